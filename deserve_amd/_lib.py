@@ -19,6 +19,7 @@ F32, F16, BF16 = 0, 1, 2
 ROUTE_OFF, ROUTE_AUTO, ROUTE_TWO_LAUNCHES, ROUTE_SHARED_LAUNCH = 0, 1, 2, 3
 APPEND_ODD_LATE = 1 << 30     # DSKV_APPEND_ODD_LATE of include/dskv.h
 LAYOUT_SEPARATE, LAYOUT_SHARED = 0, 1
+MAX_TREE_ROWS = 64         # DSKV_MAX_TREE_ROWS of include/dskv.h
 ABI_VERSION = 3          # DSKV_ABI_VERSION of the include/dskv.h these signatures were written against
 
 
@@ -48,6 +49,22 @@ class MixedStep(ctypes.Structure):
                 ("num_pages", c_int32), ("batch", c_int32), ("nnz", c_int32), ("n_qo_heads", c_int32),
                 ("n_kv_heads", c_int32), ("head_dim", c_int32), ("page_size", c_int32), ("causal", c_int32),
                 ("dtype", c_int32), ("sm_scale", c_float)]
+
+
+class StepTablesArgs(ctypes.Structure):
+    """dskv_step_tables_t of include/dskv.h."""
+    _fields_ = [(n, c_void_p) for n in (
+        "page_tables", "rows", "kv_lens", "qo_lens", "parents", "qo_indptr", "kv_page_indptr", "kv_last_page_lens",
+        "kv_page_indices", "positions", "slots", "masks")] + [("table_stride", c_int64), ("n_parents", c_int64)] + [
+        (n, c_int32) for n in ("table_rows", "table_width", "batch", "page_size", "max_tokens", "max_pages")]
+
+
+class TreeStep(ctypes.Structure):
+    """dskv_tree_step_t of include/dskv.h."""
+    _fields_ = [(n, c_void_p) for n in ("qo_indptr", "kv_page_indptr", "kv_page_indices", "kv_last_page_lens", "masks",
+                                        "workspace")] + [("workspace_bytes", c_int64), ("n_page_indices", c_int64)] + [
+        (n, c_int32) for n in ("batch", "nnz", "max_qo_len", "n_qo_heads", "n_kv_heads", "head_dim", "page_size",
+                               "num_pages", "dtype")] + [("sm_scale", c_float)]
 
 
 _lib: Optional[ctypes.CDLL] = None
@@ -129,6 +146,16 @@ _SIGNATURES = {
     "dskv_rope_append_paged_kv": (c_int32, [c_void_p, c_void_p, c_int32] + [c_void_p] * 8 +
                                   [c_int32] * 6 + [c_float, c_int32, c_void_p]),
     "dskv_upload_words": (c_int32, [c_void_p, c_void_p, c_int64, c_void_p]),
+    "dskv_step_tables": (c_int32, [POINTER(StepTablesArgs), c_void_p]),
+    "dskv_rope_append_slots": (c_int32, [c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
+                                         c_int64, c_void_p, c_void_p] + [c_int32] * 6 + [c_void_p]),
+    "dskv_tree_attn_workspace": (c_int64, [c_int32] * 7),
+    "dskv_tree_attn": (c_int32, [POINTER(TreeStep), c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
+    "dskv_verify_workspace": (c_int64, [c_int32, c_int32]),
+    "dskv_verify_drafts": (c_int32, [c_void_p] * 4 + [c_int64, c_void_p, c_int64] + [c_void_p] * 5 + [c_int64] +
+                           [c_int32] * 4 + [c_void_p]),
+    "dskv_move_rows": (c_int32, [c_void_p, c_int64, c_int32, c_int32, c_int32, c_int64] + [c_void_p] * 4 +
+                       [c_int32, c_int32, c_void_p]),
     "dskv_swap_slice": (c_int32, [c_void_p, c_int64, c_int64, c_int32, c_void_p, c_void_p,
                                   c_void_p, c_void_p]),
     "dskv_swap_create": (c_int32, [POINTER(c_void_p), c_int64]),

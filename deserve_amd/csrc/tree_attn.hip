@@ -1,0 +1,194 @@
+// Attention of a step's rows over the paged context and over the rows that they descend from: one pass over the
+// keys with a running maximum m and sum l,
+//   m' = max(m, s_j),  l' = l 2^(m - m') + 2^(s_j - m'),  O' = O 2^(m - m') + 2^(s_j - m') v_j,   out = O / l,
+// with scores in units of log 2.  A place that a row does not see has score -infinity and weight 0; a row that
+// sees nothing keeps l = 0 and gets zeros.
+#include "mfma.h"
+#include "rope_math.h"
+
+namespace dskv {
+
+struct TreeArgs {
+    const int32_t *qo_indptr, *kv_page_indptr, *kv_page_indices, *kv_last_page_lens;
+    const int64_t *masks;
+    char *out;
+    const char *q, *pages;
+    long q_stride, n_page_indices;        // q_stride in bytes
+    int batch, nnz, max_rows, n_qo_heads, n_kv_heads, head_dim, page_size, num_pages;
+    float scale;                          // sm_scale / log 2
+};
+
+// Largest b with qo_indptr[b] <= t < qo_indptr[b + 1], or -1; by a whole wave, 64 entries at a time.
+__device__ __forceinline__ int request_of_row(const int32_t *indptr, int batch, int t)
+{
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = batch;                 // entries lo .. lo + n hold the answer
+    while (n > 64) {
+        const int step = (n + 63) / 64;
+        const int at = lo + lane * step;
+        const unsigned long long le = __ballot(at < lo + n && indptr[min(at, batch)] <= t);
+        const int k = __popcll(le);
+        if (k == 0) return -1;
+        const int next = lo + (k - 1) * step;
+        n = min(step, lo + n - next);
+        lo = next;
+    }
+    const unsigned long long le = __ballot(lane < n && indptr[min(lo + lane, batch)] <= t);
+    if (le == 0) return -1;
+    const int b = lo + __popcll(le) - 1;
+    return t < indptr[b + 1] ? b : -1;
+}
+
+// Any type and head dim: one workgroup per (row, q head) whose waves take every kGenericWaves-th group of four
+// keys.  Lane (g, c) holds dims 8 c .. 8 c + 7 (and 128 more ..) of key g of the group.  Bound by the
+// latency of its loads: K and V are read once per row and q head, from the caches but for the first time.
+constexpr int kGenericWaves = 8;
+
+template <int DT> __device__ __forceinline__ void load8(const char *p, float *f)
+{
+    typedef Chunk<DT> C;
+    C::unpack(*reinterpret_cast<const u32x4 *>(p), f);
+    if (C::kElems == 4) C::unpack(*reinterpret_cast<const u32x4 *>(p + 16), f + 4);
+}
+
+template <int DT, int kChunks>
+__global__ __launch_bounds__(kGenericWaves * 64) void tree_generic_kernel(TreeArgs a)
+{
+    constexpr int E = DT == DSKV_F32 ? 4 : 2;                    // bytes of an element
+    const int t = blockIdx.x, h = blockIdx.y;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
+    const int b = request_of_row(a.qo_indptr, a.batch, t);
+    if (b < 0) return;
+    const int first = a.qo_indptr[b], n = a.qo_indptr[b + 1] - first, i = t - first;
+    if (i < 0 || i >= a.max_rows) return;
+    const int page0 = a.kv_page_indptr[b], pages = a.kv_page_indptr[b + 1] - page0;
+    const long kv_len = pages > 0 ? (long)(pages - 1) * a.page_size + min(a.kv_last_page_lens[b], a.page_size) : 0;
+    const long prior = kv_len - n;
+    const unsigned long long mask = a.masks ? (unsigned long long)a.masks[t] : 0;
+    const long seen = a.masks ? kv_len : min(kv_len, prior + i + 1);
+    const int kv_head = h / (a.n_qo_heads / a.n_kv_heads);
+    const long head_bytes = (long)a.head_dim * E, row_bytes = a.n_kv_heads * head_bytes;
+    float q[kChunks][8], o[kChunks][8];
+#pragma unroll
+    for (int k = 0; k < kChunks; k++)
+#pragma unroll
+        for (int d = 0; d < 8; d++) q[k][d] = o[k][d] = 0;
+#pragma unroll
+    for (int k = 0; k < kChunks; k++)
+        if (k * 128 + c * 8 < a.head_dim)
+            load8<DT>(a.q + t * a.q_stride + h * head_bytes + (k * 128 + c * 8) * E, q[k]);
+    float m = -INFINITY, l = 0;
+    for (long j = wave * 4 + g; j - g < seen; j += kGenericWaves * 4) {
+        bool there = j < seen;
+        if (there && a.masks && j >= prior) there = j - prior < DSKV_MAX_TREE_ROWS && (mask >> (j - prior)) & 1;
+        long page = -1;
+        if (there) {
+            const long entry = page0 + j / a.page_size;
+            if (entry >= 0 && entry < a.n_page_indices) page = a.kv_page_indices[entry];
+        }
+        there = page >= 0 && page < a.num_pages;
+        const char *key = a.pages + ((there ? page : 0) * 2 * a.page_size + (there ? j % a.page_size : 0)) * row_bytes +
+                          kv_head * head_bytes;
+        float s = 0, v[kChunks][8];
+#pragma unroll
+        for (int k = 0; k < kChunks; k++) {
+#pragma unroll
+            for (int d = 0; d < 8; d++) v[k][d] = 0;
+            if (there && k * 128 + c * 8 < a.head_dim) {
+                float x[8];
+                load8<DT>(key + (k * 128 + c * 8) * E, x);
+                load8<DT>(key + a.page_size * row_bytes + (k * 128 + c * 8) * E, v[k]);
+#pragma unroll
+                for (int d = 0; d < 8; d++) s = fmaf(q[k][d], x[d], s);
+            }
+        }
+#pragma unroll
+        for (int x = 1; x < 16; x <<= 1) s += __shfl_xor(s, x);
+        if (there) {
+            s *= a.scale;
+            const float top = fmaxf(m, s);
+            const float base = top == -INFINITY ? 0.f : top;
+            const float keep = __builtin_amdgcn_exp2f(m - base), p = __builtin_amdgcn_exp2f(s - base);
+            m = top;
+            l = l * keep + p;
+#pragma unroll
+            for (int k = 0; k < kChunks; k++)
+#pragma unroll
+                for (int d = 0; d < 8; d++) o[k][d] = fmaf(o[k][d], keep, p * v[k][d]);
+        }
+    }
+    // the 4 * kGenericWaves running sums meet in LDS
+    __shared__ float ms[kGenericWaves * 4], ls[kGenericWaves * 4];
+    __shared__ float os[kGenericWaves * 4][kChunks * 128 + 4];
+    const int part = wave * 4 + g;
+    if (c == 0) {
+        ms[part] = m;
+        ls[part] = l;
+    }
+#pragma unroll
+    for (int k = 0; k < kChunks; k++)
+#pragma unroll
+        for (int d = 0; d < 8; d++) os[part][k * 128 + c * 8 + d] = o[k][d];
+    __syncthreads();
+    float top = -INFINITY;
+    for (int p = 0; p < kGenericWaves * 4; p++) top = fmaxf(top, ms[p]);
+    const float base = top == -INFINITY ? 0.f : top;
+    for (int d = threadIdx.x; d < a.head_dim; d += kGenericWaves * 64) {
+        float sum = 0, acc = 0;
+        for (int p = 0; p < kGenericWaves * 4; p++) {
+            const float w = __builtin_amdgcn_exp2f(ms[p] - base);
+            sum += ls[p] * w;
+            acc += os[p][d] * w;
+        }
+        LoadElt<DT>::put(a.out, ((long)t * a.n_qo_heads + h) * a.head_dim + d, sum > 0 ? acc / sum : sum == 0 ? 0.f : NAN);
+    }
+}
+
+}  // namespace dskv
+
+extern "C" int64_t dskv_tree_attn_workspace(int32_t batch, int32_t nnz, int32_t max_qo_len, int32_t n_qo_heads,
+                                            int32_t n_kv_heads, int32_t head_dim, int32_t dtype)
+{
+    return 0;
+}
+
+extern "C" int dskv_tree_attn(const dskv_tree_step_t *s, void *out, const void *q, int64_t q_stride,
+                              const void *pages_layer, void *stream)
+{
+    using namespace dskv;
+    DSKV_REQUIRE(s, "tree_attn: null arguments");
+    DSKV_REQUIRE(s->batch >= 0 && s->nnz >= 0 && s->max_qo_len >= 0, "tree_attn: negative batch, nnz or rows");
+    DSKV_REQUIRE(s->dtype == DSKV_F32 || s->dtype == DSKV_F16 || s->dtype == DSKV_BF16, "tree_attn: unknown dtype %d", s->dtype);
+    DSKV_REQUIRE(s->n_kv_heads > 0 && s->n_qo_heads > 0 && s->n_qo_heads % s->n_kv_heads == 0,
+                 "tree_attn: n_qo_heads %d must be a multiple of n_kv_heads %d", s->n_qo_heads, s->n_kv_heads);
+    DSKV_REQUIRE(s->head_dim > 0 && s->head_dim % 8 == 0 && s->head_dim <= 256,
+                 "tree_attn: head_dim %d must be a multiple of 8 up to 256", s->head_dim);
+    DSKV_REQUIRE(s->page_size > 0 && s->num_pages > 0 && s->n_page_indices >= 0, "tree_attn: bad page shape");
+    DSKV_REQUIRE(!s->masks || s->max_qo_len <= DSKV_MAX_TREE_ROWS, "tree_attn: masks hold %d rows a request, max_qo_len is %d",
+                 DSKV_MAX_TREE_ROWS, s->max_qo_len);
+    if (s->batch == 0 || s->nnz == 0 || s->max_qo_len == 0) return 0;
+    const int size = s->dtype == DSKV_F32 ? 4 : 2;
+    DSKV_REQUIRE(out && q && pages_layer && s->qo_indptr && s->kv_page_indptr && s->kv_last_page_lens &&
+                 (s->kv_page_indices || s->n_page_indices == 0), "tree_attn: null pointer argument");
+    DSKV_REQUIRE(q_stride >= (int64_t)s->n_qo_heads * s->head_dim, "tree_attn: rows of q overlap");
+    DSKV_REQUIRE(((uintptr_t)out | (uintptr_t)q | (uintptr_t)pages_layer) % 16 == 0 && q_stride * size % 16 == 0,
+                 "tree_attn: tensors and their rows must be 16-byte aligned");
+    TreeArgs a = {s->qo_indptr, s->kv_page_indptr, s->kv_page_indices, s->kv_last_page_lens, s->masks, (char *)out,
+                  (const char *)q, (const char *)pages_layer, (long)q_stride * size, (long)s->n_page_indices, s->batch,
+                  s->nnz, s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->head_dim, s->page_size, s->num_pages,
+                  s->sm_scale * 1.4426950408889634f};
+    DSKV_REQUIRE(s->n_qo_heads <= 65535, "tree_attn: at most 65535 heads");
+    const dim3 grid((unsigned)s->nnz, (unsigned)s->n_qo_heads), block(kGenericWaves * 64);
+    hipStream_t st = (hipStream_t)stream;
+#define DSKV_TREE_GENERIC(DT)                                                                                  \
+    do {                                                                                                       \
+        if (s->head_dim <= 128) hipLaunchKernelGGL((tree_generic_kernel<DT, 1>), grid, block, 0, st, a);       \
+        else hipLaunchKernelGGL((tree_generic_kernel<DT, 2>), grid, block, 0, st, a);                          \
+    } while (0)
+    if (s->dtype == DSKV_F32) DSKV_TREE_GENERIC(DSKV_F32);
+    else if (s->dtype == DSKV_F16) DSKV_TREE_GENERIC(DSKV_F16);
+    else DSKV_TREE_GENERIC(DSKV_BF16);
+#undef DSKV_TREE_GENERIC
+    DSKV_LAUNCH_CHECK("tree_generic_kernel");
+    return 0;
+}

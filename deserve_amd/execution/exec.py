@@ -15,6 +15,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
+from deserve_amd.draft_ops import BatchTreeWithPagedKVCacheWrapper
 from deserve_amd.execution.result import BatchResult
 from deserve_amd.kvcache.paged.kvcache import PagedKVCache
 from deserve_amd.model.context.flash import FlashDecodeCtx, FlashPrefillCtx
@@ -35,6 +36,17 @@ def get_wrappers(device: torch.device):
         _wrappers[device] = (BatchDecodeWithPagedKVCacheWrapper(ws),
                              BatchPrefillWithPagedKVCacheWrapper(ws))
     return _wrappers[device]
+
+
+_tree_wrappers: Dict[torch.device, BatchTreeWithPagedKVCacheWrapper] = {}
+
+
+def get_tree_wrapper(device: torch.device) -> BatchTreeWithPagedKVCacheWrapper:
+    """The wrapper for steps of drafted tokens, over the workspace of get_wrappers."""
+    device = torch.device(device)
+    if device not in _tree_wrappers:
+        _tree_wrappers[device] = BatchTreeWithPagedKVCacheWrapper(get_wrappers(device)[0]._workspace)
+    return _tree_wrappers[device]
 
 
 @dataclass

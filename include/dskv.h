@@ -541,6 +541,112 @@ int dskv_swap_streams(dskv_swap_t *handle, void **out_stream, void **in_stream);
 int dskv_swap_bind_compute_stream(dskv_swap_t *handle, void *compute_stream,
                                   int32_t *independent_out);
 
+/*
+ * A step that verifies drafted tokens (no counterpart in the reference).  Request b brings n_b rows to it: row 0
+ * is the last token it was given, whose K/V its cache does not hold yet, the others are drafted tokens that form a
+ * chain or a tree behind it; a row's parent has a smaller index.  What follows keeps lengths and tables on
+ * the device - how far a request gets is known there only - so nothing here plans on the host, and all of it can be
+ * captured into a graph and replayed with other lengths.
+ */
+#define DSKV_MAX_TREE_ROWS 64          /* rows of one request in a tree, and in a verification */
+
+/*
+ * Block tables, slot map, positions and tree masks from the requests' lengths.  All arrays on the device.
+ * page_tables: table_rows rows of table_width page ids, table_stride entries apart; request b owns row rows[b]
+ * (rows null: row b).  kv_lens: tokens cached before the step; qo_lens: new rows of the step, 0 and more.
+ * masks null: rows follow one another.  Else parents: index of every row's parent within its request, ragged by
+ * qo_indptr, n_parents entries; a value outside [0, own index) is no parent, nor is one past them.
+ * Written: qo_indptr and kv_page_indptr (batch + 1), kv_last_page_lens (batch), kv_page_indices (its first
+ * kv_page_indptr[batch] of max_pages entries; those behind stay as they are), and for all max_tokens
+ * rows slots (page id * page_size + place in the page; -1 for rows behind the last request), positions
+ * (cached tokens + number of rows descended from; 0 behind the last) and, if not null, masks (bit j: the row is row j of
+ * its request or descends from it; 0 behind the last).
+ * A request whose numbers are negative, whose table row does not exist or does not hold its tokens, or that has more than
+ * DSKV_MAX_TREE_ROWS rows with masks, gets no rows and no pages, as if its lengths were 0; so does the first request
+ * that does not fit max_tokens or max_pages, with all behind it.
+ */
+typedef struct dskv_step_tables {
+    const int32_t *page_tables, *rows, *kv_lens, *qo_lens, *parents;
+    int32_t *qo_indptr, *kv_page_indptr, *kv_last_page_lens, *kv_page_indices, *positions;
+    int64_t *slots, *masks;
+    int64_t table_stride, n_parents;
+    int32_t table_rows, table_width, batch, page_size, max_tokens, max_pages;
+} dskv_step_tables_t;
+int dskv_step_tables(const dskv_step_tables_t *tables, void *stream);
+
+/*
+ * Rows of a step into the slots of a map: K[slots[t]] = rotated k[t], V[slots[t]] = v[t], q_out[t] = rotated q[t].
+ * rope_table: (nnz, head_dim) floats, row t = cos | sin of the row's angles (dskv_rope_table of the positions),
+ * with the arithmetic of dskv_apply_rope; null: nothing is rotated, q and q_out are left alone (may be null).
+ * q, k, v: rows *_stride elements apart, the heads of a row contiguous, so that they may be parts of one
+ * projection's output; rows and strides at multiples of 16 bytes.  q_out is contiguous.  A slot outside
+ * [0, num_pages * page_size) is no slot: the row's k and v go nowhere.  The slots of a call are distinct
+ * (where two are the same, every 16 bytes come from one of the two rows).
+ */
+int dskv_rope_append_slots(void *q_out, void *pages_layer, int32_t num_pages, const void *q, const void *k,
+                           const void *v, int64_t q_stride, int64_t k_stride, int64_t v_stride, const int64_t *slots,
+                           const float *rope_table, int32_t nnz, int32_t page_size, int32_t n_qo_heads,
+                           int32_t n_kv_heads, int32_t head_dim, int32_t dtype, void *stream);
+
+/*
+ * Attention of a step's rows over the paged context and over the rows that they descend from.  Row i of request b
+ * sees cached position j < kv_len_b - n_b, and new row j of its request where bit j of its mask is set (masks null:
+ * where j <= i).  A row that sees nothing gets zeros.  K and V are in the pages (kv_len_b counts the new rows).
+ * q rows are q_stride elements apart (heads contiguous), out is contiguous; rows behind qo_indptr[batch]
+ * are left as they are.  A page id outside [0, num_pages) holds no tokens, nor does a table entry past n_page_indices.
+ * max_qo_len: no request has more rows (more: the further ones are left as they are); with masks at most
+ * DSKV_MAX_TREE_ROWS.  head_dim: a multiple of 8 up to 256.
+ * workspace (16-byte aligned): at least dskv_tree_attn_workspace(..) bytes, which do not depend on the lengths; used
+ * by one call at a time.
+ */
+typedef struct dskv_tree_step {
+    const int32_t *qo_indptr, *kv_page_indptr, *kv_page_indices, *kv_last_page_lens;
+    const int64_t *masks;
+    void *workspace;
+    int64_t workspace_bytes, n_page_indices;
+    int32_t batch, nnz, max_qo_len, n_qo_heads, n_kv_heads, head_dim, page_size, num_pages, dtype;
+    float sm_scale;
+} dskv_tree_step_t;
+int64_t dskv_tree_attn_workspace(int32_t batch, int32_t nnz, int32_t max_qo_len, int32_t n_qo_heads, int32_t n_kv_heads,
+                                 int32_t head_dim, int32_t dtype);
+int dskv_tree_attn(const dskv_tree_step_t *step, void *out, const void *q, int64_t q_stride, const void *pages_layer,
+                   void *stream);
+
+/*
+ * Drafted tokens accepted or refused, from given random numbers.  target_probs row t: the target's probabilities of
+ * what follows row t (vocab of them, rows target_stride elements apart, dtype); tokens[t]: row t's token; uniforms[t] in
+ * [0, 1): row t's number, for row 0 of a request that of its last draw.  From row 0 on, the children of the row reached
+ * are tried in index order and the first that passes is followed, with p the target's row there:
+ *   draft_probs given (parents null): token x was sampled from q, row of draft_probs at the parent, and passes if
+ *     uniform * q(x) < p(x);
+ *   else: it passes if no earlier child refused there has token x and uniform * (1 - sum of p over the distinct tokens of those)
+ *     < p(x).
+ * Where none passes (or there is none) the walk ends, and the request's last token is the first t with cumulated
+ * w(0..t) > uniforms[row 0] * sum of w, where w = max(p - q, 0) if a child was refused with draft_probs, p with the refused
+ * children's tokens at 0 without, and p if w has no mass (token 0 if p has none).  A last number below 0 counts as 0, one from 1 on
+ * or that is none draws the last index with weight.  Sums in 64 bits.  Values of p and q that are
+ * negative, infinite or no number count as 0, tokens outside [0, vocab) have probability 0.
+ * Written for all nnz rows: path (row[j] of the request: index of the j-th row of the walk, row 0 first; then -1),
+ * out_tokens (tokens of the walk's rows behind row 0, then the last token; then -1); counts[b]: rows of the
+ * walk = tokens given, 0 for requests without rows or with more than DSKV_MAX_TREE_ROWS.
+ * workspace: dskv_verify_workspace(batch, vocab) bytes, 16-byte aligned, used by one call at a time.
+ */
+int64_t dskv_verify_workspace(int32_t batch, int32_t vocab);
+int dskv_verify_drafts(int32_t *counts, int32_t *path, int32_t *out_tokens, const void *target_probs,
+                       int64_t target_stride, const void *draft_probs, int64_t draft_stride, const int32_t *tokens,
+                       const float *uniforms, const int32_t *qo_indptr, const int32_t *parents, void *workspace,
+                       int64_t workspace_bytes, int32_t batch, int32_t nnz, int32_t vocab, int32_t dtype, void *stream);
+
+/*
+ * K/V of the rows of every request's walk to where its sequence goes on: row j of the walk, j >= 1, from slot
+ * slots[row path[j]] to slots[row j], K and V, in all layers.  pages: (n_layers, num_pages, 2, page_size) rows of row_bytes
+ * with layer_stride_bytes between layers, a token's K or its V.  path rises, as
+ * dskv_verify_drafts writes it; entries that do not, or lie outside their request, and slots outside the pool move nothing.
+ */
+int dskv_move_rows(void *pages, int64_t layer_stride_bytes, int32_t n_layers, int32_t num_pages, int32_t page_size,
+                   int64_t row_bytes, const int64_t *slots, const int32_t *qo_indptr, const int32_t *path,
+                   const int32_t *counts, int32_t batch, int32_t nnz, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,228 @@
+"""Attention of a step's rows over the paged context and over the rows that they descend from."""
+import numpy as np
+import pytest
+import torch
+
+from draftutil import attention, make_step
+
+CASES = [
+    # name, cached tokens, rows, tree, page, Hq, Hkv, D, dtype
+    ("one_token", [0], [1], False, 16, 32, 8, 128, "bf16"),
+    ("nothing_cached", [0, 0, 0], [5, 64, 1], True, 16, 32, 8, 128, "bf16"),
+    ("no_rows_between", [40, 0, 9, 70], [0, 0, 3, 0], False, 16, 32, 8, 128, "f16"),
+    ("tile_edges", [14, 15, 16, 30, 31, 32, 33, 62, 63, 64], [1, 2, 1, 2, 1, 1, 3, 2, 1, 5], False, 16, 32, 8, 128, "bf16"),
+    ("block_edges", [127, 128, 129, 255, 256, 257, 511], [4, 1, 7, 1, 4, 16, 2], True, 16, 32, 8, 128, "f16"),
+    ("column_edges_group4", [50] * 8, [3, 4, 5, 8, 9, 16, 17, 64], True, 16, 32, 8, 128, "bf16"),
+    ("column_edges_group7", [33] * 6, [1, 2, 3, 9, 10, 37], True, 8, 28, 4, 128, "bf16"),
+    ("group1", [100, 3], [64, 17], True, 16, 8, 8, 128, "f16"),
+    ("group32", [70, 200], [5, 64], True, 16, 32, 1, 128, "bf16"),
+    ("group40", [70], [9], False, 16, 40, 1, 128, "f16"),
+    ("odd_heads", [90, 5], [6, 30], True, 16, 15, 5, 128, "bf16"),
+    ("page1", [60, 131], [7, 20], True, 1, 16, 4, 128, "bf16"),
+    ("page3", [60, 131], [7, 20], True, 3, 16, 4, 128, "f16"),
+    ("page12", [60, 500], [7, 20], False, 12, 16, 4, 128, "bf16"),
+    ("page128", [600, 127, 128], [7, 1, 1], True, 128, 16, 4, 128, "bf16"),
+    ("dim64", [77, 300], [5, 40], True, 16, 32, 8, 64, "bf16"),
+    ("dim64_f16_page4", [1000], [12], False, 4, 12, 4, 64, "f16"),
+    ("dim80", [77, 30], [5, 9], True, 16, 8, 2, 80, "bf16"),
+    ("dim8", [77], [5], True, 16, 4, 2, 8, "f16"),
+    ("dim256", [130, 2], [5, 33], True, 16, 8, 2, 256, "bf16"),
+    ("fp32", [77, 300, 0], [5, 40, 1], True, 16, 16, 4, 128, "fp32"),
+    ("fp32_dim64", [700], [3], False, 12, 8, 8, 64, "fp32"),
+    ("fp32_dim200", [90], [12], True, 16, 4, 4, 200, "fp32"),
+    ("long", [3000], [6], False, 16, 8, 2, 128, "bf16"),
+    ("long_tree", [2500, 9], [64, 2], True, 16, 16, 2, 128, "f16"),
+    ("many_short", list(range(70)), [1 + i % 5 for i in range(70)], True, 8, 8, 2, 128, "bf16"),
+    ("many_lengths", [int(x) for x in np.random.default_rng(1).integers(0, 900, 40)], [4] * 40, False, 16, 8, 2, 128, "bf16"),
+]
+
+
+def run(step, on=None, scale=None, max_qo_len=None, masks="own", q=None, out=None):
+    from deserve_amd.execution.exec import get_tree_wrapper
+
+    on = on or step.on("cuda")
+    w = get_tree_wrapper(torch.device("cuda", 0))
+    w.begin_forward(*on["csr"], step.hq, step.hkv, step.dim, step.page,
+                    max_qo_len=int(step.rows.max()) if max_qo_len is None else max_qo_len,
+                    masks=on["masks"] if isinstance(masks, str) else masks)
+    q = on["q"] if q is None else q
+    return w.forward(q, on["pages"], scale, out=torch.full_like(q, float("nan")) if out is None else out)
+
+
+def compare(got, want, bound):
+    got = got.double().cpu().numpy()
+    assert np.isfinite(got).all()
+    off = np.abs(got - want) / bound
+    assert off.max() <= 1, (np.unravel_index(off.argmax(), off.shape), off.max())
+
+
+def case_step(case, seed=11):
+    name, kv, rows, tree, page, hq, hkv, dim, dtype = case
+    return make_step(seed, kv, rows, tree, page, hq, hkv, dim, dtype)
+
+
+@pytest.mark.parametrize("case", [c for c in CASES if c[7] == 128 and max(c[1]) < 400], ids=lambda c: c[0])
+def test_the_bound_lets_no_row_miss_a_key(case):
+    """A row without one of the tokens that it sees (its heaviest) is over its bound somewhere."""
+    step = case_step(case)
+    want, bound = attention(step)
+    for b in range(len(step.kv)):
+        lo, hi, table, length = step.request(b)
+        if hi == lo or step.sees(b)[-1].sum() < 2:
+            continue
+        held = step.pages[torch.from_numpy(table).long()].double().numpy()
+        k, v = (held[:, i].reshape(-1, step.hkv, step.dim)[:length, 0] for i in (0, 1))
+        s = np.where(step.sees(b)[-1], k @ step.q[hi - 1, 0].double().numpy() * step.dim ** -0.5, -np.inf)
+        w = np.exp(s - s.max())
+        w[w.argmax()] = 0
+        assert (np.abs(w @ v / w.sum() - want[hi - 1, 0]) > bound[hi - 1, 0]).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", CASES, ids=lambda c: c[0])
+def test_rows_match_the_definition(case):
+    print("[case] tree attention", *case, flush=True)
+    step = case_step(case)
+    on = step.on("cuda")
+    compare(run(step, on), *attention(step))
+    # what the pages hold behind a sequence is never looked at
+    for b in range(len(step.kv)):
+        _, _, table, length = step.request(b)
+        if length % step.page:
+            on["pages"][int(table[-1]), :, length % step.page:] = float("nan")
+    got = run(step, on)
+    compare(got, *attention(step))
+    assert torch.equal(got, run(step, on)), "the same call gives other bits"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dim", [("bf16", 128), ("f16", 64), ("fp32", 128), ("bf16", 80)])
+def test_rows_that_see_nothing(dtype, dim):
+    """Masks of a caller's own: no bit at all, later rows only, all rows."""
+    step = make_step(2, [0, 5, 0], [6, 4, 3], True, 16, 16, 4, dim, dtype)
+    step.masks = np.array([0, 2, 0, 63, 32, -1, 0, 15, 8, 1, 0, 0, 0], np.int64)
+    want, bound = attention(step)
+    got = run(step)
+    compare(got, want, bound + (want == 0) * 1e-30)
+    assert not got[[0, 2, 10, 11, 12]].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dim,group", [("bf16", 128, 4), ("f16", 128, 1), ("f16", 64, 8), ("fp32", 128, 4), ("fp32", 64, 2), ("bf16", 96, 4)])
+def test_infinities_and_nan_in_masked_places(dtype, dim, group):
+    """A drafted row whose K and V are no numbers reaches the rows that descend from it and no other."""
+    for value in (float("nan"), float("inf"), -float("inf")):
+        step = make_step(7, [37, 200, 0], [20, 64, 9], True, 16, 4 * group, 4, dim, dtype)
+        want, bound = attention(step)
+        on, slots = step.on("cuda"), step.slots()
+        broken = {0: [3, 7], 1: [5, 33, 62], 2: [4]}
+        hit = np.zeros(len(want), bool)
+        for b, rows in broken.items():
+            for r in rows:
+                at = int(slots[step.qo_indptr[b] + r])
+                on["pages"][at // 16, 1, at % 16, :, ::3] = value
+                on["pages"][at // 16, 0, at % 16] = float("nan")
+                hit[step.qo_indptr[b]: step.qo_indptr[b + 1]] |= step.sees(b)[:, step.kv[b] + r]
+        got = run(step, on).double().cpu().numpy()
+        off = np.abs(got[~hit] - want[~hit]) / bound[~hit]
+        assert off.max() <= 1, (value, off.max())
+        assert not np.isfinite(got[hit]).all(2).any()
+
+
+@pytest.mark.gpu
+def test_tokens_apart_scales_and_rows_left_out():
+    step = make_step(8, [130, 7, 64], [9, 3, 12], True)
+    on = step.on("cuda")
+    qkv = torch.randn((24, 48, 128), device="cuda").bfloat16()
+    qkv[:, :32] = on["q"]
+    for scale in (0.2, 0.0, -0.05):
+        compare(run(step, on, scale, q=qkv[:, :32], out=torch.empty_like(on["q"])), *attention(step, scale))
+    # a batch padded with rows that belong to nobody, and requests with more rows than max_qo_len
+    want, bound = attention(step)
+    q = torch.cat([on["q"], torch.full_like(on["q"][:5], float("nan"))])
+    masks = torch.cat([on["masks"], on["masks"][:5]])
+    out = torch.full_like(q, 7.0)
+    run(step, on, q=q, masks=masks, out=out)
+    compare(out[:24], want, bound)
+    assert (out[24:] == 7).all()
+    out.fill_(7.0)
+    run(step, on, q=q, masks=masks, max_qo_len=5, out=out)
+    left = [5, 6, 7, 8] + list(range(17, 29))
+    kept = [i for i in range(24) if i not in left]
+    compare(out[kept], want[kept], bound[kept])
+    assert (out[left] == 7).all()
+
+
+@pytest.mark.gpu
+def test_chains_longer_than_a_tree():
+    step = make_step(9, [100, 0], [150, 70], False, 16, 16, 4)
+    compare(run(step), *attention(step))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dim", [("bf16", 128), ("fp32", 64), ("f16", 96)])
+def test_pages_outside_the_pool_hold_no_tokens(dtype, dim):
+    step = make_step(10, [100, 40], [4, 3], True, 16, 8, 2, dim, dtype)
+    on = step.on("cuda")
+    want_step = make_step(10, [100, 40], [4, 3], True, 16, 8, 2, dim, dtype)
+    table = step.kv_page_indices.copy()
+    table[[2, 5, 8]] = [-1, step.pages.shape[0], 2 ** 31 - 1]
+    on["csr"] = on["csr"][:2] + (torch.from_numpy(table).cuda(),) + on["csr"][3:]
+    gone = {0: [2, 5], 1: [8 - int(step.kv_page_indptr[1])]}
+    sees = Step_without(want_step, gone)
+    compare(run(step, on), *attention(sees))
+    # a table that is shorter than its indptr says
+    on["csr"] = on["csr"][:2] + (torch.from_numpy(step.kv_page_indices[:8].copy()).cuda(),) + on["csr"][3:]
+    compare(run(step, on), *attention(Step_without(want_step, {1: [8 - int(step.kv_page_indptr[1]), 9 - int(step.kv_page_indptr[1])]})))
+
+
+def Step_without(step, gone):
+    """The step with the given pages of its requests unseen."""
+    class Without(type(step)):
+        def sees(self, b):
+            out = super().sees(b)
+            for p in gone.get(b, ()):
+                out[:, p * self.page: (p + 1) * self.page] = False
+            return out
+    return Without(**vars(step))
+
+
+@pytest.mark.gpu
+def test_another_stream_and_replays_with_other_lengths():
+    """Captured once, replayed with other lengths, trees and tables in the same arrays; eager work between."""
+    from deserve_amd.draft_ops import BatchTreeWithPagedKVCacheWrapper
+
+    steps = [make_step(20 + i, kv, rows, True, 16, 32, 8) for i, (kv, rows) in enumerate(
+        [([40, 700, 3, 0], [8, 8, 8, 8]), ([0, 1, 2000, 33], [1, 20, 4, 7]), ([5, 0, 0, 0], [0, 0, 0, 3])])]
+    pages = torch.zeros((200, 2, 16, 8, 128), dtype=torch.bfloat16, device="cuda")
+    csr = [torch.zeros(n, dtype=torch.int32, device="cuda") for n in (5, 5, 200, 4)]
+    masks = torch.zeros(32, dtype=torch.int64, device="cuda")
+    q, out = (torch.zeros((32, 32, 128), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    w = BatchTreeWithPagedKVCacheWrapper(torch.empty(128 << 20, dtype=torch.uint8, device="cuda"))
+
+    def load(step):
+        on = step.on("cuda")
+        for to, t in zip([*csr, masks, q, pages], [*on["csr"], on["masks"], on["q"], on["pages"]]):
+            to[: t.shape[0]] = t
+        out.fill_(7)
+
+    load(steps[0])
+    w.begin_forward(*csr, 32, 8, 128, 16, max_qo_len=20, masks=masks)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        eager = w.forward(q, pages, out=out).clone()
+    torch.cuda.current_stream().wait_stream(stream)
+    compare(eager[:32], *attention(steps[0]))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        w.forward(q, pages, out=out)
+    for step in (steps[0], steps[1], steps[2], steps[1], steps[0]):
+        load(step)
+        graph.replay()
+        total = int(step.rows.sum())
+        compare(out[:total], *attention(step))
+        assert (out[total:] == 7).all()
+        again = w.forward(q, pages, out=torch.full_like(out, 7))
+        assert torch.equal(again, out)
+        torch.cuda.synchronize()
