@@ -3,20 +3,10 @@
 //   m' = max(m, s_j),  l' = l 2^(m - m') + 2^(s_j - m'),  O' = O 2^(m - m') + 2^(s_j - m') v_j,   out = O / l,
 // with scores in units of log 2.  A place that a row does not see has score -infinity and weight 0; a row that
 // sees nothing keeps l = 0 and gets zeros.
-#include "mfma.h"
 #include "rope_math.h"
+#include "tree_kernel.h"
 
 namespace dskv {
-
-struct TreeArgs {
-    const int32_t *qo_indptr, *kv_page_indptr, *kv_page_indices, *kv_last_page_lens;
-    const int64_t *masks;
-    char *out;
-    const char *q, *pages;
-    long q_stride, n_page_indices;        // q_stride in bytes
-    int batch, nnz, max_rows, n_qo_heads, n_kv_heads, head_dim, page_size, num_pages;
-    float scale;                          // sm_scale / log 2
-};
 
 // Largest b with qo_indptr[b] <= t < qo_indptr[b + 1], or -1; by a whole wave, 64 entries at a time.
 __device__ __forceinline__ int request_of_row(const int32_t *indptr, int batch, int t)
@@ -43,6 +33,7 @@ __device__ __forceinline__ int request_of_row(const int32_t *indptr, int batch, 
 // keys.  Lane (g, c) holds dims 8 c .. 8 c + 7 (and 128 more ..) of key g of the group.  Bound by the
 // latency of its loads: K and V are read once per row and q head, from the caches but for the first time.
 constexpr int kGenericWaves = 8;
+constexpr int kTreeUnits = 256;        // compute units
 
 template <int DT> __device__ __forceinline__ void load8(const char *p, float *f)
 {
@@ -144,12 +135,61 @@ __global__ __launch_bounds__(kGenericWaves * 64) void tree_generic_kernel(TreeAr
     }
 }
 
+// The matrix form takes head dims 64 and 128.  Tiles of up to 64 columns: few tiles, each as narrow as it can be.
+struct TreeForm {
+    int blocks, col_tiles, shares;
+};
+static bool matrix_form(int head_dim) { return head_dim == 64 || head_dim == 128; }
+static TreeForm tree_form(int max_rows, int n_qo_heads, int n_kv_heads)
+{
+    TreeForm f;
+    const long cols = (long)max_rows * (n_qo_heads / n_kv_heads);
+    f.col_tiles = (int)((cols + 63) / 64);
+    f.blocks = (int)((cols + 16L * f.col_tiles - 1) / (16L * f.col_tiles));
+    // two workgroups a compute unit where their registers allow it
+    const int resident = kTreeUnits * (f.blocks <= 2 ? 2 : 1);
+    f.shares = resident >= n_kv_heads ? resident / n_kv_heads : 1;
+    return f;
+}
+static int64_t units_bytes(int batch) { return ((int64_t)batch + 2) / 2 * 16; }
+static int64_t slots_of(const TreeForm &f, int n_kv_heads) { return 2LL * f.shares * n_kv_heads * f.blocks * 16; }
+
+template <int DT, int kD, int kBlocks> static int launch_tree(const TreeArgs &a, const TreeForm &f, hipStream_t stream)
+{
+    typedef TreeShape<DT, kD, kBlocks> S;
+    hipLaunchKernelGGL((tree_matrix_kernel<DT, kD, kBlocks>), dim3((unsigned)(f.shares * a.n_kv_heads)),
+                       dim3(kTreeThreads), 0, stream, a);
+    DSKV_LAUNCH_CHECK("tree_matrix_kernel");
+    const int columns = 256 / (kD / 4 * 4);
+    hipLaunchKernelGGL((tree_merge_kernel<DT, kD, kBlocks>),
+                       dim3((unsigned)(a.batch * f.col_tiles), (unsigned)a.n_kv_heads, (unsigned)(S::kCols / columns)), dim3(256), 0,
+                       stream, a, f.col_tiles);
+    DSKV_LAUNCH_CHECK("tree_merge_kernel");
+    return 0;
+}
+template <int DT, int kD> static int launch_tree_blocks(const TreeArgs &a, const TreeForm &f, hipStream_t stream)
+{
+    switch (f.blocks) {
+    case 1: return launch_tree<DT, kD, 1>(a, f, stream);
+    case 2: return launch_tree<DT, kD, 2>(a, f, stream);
+    case 3: return launch_tree<DT, kD, 3>(a, f, stream);
+    default: return launch_tree<DT, kD, 4>(a, f, stream);
+    }
+}
+template <int DT> static int launch_tree_dim(const TreeArgs &a, const TreeForm &f, hipStream_t stream)
+{
+    return a.head_dim == 64 ? launch_tree_blocks<DT, 64>(a, f, stream) : launch_tree_blocks<DT, 128>(a, f, stream);
+}
+
 }  // namespace dskv
 
 extern "C" int64_t dskv_tree_attn_workspace(int32_t batch, int32_t nnz, int32_t max_qo_len, int32_t n_qo_heads,
                                             int32_t n_kv_heads, int32_t head_dim, int32_t dtype)
 {
-    return 0;
+    using namespace dskv;
+    if (batch <= 0 || nnz <= 0 || max_qo_len <= 0 || n_kv_heads <= 0 || n_qo_heads < n_kv_heads || !matrix_form(head_dim)) return 0;
+    const TreeForm f = tree_form(max_qo_len, n_qo_heads, n_kv_heads);
+    return units_bytes(batch) + slots_of(f, n_kv_heads) * (head_dim + 2) * (int64_t)sizeof(float);
 }
 
 extern "C" int dskv_tree_attn(const dskv_tree_step_t *s, void *out, const void *q, int64_t q_stride,
@@ -177,9 +217,27 @@ extern "C" int dskv_tree_attn(const dskv_tree_step_t *s, void *out, const void *
                   (const char *)q, (const char *)pages_layer, (long)q_stride * size, (long)s->n_page_indices, s->batch,
                   s->nnz, s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->head_dim, s->page_size, s->num_pages,
                   s->sm_scale * 1.4426950408889634f};
+    hipStream_t st = (hipStream_t)stream;
+    if (matrix_form(s->head_dim) && (int64_t)s->num_pages * 2 * s->page_size < INT32_MAX) {
+        const TreeForm f = tree_form(s->max_qo_len, s->n_qo_heads, s->n_kv_heads);
+        const int64_t need = dskv_tree_attn_workspace(s->batch, s->nnz, s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->head_dim, s->dtype);
+        if (!s->workspace || s->workspace_bytes < need) {
+            set_error("tree_attn: workspace of %lld bytes, %lld are needed", (long long)s->workspace_bytes, (long long)need);
+            return DSKV_E_NOMEM;
+        }
+        DSKV_REQUIRE((uintptr_t)s->workspace % 16 == 0, "tree_attn: the workspace must be 16-byte aligned");
+        DSKV_REQUIRE((int64_t)s->batch * f.col_tiles < INT32_MAX && s->n_kv_heads <= 65535, "tree_attn: too large a batch");
+        a.units_before = (int64_t *)s->workspace;
+        a.part_o = (float *)((char *)s->workspace + units_bytes(s->batch));
+        a.part_ml = a.part_o + slots_of(f, s->n_kv_heads) * s->head_dim;
+        a.n_shares = f.shares;
+        a.group = s->n_qo_heads / s->n_kv_heads;
+        if (s->dtype == DSKV_F32) return launch_tree_dim<DSKV_F32>(a, f, st);
+        if (s->dtype == DSKV_F16) return launch_tree_dim<DSKV_F16>(a, f, st);
+        return launch_tree_dim<DSKV_BF16>(a, f, st);
+    }
     DSKV_REQUIRE(s->n_qo_heads <= 65535, "tree_attn: at most 65535 heads");
     const dim3 grid((unsigned)s->nnz, (unsigned)s->n_qo_heads), block(kGenericWaves * 64);
-    hipStream_t st = (hipStream_t)stream;
 #define DSKV_TREE_GENERIC(DT)                                                                                  \
     do {                                                                                                       \
         if (s->head_dim <= 128) hipLaunchKernelGGL((tree_generic_kernel<DT, 1>), grid, block, 0, st, a);       \

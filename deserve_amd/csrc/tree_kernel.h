@@ -1,0 +1,501 @@
+// The matrix form of the tree attention: head_dim 64 and 128, all three types.  See tree_attn.hip for what is computed.
+//
+// The columns of a kv head are its (row, q head of the group) pairs; S^T = K Q^T and O^T = V^T P^T keep a column in the
+// lanes that share lane % 16, so its maximum and sum never cross more than four lanes.
+// The work is cut without a host plan: request b has ct_b column tiles of kBlocks * 16 columns and st_b subtiles
+// of kSub tokens; all (request, column tile, subtile) units lie end to end, every workgroup takes the sums over the requests for
+// itself, and share s of n covers units [s U / n, (s + 1) U / n): equal to one unit, whatever the lengths.  One
+// workgroup per (share, kv head); its four waves take the share's subtiles in turn, each with a running maximum, sum and O of
+// its own, and meet in LDS where an item (request, column tile) ends.  An item that a share boundary cuts leaves
+// a partial (maximum, sum, O in fp32) that tree_merge_kernel adds up.
+// K and V go by whole rows through registers (one subtile ahead) and a wave's own LDS: rows of 256 bytes are what
+// HBM delivers best, and a row's page is looked up once per subtile, by lane, so pages may have any size.
+#pragma once
+
+#include "kv_tile.h"
+
+namespace dskv {
+
+constexpr int kTreeWaves = 4;
+constexpr int kTreeThreads = kTreeWaves * 64;
+
+struct TreeArgs {
+    const int32_t *qo_indptr, *kv_page_indptr, *kv_page_indices, *kv_last_page_lens;
+    const int64_t *masks;
+    char *out;
+    const char *q, *pages;
+    long q_stride, n_page_indices;        // q_stride in bytes
+    int batch, nnz, max_rows, n_qo_heads, n_kv_heads, head_dim, page_size, num_pages;
+    float scale;                          // sm_scale / log 2
+    // matrix form
+    float *part_o, *part_ml;              // (2 * n_shares, n_kv_heads, columns of a tile, head_dim | 2)
+    int64_t *units_before;                // (batch + 1): units of the requests in front
+    int n_shares, group;
+};
+
+template <int DT, int kD, int kBlocks> struct TreeShape {
+    static constexpr int kElt = DT == DSKV_F32 ? 4 : 2;
+    static constexpr int kSub = DT == DSKV_F32 ? 16 : 32;            // tokens of a subtile
+    static constexpr int kTiles = kSub / 16;
+    static constexpr int kRow = kD * kElt;                           // bytes
+    static constexpr int kChunks = kRow / 16;                        // 16-byte chunks of a row
+    static constexpr int kRowsPerLoad = 64 / kChunks;
+    static constexpr int kLoads = kSub / kRowsPerLoad;
+    static constexpr int kSteps = kD * kElt / 64;                    // 16-byte operand chunks of a lane along the dims
+    static constexpr int kDimTiles = kD / 16;
+    static constexpr int kCols = kBlocks * 16;
+    static constexpr int kKPitch = kRow + 16;                        // 16 rows' chunks at one offset meet no bank twice
+    static constexpr int kVPitch = DT == DSKV_F32 ? kRow + 16 : kRow + 32;
+    static constexpr int kWaveLds = kSub * (kKPitch + kVPitch);
+    static constexpr int kOPitch = kD + 4;                           // floats
+    static constexpr int kMergeLds = kTreeWaves * kCols * (kOPitch + 2) * 4;
+    static constexpr int kLds = kTreeWaves * kWaveLds > kMergeLds ? kTreeWaves * kWaveLds : kMergeLds;
+};
+
+struct TreeRequest {
+    long first;          // its first row
+    long kv_len;
+    int page0, pages;
+    int n;               // rows that are computed
+    int rows;            // rows it has
+    int col_tiles, subtiles;
+    __device__ __forceinline__ long units() const { return (long)col_tiles * subtiles; }
+};
+
+// What the arrays say about request b, within the bounds of the tensors.
+template <int kCols, int kSub> __device__ __forceinline__ TreeRequest tree_request(const TreeArgs &a, int b)
+{
+    TreeRequest r;
+    r.first = a.qo_indptr[b];
+    r.rows = a.qo_indptr[b + 1] - (int)r.first;
+    r.page0 = a.kv_page_indptr[b];
+    r.pages = a.kv_page_indptr[b + 1] - r.page0;
+    const int last = a.kv_last_page_lens[b];
+    r.kv_len = r.pages > 0 ? max((long)(r.pages - 1) * a.page_size + min(last, a.page_size), 0L) : 0;
+    r.n = r.first < 0 ? 0 : (int)max(min(min((long)r.rows, (long)a.max_rows), (long)a.nnz - r.first), 0L);
+    r.col_tiles = (r.n * a.group + kCols - 1) / kCols;
+    r.subtiles = max((int)((r.kv_len + kSub - 1) / kSub), 1);        // a row that sees nothing is written too
+    return r;
+}
+
+__device__ __forceinline__ long share_begin(long s, long units, long shares) { return s * units / shares; }
+
+// Shares that are in use: a workgroup's waves have a subtile each, if there are as many.
+__device__ __forceinline__ long shares_of(const TreeArgs &a, long units)
+{
+    return max(min((long)a.n_shares, (units + kTreeWaves - 1) / kTreeWaves), 1L);
+}
+
+// Row of the pool (page * 2 P + place) of token t of a request, -1 if there is none.  K half; V lies P rows on.
+__device__ __forceinline__ int pool_row(const TreeArgs &a, const TreeRequest &r, long t, int &entry_id)
+{
+    const int page = entry_id;
+    return t < r.kv_len && page >= 0 && page < a.num_pages ? page * 2 * a.page_size + (int)(t % a.page_size) : -1;
+}
+__device__ __forceinline__ int page_of(const TreeArgs &a, const TreeRequest &r, long t)
+{
+    const long entry = r.page0 + t / a.page_size;
+    return t < r.kv_len && entry >= 0 && entry < a.n_page_indices ? a.kv_page_indices[entry] : -1;
+}
+
+template <int DT, int kD, int kBlocks> struct TreeRegs {
+    typedef TreeShape<DT, kD, kBlocks> S;
+    u32x4 k[S::kLoads], v[S::kLoads];
+};
+
+template <int DT, int kD, int kBlocks>
+__global__ __launch_bounds__(kTreeThreads, kBlocks <= 2 ? 2 : 1) void tree_matrix_kernel(TreeArgs a)
+{
+    typedef TreeShape<DT, kD, kBlocks> S;
+    __shared__ __align__(16) char lds[S::kLds];
+    __shared__ long scan[kTreeWaves], found[3];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, c = lane & 15;
+    const int share = blockIdx.x / a.n_kv_heads, head = blockIdx.x % a.n_kv_heads;
+
+    // ---- where the share begins
+    const int per = (a.batch + kTreeThreads - 1) / kTreeThreads;
+    const int b0 = threadIdx.x * per, b1 = min(b0 + per, a.batch);
+    long mine = 0;
+    for (int b = b0; b < b1; b++) mine += tree_request<S::kCols, S::kSub>(a, b).units();
+    long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const long x = __shfl_up(upto, o);
+        if (lane >= o) upto += x;
+    }
+    if (lane == 63) scan[wave] = upto;
+    __syncthreads();
+    long units = 0;
+#pragma unroll
+    for (int w = 0; w < kTreeWaves; w++) {
+        if (w == wave) upto += units;
+        units += scan[w];
+    }
+    const long shares = shares_of(a, units);
+    const bool idle = share >= shares || units == 0;
+    const long begin = share_begin(share, units, shares), end = share_begin(share + 1, units, shares);
+    long before = upto - mine;
+    const bool tells = blockIdx.x == 0;
+    if (tells || (before <= begin && begin < upto)) {
+        for (int b = b0; b < b1; b++) {
+            const long u = tree_request<S::kCols, S::kSub>(a, b).units();
+            if (tells) a.units_before[b] = before;
+            if (before <= begin && begin < before + u) {
+                found[0] = b;
+                found[1] = before;
+            }
+            before += u;
+        }
+        if (tells && b1 == a.batch) a.units_before[a.batch] = units;
+    }
+    __syncthreads();
+    if (idle) return;
+    int b = __builtin_amdgcn_readfirstlane((int)found[0]);
+    long unit = begin, base = found[1];                       // base: units in front of request b
+
+    char *const k_lds = lds + wave * S::kWaveLds, *const v_lds = k_lds + S::kSub * S::kKPitch;
+    const long row_bytes = (long)a.n_kv_heads * S::kRow;
+    const int load_row = lane / S::kChunks, load_chunk = lane % S::kChunks;
+    const char *const pool = a.pages + head * S::kRow + load_chunk * 16;
+
+    while (unit < end) {
+        const TreeRequest r = tree_request<S::kCols, S::kSub>(a, b);
+        const long r_units = r.units();
+        if (unit >= base + r_units) {                         // on to the next request that has rows
+            base += r_units;
+            b++;
+            continue;
+        }
+        const int ct = (int)((unit - base) / r.subtiles);
+        const long item = base + (long)ct * r.subtiles;       // the item's first unit
+        const int st0 = (int)(unit - item), st1 = (int)min(end - item, (long)r.subtiles);
+        const int cols = min(r.n * a.group - ct * S::kCols, S::kCols);
+        const long prior = r.kv_len - r.rows;
+
+        // ---- columns: q and what they see
+        u32x4 q[kBlocks][S::kSteps];
+        unsigned long long mask[kBlocks];
+        int limit[kBlocks];
+#pragma unroll
+        for (int k = 0; k < kBlocks; k++) {
+            const int col = ct * S::kCols + k * 16 + c;
+            const int i = col / a.group, hq = head * a.group + col - i * a.group;
+            const bool there = k * 16 + c < cols;
+            const char *row = a.q + (r.first + (there ? i : 0)) * a.q_stride + (there ? hq : 0) * S::kRow + g * 16;
+#pragma unroll
+            for (int s = 0; s < S::kSteps; s++) {
+                q[k][s] = u32x4{0, 0, 0, 0};
+                if (there) q[k][s] = *reinterpret_cast<const u32x4 *>(row + s * 64);
+            }
+            mask[k] = !a.masks ? ~0ull : there ? (unsigned long long)a.masks[r.first + i] : 0;
+            // tokens from `limit` on are not seen whatever the mask says
+            const long lim = a.masks ? min(r.kv_len, prior + DSKV_MAX_TREE_ROWS) : min(r.kv_len, prior + i + 1);
+            limit[k] = there ? (int)max(lim, 0L) : 0;
+        }
+
+        f32x4 o[kBlocks][S::kDimTiles];
+        float m[kBlocks], l[kBlocks];
+#pragma unroll
+        for (int k = 0; k < kBlocks; k++) {
+            m[k] = -INFINITY;
+            l[k] = 0;
+#pragma unroll
+            for (int d = 0; d < S::kDimTiles; d++) o[k][d] = f32x4{0, 0, 0, 0};
+        }
+
+        // ---- the wave's subtiles, one ahead in registers, the page ids another one ahead
+        TreeRegs<DT, kD, kBlocks> next;
+        auto id_of = [&](int st) { return page_of(a, r, (long)st * S::kSub + (lane & (S::kSub - 1))); };
+        auto row_of = [&](int st, int id) { return pool_row(a, r, (long)st * S::kSub + (lane & (S::kSub - 1)), id); };
+        auto request = [&](int rows) {
+#pragma unroll
+            for (int i = 0; i < S::kLoads; i++) {
+                const int row = __shfl(rows, load_row + S::kRowsPerLoad * i);
+                next.k[i] = next.v[i] = u32x4{0, 0, 0, 0};
+                if (row >= 0) {
+                    const char *p = pool + (unsigned long)(unsigned)row * row_bytes;
+                    next.k[i] = *reinterpret_cast<const u32x4 *>(p);
+                    next.v[i] = *reinterpret_cast<const u32x4 *>(p + a.page_size * row_bytes);
+                }
+            }
+        };
+        int rows_now = -1, id_next = -1;
+        if (st0 + wave < st1) {
+            rows_now = row_of(st0 + wave, id_of(st0 + wave));
+            request(rows_now);
+        }
+        if (st0 + wave + kTreeWaves < st1) id_next = id_of(st0 + wave + kTreeWaves);
+        for (int st = st0 + wave; st < st1; st += kTreeWaves) {
+            const int t0 = st * S::kSub;
+            const unsigned long long held = __ballot(rows_now >= 0);       // tokens that there are (lanes repeat)
+            const bool whole = held == ~0ull && t0 + S::kSub <= prior + (a.masks ? 0 : 1) && true;
+            unsigned bad = 0;                                              // tokens whose V is no number, masked somewhere
+            __builtin_amdgcn_wave_barrier();
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < S::kLoads; i++) {
+                    bool odd = false;
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        const uint32_t x = next.v[i][w];
+                        if (DT == DSKV_F32) odd |= (x & 0x7F800000u) == 0x7F800000u;
+                        else if (DT == DSKV_BF16) odd |= (x & 0x7F80u) == 0x7F80u || (x & 0x7F800000u) == 0x7F800000u;
+                        else odd |= (x & 0x7C00u) == 0x7C00u || (x & 0x7C000000u) == 0x7C000000u;
+                    }
+                    const unsigned long long odd_lanes = __ballot(odd);
+#pragma unroll
+                    for (int j = 0; j < S::kRowsPerLoad; j++) {
+                        const unsigned long long of_row = (S::kChunks == 64 ? ~0ull : (1ull << S::kChunks) - 1) << (j * S::kChunks);
+                        if (odd_lanes & of_row) bad |= 1u << (j + S::kRowsPerLoad * i);
+                    }
+                    if ((bad >> (load_row + S::kRowsPerLoad * i)) & 1) next.v[i] = u32x4{0, 0, 0, 0};
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < S::kLoads; i++) {
+                const int row = load_row + S::kRowsPerLoad * i;
+                *reinterpret_cast<u32x4 *>(k_lds + row * S::kKPitch + load_chunk * 16) = next.k[i];
+                *reinterpret_cast<u32x4 *>(v_lds + row * S::kVPitch + load_chunk * 16) = next.v[i];
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            const int rows_of_this = rows_now;
+            if (st + kTreeWaves < st1) {
+                rows_now = row_of(st + kTreeWaves, id_next);
+                request(rows_now);
+                if (st + 2 * kTreeWaves < st1) id_next = id_of(st + 2 * kTreeWaves);
+            }
+
+            // ---- scores
+            f32x4 s[kBlocks][S::kTiles];
+#pragma unroll
+            for (int t = 0; t < S::kTiles; t++) {
+#pragma unroll
+                for (int k = 0; k < kBlocks; k++) s[k][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int e = 0; e < S::kSteps; e++) {
+                    const u32x4 key = *reinterpret_cast<const u32x4 *>(k_lds + (t * 16 + c) * S::kKPitch + e * 64 + g * 16);
+#pragma unroll
+                    for (int k = 0; k < kBlocks; k++) {
+                        if constexpr (DT == DSKV_F32) {
+                            const f32x4 kf = __builtin_bit_cast(f32x4, key), qf = __builtin_bit_cast(f32x4, q[k][e]);
+#pragma unroll
+                            for (int j = 0; j < 4; j++)
+                                s[k][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j], qf[j], s[k][t], 0, 0, 0);
+                        } else {
+                            s[k][t] = Elt<DT>::mfma_k32(key, q[k][e], s[k][t]);
+                        }
+                    }
+                }
+            }
+            // ---- weights
+            u32x4 p[kBlocks];                                  // 16-bit: the operand; fp32: four floats
+            auto sees = [&](int k, int token) {                // token of the subtile
+                const long at = t0 + token;
+                const long j = at - prior;
+                return at < limit[k] && ((held >> token) & 1) && (j < 0 || ((mask[k] >> (j & 63)) & 1));
+            };
+#pragma unroll
+            for (int k = 0; k < kBlocks; k++) {
+                float x[S::kTiles * 4];
+#pragma unroll
+                for (int t = 0; t < S::kTiles; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[t * 4 + e] = s[k][t][e] * a.scale;
+                if (!whole) {
+#pragma unroll
+                    for (int t = 0; t < S::kTiles; t++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (!sees(k, t * 16 + 4 * g + e)) x[t * 4 + e] = -INFINITY;
+                }
+                float top = x[0];
+#pragma unroll
+                for (int e = 1; e < S::kTiles * 4; e++) top = fmaxf(top, x[e]);
+                top = fmaxf(m[k], quad_rows_max(top));
+                const float from = top == -INFINITY ? 0.f : top;
+                const float keep = __builtin_amdgcn_exp2f(m[k] - from);
+                m[k] = top;
+                float sum = 0;
+#pragma unroll
+                for (int e = 0; e < S::kTiles * 4; e++) {
+                    x[e] = __builtin_amdgcn_exp2f(x[e] - from);
+                    sum += x[e];
+                }
+                l[k] = l[k] * keep + sum;
+#pragma unroll
+                for (int d = 0; d < S::kDimTiles; d++) o[k][d] *= keep;
+                if constexpr (DT == DSKV_F32) {
+                    p[k] = __builtin_bit_cast(u32x4, f32x4{x[0], x[1], x[2], x[3]});
+                } else {
+                    // rounded to 16 bits for the matrix product: half a step of each weight
+#pragma unroll
+                    for (int e = 0; e < 4; e++) p[k][e] = Elt<DT>::pack2(x[2 * e], x[2 * e + 1]);
+                }
+            }
+            // ---- output
+#pragma unroll
+            for (int d = 0; d < S::kDimTiles; d++) {
+                if constexpr (DT == DSKV_F32) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float value = *reinterpret_cast<const float *>(v_lds + (4 * g + e) * S::kVPitch + (d * 16 + c) * 4);
+#pragma unroll
+                        for (int k = 0; k < kBlocks; k++)
+                            o[k][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                value, __builtin_bit_cast(f32x4, p[k])[e], o[k][d], 0, 0, 0);
+                    }
+                } else {
+                    const char *at = v_lds + (4 * g + (c >> 2)) * S::kVPitch + d * 32 + (c & 3) * 8;
+                    const u32x2 lo = read_transposed(at), hi = read_transposed(at + 16 * S::kVPitch);
+                    const u32x4 value = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+                    for (int k = 0; k < kBlocks; k++) o[k][d] = Elt<DT>::mfma_k32(value, p[k], o[k][d]);
+                }
+            }
+            // A weight of 0 times a V that is no number would reach columns that do not see the token: such tokens
+            // were left out above and are added here, to the columns that see them.
+            while (__builtin_expect(bad != 0, 0)) {
+                const int token = __builtin_ctz(bad);
+                bad &= bad - 1;
+                const int row = __shfl(rows_of_this, token);
+                if (row < 0) continue;
+                const char *value = a.pages + (unsigned long)(unsigned)row * row_bytes + a.page_size * row_bytes + head * S::kRow;
+                const int owner = ((token & 15) >> 2) * 16 + c;             // lane that holds the column's weight
+#pragma unroll
+                for (int k = 0; k < kBlocks; k++) {
+                    float weight = 0;
+#pragma unroll
+                    for (int e = 0; e < S::kTiles * 4; e++) {
+                        float w;
+                        if constexpr (DT == DSKV_F32) w = __builtin_bit_cast(f32x4, p[k])[e];
+                        else {
+                            float lo, hi;
+                            Elt<DT>::unpack2(p[k][e >> 1], lo, hi);
+                            w = e & 1 ? hi : lo;
+                        }
+                        w = __shfl(w, owner);
+                        if (e == (token >> 4) * 4 + (token & 3)) weight = w;
+                    }
+                    if (sees(k, token)) {
+#pragma unroll
+                        for (int d = 0; d < S::kDimTiles; d++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                o[k][d][e] += weight * LoadElt<DT>::get(value, d * 16 + 4 * g + e);
+                    }
+                }
+            }
+        }
+
+        // ---- the waves' results meet
+        float *const o_lds = reinterpret_cast<float *>(lds);
+        float *const ml_lds = o_lds + kTreeWaves * S::kCols * S::kOPitch;
+        __syncthreads();                                       // all waves are through with their K and V
+#pragma unroll
+        for (int k = 0; k < kBlocks; k++) {
+            l[k] = quad_rows_sum(l[k]);
+            const int col = wave * S::kCols + k * 16 + c;
+            if (g == 0) {
+                ml_lds[col * 2] = m[k];
+                ml_lds[col * 2 + 1] = l[k];
+            }
+#pragma unroll
+            for (int d = 0; d < S::kDimTiles; d++)
+                *reinterpret_cast<f32x4 *>(o_lds + col * S::kOPitch + d * 16 + 4 * g) = o[k][d];
+        }
+        __syncthreads();
+        const bool cut = st0 > 0 || st1 < r.subtiles;
+        const long slot = 2L * share + (unit > begin ? 1 : 0);
+        const long part = (slot * a.n_kv_heads + head) * S::kCols;
+        constexpr int kQuads = kD / 4;
+        for (int x = threadIdx.x; x < cols * kQuads; x += kTreeThreads) {
+            const int col = x / kQuads, quad = x % kQuads;
+            float top = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kTreeWaves; w++) top = fmaxf(top, ml_lds[(w * S::kCols + col) * 2]);
+            const float from = top == -INFINITY ? 0.f : top;
+            float sum = 0;
+            f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+            for (int w = 0; w < kTreeWaves; w++) {
+                const float weight = __builtin_amdgcn_exp2f(ml_lds[(w * S::kCols + col) * 2] - from);
+                sum += ml_lds[(w * S::kCols + col) * 2 + 1] * weight;
+                acc += *reinterpret_cast<const f32x4 *>(o_lds + (w * S::kCols + col) * S::kOPitch + quad * 4) * weight;
+            }
+            if (cut) {
+                *reinterpret_cast<f32x4 *>(a.part_o + (part + col) * kD + quad * 4) = acc;
+                if (quad == 0) {
+                    a.part_ml[(part + col) * 2] = top;
+                    a.part_ml[(part + col) * 2 + 1] = sum;
+                }
+            } else {
+                const int at = ct * S::kCols + col, i = at / a.group, hq = head * a.group + at - i * a.group;
+                const float inv = sum == 0 ? 0.f : 1.f / sum;
+                char *dst = a.out + ((r.first + i) * a.n_qo_heads + hq) * S::kRow + quad * 4 * S::kElt;
+                if constexpr (DT == DSKV_F32) *reinterpret_cast<f32x4 *>(dst) = acc * inv;
+                else *reinterpret_cast<u32x2 *>(dst) = u32x2{Elt<DT>::pack2(acc.x * inv, acc.y * inv), Elt<DT>::pack2(acc.z * inv, acc.w * inv)};
+            }
+        }
+        __syncthreads();
+        unit = item + st1;
+    }
+}
+
+// Items that were cut: one workgroup per (item, kv head, two columns); its threads are four groups that take
+// every fourth part, and meet in LDS.
+template <int DT, int kD, int kBlocks> __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int max_col_tiles)
+{
+    typedef TreeShape<DT, kD, kBlocks> S;
+    constexpr int kQuads = kD / 4, kGroups = 4, kColumns = 256 / (kQuads * kGroups);
+    __shared__ f32x4 acc_of[kGroups][kColumns * kQuads];
+    __shared__ float ml_of[kGroups][kColumns][2];
+    const int b = blockIdx.x / max_col_tiles, ct = blockIdx.x % max_col_tiles, head = blockIdx.y;
+    const int quad = threadIdx.x % kQuads, column = threadIdx.x / kQuads % kColumns, group = threadIdx.x / (kQuads * kColumns);
+    const TreeRequest r = tree_request<S::kCols, S::kSub>(a, b);
+    const long units = a.units_before[a.batch], shares = shares_of(a, units);
+    const int col = blockIdx.z * kColumns + column;
+    if (ct >= r.col_tiles || ct * S::kCols + blockIdx.z * kColumns >= (unsigned)(r.n * a.group)) return;
+    const bool there = ct * S::kCols + col < r.n * a.group;
+    const long first = a.units_before[b] + (long)ct * r.subtiles, last = first + r.subtiles - 1;
+    const long s0 = ((first + 1) * shares + units - 1) / units - 1, s1 = ((last + 1) * shares + units - 1) / units - 1;
+    if (s0 == s1) return;
+    float top = -INFINITY, sum = 0;
+    f32x4 acc = {0, 0, 0, 0};
+    if (there)
+        for (long s = s0 + group; s <= s1; s += kGroups) {
+            const long slot = 2 * s + (s == s0 && share_begin(s, units, shares) < first ? 1 : 0);
+            const long part = (slot * a.n_kv_heads + head) * S::kCols + col;
+            const float pm = a.part_ml[part * 2], pl = a.part_ml[part * 2 + 1];
+            const f32x4 po = *reinterpret_cast<const f32x4 *>(a.part_o + part * kD + quad * 4);
+            const float m = fmaxf(top, pm), from = m == -INFINITY ? 0.f : m;
+            const float w0 = __builtin_amdgcn_exp2f(top - from), w1 = __builtin_amdgcn_exp2f(pm - from);
+            top = m;
+            sum = sum * w0 + pl * w1;
+            acc = acc * w0 + po * w1;
+        }
+    acc_of[group][column * kQuads + quad] = acc;
+    if (quad == 0) {
+        ml_of[group][column][0] = top;
+        ml_of[group][column][1] = sum;
+    }
+    __syncthreads();
+    if (group > 0 || !there) return;
+#pragma unroll
+    for (int w = 1; w < kGroups; w++) {
+        const float pm = ml_of[w][column][0], pl = ml_of[w][column][1];
+        const float m = fmaxf(top, pm), from = m == -INFINITY ? 0.f : m;
+        const float w0 = __builtin_amdgcn_exp2f(top - from), w1 = __builtin_amdgcn_exp2f(pm - from);
+        top = m;
+        sum = sum * w0 + pl * w1;
+        acc = acc * w0 + acc_of[w][column * kQuads + quad] * w1;
+    }
+    const int at = ct * S::kCols + col, i = at / a.group, hq = head * a.group + at - i * a.group;
+    const float inv = sum == 0 ? 0.f : 1.f / sum;
+    char *dst = a.out + ((r.first + i) * a.n_qo_heads + hq) * S::kRow + quad * 4 * S::kElt;
+    if constexpr (DT == DSKV_F32) *reinterpret_cast<f32x4 *>(dst) = acc * inv;
+    else *reinterpret_cast<u32x2 *>(dst) = u32x2{Elt<DT>::pack2(acc.x * inv, acc.y * inv), Elt<DT>::pack2(acc.z * inv, acc.w * inv)};
+}
+
+}  // namespace dskv
