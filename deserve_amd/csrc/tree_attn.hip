@@ -4,7 +4,7 @@
 // with scores in units of log 2.  A place that a row does not see has score -infinity and weight 0; a row that
 // sees nothing keeps l = 0 and gets zeros.
 #include "rope_math.h"
-#include "tree_kernel.h"
+#include "tree_wide_kernel.h"
 
 namespace dskv {
 
@@ -135,40 +135,69 @@ __global__ __launch_bounds__(kGenericWaves * 64) void tree_generic_kernel(TreeAr
     }
 }
 
-// The matrix form takes head dims 64 and 128.  Tiles of up to 64 columns: few tiles, each as narrow as it can be.
+// How a step is computed.  wide_waves > 0: tree_wide_kernel.h with so many waves; else the matrix form of tree_kernel.h with
+// tiles of `blocks` * 16 columns: few tiles, each as narrow as it can be.
 struct TreeForm {
-    int blocks, col_tiles, shares;
+    int wide_waves, blocks, cols, col_tiles, shares, least;
 };
 static bool matrix_form(int head_dim) { return head_dim == 64 || head_dim == 128; }
-static TreeForm tree_form(int max_rows, int n_qo_heads, int n_kv_heads)
+static TreeForm tree_form(bool wide, int max_rows, int n_qo_heads, int n_kv_heads)
 {
     TreeForm f;
     const long cols = (long)max_rows * (n_qo_heads / n_kv_heads);
-    f.col_tiles = (int)((cols + 63) / 64);
-    f.blocks = (int)((cols + 16L * f.col_tiles - 1) / (16L * f.col_tiles));
-    // two workgroups a compute unit where their registers allow it
-    const int resident = kTreeUnits * (f.blocks <= 2 ? 2 : 1);
+    f.wide_waves = !wide ? 0 : cols <= 128 ? 4 : 8;
+    const int widest = wide ? f.wide_waves * 32 : 64;
+    f.col_tiles = (int)((cols + widest - 1) / widest);
+    f.blocks = wide ? 0 : (int)((cols + 16L * f.col_tiles - 1) / (16L * f.col_tiles));
+    f.cols = wide ? widest : f.blocks * 16;
+    f.least = wide ? kWideLeast : kTreeWaves;
+    // two workgroups a compute unit where their registers and LDS allow it
+    const int resident = kTreeUnits * ((wide ? f.wide_waves == 4 : f.blocks <= 2) ? 2 : 1);
     f.shares = resident >= n_kv_heads ? resident / n_kv_heads : 1;
     return f;
 }
+static bool wide_form(int max_rows, int n_qo_heads, int n_kv_heads, int head_dim, int dtype)
+{
+    return head_dim == 128 && dtype != DSKV_F32 && (long)max_rows * (n_qo_heads / n_kv_heads) > 64;
+}
 static int64_t units_bytes(int batch) { return ((int64_t)batch + 2) / 2 * 16; }
-static int64_t slots_of(const TreeForm &f, int n_kv_heads) { return 2LL * f.shares * n_kv_heads * f.blocks * 16; }
+static int64_t slots_of(const TreeForm &f, int n_kv_heads) { return 2LL * f.shares * n_kv_heads * f.cols; }
+static int64_t form_bytes(const TreeForm &f, int batch, int n_kv_heads, int head_dim)
+{
+    return units_bytes(batch) + slots_of(f, n_kv_heads) * (head_dim + 2) * (int64_t)sizeof(float);
+}
 
+template <int DT, int kD, int kCols, int kSub> static int launch_tree_merge(const TreeArgs &a, const TreeForm &f, hipStream_t stream)
+{
+    // few items are cut into many parts each, many into few
+    const bool many_parts = (long)a.batch * f.col_tiles * 4 < f.shares;
+    const int columns = 256 / (kD / 4 * (many_parts ? 4 : 1));
+    const dim3 grid((unsigned)(a.batch * f.col_tiles), (unsigned)a.n_kv_heads, (unsigned)((kCols + columns - 1) / columns));
+    if (many_parts) hipLaunchKernelGGL((tree_merge_kernel<DT, kD, kCols, kSub, 4>), grid, dim3(256), 0, stream, a, f.col_tiles, f.least);
+    else hipLaunchKernelGGL((tree_merge_kernel<DT, kD, kCols, kSub, 1>), grid, dim3(256), 0, stream, a, f.col_tiles, f.least);
+    DSKV_LAUNCH_CHECK("tree_merge_kernel");
+    return 0;
+}
 template <int DT, int kD, int kBlocks> static int launch_tree(const TreeArgs &a, const TreeForm &f, hipStream_t stream)
 {
     typedef TreeShape<DT, kD, kBlocks> S;
     hipLaunchKernelGGL((tree_matrix_kernel<DT, kD, kBlocks>), dim3((unsigned)(f.shares * a.n_kv_heads)),
                        dim3(kTreeThreads), 0, stream, a);
     DSKV_LAUNCH_CHECK("tree_matrix_kernel");
-    const int columns = 256 / (kD / 4 * 4);
-    hipLaunchKernelGGL((tree_merge_kernel<DT, kD, kBlocks>),
-                       dim3((unsigned)(a.batch * f.col_tiles), (unsigned)a.n_kv_heads, (unsigned)(S::kCols / columns)), dim3(256), 0,
-                       stream, a, f.col_tiles);
-    DSKV_LAUNCH_CHECK("tree_merge_kernel");
-    return 0;
+    return launch_tree_merge<DT, kD, S::kCols, S::kSub>(a, f, stream);
+}
+template <int DT, int kWaves> static int launch_tree_wide(const TreeArgs &a, const TreeForm &f, hipStream_t stream)
+{
+    hipLaunchKernelGGL((tree_wide_kernel<DT, kWaves>), dim3((unsigned)(f.shares * a.n_kv_heads)), dim3(kWaves * 64), 0, stream, a);
+    DSKV_LAUNCH_CHECK("tree_wide_kernel");
+    return launch_tree_merge<DT, 128, kWaves * 32, kWideBlock>(a, f, stream);
 }
 template <int DT, int kD> static int launch_tree_blocks(const TreeArgs &a, const TreeForm &f, hipStream_t stream)
 {
+    if constexpr (DT != DSKV_F32 && kD == 128) {
+        if (f.wide_waves == 4) return launch_tree_wide<DT, 4>(a, f, stream);
+        if (f.wide_waves == 8) return launch_tree_wide<DT, 8>(a, f, stream);
+    }
     switch (f.blocks) {
     case 1: return launch_tree<DT, kD, 1>(a, f, stream);
     case 2: return launch_tree<DT, kD, 2>(a, f, stream);
@@ -188,8 +217,10 @@ extern "C" int64_t dskv_tree_attn_workspace(int32_t batch, int32_t nnz, int32_t 
 {
     using namespace dskv;
     if (batch <= 0 || nnz <= 0 || max_qo_len <= 0 || n_kv_heads <= 0 || n_qo_heads < n_kv_heads || !matrix_form(head_dim)) return 0;
-    const TreeForm f = tree_form(max_qo_len, n_qo_heads, n_kv_heads);
-    return units_bytes(batch) + slots_of(f, n_kv_heads) * (head_dim + 2) * (int64_t)sizeof(float);
+    const int64_t narrow = form_bytes(tree_form(false, max_qo_len, n_qo_heads, n_kv_heads), batch, n_kv_heads, head_dim);
+    if (!wide_form(max_qo_len, n_qo_heads, n_kv_heads, head_dim, dtype)) return narrow;
+    const int64_t wide = form_bytes(tree_form(true, max_qo_len, n_qo_heads, n_kv_heads), batch, n_kv_heads, head_dim);
+    return narrow > wide ? narrow : wide;
 }
 
 extern "C" int dskv_tree_attn(const dskv_tree_step_t *s, void *out, const void *q, int64_t q_stride,
@@ -218,8 +249,11 @@ extern "C" int dskv_tree_attn(const dskv_tree_step_t *s, void *out, const void *
                   s->nnz, s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->head_dim, s->page_size, s->num_pages,
                   s->sm_scale * 1.4426950408889634f};
     hipStream_t st = (hipStream_t)stream;
-    if (matrix_form(s->head_dim) && (int64_t)s->num_pages * 2 * s->page_size < INT32_MAX) {
-        const TreeForm f = tree_form(s->max_qo_len, s->n_qo_heads, s->n_kv_heads);
+    // (rows of the pool and tokens of a request are numbered in 32 bits there)
+    if (matrix_form(s->head_dim) && (int64_t)s->num_pages * 2 * s->page_size < INT32_MAX &&
+        s->n_page_indices < (1 << 30) / s->page_size && s->max_qo_len <= kTreeMostRows) {
+        const TreeForm f = tree_form(s->sm_scale > 0 && wide_form(s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->head_dim, s->dtype),
+                                     s->max_qo_len, s->n_qo_heads, s->n_kv_heads);
         const int64_t need = dskv_tree_attn_workspace(s->batch, s->nnz, s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->head_dim, s->dtype);
         if (!s->workspace || s->workspace_bytes < need) {
             set_error("tree_attn: workspace of %lld bytes, %lld are needed", (long long)s->workspace_bytes, (long long)need);

@@ -13,11 +13,13 @@
 #pragma once
 
 #include "kv_tile.h"
+#include "rope_math.h"
 
 namespace dskv {
 
 constexpr int kTreeWaves = 4;
 constexpr int kTreeThreads = kTreeWaves * 64;
+constexpr int kTreeMostRows = 1024;         // of a request in the matrix forms; longer chunks are a prefill's
 
 struct TreeArgs {
     const int32_t *qo_indptr, *kv_page_indptr, *kv_page_indices, *kv_last_page_lens;
@@ -54,10 +56,10 @@ template <int DT, int kD, int kBlocks> struct TreeShape {
 
 struct TreeRequest {
     long first;          // its first row
-    long kv_len;
+    long kv_len;         // tokens that its rows may see
+    long prior;          // tokens in front of its rows
     int page0, pages;
     int n;               // rows that are computed
-    int rows;            // rows it has
     int col_tiles, subtiles;
     __device__ __forceinline__ long units() const { return (long)col_tiles * subtiles; }
 };
@@ -67,12 +69,14 @@ template <int kCols, int kSub> __device__ __forceinline__ TreeRequest tree_reque
 {
     TreeRequest r;
     r.first = a.qo_indptr[b];
-    r.rows = a.qo_indptr[b + 1] - (int)r.first;
+    const long rows = (long)a.qo_indptr[b + 1] - r.first;
     r.page0 = a.kv_page_indptr[b];
     r.pages = a.kv_page_indptr[b + 1] - r.page0;
     const int last = a.kv_last_page_lens[b];
     r.kv_len = r.pages > 0 ? max((long)(r.pages - 1) * a.page_size + min(last, a.page_size), 0L) : 0;
-    r.n = r.first < 0 ? 0 : (int)max(min(min((long)r.rows, (long)a.max_rows), (long)a.nnz - r.first), 0L);
+    r.n = r.first < 0 ? 0 : (int)max(min(min(rows, (long)a.max_rows), (long)a.nnz - r.first), 0L);
+    r.prior = r.kv_len - rows;
+    r.kv_len = max(min(r.kv_len, r.prior + (a.masks ? DSKV_MAX_TREE_ROWS : r.n)), 0L);
     r.col_tiles = (r.n * a.group + kCols - 1) / kCols;
     r.subtiles = max((int)((r.kv_len + kSub - 1) / kSub), 1);        // a row that sees nothing is written too
     return r;
@@ -80,10 +84,68 @@ template <int kCols, int kSub> __device__ __forceinline__ TreeRequest tree_reque
 
 __device__ __forceinline__ long share_begin(long s, long units, long shares) { return s * units / shares; }
 
-// Shares that are in use: a workgroup's waves have a subtile each, if there are as many.
-__device__ __forceinline__ long shares_of(const TreeArgs &a, long units)
+// Shares that are in use: none has fewer than `least` units, if there are as many.
+__device__ __forceinline__ long shares_of(const TreeArgs &a, long units, int least)
 {
-    return max(min((long)a.n_shares, (units + kTreeWaves - 1) / kTreeWaves), 1L);
+    return max(min((long)a.n_shares, (units + least - 1) / least), 1L);
+}
+
+// Where the workgroup's share begins and ends, by all of its kThreads threads; the first workgroup leaves the
+// sums for the merge launch.
+struct TreePlace {
+    long begin, end;     // units; equal: nothing to do
+    long base;           // units in front of request b
+    int b;
+};
+template <int kCols, int kSub, int kThreads>
+__device__ __forceinline__ TreePlace tree_place(const TreeArgs &a, long share, int least)
+{
+    __shared__ long scan[kThreads / 64], found[2];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int per = (a.batch + kThreads - 1) / kThreads;
+    const int b0 = threadIdx.x * per, b1 = min(b0 + per, a.batch);
+    long mine = 0;
+    for (int b = b0; b < b1; b++) mine += tree_request<kCols, kSub>(a, b).units();
+    long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const long x = __shfl_up(upto, o);
+        if (lane >= o) upto += x;
+    }
+    if (lane == 63) scan[wave] = upto;
+    __syncthreads();
+    long units = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; w++) {
+        if (w == wave) upto += units;
+        units += scan[w];
+    }
+    TreePlace at = {0, 0, 0, 0};
+    const long shares = shares_of(a, units, least);
+    if (share < shares) {
+        at.begin = share_begin(share, units, shares);
+        at.end = share_begin(share + 1, units, shares);
+    }
+    long before = upto - mine;
+    const bool tells = blockIdx.x == 0;
+    if (tells || (before <= at.begin && at.begin < upto)) {
+        for (int b = b0; b < b1; b++) {
+            const long u = tree_request<kCols, kSub>(a, b).units();
+            if (tells) a.units_before[b] = before;
+            if (before <= at.begin && at.begin < before + u) {
+                found[0] = b;
+                found[1] = before;
+            }
+            before += u;
+        }
+        if (tells && b1 == a.batch) a.units_before[a.batch] = units;
+    }
+    __syncthreads();
+    if (at.begin < at.end) {
+        at.b = __builtin_amdgcn_readfirstlane((int)found[0]);
+        at.base = found[1];
+    }
+    return at;
 }
 
 // Row of the pool (page * 2 P + place) of token t of a request, -1 if there is none.  K half; V lies P rows on.
@@ -108,51 +170,15 @@ __global__ __launch_bounds__(kTreeThreads, kBlocks <= 2 ? 2 : 1) void tree_matri
 {
     typedef TreeShape<DT, kD, kBlocks> S;
     __shared__ __align__(16) char lds[S::kLds];
-    __shared__ long scan[kTreeWaves], found[3];
+    __shared__ unsigned bad_at[kTreeMostRows / S::kSub + 2];    // bit per token of a subtile with new rows: its V is no number
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, c = lane & 15;
     const int share = blockIdx.x / a.n_kv_heads, head = blockIdx.x % a.n_kv_heads;
 
-    // ---- where the share begins
-    const int per = (a.batch + kTreeThreads - 1) / kTreeThreads;
-    const int b0 = threadIdx.x * per, b1 = min(b0 + per, a.batch);
-    long mine = 0;
-    for (int b = b0; b < b1; b++) mine += tree_request<S::kCols, S::kSub>(a, b).units();
-    long upto = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const long x = __shfl_up(upto, o);
-        if (lane >= o) upto += x;
-    }
-    if (lane == 63) scan[wave] = upto;
-    __syncthreads();
-    long units = 0;
-#pragma unroll
-    for (int w = 0; w < kTreeWaves; w++) {
-        if (w == wave) upto += units;
-        units += scan[w];
-    }
-    const long shares = shares_of(a, units);
-    const bool idle = share >= shares || units == 0;
-    const long begin = share_begin(share, units, shares), end = share_begin(share + 1, units, shares);
-    long before = upto - mine;
-    const bool tells = blockIdx.x == 0;
-    if (tells || (before <= begin && begin < upto)) {
-        for (int b = b0; b < b1; b++) {
-            const long u = tree_request<S::kCols, S::kSub>(a, b).units();
-            if (tells) a.units_before[b] = before;
-            if (before <= begin && begin < before + u) {
-                found[0] = b;
-                found[1] = before;
-            }
-            before += u;
-        }
-        if (tells && b1 == a.batch) a.units_before[a.batch] = units;
-    }
-    __syncthreads();
-    if (idle) return;
-    int b = __builtin_amdgcn_readfirstlane((int)found[0]);
-    long unit = begin, base = found[1];                       // base: units in front of request b
+    TreePlace place = tree_place<S::kCols, S::kSub, kTreeThreads>(a, share, kTreeWaves);
+    const long begin = place.begin, end = place.end;
+    long unit = begin, base = place.base;
+    int b = place.b;
 
     char *const k_lds = lds + wave * S::kWaveLds, *const v_lds = k_lds + S::kSub * S::kKPitch;
     const long row_bytes = (long)a.n_kv_heads * S::kRow;
@@ -171,7 +197,8 @@ __global__ __launch_bounds__(kTreeThreads, kBlocks <= 2 ? 2 : 1) void tree_matri
         const long item = base + (long)ct * r.subtiles;       // the item's first unit
         const int st0 = (int)(unit - item), st1 = (int)min(end - item, (long)r.subtiles);
         const int cols = min(r.n * a.group - ct * S::kCols, S::kCols);
-        const long prior = r.kv_len - r.rows;
+        const long prior = r.prior;
+        const int new_from = (int)(max(prior, 0L) / S::kSub);       // first subtile with new rows
 
         // ---- columns: q and what they see
         u32x4 q[kBlocks][S::kSteps];
@@ -229,10 +256,12 @@ __global__ __launch_bounds__(kTreeThreads, kBlocks <= 2 ? 2 : 1) void tree_matri
         for (int st = st0 + wave; st < st1; st += kTreeWaves) {
             const int t0 = st * S::kSub;
             const unsigned long long held = __ballot(rows_now >= 0);       // tokens that there are (lanes repeat)
-            const bool whole = held == ~0ull && t0 + S::kSub <= prior + (a.masks ? 0 : 1) && true;
-            unsigned bad = 0;                                              // tokens whose V is no number, masked somewhere
+            const bool whole = held == ~0ull && t0 + S::kSub <= prior + (a.masks ? 0 : 1);
             __builtin_amdgcn_wave_barrier();
-            if (!whole) {
+            // A weight of 0 times a V that is no number would reach columns that do not see the token: such tokens among the
+            // new ones are taken out here and added behind the walk.
+            if (st >= new_from) {
+                unsigned bad = 0;
 #pragma unroll
                 for (int i = 0; i < S::kLoads; i++) {
                     bool odd = false;
@@ -251,6 +280,7 @@ __global__ __launch_bounds__(kTreeThreads, kBlocks <= 2 ? 2 : 1) void tree_matri
                     }
                     if ((bad >> (load_row + S::kRowsPerLoad * i)) & 1) next.v[i] = u32x4{0, 0, 0, 0};
                 }
+                if (lane == 0) bad_at[st - new_from] = bad;
             }
 #pragma unroll
             for (int i = 0; i < S::kLoads; i++) {
@@ -260,7 +290,6 @@ __global__ __launch_bounds__(kTreeThreads, kBlocks <= 2 ? 2 : 1) void tree_matri
             }
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
-            const int rows_of_this = rows_now;
             if (st + kTreeWaves < st1) {
                 rows_now = row_of(st + kTreeWaves, id_next);
                 request(rows_now);
@@ -354,31 +383,35 @@ __global__ __launch_bounds__(kTreeThreads, kBlocks <= 2 ? 2 : 1) void tree_matri
                     for (int k = 0; k < kBlocks; k++) o[k][d] = Elt<DT>::mfma_k32(value, p[k], o[k][d]);
                 }
             }
-            // A weight of 0 times a V that is no number would reach columns that do not see the token: such tokens
-            // were left out above and are added here, to the columns that see them.
+        }
+
+        // ---- the wave's tokens that were taken out, for the columns that see them
+        for (int st = st0 + wave; st < st1; st += kTreeWaves) {
+            if (st < new_from) continue;
+            unsigned bad = __builtin_amdgcn_readfirstlane(bad_at[st - new_from]);
             while (__builtin_expect(bad != 0, 0)) {
                 const int token = __builtin_ctz(bad);
                 bad &= bad - 1;
-                const int row = __shfl(rows_of_this, token);
+                const long t = (long)st * S::kSub + token;
+                int id = page_of(a, r, t);
+                const int row = pool_row(a, r, t, id);
                 if (row < 0) continue;
-                const char *value = a.pages + (unsigned long)(unsigned)row * row_bytes + a.page_size * row_bytes + head * S::kRow;
-                const int owner = ((token & 15) >> 2) * 16 + c;             // lane that holds the column's weight
+                const char *key = a.pages + (unsigned long)(unsigned)row * row_bytes + head * S::kRow;
+                const char *value = key + a.page_size * row_bytes;
 #pragma unroll
                 for (int k = 0; k < kBlocks; k++) {
-                    float weight = 0;
+                    float s = 0;
 #pragma unroll
-                    for (int e = 0; e < S::kTiles * 4; e++) {
-                        float w;
-                        if constexpr (DT == DSKV_F32) w = __builtin_bit_cast(f32x4, p[k])[e];
-                        else {
-                            float lo, hi;
-                            Elt<DT>::unpack2(p[k][e >> 1], lo, hi);
-                            w = e & 1 ? hi : lo;
-                        }
-                        w = __shfl(w, owner);
-                        if (e == (token >> 4) * 4 + (token & 3)) weight = w;
+                    for (int e = 0; e < S::kSteps; e++) {
+                        constexpr int E = Chunk<DT>::kElems;
+                        float x[E], y[E];
+                        Chunk<DT>::unpack(*reinterpret_cast<const u32x4 *>(key + e * 64 + g * 16), x);
+                        Chunk<DT>::unpack(q[k][e], y);
+#pragma unroll
+                        for (int d = 0; d < E; d++) s = fmaf(x[d], y[d], s);
                     }
-                    if (sees(k, token)) {
+                    const float weight = __builtin_amdgcn_exp2f(quad_rows_sum(s) * a.scale - (m[k] == -INFINITY ? 0.f : m[k]));
+                    if (t < limit[k] && (t < prior || ((mask[k] >> ((t - prior) & 63)) & 1))) {
 #pragma unroll
                         for (int d = 0; d < S::kDimTiles; d++)
 #pragma unroll
@@ -443,57 +476,69 @@ __global__ __launch_bounds__(kTreeThreads, kBlocks <= 2 ? 2 : 1) void tree_matri
     }
 }
 
-// Items that were cut: one workgroup per (item, kv head, two columns); its threads are four groups that take
-// every fourth part, and meet in LDS.
-template <int DT, int kD, int kBlocks> __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int max_col_tiles)
+// Items that were cut: a thread per (column, four dims) and group of parts.  kGroups > 1, for items in many parts: each takes
+// every kGroups-th part, and they meet in LDS.
+template <int DT, int kD, int kCols, int kSub, int kGroups>
+__global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int max_col_tiles, int least)
 {
-    typedef TreeShape<DT, kD, kBlocks> S;
-    constexpr int kQuads = kD / 4, kGroups = 4, kColumns = 256 / (kQuads * kGroups);
-    __shared__ f32x4 acc_of[kGroups][kColumns * kQuads];
-    __shared__ float ml_of[kGroups][kColumns][2];
+    constexpr int kElt = DT == DSKV_F32 ? 4 : 2;
+    constexpr int kQuads = kD / 4, kColumns = 256 / (kQuads * kGroups);
     const int b = blockIdx.x / max_col_tiles, ct = blockIdx.x % max_col_tiles, head = blockIdx.y;
     const int quad = threadIdx.x % kQuads, column = threadIdx.x / kQuads % kColumns, group = threadIdx.x / (kQuads * kColumns);
-    const TreeRequest r = tree_request<S::kCols, S::kSub>(a, b);
-    const long units = a.units_before[a.batch], shares = shares_of(a, units);
+    const TreeRequest r = tree_request<kCols, kSub>(a, b);
+    const long before = a.units_before[b], units = a.units_before[a.batch];
     const int col = blockIdx.z * kColumns + column;
-    if (ct >= r.col_tiles || ct * S::kCols + blockIdx.z * kColumns >= (unsigned)(r.n * a.group)) return;
-    const bool there = ct * S::kCols + col < r.n * a.group;
-    const long first = a.units_before[b] + (long)ct * r.subtiles, last = first + r.subtiles - 1;
+    if (ct >= r.col_tiles || ct * kCols + (int)blockIdx.z * kColumns >= r.n * a.group) return;
+    const long shares = shares_of(a, units, least);
+    const bool there = ct * kCols + col < r.n * a.group;
+    const long first = before + (long)ct * r.subtiles, last = first + r.subtiles - 1;
     const long s0 = ((first + 1) * shares + units - 1) / units - 1, s1 = ((last + 1) * shares + units - 1) / units - 1;
     if (s0 == s1) return;
     float top = -INFINITY, sum = 0;
     f32x4 acc = {0, 0, 0, 0};
-    if (there)
-        for (long s = s0 + group; s <= s1; s += kGroups) {
-            const long slot = 2 * s + (s == s0 && share_begin(s, units, shares) < first ? 1 : 0);
-            const long part = (slot * a.n_kv_heads + head) * S::kCols + col;
-            const float pm = a.part_ml[part * 2], pl = a.part_ml[part * 2 + 1];
-            const f32x4 po = *reinterpret_cast<const f32x4 *>(a.part_o + part * kD + quad * 4);
-            const float m = fmaxf(top, pm), from = m == -INFINITY ? 0.f : m;
-            const float w0 = __builtin_amdgcn_exp2f(top - from), w1 = __builtin_amdgcn_exp2f(pm - from);
-            top = m;
-            sum = sum * w0 + pl * w1;
-            acc = acc * w0 + po * w1;
-        }
-    acc_of[group][column * kQuads + quad] = acc;
-    if (quad == 0) {
-        ml_of[group][column][0] = top;
-        ml_of[group][column][1] = sum;
-    }
-    __syncthreads();
-    if (group > 0 || !there) return;
-#pragma unroll
-    for (int w = 1; w < kGroups; w++) {
-        const float pm = ml_of[w][column][0], pl = ml_of[w][column][1];
+    auto add = [&](float pm, float pl, f32x4 po) {
         const float m = fmaxf(top, pm), from = m == -INFINITY ? 0.f : m;
         const float w0 = __builtin_amdgcn_exp2f(top - from), w1 = __builtin_amdgcn_exp2f(pm - from);
         top = m;
         sum = sum * w0 + pl * w1;
-        acc = acc * w0 + acc_of[w][column * kQuads + quad] * w1;
+        acc = acc * w0 + po * w1;
+    };
+    if (there) {
+        constexpr int kAhead = 4;                  // parts requested together
+        for (long s = s0 + group; s <= s1; s += kAhead * kGroups) {
+            float pm[kAhead], pl[kAhead];
+            f32x4 po[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; i++) {
+                const long si = min(s + i * kGroups, s1);
+                const long slot = 2 * si + (si == s0 && share_begin(si, units, shares) < first ? 1 : 0);
+                const long part = (slot * a.n_kv_heads + head) * kCols + col;
+                pm[i] = a.part_ml[part * 2];
+                pl[i] = a.part_ml[part * 2 + 1];
+                po[i] = *reinterpret_cast<const f32x4 *>(a.part_o + part * kD + quad * 4);
+            }
+#pragma unroll
+            for (int i = 0; i < kAhead; i++)
+                if (s + i * kGroups <= s1) add(pm[i], pl[i], po[i]);
+        }
     }
-    const int at = ct * S::kCols + col, i = at / a.group, hq = head * a.group + at - i * a.group;
+    if constexpr (kGroups > 1) {
+        __shared__ f32x4 acc_of[kGroups][kColumns * kQuads];
+        __shared__ float ml_of[kGroups][kColumns][2];
+        acc_of[group][column * kQuads + quad] = acc;
+        if (quad == 0) {
+            ml_of[group][column][0] = top;
+            ml_of[group][column][1] = sum;
+        }
+        __syncthreads();
+        if (group > 0) return;
+#pragma unroll
+        for (int w = 1; w < kGroups; w++) add(ml_of[w][column][0], ml_of[w][column][1], acc_of[w][column * kQuads + quad]);
+    }
+    if (!there) return;
+    const int at = ct * kCols + col, i = at / a.group, hq = head * a.group + at - i * a.group;
     const float inv = sum == 0 ? 0.f : 1.f / sum;
-    char *dst = a.out + ((r.first + i) * a.n_qo_heads + hq) * S::kRow + quad * 4 * S::kElt;
+    char *dst = a.out + (((r.first + i) * a.n_qo_heads + hq) * kD + quad * 4) * kElt;
     if constexpr (DT == DSKV_F32) *reinterpret_cast<f32x4 *>(dst) = acc * inv;
     else *reinterpret_cast<u32x2 *>(dst) = u32x2{Elt<DT>::pack2(acc.x * inv, acc.y * inv), Elt<DT>::pack2(acc.z * inv, acc.w * inv)};
 }

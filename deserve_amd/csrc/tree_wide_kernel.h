@@ -1,0 +1,393 @@
+// The tree attention for more columns than fit a wave (head_dim 128, 16 bits): the columns are split over the waves of
+// a workgroup, 32 each, and all of them read the same 32-token blocks of K and V from LDS, which go there straight from
+// memory.  See tree_kernel.h for how the work is cut.  sm_scale is positive: a masked score is -infinity before it is
+// scaled.
+//
+// Bound by the matrix pipeline and the vector instructions beside it: 16 of 32x32x16 per block and wave, 16 exponentials a
+// lane.  Iteration j of a walk multiplies P(j - 1) into V(j - 1), turns S(j) into P(j) and computes S(j + 1), so that all of
+// its matrix instructions are independent of its exponentials.  Blocks lie in four stages of K and of V; iteration j
+// requests K(j + 3) and V(j + 2) behind its only barrier.  The running maximum of a column is raised only when
+// a block's weights under it sum to more than kMostWeight in a lane.
+// Where a token lies in the pool is looked up for some thousand tokens at a time and kept in LDS (row numbers, a bit per token that
+// there is), so that pages may have any size and the loop's loads wait for nothing but LDS.
+#pragma once
+
+#include "tree_kernel.h"
+
+namespace dskv {
+
+constexpr int kWideBlock = 32;
+constexpr int kWideRegion = 1088;           // four rows, chunk by chunk ((4 c + row) * 16), and 64 bytes of padding
+constexpr int kWideStage = kWideBlock / 4 * kWideRegion;
+constexpr int kWideLeast = 8;               // units a share has at least: what fills the stages takes about as long
+constexpr float kMostWeight = 256.f;
+constexpr int kBadBlocks = kTreeMostRows / kWideBlock + 2;       // that new rows reach into
+
+static __device__ const u32x4 kNoRow[16] = {};          // what a token that there is not reads as
+
+template <int kWaves> struct WideShape {
+    static constexpr int kThreads = kWaves * 64;
+    static constexpr int kCols = kWaves * 32;
+    static constexpr int kGroups = 8 / kWaves;           // regions of a block that a wave requests
+    static constexpr int kHalf = kWaves == 8 ? 64 : 32;  // blocks that are looked up at a time; two such halves are kept
+    static constexpr int kTokens = 2 * kHalf * kWideBlock;
+};
+
+template <int DT, int kWaves>
+__global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
+{
+    typedef Elt<DT> E;
+    typedef WideShape<kWaves> W;
+    __shared__ __align__(16) char lds[8 * kWideStage];
+    __shared__ int32_t row_at[W::kTokens];               // row of the pool (page * 2 P + place), -1: none
+    __shared__ uint32_t held_at[2 * W::kHalf];           // bit per token of a block: there is one
+    __shared__ uint32_t bad_at[kBadBlocks];              // bit per token of a block with new rows: its V is no number
+    __shared__ int holes;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, c = lane & 15, h = lane >> 5, r32 = lane & 31;
+    const int share = blockIdx.x / a.n_kv_heads, head = blockIdx.x % a.n_kv_heads;
+    TreePlace place = tree_place<W::kCols, kWideBlock, W::kThreads>(a, share, kWideLeast);
+    const long begin = place.begin, end = place.end;
+    long unit = begin, base = place.base;
+    int b = place.b;
+
+    auto k_stage = [&](int i) { return lds + i * kWideStage; };
+    auto v_stage = [&](int i) { return lds + (4 + i) * kWideStage; };
+    const int row_bytes = a.n_kv_heads * 256;
+    const long half_bytes = (long)a.page_size * row_bytes;
+    // lane p of a load fetches chunk p / 4 of row p % 4 of a region
+    const char *const pool = a.pages + head * 256 + (lane >> 2) * 16;
+    const char *const none = reinterpret_cast<const char *>(kNoRow) + (lane >> 2) * 16;
+
+    while (unit < end) {
+        const TreeRequest r = tree_request<W::kCols, kWideBlock>(a, b);
+        if (unit >= base + r.units()) {
+            base += r.units();
+            b++;
+            continue;
+        }
+        const int ct = (int)((unit - base) / r.subtiles);
+        const long item = base + (long)ct * r.subtiles;
+        const int st0 = (int)(unit - item), st1 = (int)min(end - item, (long)r.subtiles);
+        const int blocks = st1 - st0;
+        const int cols = min(r.n * a.group - ct * W::kCols, W::kCols);
+        const int prior = (int)max(r.prior, (long)-INT32_MAX);
+        const int t_end = (int)min(r.kv_len, (long)st1 * kWideBlock);
+        const bool works = wave * 32 < cols;
+
+        // ---- the column
+        const int col = ct * W::kCols + wave * 32 + r32, row_i = col / a.group;
+        const bool there = wave * 32 + r32 < cols;
+        const long q_row = r.first + (there ? row_i : 0);
+        const int hq = head * a.group + (there ? col - row_i * a.group : 0);
+        unsigned long long mask = ~0ull;
+        int limit = 0;                                  // tokens from here on are not seen
+        if (there) {
+            if (a.masks) mask = (unsigned long long)a.masks[q_row];
+            const long lim = a.masks ? (long)prior + DSKV_MAX_TREE_ROWS : (long)prior + row_i + 1;
+            limit = (int)max(min(lim, (long)t_end), 0L);
+        }
+        u32x4 q[8];
+        {
+            const char *row = a.q + q_row * a.q_stride + hq * 256 + h * 16;
+#pragma unroll
+            for (int s = 0; s < 8; s++) {
+                q[s] = u32x4{0, 0, 0, 0};
+                if (there) q[s] = *reinterpret_cast<const u32x4 *>(row + s * 32);
+            }
+        }
+        // blocks that reach behind here need their scores masked
+        const int first_i = (ct * W::kCols + wave * 32) / a.group;
+        int mask_from = min(a.masks ? prior : prior + first_i + 1, t_end);
+
+        f32x16 acc[4], xs[2];
+        float m_run = -__FLT_MAX__, l_run = 0;
+        u32x4 pb[2][2];
+#pragma unroll
+        for (int d = 0; d < 4; d++)
+#pragma unroll
+            for (int v = 0; v < 16; v++) acc[d][v] = 0;
+        pb[1][0] = pb[1][1] = u32x4{0, 0, 0, 0};
+
+        // ---- rows of the pool, kHalf blocks at a time: half x of the walk into half x % 2
+        auto look_up = [&](int x) {
+            for (int i = threadIdx.x; i < W::kHalf * kWideBlock; i += W::kThreads) {
+                const int t = (st0 + x * W::kHalf) * kWideBlock + i;
+                int row = -1;
+                if (t < t_end) {
+                    int id = page_of(a, r, t);
+                    row = pool_row(a, r, t, id);
+                    if (row < 0) holes = 1;
+                }
+                const int at = (x & 1) * W::kHalf * kWideBlock + i;
+                row_at[at] = row;
+                const unsigned long long there64 = __ballot(row >= 0);
+                if ((lane & 31) == 0) held_at[at / kWideBlock] = (uint32_t)(there64 >> (lane & 32));
+            }
+        };
+        // address of the lane's 16 bytes of K of block j (V: half_bytes on)
+        struct Where {
+            const char *p[W::kGroups];
+            bool is[W::kGroups];
+        };
+        auto where = [&](int j, Where &w) {
+#pragma unroll
+            for (int i = 0; i < W::kGroups; i++) {
+                const int at = (j & (2 * W::kHalf - 1)) * kWideBlock + (wave * W::kGroups + i) * 4 + (lane & 3);
+                const int row = j < blocks ? row_at[at] : -1;      // (behind the walk nothing was looked up)
+                w.is[i] = row >= 0;
+                w.p[i] = row >= 0 ? pool + (unsigned long)(unsigned)row * (unsigned)row_bytes : none;
+            }
+        };
+        typedef __attribute__((address_space(3))) void *lds_ptr;
+        // Written out as instructions: through the compiler's builtin every later LDS read waits for all of these loads.  What it does
+        // not know it does not wait for: the waits are the explicit ones below.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+        auto request = [&](const Where &w, char *stage, long more) {
+#pragma unroll
+            for (int i = 0; i < W::kGroups; i++) {
+                const uint32_t to = (uint32_t)(uintptr_t)(lds_ptr)(stage + (wave * W::kGroups + i) * kWideRegion);
+                const char *p = w.is[i] ? w.p[i] + more : w.p[i];
+                asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off"
+                             :
+                             : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(p)
+                             : "memory", "m0");
+            }
+        };
+#pragma clang diagnostic pop
+        // until at most n of the wave's vector-memory operations are on their way
+#define DSKV_WAIT_VMEM(n) __builtin_amdgcn_s_waitcnt(((n) & 15) | 0x70 | 0xF00 | (((n) >> 4) << 14))
+
+        // ---- parts of an iteration
+        auto scores = [&](const char *stage, f32x16 &x) {
+            // token r32 = row r32 & 3 of region r32 >> 2; chunk 2 s + h
+            const char *rows = stage + (r32 >> 2) * kWideRegion + h * 64 + (r32 & 3) * 16;
+#pragma unroll
+            for (int v = 0; v < 16; v++) x[v] = 0;
+#pragma unroll
+            for (int s = 0; s < 8; s++) x = E::mfma_32x32(*reinterpret_cast<const u32x4 *>(rows + s * 128), q[s], x);
+        };
+        // Bits of block j's tokens that the column sees.
+        auto seen_of = [&](int j, uint32_t held) {
+            const int t = (st0 + j) * kWideBlock, from = t - prior;         // its first token among the new ones
+            uint32_t bits;
+            if (from >= 0) bits = from < 64 ? (uint32_t)(mask >> from) : a.masks ? 0u : ~0u;
+            else if (from > -32) bits = (uint32_t)(mask << -from) | ((1u << -from) - 1);
+            else bits = ~0u;
+            if (!a.masks) bits = ~0u;
+            const int left = limit - t;
+            bits &= left <= 0 ? 0u : left >= 32 ? ~0u : (1u << left) - 1;
+            return bits & held;
+        };
+        auto seen = [&](int j) { return j < blocks ? seen_of(j, held_at[j & (2 * W::kHalf - 1)]) : 0u; };
+        auto mask_scores = [&](int j, f32x16 &x) {
+            asm volatile("" : "+v"(x));                 // keeps this a branch that most blocks do not take
+            uint32_t bits = seen(j) >> (4 * h);
+            asm volatile("" : "+v"(bits));
+#pragma unroll
+            for (int v = 0; v < 16; v++)
+                if (!((bits >> (8 * (v >> 2) + (v & 3))) & 1)) x[v] = -INFINITY;
+        };
+        auto weights = [&](const f32x16 &x, int s, u32x4 &out, float &sum) {
+            float p[8];
+#pragma unroll
+            for (int v = 0; v < 8; v++) {
+                p[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * s + v], a.scale, -m_run));
+                sum += p[v];
+            }
+            out = u32x4{E::pack2(p[0], p[1]), E::pack2(p[2], p[3]), E::pack2(p[4], p[5]), E::pack2(p[6], p[7])};
+        };
+        auto raise = [&](const f32x16 &x) {
+            float m = x[0] * a.scale;
+#pragma unroll
+            for (int v = 1; v < 16; v++) m = fmaxf(m, x[v] * a.scale);
+            float other = m;
+            swap_halves32(m, other);
+            const float m_new = fmaxf(m_run, fmaxf(m, other));
+            const float keep = __builtin_amdgcn_exp2f(m_run - m_new);
+            m_run = m_new;
+            l_run *= keep;
+#pragma unroll
+            for (int d = 0; d < 4; d++) acc[d] *= keep;
+        };
+        const int v_off = h * kWideRegion + (2 * (g & 1) + ((c & 3) >> 1)) * 64 + (c >> 2) * 16 + (c & 1) * 8;
+        // A weight of 0 times a V that is no number would reach columns that do not see the token: such tokens among the new
+        // ones are taken out of the block here, by the wave that requested them, and added behind the walk.
+        const int new_from = max((max(prior, 0) >> 5) - st0, 0), new_to = min(((int)r.kv_len + 31) / 32 - st0, blocks);
+        auto set_aside = [&](int j) {
+#pragma unroll
+            for (int i = 0; i < W::kGroups; i++) {
+                const int region = wave * W::kGroups + i;
+                u32x4 *at = reinterpret_cast<u32x4 *>(v_stage(j & 3) + region * kWideRegion + lane * 16);
+                const u32x4 x = *at;
+                bool odd = false;
+#pragma unroll
+                for (int w = 0; w < 4; w++)
+                    odd |= DT == DSKV_BF16 ? (x[w] & 0x7F80u) == 0x7F80u || (x[w] & 0x7F800000u) == 0x7F800000u
+                                           : (x[w] & 0x7C00u) == 0x7C00u || (x[w] & 0x7C000000u) == 0x7C000000u;
+                const unsigned long long lanes = __ballot(odd);
+                if (__builtin_expect(lanes != 0, 0)) {
+                    uint32_t rows = 0;
+#pragma unroll
+                    for (int row = 0; row < 4; row++)
+                        if (lanes & (0x1111111111111111ull << row)) rows |= 1u << row;
+                    if ((rows >> (lane & 3)) & 1) *at = u32x4{0, 0, 0, 0};
+                    if (lane == 0) atomicOr(&bad_at[j - new_from], rows << (4 * region));
+                }
+            }
+        };
+        // ---- the walk
+        __syncthreads();                                 // the item before is through with LDS
+        if (threadIdx.x == 0) holes = 0;
+        for (int i = threadIdx.x; i < kBadBlocks; i += W::kThreads) bad_at[i] = 0;
+        __syncthreads();
+        look_up(0);
+        for (int i = threadIdx.x; i < kWideStage / 16; i += W::kThreads)
+            reinterpret_cast<u32x4 *>(v_stage(3))[i] = u32x4{0, 0, 0, 0};          // V(-1), which P(-1) = 0 is multiplied by
+        __syncthreads();
+        if (holes) mask_from = 0;
+        Where at2, at3;                                  // of blocks j + 2 and j + 3
+        {
+            Where w0, w1;
+            where(0, w0);
+            where(1, w1);
+            where(2, at2);
+            request(w0, k_stage(0), 0);
+            request(w1, k_stage(1), 0);
+            request(w0, v_stage(0), half_bytes);
+            request(at2, k_stage(2), 0);
+            request(w1, v_stage(1), half_bytes);
+            where(3, at3);
+            DSKV_WAIT_VMEM(4 * W::kGroups);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (works) {
+            scores(k_stage(0), xs[0]);
+            if ((st0 + 1) * kWideBlock > mask_from) mask_scores(0, xs[0]);
+        }
+        auto iteration = [&](int j, int phase) {         // phase = j % 4, a literal
+            // this wave's rows of K(j + 1) and V(j - 1) have landed
+            DSKV_WAIT_VMEM(3 * W::kGroups);
+            asm volatile("" ::: "memory");
+            if (j > new_from && j <= new_to) set_aside(j - 1);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            request(at3, k_stage((phase + 3) & 3), 0);                              // K(j + 3)
+            request(at2, v_stage((phase + 2) & 3), half_bytes);                     // V(j + 2)
+            at2 = at3;
+            where(j + 4, at3);
+            if (!works || j > blocks) return;
+            const int cur = phase & 1, nxt = cur ^ 1;
+            const char *rows = v_stage((phase + 3) & 3) + v_off;                    // V(j - 1)
+            u32x4 va[4][2];
+#pragma unroll
+            for (int d = 0; d < 4; d++)
+#pragma unroll
+                for (int s = 0; s < 2; s++) {
+                    const char *p = rows + s * 4 * kWideRegion + d * 256;
+                    const u32x2 lo = read_transposed(p), hi = read_transposed(p + 2 * kWideRegion);
+                    va[d][s] = u32x4{lo.x, lo.y, hi.x, hi.y};
+                }
+            scores(k_stage((phase + 1) & 3), xs[nxt]);                              // S(j + 1)
+            float sum = 0;
+            weights(xs[cur], 0, pb[cur][0], sum);
+            if ((st0 + j + 2) * kWideBlock > mask_from) mask_scores(j + 1, xs[nxt]);
+#pragma unroll
+            for (int d = 0; d < 4; d++)
+#pragma unroll
+                for (int s = 0; s < 2; s++) acc[d] = E::mfma_32x32(va[d][s], pb[nxt][s], acc[d]);   // P(j - 1)
+            weights(xs[cur], 1, pb[cur][1], sum);
+            if (__builtin_expect(__builtin_amdgcn_ballot_w64(sum > kMostWeight) != 0, 0)) {
+                raise(xs[cur]);
+                __builtin_amdgcn_sched_barrier(0);
+                sum = 0;
+                weights(xs[cur], 0, pb[cur][0], sum);
+                weights(xs[cur], 1, pb[cur][1], sum);
+            }
+            l_run += sum;
+        };
+        for (int j = 0; j <= blocks; j += 4) {
+            if (j % W::kHalf == W::kHalf / 2 && j + W::kHalf / 2 < blocks) look_up(j / W::kHalf + 1);
+            iteration(j, 0);
+            if (holes) mask_from = 0;
+            iteration(j + 1, 1);
+            iteration(j + 2, 2);
+            iteration(j + 3, 3);
+        }
+        DSKV_WAIT_VMEM(0);                               // nothing of this wave is still on its way into LDS
+
+        // ---- tokens that were taken out, for the columns that see them
+        for (int j = new_from; j < new_to; j++) {
+            uint32_t bad = bad_at[j - new_from];
+            if (__builtin_expect(bad == 0, 1)) continue;
+            const uint32_t bits = seen_of(j, ~0u);
+            while (bad) {
+                const int token = __builtin_ctz(bad);
+                bad &= bad - 1;
+                const int t = (st0 + j) * kWideBlock + token;
+                int id = page_of(a, r, t);
+                const int row = pool_row(a, r, t, id);
+                if (row < 0) continue;
+                const char *key = a.pages + (unsigned long)(unsigned)row * (unsigned)row_bytes + head * 256;
+                float s = 0;
+                for (int k = 0; k < 8; k++) {
+                    float x[8], y[8];
+                    Chunk<DT>::unpack(*reinterpret_cast<const u32x4 *>(key + k * 32 + h * 16), x);
+                    u32x4 mine = q[0];
+#pragma unroll
+                    for (int i = 1; i < 8; i++) mine = k == i ? q[i] : mine;
+                    Chunk<DT>::unpack(mine, y);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) s = fmaf(x[e], y[e], s);
+                }
+                float other = s;
+                swap_halves32(s, other);
+                const float weight = __builtin_amdgcn_exp2f(fmaf(s + other, a.scale, -m_run));
+                if ((bits >> token) & 1)
+#pragma unroll
+                    for (int d = 0; d < 4; d++)
+#pragma unroll
+                        for (int v = 0; v < 16; v++)
+                            acc[d][v] += weight * LoadElt<DT>::get(key + half_bytes, d * 32 + 8 * (v >> 2) + 4 * h + (v & 3));
+            }
+        }
+
+        // ---- the item's result
+        float l_other = l_run;
+        swap_halves32(l_run, l_other);
+        const float l = l_run + l_other;
+        const bool cut = st0 > 0 || st1 < r.subtiles;
+        if (there && cut) {
+            const long slot = 2L * share + (unit > begin ? 1 : 0);
+            const long part = (slot * a.n_kv_heads + head) * W::kCols + wave * 32 + r32;
+#pragma unroll
+            for (int d = 0; d < 4; d++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    *reinterpret_cast<f32x4 *>(a.part_o + part * 128 + d * 32 + 8 * i + 4 * h) =
+                        f32x4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+            if (h == 0) {
+                a.part_ml[part * 2] = m_run;
+                a.part_ml[part * 2 + 1] = l;
+            }
+        } else if (there) {
+            const float inv = l == 0 ? 0.f : 1.f / l;
+            char *dst = a.out + ((q_row * a.n_qo_heads + hq) * 128 + 4 * h) * 2;
+#pragma unroll
+            for (int d = 0; d < 4; d++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    *reinterpret_cast<u32x2 *>(dst + (d * 32 + 8 * i) * 2) =
+                        u32x2{E::pack2(acc[d][4 * i] * inv, acc[d][4 * i + 1] * inv),
+                              E::pack2(acc[d][4 * i + 2] * inv, acc[d][4 * i + 3] * inv)};
+        }
+        unit = item + st1;
+    }
+}
+#undef DSKV_WAIT_VMEM
+
+}  // namespace dskv

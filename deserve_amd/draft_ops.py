@@ -30,22 +30,30 @@ from deserve_amd import _lib
 MAX_TREE_ROWS = _lib.MAX_TREE_ROWS
 
 
-def _on_device(device: torch.device, others) -> None:
-    """The kernels read device memory only, and one device's."""
-    if device.type != "cuda":
-        raise ValueError(f"tensors must be on the GPU, got one on {device}")
+# (the functions behind torch.cuda.current_device() and current_stream(), whose own work costs a short step half of
+# its host time)
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _on_device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+    """Index of the device that all of them are on: the kernels read device memory only, and one device's."""
+    index = first.get_device()
+    if index < 0 or not first.is_cuda:
+        raise ValueError(f"tensors must be on the GPU, got one on {first.device}")
     for t in others:
-        if t is not None and t.device != device:
-            raise ValueError(f"tensors on different devices: {device} and {t.device}")
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
+    return index
 
 
-def _call(what: str, device: torch.device, fn, *args) -> None:
-    """Enqueues on the current stream of `device`, whichever device is the current one."""
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, _lib.current_stream())
+def _call(what: str, index: int, fn, *args) -> None:
+    """Enqueues on the current stream of device `index`, whichever device is the current one."""
+    if index == _current_device():
+        rc = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, _lib.current_stream())
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
     if rc:
         _lib.check(rc, what)
 
@@ -53,8 +61,8 @@ def _call(what: str, device: torch.device, fn, *args) -> None:
 def _check_vector(name: str, t: torch.Tensor, dtype: torch.dtype, least: int) -> None:
     if t.dtype is not dtype or t.dim() != 1 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous one-dimensional {dtype} tensor")
-    if t.shape[0] < least:
-        raise ValueError(f"{name} holds {t.shape[0]} entries, {least} are needed")
+    if t.numel() < least:
+        raise ValueError(f"{name} holds {t.numel()} entries, {least} are needed")
 
 
 @dataclass
@@ -70,9 +78,12 @@ class StepTables:
 
     @classmethod
     def empty(cls, batch: int, max_tokens: int, max_pages: int, device: torch.device, tree: bool) -> "StepTables":
-        new = lambda n, dtype=torch.int32: torch.empty((n,), dtype=dtype, device=device)
-        return cls(new(batch + 1), new(batch + 1), new(max_pages), new(batch), new(max_tokens),
-                   new(max_tokens, torch.int64), new(max_tokens, torch.int64) if tree else None)
+        # one allocation; the 64-bit arrays first
+        words = [2 * max_tokens, 2 * max_tokens if tree else 0, batch + 1, batch + 1, max_pages, batch, max_tokens]
+        slots, masks, qo_indptr, kv_indptr, indices, last, positions = \
+            torch.empty((sum(words),), dtype=torch.int32, device=device).split(words)
+        return cls(qo_indptr, kv_indptr, indices, last, positions, slots.view(torch.int64),
+                   masks.view(torch.int64) if tree else None)
 
     @property
     def csr(self) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -83,7 +94,7 @@ class StepTables:
         """(max_tokens, head_dim) floats, row t = cosines | sines of the angles of row t's position: what
         rope_append_slots rotates by, the same for every layer of the step."""
         table = torch.empty((self.positions.shape[0], head_dim), dtype=torch.float32, device=self.positions.device)
-        _call("rope table", table.device, _lib.lib().dskv_rope_table, table.data_ptr(), self.positions.data_ptr(),
+        _call("rope table", _on_device(table), _lib.lib().dskv_rope_table, table.data_ptr(), self.positions.data_ptr(),
               table.shape[0], head_dim, float(rope_theta))
         return table
 
@@ -105,21 +116,20 @@ def build_step_tables(page_tables: torch.Tensor, kv_lens: torch.Tensor, qo_lens:
             (page_tables.numel() > 0 and (page_tables.stride(1) != 1 and page_tables.shape[1] > 1)) or \
             (page_tables.shape[0] > 1 and page_tables.stride(0) < page_tables.shape[1]):
         raise ValueError("page_tables must be int32 (rows, width) with contiguous rows")
-    batch = kv_lens.shape[0] if kv_lens.dim() == 1 else -1
     _check_vector("kv_lens", kv_lens, torch.int32, 0)
     _check_vector("qo_lens", qo_lens, torch.int32, 0)
-    if qo_lens.shape[0] != batch:
-        raise ValueError(f"kv_lens and qo_lens disagree about the batch: {batch} and {qo_lens.shape[0]}")
+    batch = kv_lens.numel()
+    if qo_lens.numel() != batch:
+        raise ValueError(f"kv_lens and qo_lens disagree about the batch: {batch} and {qo_lens.numel()}")
     if rows is not None:
         _check_vector("rows", rows, torch.int32, batch)
     if parents is not None:
         _check_vector("parents", parents, torch.int32, 0)
     if page_size <= 0 or max_tokens < 0 or max_pages < 0:
         raise ValueError("page_size must be positive, max_tokens and max_pages not negative")
-    device = kv_lens.device
     if out is None:
-        _on_device(device, (page_tables, qo_lens, rows, parents))
-        out = StepTables.empty(batch, max_tokens, max_pages, device, parents is not None)
+        index = _on_device(kv_lens, page_tables, qo_lens, rows, parents)
+        out = StepTables.empty(batch, max_tokens, max_pages, kv_lens.device, parents is not None)
     else:
         for name, dtype, n in (("qo_indptr", torch.int32, batch + 1), ("kv_page_indptr", torch.int32, batch + 1),
                                ("kv_page_indices", torch.int32, max_pages), ("kv_last_page_lens", torch.int32, batch),
@@ -132,14 +142,15 @@ def build_step_tables(page_tables: torch.Tensor, kv_lens: torch.Tensor, qo_lens:
             raise ValueError("out has masks exactly where there are parents")
         if out.masks is not None:
             _check_vector("out.masks", out.masks, torch.int64, max_tokens)
-        _on_device(device, (page_tables, qo_lens, rows, parents, *out.csr, out.positions, out.slots, out.masks))
+        index = _on_device(kv_lens, page_tables, qo_lens, rows, parents, *out.csr, out.positions, out.slots, out.masks)
+    table_rows, width = page_tables.shape
     args = _lib.StepTablesArgs(
         page_tables.data_ptr(), _lib.ptr(rows), kv_lens.data_ptr(), qo_lens.data_ptr(), _lib.ptr(parents),
         out.qo_indptr.data_ptr(), out.kv_page_indptr.data_ptr(), out.kv_last_page_lens.data_ptr(),
         out.kv_page_indices.data_ptr(), out.positions.data_ptr(), out.slots.data_ptr(), _lib.ptr(out.masks),
-        page_tables.stride(0) if page_tables.shape[0] > 1 else page_tables.shape[1], 0 if parents is None else parents.shape[0],
-        page_tables.shape[0], page_tables.shape[1], batch, page_size, max_tokens, max_pages)
-    _call("build_step_tables", device, _lib.lib().dskv_step_tables, ctypes.byref(args))
+        page_tables.stride(0) if table_rows > 1 else width, 0 if parents is None else parents.numel(),
+        table_rows, width, batch, page_size, max_tokens, max_pages)
+    _call("build_step_tables", index, _lib.lib().dskv_step_tables, ctypes.byref(args))
     return out
 
 
@@ -150,14 +161,19 @@ def _token_rows(name: str, t: torch.Tensor, dtype: torch.dtype, heads: Optional[
             (tokens is not None and t.shape[0] != tokens):
         raise ValueError(f"{name} must be ({'tokens' if tokens is None else tokens}, {'heads' if heads is None else heads}, "
                          f"{dim}) of the pool's dtype, got {tuple(t.shape)} of {t.dtype}")
-    size = t.element_size()
-    fine = (dim == 1 or t.stride(2) == 1) and (t.shape[1] == 1 or t.stride(1) == dim) and \
-        (t.shape[0] <= 1 or t.stride(0) >= t.shape[1] * dim and t.stride(0) * size % 16 == 0) and t.data_ptr() % 16 == 0
-    return t if fine else t.clone(memory_format=torch.contiguous_format)
+    n, h, _ = t.shape
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():
+            return t
+        step, head, one = t.stride()
+        if (dim == 1 or one == 1) and (h == 1 or head == dim) and (n <= 1 or step >= h * dim and step * t.element_size() % 16 == 0):
+            return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _row_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+    n, h, d = t.shape
+    return t.stride(0) if n > 1 else h * d
 
 
 def rope_append_slots(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor,
@@ -172,7 +188,7 @@ def rope_append_slots(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tenso
     if paged_kv_data.dim() != 5 or paged_kv_data.shape[1] != 2 or not paged_kv_data.is_contiguous():
         raise ValueError("paged_kv_data must be a contiguous (num_pages, 2, P, Hkv, D) tensor")
     num_pages, _, page, hkv, dim = paged_kv_data.shape
-    dtype, device = paged_kv_data.dtype, paged_kv_data.device
+    dtype = paged_kv_data.dtype
     k = _token_rows("k", k, dtype, hkv, dim, None)
     nnz = k.shape[0]
     v = _token_rows("v", v, dtype, hkv, dim, nnz)
@@ -186,16 +202,16 @@ def rope_append_slots(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tenso
                 rope_table.shape[0] < nnz or not rope_table.is_contiguous():
             raise ValueError(f"rope_table must be a contiguous float32 ({nnz}, {dim}) tensor")
         if out is None:
-            result = torch.empty(q.shape, dtype=dtype, device=device)
+            result = torch.empty(q.shape, dtype=dtype, device=q.device)
         elif out.shape != q.shape or out.dtype is not dtype or not out.is_contiguous():
             raise ValueError("out must be contiguous and of q's shape and dtype")
         else:
             result = out
     elif out is not None:
         raise ValueError("out is for the rotated q: rope_table is missing")
-    _on_device(device, (q, k, v, slots, rope_table, result))
+    index = _on_device(paged_kv_data, q, k, v, slots, rope_table, result)
     rotated = rope_table is not None
-    _call("rope_append_slots", device, _lib.lib().dskv_rope_append_slots, result.data_ptr() if rotated else None,
+    _call("rope_append_slots", index, _lib.lib().dskv_rope_append_slots, result.data_ptr() if rotated else None,
           paged_kv_data.data_ptr(), num_pages, q.data_ptr() if rotated else None, k.data_ptr(), v.data_ptr(),
           _row_stride(q) if rotated else 0, _row_stride(k), _row_stride(v), slots.data_ptr(), _lib.ptr(rope_table), nnz,
           page, q.shape[1] if rotated else hkv, hkv, dim, _lib.dtype_code(dtype))
@@ -223,11 +239,11 @@ class BatchTreeWithPagedKVCacheWrapper:
         masks (tokens) int64, bit j: the row sees new row j of its request, at most MAX_TREE_ROWS rows a request;
         None: it sees the rows up to itself."""
         _check_vector("qo_indptr", qo_indptr, torch.int32, 1)
-        batch = qo_indptr.shape[0] - 1
+        batch = qo_indptr.numel() - 1
         _check_vector("paged_kv_indptr", paged_kv_indptr, torch.int32, batch + 1)
         _check_vector("paged_kv_indices", paged_kv_indices, torch.int32, 0)
         _check_vector("paged_kv_last_page_len", paged_kv_last_page_len, torch.int32, batch)
-        if paged_kv_indptr.shape[0] != batch + 1:
+        if paged_kv_indptr.numel() != batch + 1:
             raise ValueError("qo_indptr and paged_kv_indptr disagree about the batch")
         if masks is not None:
             _check_vector("masks", masks, torch.int64, 0)
@@ -239,12 +255,12 @@ class BatchTreeWithPagedKVCacheWrapper:
             raise ValueError(f"head_dim {head_dim} must be a multiple of 8 up to 256")
         if page_size <= 0 or max_qo_len < 0:
             raise ValueError("page_size must be positive, max_qo_len not negative")
-        _on_device(qo_indptr.device, (paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len, masks, self._workspace))
+        _on_device(qo_indptr, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len, masks, self._workspace)
         self._held = (qo_indptr, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len, masks)
         self._step = _lib.TreeStep(
             qo_indptr.data_ptr(), paged_kv_indptr.data_ptr(), paged_kv_indices.data_ptr(),
             paged_kv_last_page_len.data_ptr(), _lib.ptr(masks), self._workspace.data_ptr(),
-            self._workspace.numel() * self._workspace.element_size(), paged_kv_indices.shape[0], batch, 0, max_qo_len,
+            self._workspace.numel() * self._workspace.element_size(), paged_kv_indices.numel(), batch, 0, max_qo_len,
             num_qo_heads, num_kv_heads, head_dim, page_size)
 
     def forward(self, q: torch.Tensor, paged_kv_data: torch.Tensor, sm_scale: Optional[float] = None, *,
@@ -261,17 +277,18 @@ class BatchTreeWithPagedKVCacheWrapper:
                              f"tensor as given to begin_forward, got {tuple(page)}")
         dtype = paged_kv_data.dtype
         q = _token_rows("q", q, dtype, s.n_qo_heads, s.head_dim, None)
-        if self._held[4] is not None and self._held[4].shape[0] < q.shape[0]:
-            raise ValueError(f"masks hold {self._held[4].shape[0]} rows, q has {q.shape[0]}")
+        nnz, masks = q.shape[0], self._held[4]
+        if masks is not None and masks.numel() < nnz:
+            raise ValueError(f"masks hold {masks.numel()} rows, q has {nnz}")
         if out is None:
             out = torch.empty(q.shape, dtype=dtype, device=q.device)
         elif out.shape != q.shape or out.dtype is not dtype or not out.is_contiguous():
             raise ValueError("out must be contiguous and of q's shape and dtype")
-        _on_device(self._held[0].device, (q, paged_kv_data, out))
+        index = _on_device(q, paged_kv_data, out, self._held[0])
         step = _lib.TreeStep.from_buffer_copy(s)      # calls from several threads do not share it
-        step.nnz, step.num_pages, step.dtype = q.shape[0], page[0], _lib.dtype_code(dtype)
+        step.nnz, step.num_pages, step.dtype = nnz, page[0], _lib.dtype_code(dtype)
         step.sm_scale = 1.0 / math.sqrt(s.head_dim) if sm_scale is None else sm_scale
-        _call("tree forward", q.device, _lib.lib().dskv_tree_attn, ctypes.byref(step), out.data_ptr(), q.data_ptr(),
+        _call("tree forward", index, _lib.lib().dskv_tree_attn, ctypes.byref(step), out.data_ptr(), q.data_ptr(),
               _row_stride(q), paged_kv_data.data_ptr())
         return out
 
@@ -318,15 +335,14 @@ def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, uniforms: to
     _check_vector("qo_indptr", qo_indptr, torch.int32, 1)
     if parents is not None:
         _check_vector("parents", parents, torch.int32, nnz)
-    dtype, device, batch = _lib.dtype_code(target_probs.dtype), target_probs.device, qo_indptr.shape[0] - 1
-    _on_device(device, (tokens, uniforms, qo_indptr, parents, draft_probs))
+    dtype, batch = _lib.dtype_code(target_probs.dtype), qo_indptr.numel() - 1
+    index = _on_device(target_probs, tokens, uniforms, qo_indptr, parents, draft_probs)
     lib = _lib.lib()
     need = lib.dskv_verify_workspace(batch, vocab)
-    # from the caching allocator, per call: calls on several streams do not share it
-    workspace = torch.empty((need,), dtype=torch.uint8, device=device)
-    ints = torch.empty((batch + 2 * nnz,), dtype=torch.int32, device=device)
-    counts, path, given = ints.split((batch, nnz, nnz))
-    _call("verify_drafts", device, lib.dskv_verify_drafts, counts.data_ptr(), path.data_ptr(), given.data_ptr(),
+    # workspace and results, from the caching allocator for every call: calls on several streams share nothing
+    workspace, counts, path, given = torch.empty((need // 4 + batch + 2 * nnz,), dtype=torch.int32,
+                                                 device=target_probs.device).split((need // 4, batch, nnz, nnz))
+    _call("verify_drafts", index, lib.dskv_verify_drafts, counts.data_ptr(), path.data_ptr(), given.data_ptr(),
           target_probs.data_ptr(), target_probs.stride(0) if nnz > 1 else vocab, _lib.ptr(draft_probs),
           0 if draft_probs is None else draft_probs.stride(0) if nnz > 1 else vocab, tokens.data_ptr(), uniforms.data_ptr(),
           qo_indptr.data_ptr(), _lib.ptr(parents), workspace.data_ptr(), need, batch, nnz, vocab, dtype)
@@ -339,20 +355,21 @@ def move_accepted_rows(pages: torch.Tensor, slots: torch.Tensor, qo_indptr: torc
     (verify_drafts) to where its sequence goes on, row j of the walk from slots[row path[j]] to slots[row j], in
     all layers.  Accepted chains are there already.  Rows that were refused stay behind the sequence, where the
     next step writes over them."""
-    if pages.dim() != 6 or pages.shape[2] != 2 or (pages.shape[0] > 0 and not pages[0].is_contiguous()):
+    if pages.dim() != 6 or pages.shape[2] != 2 or not (pages.is_contiguous() or pages.shape[0] == 0 or pages[0].is_contiguous()):
         raise ValueError("pages must be (L, num_pages, 2, P, Hkv, D) with contiguous layers")
     layers, num_pages, _, page, hkv, dim = pages.shape
     size = pages.element_size()
     if hkv * dim * size % 16:
         raise ValueError(f"a token's K must be a multiple of 16 bytes, not {hkv * dim * size}")
     _check_vector("qo_indptr", qo_indptr, torch.int32, 1)
-    batch = qo_indptr.shape[0] - 1
+    batch = qo_indptr.numel() - 1
     _check_vector("path", path, torch.int32, 0)
-    _check_vector("slots", slots, torch.int64, path.shape[0])
+    nnz = path.numel()
+    _check_vector("slots", slots, torch.int64, nnz)
     _check_vector("counts", counts, torch.int32, batch)
-    _on_device(pages.device, (slots, qo_indptr, path, counts))
-    if layers == 0 or num_pages == 0 or path.shape[0] == 0:
+    index = _on_device(pages, slots, qo_indptr, path, counts)
+    if layers == 0 or num_pages == 0 or nnz == 0:
         return
-    _call("move_accepted_rows", pages.device, _lib.lib().dskv_move_rows, pages.data_ptr(), pages.stride(0) * size, layers,
+    _call("move_accepted_rows", index, _lib.lib().dskv_move_rows, pages.data_ptr(), pages.stride(0) * size, layers,
           num_pages, page, hkv * dim * size, slots.data_ptr(), qo_indptr.data_ptr(), path.data_ptr(), counts.data_ptr(), batch,
-          path.shape[0])
+          nnz)

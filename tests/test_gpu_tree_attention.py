@@ -32,6 +32,11 @@ CASES = [
     ("fp32_dim200", [90], [12], True, 16, 4, 4, 200, "fp32"),
     ("long", [3000], [6], False, 16, 8, 2, 128, "bf16"),
     ("long_tree", [2500, 9], [64, 2], True, 16, 16, 2, 128, "f16"),
+    ("wide_edges", [0, 31, 32, 33, 95, 96, 127, 128], [17, 33, 64, 20, 31, 32, 5, 18], True, 16, 32, 8, 128, "bf16"),
+    ("wide_group8", [70, 1000, 5], [64, 17, 33], True, 16, 64, 8, 128, "f16"),
+    ("wide_group7_page3", [70, 500], [30, 64], True, 3, 14, 2, 128, "bf16"),
+    ("wide_segments", [2047, 2048, 1023, 1024, 4100], [20, 20, 33, 5, 64], True, 16, 16, 4, 128, "bf16"),
+    ("wide_chains", [300, 20], [40, 64], False, 12, 32, 8, 128, "f16"),
     ("many_short", list(range(70)), [1 + i % 5 for i in range(70)], True, 8, 8, 2, 128, "bf16"),
     ("many_lengths", [int(x) for x in np.random.default_rng(1).integers(0, 900, 40)], [4] * 40, False, 16, 8, 2, 128, "bf16"),
 ]
@@ -108,7 +113,7 @@ def test_rows_that_see_nothing(dtype, dim):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dtype,dim,group", [("bf16", 128, 4), ("f16", 128, 1), ("f16", 64, 8), ("fp32", 128, 4), ("fp32", 64, 2), ("bf16", 96, 4)])
+@pytest.mark.parametrize("dtype,dim,group", [("bf16", 128, 4), ("f16", 128, 1), ("f16", 128, 6), ("bf16", 128, 8), ("f16", 64, 8), ("fp32", 128, 4), ("fp32", 64, 2), ("bf16", 96, 4)])
 def test_infinities_and_nan_in_masked_places(dtype, dim, group):
     """A drafted row whose K and V are no numbers reaches the rows that descend from it and no other."""
     for value in (float("nan"), float("inf"), -float("inf")):
@@ -155,16 +160,19 @@ def test_tokens_apart_scales_and_rows_left_out():
 
 @pytest.mark.gpu
 def test_chains_longer_than_a_tree():
-    step = make_step(9, [100, 0], [150, 70], False, 16, 16, 4)
+    for dim, dtype in ((128, "bf16"), (64, "f16"), (128, "fp32")):
+        step = make_step(9, [100, 0], [150, 70], False, 16, 16, 4, dim, dtype)
+        compare(run(step), *attention(step))
+    step = make_step(9, [40, 9], [1100, 3], False, 16, 2, 2)
     compare(run(step), *attention(step))
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dtype,dim", [("bf16", 128), ("fp32", 64), ("f16", 96)])
-def test_pages_outside_the_pool_hold_no_tokens(dtype, dim):
-    step = make_step(10, [100, 40], [4, 3], True, 16, 8, 2, dim, dtype)
+@pytest.mark.parametrize("dtype,dim,hq", [("bf16", 128, 8), ("bf16", 128, 64), ("fp32", 64, 8), ("f16", 96, 8)])
+def test_pages_outside_the_pool_hold_no_tokens(dtype, dim, hq):
+    step = make_step(10, [100, 40], [4, 3], True, 16, hq, 2, dim, dtype)
     on = step.on("cuda")
-    want_step = make_step(10, [100, 40], [4, 3], True, 16, 8, 2, dim, dtype)
+    want_step = make_step(10, [100, 40], [4, 3], True, 16, hq, 2, dim, dtype)
     table = step.kv_page_indices.copy()
     table[[2, 5, 8]] = [-1, step.pages.shape[0], 2 ** 31 - 1]
     on["csr"] = on["csr"][:2] + (torch.from_numpy(table).cuda(),) + on["csr"][3:]
