@@ -154,6 +154,7 @@ static TreeForm tree_form(bool wide, int max_rows, int n_qo_heads, int n_kv_head
     // two workgroups a compute unit where their registers and LDS allow it
     const int resident = kTreeUnits * ((wide ? f.wide_waves == 4 : f.blocks <= 2) ? 2 : 1);
     f.shares = resident >= n_kv_heads ? resident / n_kv_heads : 1;
+    if (f.shares > 8) f.shares = f.shares / 8 * 8;         // (see share_and_head)
     return f;
 }
 static bool wide_form(int max_rows, int n_qo_heads, int n_kv_heads, int head_dim, int dtype)

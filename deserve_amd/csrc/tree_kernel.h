@@ -61,6 +61,7 @@ struct TreeRequest {
     int page0, pages;
     int n;               // rows that are computed
     int col_tiles, subtiles;
+    int tile;            // columns of a tile: its tiles are as even as 32 columns a wave allow
     __device__ __forceinline__ long units() const { return (long)col_tiles * subtiles; }
 };
 
@@ -78,11 +79,28 @@ template <int kCols, int kSub> __device__ __forceinline__ TreeRequest tree_reque
     r.prior = r.kv_len - rows;
     r.kv_len = max(min(r.kv_len, r.prior + (a.masks ? DSKV_MAX_TREE_ROWS : r.n)), 0L);
     r.col_tiles = (r.n * a.group + kCols - 1) / kCols;
+    r.tile = kCols;
+    if (kCols > 64 && r.col_tiles > 1) r.tile = (r.n * a.group + 32 * r.col_tiles - 1) / (32 * r.col_tiles) * 32;
     r.subtiles = max((int)((r.kv_len + kSub - 1) / kSub), 1);        // a row that sees nothing is written too
     return r;
 }
 
 __device__ __forceinline__ long share_begin(long s, long units, long shares) { return s * units / shares; }
+
+// Share and kv head of a workgroup.  Workgroups go round the eight XCDs in turn; the heads of a share belong on
+// one, since their rows of a token lie side by side: with a head per XCD every one of its L2s would be
+// asked for every eighth 256 bytes, by two of its sixteen channels.
+__device__ __forceinline__ void share_and_head(const TreeArgs &a, int &share, int &head)
+{
+    const int wg = blockIdx.x;
+    if (a.n_shares % 8 == 0) {
+        share = wg % 8 + wg / 8 / a.n_kv_heads * 8;
+        head = wg / 8 % a.n_kv_heads;
+    } else {
+        share = wg / a.n_kv_heads;
+        head = wg % a.n_kv_heads;
+    }
+}
 
 // Shares that are in use: none has fewer than `least` units, if there are as many.
 __device__ __forceinline__ long shares_of(const TreeArgs &a, long units, int least)
@@ -173,7 +191,8 @@ __global__ __launch_bounds__(kTreeThreads, kBlocks <= 2 ? 2 : 1) void tree_matri
     __shared__ unsigned bad_at[kTreeMostRows / S::kSub + 2];    // bit per token of a subtile with new rows: its V is no number
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, c = lane & 15;
-    const int share = blockIdx.x / a.n_kv_heads, head = blockIdx.x % a.n_kv_heads;
+    int share, head;
+    share_and_head(a, share, head);
 
     TreePlace place = tree_place<S::kCols, S::kSub, kTreeThreads>(a, share, kTreeWaves);
     const long begin = place.begin, end = place.end;
@@ -488,9 +507,10 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int max_col
     const TreeRequest r = tree_request<kCols, kSub>(a, b);
     const long before = a.units_before[b], units = a.units_before[a.batch];
     const int col = blockIdx.z * kColumns + column;
-    if (ct >= r.col_tiles || ct * kCols + (int)blockIdx.z * kColumns >= r.n * a.group) return;
+    const int cols = min(r.n * a.group - ct * r.tile, r.tile);
+    if (ct >= r.col_tiles || (int)blockIdx.z * kColumns >= cols) return;
     const long shares = shares_of(a, units, least);
-    const bool there = ct * kCols + col < r.n * a.group;
+    const bool there = col < cols;
     const long first = before + (long)ct * r.subtiles, last = first + r.subtiles - 1;
     const long s0 = ((first + 1) * shares + units - 1) / units - 1, s1 = ((last + 1) * shares + units - 1) / units - 1;
     if (s0 == s1) return;
@@ -536,7 +556,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int max_col
         for (int w = 1; w < kGroups; w++) add(ml_of[w][column][0], ml_of[w][column][1], acc_of[w][column * kQuads + quad]);
     }
     if (!there) return;
-    const int at = ct * kCols + col, i = at / a.group, hq = head * a.group + at - i * a.group;
+    const int at = ct * r.tile + col, i = at / a.group, hq = head * a.group + at - i * a.group;
     const float inv = sum == 0 ? 0.f : 1.f / sum;
     char *dst = a.out + (((r.first + i) * a.n_qo_heads + hq) * kD + quad * 4) * kElt;
     if constexpr (DT == DSKV_F32) *reinterpret_cast<f32x4 *>(dst) = acc * inv;

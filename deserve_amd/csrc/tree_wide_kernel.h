@@ -6,7 +6,7 @@
 // Bound by the matrix pipeline and the vector instructions beside it: 16 of 32x32x16 per block and wave, 16 exponentials a
 // lane.  Iteration j of a walk multiplies P(j - 1) into V(j - 1), turns S(j) into P(j) and computes S(j + 1), so that all of
 // its matrix instructions are independent of its exponentials.  Blocks lie in four stages of K and of V; iteration j
-// requests K(j + 3) and V(j + 2) behind its only barrier.  The running maximum of a column is raised only when
+// requests K(j + 4) and V(j + 2) behind its only barrier, and reads the operands of K(j + 2) at its end.  The running maximum of a column is raised only when
 // a block's weights under it sum to more than kMostWeight in a lane.
 // Where a token lies in the pool is looked up for some thousand tokens at a time and kept in LDS (row numbers, a bit per token that
 // there is), so that pages may have any size and the loop's loads wait for nothing but LDS.
@@ -45,7 +45,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
     __shared__ int holes;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, c = lane & 15, h = lane >> 5, r32 = lane & 31;
-    const int share = blockIdx.x / a.n_kv_heads, head = blockIdx.x % a.n_kv_heads;
+    int share, head;
+    share_and_head(a, share, head);
     TreePlace place = tree_place<W::kCols, kWideBlock, W::kThreads>(a, share, kWideLeast);
     const long begin = place.begin, end = place.end;
     long unit = begin, base = place.base;
@@ -70,13 +71,13 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
         const long item = base + (long)ct * r.subtiles;
         const int st0 = (int)(unit - item), st1 = (int)min(end - item, (long)r.subtiles);
         const int blocks = st1 - st0;
-        const int cols = min(r.n * a.group - ct * W::kCols, W::kCols);
+        const int cols = min(r.n * a.group - ct * r.tile, r.tile);
         const int prior = (int)max(r.prior, (long)-INT32_MAX);
         const int t_end = (int)min(r.kv_len, (long)st1 * kWideBlock);
         const bool works = wave * 32 < cols;
 
         // ---- the column
-        const int col = ct * W::kCols + wave * 32 + r32, row_i = col / a.group;
+        const int col = ct * r.tile + wave * 32 + r32, row_i = col / a.group;
         const bool there = wave * 32 + r32 < cols;
         const long q_row = r.first + (there ? row_i : 0);
         const int hq = head * a.group + (there ? col - row_i * a.group : 0);
@@ -97,7 +98,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
             }
         }
         // blocks that reach behind here need their scores masked
-        const int first_i = (ct * W::kCols + wave * 32) / a.group;
+        const int first_i = (ct * r.tile + wave * 32) / a.group;
         int mask_from = min(a.masks ? prior : prior + first_i + 1, t_end);
 
         f32x16 acc[4], xs[2];
@@ -160,13 +161,18 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
 #define DSKV_WAIT_VMEM(n) __builtin_amdgcn_s_waitcnt(((n) & 15) | 0x70 | 0xF00 | (((n) >> 4) << 14))
 
         // ---- parts of an iteration
-        auto scores = [&](const char *stage, f32x16 &x) {
+        u32x4 key[8];                                    // K operand: token r32, dims 16 s + 8 h ..
+        auto read_keys = [&](const char *stage) {
             // token r32 = row r32 & 3 of region r32 >> 2; chunk 2 s + h
             const char *rows = stage + (r32 >> 2) * kWideRegion + h * 64 + (r32 & 3) * 16;
 #pragma unroll
+            for (int s = 0; s < 8; s++) key[s] = *reinterpret_cast<const u32x4 *>(rows + s * 128);
+        };
+        auto scores = [&](f32x16 &x) {
+#pragma unroll
             for (int v = 0; v < 16; v++) x[v] = 0;
 #pragma unroll
-            for (int s = 0; s < 8; s++) x = E::mfma_32x32(*reinterpret_cast<const u32x4 *>(rows + s * 128), q[s], x);
+            for (int s = 0; s < 8; s++) x = E::mfma_32x32(key[s], q[s], x);
         };
         // Bits of block j's tokens that the column sees.
         auto seen_of = [&](int j, uint32_t held) {
@@ -197,6 +203,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
                 sum += p[v];
             }
             out = u32x4{E::pack2(p[0], p[1]), E::pack2(p[2], p[3]), E::pack2(p[4], p[5]), E::pack2(p[6], p[7])};
+            asm volatile("" ::"v"(out), "v"(sum));      // keeps them in their half of the iteration
         };
         auto raise = [&](const f32x16 &x) {
             float m = x[0] * a.scale;
@@ -247,39 +254,48 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
             reinterpret_cast<u32x4 *>(v_stage(3))[i] = u32x4{0, 0, 0, 0};          // V(-1), which P(-1) = 0 is multiplied by
         __syncthreads();
         if (holes) mask_from = 0;
-        Where at2, at3;                                  // of blocks j + 2 and j + 3
+        Where at2, at3, at4;                             // of blocks j + 2, j + 3, j + 4
         {
             Where w0, w1;
             where(0, w0);
             where(1, w1);
             where(2, at2);
+            where(3, at3);
+            // q and the mask are waited for here: left to the loop, that would be a wait for all of its loads
+#pragma unroll
+            for (int s = 0; s < 8; s++) asm volatile("" : "+v"(q[s]));
+            asm volatile("" : "+v"(mask));
             request(w0, k_stage(0), 0);
             request(w1, k_stage(1), 0);
-            request(w0, v_stage(0), half_bytes);
             request(at2, k_stage(2), 0);
+            request(w0, v_stage(0), half_bytes);
+            request(at3, k_stage(3), 0);
             request(w1, v_stage(1), half_bytes);
-            where(3, at3);
-            DSKV_WAIT_VMEM(4 * W::kGroups);
+            where(4, at4);
+            DSKV_WAIT_VMEM(4 * W::kGroups);              // K(0) and K(1)
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         if (works) {
-            scores(k_stage(0), xs[0]);
+            read_keys(k_stage(0));
+            scores(xs[0]);
             if ((st0 + 1) * kWideBlock > mask_from) mask_scores(0, xs[0]);
+            read_keys(k_stage(1));
         }
         auto iteration = [&](int j, int phase) {         // phase = j % 4, a literal
-            // this wave's rows of K(j + 1) and V(j - 1) have landed
+            // this wave's rows of K(j + 2) and V(j - 1) have landed
             DSKV_WAIT_VMEM(3 * W::kGroups);
             asm volatile("" ::: "memory");
             if (j > new_from && j <= new_to) set_aside(j - 1);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            request(at3, k_stage((phase + 3) & 3), 0);                              // K(j + 3)
+            request(at4, k_stage(phase), 0);                                        // K(j + 4)
             request(at2, v_stage((phase + 2) & 3), half_bytes);                     // V(j + 2)
             at2 = at3;
-            where(j + 4, at3);
+            at3 = at4;
+            where(j + 5, at4);
             if (!works || j > blocks) return;
             const int cur = phase & 1, nxt = cur ^ 1;
             const char *rows = v_stage((phase + 3) & 3) + v_off;                    // V(j - 1)
@@ -292,7 +308,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
                     const u32x2 lo = read_transposed(p), hi = read_transposed(p + 2 * kWideRegion);
                     va[d][s] = u32x4{lo.x, lo.y, hi.x, hi.y};
                 }
-            scores(k_stage((phase + 1) & 3), xs[nxt]);                              // S(j + 1)
+            scores(xs[nxt]);                                                        // S(j + 1)
             float sum = 0;
             weights(xs[cur], 0, pb[cur][0], sum);
             if ((st0 + j + 2) * kWideBlock > mask_from) mask_scores(j + 1, xs[nxt]);
@@ -300,6 +316,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
             for (int d = 0; d < 4; d++)
 #pragma unroll
                 for (int s = 0; s < 2; s++) acc[d] = E::mfma_32x32(va[d][s], pb[nxt][s], acc[d]);   // P(j - 1)
+            read_keys(k_stage((phase + 2) & 3));                                    // K(j + 2)
             weights(xs[cur], 1, pb[cur][1], sum);
             if (__builtin_expect(__builtin_amdgcn_ballot_w64(sum > kMostWeight) != 0, 0)) {
                 raise(xs[cur]);
