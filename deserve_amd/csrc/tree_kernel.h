@@ -94,7 +94,7 @@ __device__ __forceinline__ void share_and_head(const TreeArgs &a, int &share, in
 {
     const int wg = blockIdx.x;
     if (a.n_shares % 8 == 0) {
-        share = wg % 8 + wg / 8 / a.n_kv_heads * 8;
+        share = wg % 8 * (a.n_shares / 8) + wg / 8 / a.n_kv_heads;
         head = wg / 8 % a.n_kv_heads;
     } else {
         share = wg / a.n_kv_heads;

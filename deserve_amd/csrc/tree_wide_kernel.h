@@ -5,8 +5,8 @@
 //
 // Bound by the matrix pipeline and the vector instructions beside it: 16 of 32x32x16 per block and wave, 16 exponentials a
 // lane.  Iteration j of a walk multiplies P(j - 1) into V(j - 1), turns S(j) into P(j) and computes S(j + 1), so that all of
-// its matrix instructions are independent of its exponentials.  Blocks lie in four stages of K and of V; iteration j
-// requests K(j + 4) and V(j + 2) behind its only barrier, and reads the operands of K(j + 2) at its end.  The running maximum of a column is raised only when
+// its matrix instructions are independent of its exponentials.  Blocks lie in kStages stages of K and of V; iteration j
+// requests K(j + kStages) and V(j + kStages - 2) behind its only barrier, and reads the operands of K(j + 2) at its end.  The running maximum of a column is raised only when
 // a block's weights under it sum to more than kMostWeight in a lane.
 // Where a token lies in the pool is looked up for some thousand tokens at a time and kept in LDS (row numbers, a bit per token that
 // there is), so that pages may have any size and the loop's loads wait for nothing but LDS.
@@ -31,6 +31,7 @@ template <int kWaves> struct WideShape {
     static constexpr int kGroups = 8 / kWaves;           // regions of a block that a wave requests
     static constexpr int kHalf = kWaves == 8 ? 64 : 32;  // blocks that are looked up at a time; two such halves are kept
     static constexpr int kTokens = 2 * kHalf * kWideBlock;
+    static constexpr int kStages = kWaves == 8 ? 8 : 4;  // blocks of K, and of V, in LDS: as many as fit beside the other workgroup
 };
 
 template <int DT, int kWaves>
@@ -38,7 +39,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
 {
     typedef Elt<DT> E;
     typedef WideShape<kWaves> W;
-    __shared__ __align__(16) char lds[8 * kWideStage];
+    __shared__ __align__(16) char lds[2 * W::kStages * kWideStage];
     __shared__ int32_t row_at[W::kTokens];               // row of the pool (page * 2 P + place), -1: none
     __shared__ uint32_t held_at[2 * W::kHalf];           // bit per token of a block: there is one
     __shared__ uint32_t bad_at[kBadBlocks];              // bit per token of a block with new rows: its V is no number
@@ -53,7 +54,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
     int b = place.b;
 
     auto k_stage = [&](int i) { return lds + i * kWideStage; };
-    auto v_stage = [&](int i) { return lds + (4 + i) * kWideStage; };
+    auto v_stage = [&](int i) { return lds + (W::kStages + i) * kWideStage; };
+    constexpr int kLast = W::kStages - 1;
     const int row_bytes = a.n_kv_heads * 256;
     const long half_bytes = (long)a.page_size * row_bytes;
     // lane p of a load fetches chunk p / 4 of row p % 4 of a region
@@ -226,7 +228,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
 #pragma unroll
             for (int i = 0; i < W::kGroups; i++) {
                 const int region = wave * W::kGroups + i;
-                u32x4 *at = reinterpret_cast<u32x4 *>(v_stage(j & 3) + region * kWideRegion + lane * 16);
+                u32x4 *at = reinterpret_cast<u32x4 *>(v_stage(j & kLast) + region * kWideRegion + lane * 16);
                 const u32x4 x = *at;
                 bool odd = false;
 #pragma unroll
@@ -251,28 +253,28 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
         __syncthreads();
         look_up(0);
         for (int i = threadIdx.x; i < kWideStage / 16; i += W::kThreads)
-            reinterpret_cast<u32x4 *>(v_stage(3))[i] = u32x4{0, 0, 0, 0};          // V(-1), which P(-1) = 0 is multiplied by
+            reinterpret_cast<u32x4 *>(v_stage(kLast))[i] = u32x4{0, 0, 0, 0};          // V(-1), which P(-1) = 0 is multiplied by
         __syncthreads();
         if (holes) mask_from = 0;
-        Where at2, at3, at4;                             // of blocks j + 2, j + 3, j + 4
-        {
-            Where w0, w1;
-            where(0, w0);
-            where(1, w1);
-            where(2, at2);
-            where(3, at3);
-            // q and the mask are waited for here: left to the loop, that would be a wait for all of its loads
+        // q and the mask are waited for here: left to the loop, that would be a wait for all of its loads
 #pragma unroll
-            for (int s = 0; s < 8; s++) asm volatile("" : "+v"(q[s]));
-            asm volatile("" : "+v"(mask));
-            request(w0, k_stage(0), 0);
-            request(w1, k_stage(1), 0);
-            request(at2, k_stage(2), 0);
-            request(w0, v_stage(0), half_bytes);
-            request(at3, k_stage(3), 0);
-            request(w1, v_stage(1), half_bytes);
-            where(4, at4);
-            DSKV_WAIT_VMEM(4 * W::kGroups);              // K(0) and K(1)
+        for (int s = 0; s < 8; s++) asm volatile("" : "+v"(q[s]));
+        asm volatile("" : "+v"(mask));
+        Where at_v, at_between, at_k;                    // of blocks j + kStages - 2, - 1 and j + kStages
+        {
+            // as iterations -kStages .. -1 would request them
+            Where w[W::kStages];
+#pragma unroll
+            for (int i = 0; i < W::kStages; i++) where(i, w[i]);
+#pragma unroll
+            for (int i = 0; i < W::kStages; i++) {
+                request(w[i], k_stage(i), 0);
+                if (i >= 2) request(w[i - 2], v_stage(i - 2), half_bytes);
+            }
+            at_v = w[W::kStages - 2];
+            at_between = w[W::kStages - 1];
+            where(W::kStages, at_k);
+            DSKV_WAIT_VMEM(2 * (W::kStages - 2) * W::kGroups);              // K(0) and K(1)
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
@@ -284,21 +286,22 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
             read_keys(k_stage(1));
         }
         auto iteration = [&](int j, int phase) {         // phase = j % 4, a literal
+            const int hi = W::kStages == 8 ? j & 4 : 0;  // stage of block j: phase + hi
             // this wave's rows of K(j + 2) and V(j - 1) have landed
-            DSKV_WAIT_VMEM(3 * W::kGroups);
+            DSKV_WAIT_VMEM((2 * W::kStages - 5) * W::kGroups);
             asm volatile("" ::: "memory");
             if (j > new_from && j <= new_to) set_aside(j - 1);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            request(at4, k_stage(phase), 0);                                        // K(j + 4)
-            request(at2, v_stage((phase + 2) & 3), half_bytes);                     // V(j + 2)
-            at2 = at3;
-            at3 = at4;
-            where(j + 5, at4);
+            request(at_k, k_stage(phase + hi), 0);                                  // K(j + kStages)
+            request(at_v, v_stage((phase + hi + kLast - 1) & kLast), half_bytes);   // V(j + kStages - 2)
+            at_v = at_between;
+            at_between = at_k;
+            where(j + W::kStages + 1, at_k);
             if (!works || j > blocks) return;
             const int cur = phase & 1, nxt = cur ^ 1;
-            const char *rows = v_stage((phase + 3) & 3) + v_off;                    // V(j - 1)
+            const char *rows = v_stage((phase + hi + kLast) & kLast) + v_off;                  // V(j - 1)
             u32x4 va[4][2];
 #pragma unroll
             for (int d = 0; d < 4; d++)
@@ -316,7 +319,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
             for (int d = 0; d < 4; d++)
 #pragma unroll
                 for (int s = 0; s < 2; s++) acc[d] = E::mfma_32x32(va[d][s], pb[nxt][s], acc[d]);   // P(j - 1)
-            read_keys(k_stage((phase + 2) & 3));                                    // K(j + 2)
+            read_keys(k_stage((phase + hi + 2) & kLast));                                  // K(j + 2)
             weights(xs[cur], 1, pb[cur][1], sum);
             if (__builtin_expect(__builtin_amdgcn_ballot_w64(sum > kMostWeight) != 0, 0)) {
                 raise(xs[cur]);
