@@ -21,7 +21,7 @@ struct SlotRows {
 };
 
 template <int DT>
-__global__ __launch_bounds__(256) void append_slots_kernel(SlotRows a)
+__global__ __launch_bounds__(256, 6) void append_slots_kernel(SlotRows a)
 {
     typedef Chunk<DT> C;
     constexpr int E = C::kElems;
@@ -48,11 +48,13 @@ __global__ __launch_bounds__(256) void append_slots_kernel(SlotRows a)
     if (threadIdx.x * 16L < row_bytes) v_raw = *reinterpret_cast<const u32x4 *>(v_row + threadIdx.x * 16L);
     float cs[E / 2], sn[E / 2];
     if (a.table && works) {
+        typedef float Half __attribute__((ext_vector_type(E / 2)));
         const float *cosines = a.table + t * a.head_dim + col * (E / 2);
+        const Half c = *reinterpret_cast<const Half *>(cosines), s = *reinterpret_cast<const Half *>(cosines + a.head_dim / 2);
 #pragma unroll
         for (int j = 0; j < E / 2; j++) {
-            cs[j] = cosines[j];
-            sn[j] = cosines[a.head_dim / 2 + j];
+            cs[j] = c[j];
+            sn[j] = s[j];
         }
     }
     const bool there = slot >= 0 && slot < a.n_slots;
@@ -160,7 +162,7 @@ extern "C" int dskv_rope_append_slots(void *q_out, void *pages_layer, int32_t nu
     DSKV_REQUIRE(n_qo_heads > 0 && n_kv_heads > 0 && page_size > 0 && num_pages > 0, "rope_append_slots: bad shape");
     DSKV_REQUIRE((!rope_table || q_stride >= (int64_t)n_qo_heads * head_dim) && k_stride >= (int64_t)n_kv_heads * head_dim &&
                  v_stride >= (int64_t)n_kv_heads * head_dim, "rope_append_slots: rows overlap");
-    DSKV_REQUIRE((((uintptr_t)q_out | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)pages_layer) % 16 == 0) &&
+    DSKV_REQUIRE((((uintptr_t)q_out | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)pages_layer | (uintptr_t)rope_table) % 16 == 0) &&
                  ((rope_table ? q_stride : 0) | k_stride | v_stride) * size % 16 == 0,
                  "rope_append_slots: tensors and their rows must be 16-byte aligned");
     SlotRows a = {(char *)q_out, (char *)pages_layer, (const char *)q, (const char *)k, (const char *)v,

@@ -58,69 +58,79 @@ __device__ __forceinline__ Sums block_scan(Sums v, Sums &all, Sums *of_wave)
         all.tokens += of_wave[w].tokens;
         all.pages += of_wave[w].pages;
     }
-    __syncthreads();
     return v;
 }
 
+constexpr int kTableAhead = 8;          // table entries a thread requests before it knows where they go
+
 __global__ __launch_bounds__(kTableThreads) void step_tables_kernel(dskv_step_tables_t a)
 {
-    __shared__ Sums of_wave[kTableThreads / 64];
-    __shared__ long mine[5];           // first row and page of the request, its cached tokens, rows and pages
-    __shared__ long shared_row, fit_tokens, fit_pages;
-    const int b = blockIdx.x, t = threadIdx.x;
-    if (t == 0) {
-        fit_tokens = fit_pages = 0;
-        mine[0] = mine[1] = mine[2] = mine[3] = mine[4] = shared_row = 0;
-    }
-    __syncthreads();
-    Sums before = {0, 0};
+    __shared__ Sums of_wave[2][kTableThreads / 64], fit_of_wave[2][kTableThreads / 64];
+    __shared__ int fits_in_wave[2][kTableThreads / 64];
+    const int b = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    // the request's own entries first, and what of its table row they ask for: the sums below take as long
+    long kv = 0, n = 0, pages = 0, table_row = 0;
+    if (b < a.batch) request_of(a, b, kv, n, pages, table_row);
+    const int32_t *table = a.page_tables + table_row * a.table_stride;
+    int32_t held[kTableAhead], page_of_row = 0;
+#pragma unroll
+    for (int i = 0; i < kTableAhead; i++)
+        if (t + i * kTableThreads < pages) held[i] = table[t + i * kTableThreads];
+    if (t < n) page_of_row = table[(kv + t) / a.page_size];
+
     // Sums grow, so from the first request on that does not fit the arrays none does: it and all behind it get
     // nothing, and the entries stay at the sums of those that fit.
-    for (int first = 0; first <= b && first < a.batch; first += kTableThreads) {
+    Sums before = {0, 0}, fit = {0, 0};
+    bool b_fits = false;
+    for (int first = 0, turn = 0; first <= b && first < a.batch; first += kTableThreads, turn ^= 1) {
         const int r = first + t;
-        long kv = 0, rows = 0, pages = 0, table_row = 0;
-        if (r <= b && r < a.batch) request_of(a, r, kv, rows, pages, table_row);
+        const bool there = r <= b && r < a.batch;
+        long r_kv, r_rows = 0, r_pages = 0, r_table;
+        if (there) request_of(a, r, r_kv, r_rows, r_pages, r_table);
         Sums all;
-        Sums upto = block_scan({rows, pages}, all, of_wave);
+        Sums upto = block_scan({r_rows, r_pages}, all, of_wave[turn]);
         upto.tokens += before.tokens;
         upto.pages += before.pages;
-        const bool fits = upto.tokens <= a.max_tokens && upto.pages <= a.max_pages;
-        if (r <= b && r < a.batch && fits) {
-            atomicMax((unsigned long long *)&fit_tokens, (unsigned long long)upto.tokens);
-            atomicMax((unsigned long long *)&fit_pages, (unsigned long long)upto.pages);
-        }
-        if (r == b && fits) {
-            mine[0] = upto.tokens - rows;
-            mine[1] = upto.pages - pages;
-            mine[2] = kv;
-            mine[3] = rows;
-            mine[4] = pages;
-            shared_row = table_row;
-        }
+        const unsigned long long fits = __ballot(there && upto.tokens <= a.max_tokens && upto.pages <= a.max_pages);
+        if (fits && lane == 63 - __builtin_clzll(fits)) fit_of_wave[turn][wave] = upto;
+        if (lane == 0) fits_in_wave[turn][wave] = __popcll(fits);
+        __syncthreads();
+        int fitting = 0;
+#pragma unroll
+        for (int w = 0; w < kTableThreads / 64; w++)
+            if (fits_in_wave[turn][w]) {
+                fit = fit_of_wave[turn][w];
+                fitting += fits_in_wave[turn][w];
+            }
+        b_fits = fitting > b - first;
         before.tokens += all.tokens;
         before.pages += all.pages;
-        __syncthreads();
     }
-    const long row0 = mine[0], page0 = mine[1], kv = mine[2], n = mine[3], pages = mine[4];
-    const int32_t *table = a.page_tables + shared_row * a.table_stride;
+    if (!b_fits) kv = n = pages = 0;
+    const long row0 = fit.tokens - n, page0 = fit.pages - pages;
     if (t == 0) {
         if (b == 0) a.qo_indptr[0] = a.kv_page_indptr[0] = 0;
         if (b < a.batch) {
-            a.qo_indptr[b + 1] = (int32_t)fit_tokens;
-            a.kv_page_indptr[b + 1] = (int32_t)fit_pages;
+            a.qo_indptr[b + 1] = (int32_t)fit.tokens;
+            a.kv_page_indptr[b + 1] = (int32_t)fit.pages;
             a.kv_last_page_lens[b] = kv + n > 0 ? (int32_t)((kv + n - 1) % a.page_size) + 1 : 0;
         }
     }
-    for (long i = t; i < pages; i += kTableThreads) a.kv_page_indices[page0 + i] = table[i];
+    // a tree's parents lie by row, so they are requested last
     const bool tree = a.masks != nullptr;
+    int up = -1;
+    if (tree && t < n && row0 + t < a.n_parents) up = a.parents[row0 + t];
+#pragma unroll
+    for (int i = 0; i < kTableAhead; i++)
+        if (t + i * kTableThreads < pages) a.kv_page_indices[page0 + t + i * kTableThreads] = held[i];
+    for (long i = t + kTableAhead * kTableThreads; i < pages; i += kTableThreads) a.kv_page_indices[page0 + i] = table[i];
     for (long i = t; i < n; i += kTableThreads) {
         const long at = kv + i;
-        const long page = table[at / a.page_size];
+        const long page = i == t ? page_of_row : table[at / a.page_size];
         a.slots[row0 + i] = page < 0 ? -1 : page * a.page_size + at % a.page_size;
         if (!tree) a.positions[row0 + i] = (int32_t)at;
     }
-    if (tree && t < 64 && n > 0) {
-        int up = t < n && row0 + t < a.n_parents ? a.parents[row0 + t] : -1;
+    if (tree && wave == 0 && n > 0) {
         if (up >= t || up < 0) up = -1;            // a row without a parent among the rows before it
         unsigned long long mask = 1ull << t;
 #pragma unroll
@@ -139,7 +149,7 @@ __global__ __launch_bounds__(kTableThreads) void step_tables_kernel(dskv_step_ta
     }
     // rows behind the last request have no slot
     if (b == (int)gridDim.x - 1)
-        for (long i = fit_tokens + t; i < a.max_tokens; i += kTableThreads) {
+        for (long i = fit.tokens + t; i < a.max_tokens; i += kTableThreads) {
             a.slots[i] = -1;
             a.positions[i] = 0;
             if (tree) a.masks[i] = 0;

@@ -8,8 +8,8 @@
 // move by whole tokens, and a product of two 32-bit numbers is exact in 64.
 //
 // Bound by reading that row (of p, and of q) where there are requests enough, by the chain of two launches otherwise.
-// Two launches: the first sums parts of kPart weights, each workgroup taking the walk for itself (a few hundred
-// bytes from L2), the second finds the part by the parts' sums and the token in it.
+// Two launches: in the first every workgroup takes the walk for itself (a few hundred bytes from L2) and sums a part of kPart
+// weights; a request's first workgroup writes the walk down.  The second finds the part by the parts' sums and the token in it.
 #include "common.h"
 
 namespace dskv {
@@ -39,7 +39,17 @@ struct VerifyArgs {
     const float *uniforms;
     int32_t *counts, *path, *out_tokens;
     double *sums;                          // (batch, parts): sum of w, then the same of p
+    struct SharedWalk *walks;              // (batch)
     int batch, nnz, vocab, parts;
+};
+
+// What the workgroups need to know of a walk.
+struct SharedWalk {
+    long row, first;                       // the row reached, and the request's row 0, of all rows
+    int count, n_refused;
+    int minus_draft;
+    float uniform;                         // of row 0
+    int refused[DSKV_MAX_TREE_ROWS];       // tokens
 };
 
 // What is no probability counts as none.
@@ -55,6 +65,7 @@ struct Walk {
     long first;
     bool minus_draft;              // w = max(p - q, 0)
     unsigned long long refused;    // children refused there
+    float uniform;                 // of row 0
     int path;                      // lane j: j-th row of the walk
     int token, token_of_path;      // lane i: token of row i; lane j: token of the j-th row of the walk
 };
@@ -64,16 +75,17 @@ template <int DT> __device__ __forceinline__ Walk walk_drafts(const VerifyArgs &
 {
     typedef typename Prob<DT>::T T;
     const int lane = threadIdx.x & 63;
-    Walk w = {0, 0, 0, 0, false, 0, -1, -1, -1};
+    Walk w = {0, 0, 0, 0, false, 0, 0.f, -1, -1, -1};
     const long first = a.qo_indptr[b], n = a.qo_indptr[b + 1] - first;
     w.first = first;
     if (first < 0 || n <= 0 || n > DSKV_MAX_TREE_ROWS || first + n > a.nnz) return w;
     w.n = (int)n;
     int up = -1, token = -1;
-    double p = 0, q = 0, u = 0;
+    double p = 0, q = 0;
+    float u32 = 0;
     if (lane < n) {
         token = a.tokens[first + lane];
-        u = a.uniforms[first + lane];
+        u32 = a.uniforms[first + lane];
         up = lane == 0 ? -1 : a.parents ? a.parents[first + lane] : lane - 1;
         if (up >= lane) up = -1;
         if (up >= 0 && token >= 0 && token < a.vocab) {
@@ -81,6 +93,8 @@ template <int DT> __device__ __forceinline__ Walk walk_drafts(const VerifyArgs &
             if (a.draft) q = weight_of<DT>(((const T *)a.draft)[(first + up) * a.draft_stride + token]);
         }
     }
+    const double u = u32;
+    w.uniform = __shfl(u32, 0);
     const bool drafted = a.draft != nullptr;
     const bool chain_passes = drafted && up >= 0 && u * q < p;
     int at = 0, count = 1;
@@ -127,41 +141,54 @@ template <int DT> __device__ __forceinline__ Walk walk_drafts(const VerifyArgs &
 }
 
 // The walk for the workgroup's other waves.
-struct SharedWalk {
-    long row;
-    int count, n_refused;
-    bool minus_draft;
-    int refused[DSKV_MAX_TREE_ROWS];       // tokens
-};
 __device__ __forceinline__ void share_walk(const Walk &w, SharedWalk &s, bool drafted)
 {
     const int lane = threadIdx.x & 63;
     if (lane == 0) {
         s.row = w.row;
+        s.first = w.first;
         s.count = w.count;
         s.minus_draft = w.minus_draft;
+        s.uniform = w.uniform;
         s.n_refused = drafted ? 0 : __popcll(w.refused);
     }
     if (!drafted && ((w.refused >> lane) & 1)) s.refused[__popcll(w.refused & ((1ull << lane) - 1))] = w.token;
 }
 
-// Thread t's weights of a part: elements t * kPerThread .. of it.
+// Weights e0 .. e0 + 15 bytes' worth of the row, as many as a 16-byte load holds; rows start at any element.
 template <int DT>
-__device__ __forceinline__ void load_weights(const VerifyArgs &a, const SharedWalk &s, long part, float (&p)[kPerThread],
+__device__ __forceinline__ void load_probs(const typename Prob<DT>::T *row, long e0, int vocab, float *p)
+{
+    typedef typename Prob<DT>::T T;
+    constexpr int kN = 16 / sizeof(T);
+    T x[kN];
+    if (e0 + kN <= vocab) {
+        __builtin_memcpy(x, row + e0, 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kN; i++) x[i] = e0 + i < vocab ? row[e0 + i] : T(0);
+    }
+#pragma unroll
+    for (int i = 0; i < kN; i++) p[i] = weight_of<DT>(x[i]);
+}
+
+// The thread's weights of a part: kPerThread / kN runs of kN, the first at e0, kStep elements apart.
+template <int DT, int kStep>
+__device__ __forceinline__ void load_weights(const VerifyArgs &a, const SharedWalk &s, long e0, float (&p)[kPerThread],
                                              double (&w)[kPerThread])
 {
     typedef typename Prob<DT>::T T;
-    const long e0 = part * kPart + threadIdx.x * kPerThread;
+    constexpr int kN = 16 / sizeof(T);
     const T *target = (const T *)a.target + s.row * a.target_stride;
     const T *draft = (const T *)a.draft + s.row * a.draft_stride;
 #pragma unroll
-    for (int i = 0; i < kPerThread; i++) p[i] = e0 + i < a.vocab ? weight_of<DT>(target[e0 + i]) : 0.f;
+    for (int i = 0; i < kPerThread / kN; i++) load_probs<DT>(target, e0 + i * kStep, a.vocab, p + i * kN);
     if (s.minus_draft) {
+        float q[kPerThread];
 #pragma unroll
-        for (int i = 0; i < kPerThread; i++) {
-            const float q = e0 + i < a.vocab ? weight_of<DT>(draft[e0 + i]) : 0.f;
-            w[i] = fmax((double)p[i] - (double)q, 0.0);
-        }
+        for (int i = 0; i < kPerThread / kN; i++) load_probs<DT>(draft, e0 + i * kStep, a.vocab, q + i * kN);
+#pragma unroll
+        for (int i = 0; i < kPerThread; i++) w[i] = p[i] > q[i] ? (double)p[i] - (double)q[i] : 0.0;
     } else {
 #pragma unroll
         for (int i = 0; i < kPerThread; i++) w[i] = p[i];
@@ -169,7 +196,7 @@ __device__ __forceinline__ void load_weights(const VerifyArgs &a, const SharedWa
             const long at = s.refused[r] - e0;
 #pragma unroll
             for (int i = 0; i < kPerThread; i++)
-                if (at == i) w[i] = 0;
+                if (at == i / kN * kStep + i % kN) w[i] = 0;
         }
     }
 }
@@ -186,12 +213,37 @@ template <int DT> __global__ __launch_bounds__(kVerifyThreads) void verify_sums_
     __shared__ SharedWalk s;
     __shared__ double of_wave[kVerifyThreads / 64][2];
     const int b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (wave == 0) share_walk(walk_drafts<DT>(a, b), s, a.draft != nullptr);
+    const bool tells = blockIdx.x == 0;
+    // rows behind the last request
+    if (tells && b >= a.batch - 1) {
+        const long end = max((long)a.qo_indptr[a.batch], 0L);
+        for (long t = end + threadIdx.x; t < a.nnz; t += kVerifyThreads) a.path[t] = a.out_tokens[t] = -1;
+        if (b >= a.batch) return;                                  // no requests at all
+    }
+    if (wave == 0) {
+        const Walk w = walk_drafts<DT>(a, b);
+        share_walk(w, s, a.draft != nullptr);
+        if (tells) {
+            share_walk(w, a.walks[b], a.draft != nullptr);
+            const int next = __shfl(w.token_of_path, min(lane + 1, 63));
+            if (lane < w.n) {
+                a.path[w.first + lane] = lane < w.count ? w.path : -1;
+                if (lane != w.count - 1) a.out_tokens[w.first + lane] = lane < w.count ? next : -1;
+            }
+            if (lane == 0) a.counts[b] = w.count;
+        }
+    }
     __syncthreads();
-    if (s.count == 0) return;
+    if (s.count == 0) {                                            // no rows, or too many
+        const long lo = max((long)a.qo_indptr[b], 0L), hi = min((long)a.qo_indptr[b + 1], (long)a.nnz);
+        if (tells)
+            for (long t = lo + threadIdx.x; t < hi; t += kVerifyThreads) a.path[t] = a.out_tokens[t] = -1;
+        return;
+    }
+    constexpr int kN = 16 / sizeof(typename Prob<DT>::T);
     float p[kPerThread];
     double w[kPerThread], sw = 0, sp = 0;
-    load_weights<DT>(a, s, blockIdx.x, p, w);
+    load_weights<DT, kVerifyThreads * kN>(a, s, (long)blockIdx.x * kPart + threadIdx.x * kN, p, w);
 #pragma unroll
     for (int i = 0; i < kPerThread; i++) {
         sw += w[i];
@@ -212,71 +264,70 @@ template <int DT> __global__ __launch_bounds__(kVerifyThreads) void verify_sums_
     }
 }
 
+// Sums up to and with this lane's over a wave.
+__device__ __forceinline__ double wave_scan64(double v)
+{
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const double x = __shfl_up(v, o);
+        if (lane >= o) v += x;
+    }
+    return v;
+}
+
 template <int DT> __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs a)
 {
     __shared__ SharedWalk s;
     __shared__ double of_wave[kVerifyThreads / 64];
     __shared__ int drawn, last_with_mass;
     const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    Walk walk = {};
-    if (wave == 0 && b < a.batch) {
-        walk = walk_drafts<DT>(a, b);
-        share_walk(walk, s, a.draft != nullptr);
-    }
+    static_assert(sizeof(SharedWalk) % 4 == 0 && sizeof(SharedWalk) / 4 <= kVerifyThreads, "a word a thread");
+    if (threadIdx.x < sizeof(SharedWalk) / 4) ((int *)&s)[threadIdx.x] = ((const int *)(a.walks + b))[threadIdx.x];
     if (threadIdx.x == 0) drawn = 0x7fffffff, last_with_mass = -1;
-    // rows behind the last request, and those of requests that are left out
-    if (b >= a.batch - 1) {
-        const long end = max((long)a.qo_indptr[a.batch], 0L);
-        for (long t = end + threadIdx.x; t < a.nnz; t += kVerifyThreads) a.path[t] = a.out_tokens[t] = -1;
-    }
-    if (b >= a.batch) return;                  // no requests at all
+    // sums of the parts, of w and of p, 64 at a time by every wave alike
+    const double *of_w = a.sums + (long)b * a.parts, *of_p = of_w + (long)a.batch * a.parts;
+    double first_w = lane < a.parts ? of_w[lane] : 0, first_p = lane < a.parts ? of_p[lane] : 0;
     __syncthreads();
-    if (s.count == 0) {
-        const long lo = max((long)a.qo_indptr[b], 0L), hi = min((long)a.qo_indptr[b + 1], (long)a.nnz);
-        for (long t = lo + threadIdx.x; t < hi; t += kVerifyThreads) a.path[t] = a.out_tokens[t] = -1;
-        if (threadIdx.x == 0) a.counts[b] = 0;
-        return;
+    if (s.count == 0) return;
+    const double u = s.uniform;
+    double scan_w = wave_scan64(first_w), total = __shfl(scan_w, 63);
+    for (int i = 64; i < a.parts; i += 64) total += wave_sum64(i + lane < a.parts ? of_w[i + lane] : 0);
+    const bool from_p = !(total > 0);            // w has no mass
+    const double *sums = from_p ? of_p : of_w;
+    if (from_p) {
+        scan_w = wave_scan64(first_p);
+        total = __shfl(scan_w, 63);
+        for (int i = 64; i < a.parts; i += 64) total += wave_sum64(i + lane < a.parts ? of_p[i + lane] : 0);
     }
-    // the part that the draw falls into: sums of the parts in order, by every thread alike
-    const double *sums = a.sums + (long)b * a.parts;
-    double total = 0;
-    for (int i = 0; i < a.parts; i++) total += sums[i];
-    const bool of_p = !(total > 0);            // w has no mass
-    if (of_p) {
-        sums += (long)a.batch * a.parts;
-        total = 0;
-        for (int i = 0; i < a.parts; i++) total += sums[i];
-    }
-    const double u = a.uniforms[a.qo_indptr[b]];
     const double target = u < 0 ? 0 : u * total;
-    double before = 0;
+    // the first part whose sum passes the target; if rounding or u lets none, the last with mass
+    double before = 0, before_part = 0;
     int part = -1;
-    double before_part = 0;
-    for (int i = 0; i < a.parts; i++) {
-        const double sum = sums[i];
-        if (sum > 0) {
-            part = i;                          // the last with mass, if the draw is behind all of them
-            before_part = before;
+    for (int i = 0; i < a.parts; i += 64) {
+        const double sum = i == 0 ? (from_p ? first_p : first_w) : i + lane < a.parts ? sums[i + lane] : 0;
+        const double upto = i == 0 ? scan_w : before + wave_scan64(sum);
+        const unsigned long long mass = __ballot(sum > 0), over = __ballot(sum > 0 && upto > target);
+        if (mass) {
+            const int at = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(mass);
+            part = i + at;
+            before_part = __shfl(upto - sum, at);
         }
-        before += sum;
-        if (before > target) break;
+        if (over) break;
+        before = __shfl(upto, 63);
     }
     int token = 0;
     if (part >= 0) {
+        constexpr int kN = 16 / sizeof(typename Prob<DT>::T);
         float p[kPerThread];
         double w[kPerThread], mine = 0;
-        load_weights<DT>(a, s, part, p, w);
+        load_weights<DT, kN>(a, s, (long)part * kPart + threadIdx.x * kPerThread, p, w);
 #pragma unroll
         for (int i = 0; i < kPerThread; i++) {
-            if (of_p) w[i] = p[i];
+            if (from_p) w[i] = p[i];
             mine += w[i];
         }
-        double upto = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const double v = __shfl_up(upto, o);
-            if (lane >= o) upto += v;
-        }
+        const double upto = wave_scan64(mine);
         if (lane == 63) of_wave[wave] = upto;
         __syncthreads();
         double cum = before_part + upto - mine;
@@ -299,12 +350,7 @@ template <int DT> __global__ __launch_bounds__(kVerifyThreads) void verify_draw_
         // rounding may leave the sum of the part below what its whole sum promised
         token = part * kPart + (drawn != 0x7fffffff ? drawn : max(last_with_mass, 0));
     }
-    if (wave == 0 && lane < walk.n) {
-        const int next = __shfl(walk.token_of_path, min(lane + 1, 63));
-        a.path[walk.first + lane] = lane < walk.count ? walk.path : -1;
-        a.out_tokens[walk.first + lane] = lane < walk.count - 1 ? next : lane == walk.count - 1 ? token : -1;
-        if (lane == 0) a.counts[b] = walk.count;
-    }
+    if (threadIdx.x == 0) a.out_tokens[s.first + s.count - 1] = token;
 }
 
 static int verify_parts(int vocab) { return (vocab + kPart - 1) / kPart; }
@@ -314,7 +360,7 @@ static int verify_parts(int vocab) { return (vocab + kPart - 1) / kPart; }
 extern "C" int64_t dskv_verify_workspace(int32_t batch, int32_t vocab)
 {
     if (batch <= 0 || vocab <= 0) return 0;
-    return (int64_t)batch * dskv::verify_parts(vocab) * 2 * (int64_t)sizeof(double);
+    return batch * (dskv::verify_parts(vocab) * 2 * (int64_t)sizeof(double) + (int64_t)sizeof(dskv::SharedWalk));
 }
 
 extern "C" int dskv_verify_drafts(int32_t *counts, int32_t *path, int32_t *out_tokens, const void *target_probs,
@@ -341,18 +387,18 @@ extern "C" int dskv_verify_drafts(int32_t *counts, int32_t *path, int32_t *out_t
     DSKV_REQUIRE((uintptr_t)workspace % 16 == 0, "verify_drafts: the workspace must be 16-byte aligned");
     const int parts = verify_parts(vocab);
     VerifyArgs a = {target_probs, draft_probs, (long)target_stride, (long)draft_stride, tokens, qo_indptr, parents,
-                    uniforms, counts, path, out_tokens, (double *)workspace, batch, nnz, vocab, parts};
+                    uniforms, counts, path, out_tokens, (double *)workspace,
+                    (SharedWalk *)((double *)workspace + (int64_t)batch * parts * 2), batch, nnz, vocab, parts};
     hipStream_t s = (hipStream_t)stream;
 #define DSKV_LAUNCH_VERIFY(DT)                                                                                      \
     do {                                                                                                            \
-        if (batch > 0) {                                                                                            \
-            hipLaunchKernelGGL((verify_sums_kernel<DT>), dim3((unsigned)parts, (unsigned)batch),                    \
-                               dim3(kVerifyThreads), 0, s, a);                                                      \
-            DSKV_LAUNCH_CHECK("verify_sums_kernel");                                                                \
-        }                                                                                                           \
-        hipLaunchKernelGGL((verify_draw_kernel<DT>), dim3((unsigned)(batch > 0 ? batch : 1)),                       \
+        hipLaunchKernelGGL((verify_sums_kernel<DT>), dim3((unsigned)parts, (unsigned)(batch > 0 ? batch : 1)),      \
                            dim3(kVerifyThreads), 0, s, a);                                                          \
-        DSKV_LAUNCH_CHECK("verify_draw_kernel");                                                                    \
+        DSKV_LAUNCH_CHECK("verify_sums_kernel");                                                                    \
+        if (batch > 0) {                                                                                            \
+            hipLaunchKernelGGL((verify_draw_kernel<DT>), dim3((unsigned)batch), dim3(kVerifyThreads), 0, s, a);     \
+            DSKV_LAUNCH_CHECK("verify_draw_kernel");                                                                \
+        }                                                                                                           \
     } while (0)
     if (dtype == DSKV_F32) DSKV_LAUNCH_VERIFY(DSKV_F32);
     else if (dtype == DSKV_F16) DSKV_LAUNCH_VERIFY(DSKV_F16);

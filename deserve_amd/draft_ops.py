@@ -154,26 +154,26 @@ def build_step_tables(page_tables: torch.Tensor, kv_lens: torch.Tensor, qo_lens:
     return out
 
 
-def _token_rows(name: str, t: torch.Tensor, dtype: torch.dtype, heads: Optional[int], dim: int, tokens: Optional[int]) -> torch.Tensor:
-    """(tokens, heads, dim) with the heads of a token contiguous; tokens may lie apart, as parts of one projection's
-    output do.  Anything else is copied."""
-    if t.dim() != 3 or t.shape[2] != dim or t.dtype is not dtype or (heads is not None and t.shape[1] != heads) or \
-            (tokens is not None and t.shape[0] != tokens):
+def _token_rows(name: str, t: torch.Tensor, dtype: torch.dtype, heads: Optional[int], dim: int,
+                tokens: Optional[int]) -> Tuple[torch.Tensor, int]:
+    """(tokens, heads, dim) with the heads of a token contiguous, and how many elements tokens are apart: they may lie apart, as
+    parts of one projection's output do.  Anything else is copied."""
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != dim or t.dtype is not dtype or (heads is not None and shape[1] != heads) or \
+            (tokens is not None and shape[0] != tokens):
         raise ValueError(f"{name} must be ({'tokens' if tokens is None else tokens}, {'heads' if heads is None else heads}, "
-                         f"{dim}) of the pool's dtype, got {tuple(t.shape)} of {t.dtype}")
-    n, h, _ = t.shape
+                         f"{dim}) of the pool's dtype, got {tuple(shape)} of {t.dtype}")
+    n, h, _ = shape
     if t.data_ptr() % 16 == 0:
         if t.is_contiguous():
-            return t
+            return t, h * dim
         step, head, one = t.stride()
-        if (dim == 1 or one == 1) and (h == 1 or head == dim) and (n <= 1 or step >= h * dim and step * t.element_size() % 16 == 0):
-            return t
-    return t.clone(memory_format=torch.contiguous_format)
-
-
-def _row_stride(t: torch.Tensor) -> int:
-    n, h, d = t.shape
-    return t.stride(0) if n > 1 else h * d
+        if (dim == 1 or one == 1) and (h == 1 or head == dim):
+            if n <= 1:
+                return t, h * dim
+            if step >= h * dim and step * t.element_size() % 16 == 0:
+                return t, step
+    return t.clone(memory_format=torch.contiguous_format), h * dim
 
 
 def rope_append_slots(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor,
@@ -189,20 +189,21 @@ def rope_append_slots(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tenso
         raise ValueError("paged_kv_data must be a contiguous (num_pages, 2, P, Hkv, D) tensor")
     num_pages, _, page, hkv, dim = paged_kv_data.shape
     dtype = paged_kv_data.dtype
-    k = _token_rows("k", k, dtype, hkv, dim, None)
+    k, k_stride = _token_rows("k", k, dtype, hkv, dim, None)
     nnz = k.shape[0]
-    v = _token_rows("v", v, dtype, hkv, dim, nnz)
+    v, v_stride = _token_rows("v", v, dtype, hkv, dim, nnz)
     _check_vector("slots", slots, torch.int64, nnz)
-    result = q
+    result, q_stride, heads = q, 0, hkv
     if rope_table is not None:
         if q is None:
             raise ValueError("rope_table rotates q and k: q is missing")
-        q = _token_rows("q", q, dtype, None, dim, nnz)
-        if rope_table.dtype is not torch.float32 or rope_table.dim() != 2 or rope_table.shape[1] != dim or \
-                rope_table.shape[0] < nnz or not rope_table.is_contiguous():
-            raise ValueError(f"rope_table must be a contiguous float32 ({nnz}, {dim}) tensor")
+        q, q_stride = _token_rows("q", q, dtype, None, dim, nnz)
+        heads = q.shape[1]
+        table = rope_table.shape
+        if rope_table.dtype is not torch.float32 or len(table) != 2 or table[1] != dim or table[0] < nnz or not rope_table.is_contiguous() or rope_table.data_ptr() % 16:
+            raise ValueError(f"rope_table must be a contiguous, 16-byte aligned float32 ({nnz}, {dim}) tensor")
         if out is None:
-            result = torch.empty(q.shape, dtype=dtype, device=q.device)
+            result = q.new_empty(q.shape)
         elif out.shape != q.shape or out.dtype is not dtype or not out.is_contiguous():
             raise ValueError("out must be contiguous and of q's shape and dtype")
         else:
@@ -213,8 +214,8 @@ def rope_append_slots(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tenso
     rotated = rope_table is not None
     _call("rope_append_slots", index, _lib.lib().dskv_rope_append_slots, result.data_ptr() if rotated else None,
           paged_kv_data.data_ptr(), num_pages, q.data_ptr() if rotated else None, k.data_ptr(), v.data_ptr(),
-          _row_stride(q) if rotated else 0, _row_stride(k), _row_stride(v), slots.data_ptr(), _lib.ptr(rope_table), nnz,
-          page, q.shape[1] if rotated else hkv, hkv, dim, _lib.dtype_code(dtype))
+          q_stride, k_stride, v_stride, slots.data_ptr(), _lib.ptr(rope_table), nnz, page, heads, hkv, dim,
+          _lib.dtype_code(dtype))
     return result
 
 
@@ -276,12 +277,12 @@ class BatchTreeWithPagedKVCacheWrapper:
             raise ValueError(f"paged_kv_data must be a contiguous (num_pages, 2, {s.page_size}, {s.n_kv_heads}, {s.head_dim}) "
                              f"tensor as given to begin_forward, got {tuple(page)}")
         dtype = paged_kv_data.dtype
-        q = _token_rows("q", q, dtype, s.n_qo_heads, s.head_dim, None)
+        q, q_stride = _token_rows("q", q, dtype, s.n_qo_heads, s.head_dim, None)
         nnz, masks = q.shape[0], self._held[4]
         if masks is not None and masks.numel() < nnz:
             raise ValueError(f"masks hold {masks.numel()} rows, q has {nnz}")
         if out is None:
-            out = torch.empty(q.shape, dtype=dtype, device=q.device)
+            out = q.new_empty(q.shape)
         elif out.shape != q.shape or out.dtype is not dtype or not out.is_contiguous():
             raise ValueError("out must be contiguous and of q's shape and dtype")
         index = _on_device(q, paged_kv_data, out, self._held[0])
@@ -289,7 +290,7 @@ class BatchTreeWithPagedKVCacheWrapper:
         step.nnz, step.num_pages, step.dtype = nnz, page[0], _lib.dtype_code(dtype)
         step.sm_scale = 1.0 / math.sqrt(s.head_dim) if sm_scale is None else sm_scale
         _call("tree forward", index, _lib.lib().dskv_tree_attn, ctypes.byref(step), out.data_ptr(), q.data_ptr(),
-              _row_stride(q), paged_kv_data.data_ptr())
+              q_stride, paged_kv_data.data_ptr())
         return out
 
     def end_forward(self) -> None:
@@ -340,8 +341,7 @@ def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, uniforms: to
     lib = _lib.lib()
     need = lib.dskv_verify_workspace(batch, vocab)
     # workspace and results, from the caching allocator for every call: calls on several streams share nothing
-    workspace, counts, path, given = torch.empty((need // 4 + batch + 2 * nnz,), dtype=torch.int32,
-                                                 device=target_probs.device).split((need // 4, batch, nnz, nnz))
+    workspace, counts, path, given = tokens.new_empty((need // 4 + batch + 2 * nnz,)).split((need // 4, batch, nnz, nnz))
     _call("verify_drafts", index, lib.dskv_verify_drafts, counts.data_ptr(), path.data_ptr(), given.data_ptr(),
           target_probs.data_ptr(), target_probs.stride(0) if nnz > 1 else vocab, _lib.ptr(draft_probs),
           0 if draft_probs is None else draft_probs.stride(0) if nnz > 1 else vocab, tokens.data_ptr(), uniforms.data_ptr(),
