@@ -94,7 +94,7 @@ __device__ __forceinline__ void share_and_head(const TreeArgs &a, int &share, in
 {
     const int wg = blockIdx.x;
     if (a.n_shares % 8 == 0) {
-        share = wg % 8 * (a.n_shares / 8) + wg / 8 / a.n_kv_heads;
+        share = wg % 8 + wg / 8 / a.n_kv_heads * 8;        // (few shares in use are spread over the XCDs)
         head = wg / 8 % a.n_kv_heads;
     } else {
         share = wg / a.n_kv_heads;
@@ -261,8 +261,8 @@ __global__ __launch_bounds__(kTreeThreads, kBlocks <= 2 ? 2 : 1) void tree_matri
                 next.k[i] = next.v[i] = u32x4{0, 0, 0, 0};
                 if (row >= 0) {
                     const char *p = pool + (unsigned long)(unsigned)row * row_bytes;
-                    next.k[i] = *reinterpret_cast<const u32x4 *>(p);
-                    next.v[i] = *reinterpret_cast<const u32x4 *>(p + a.page_size * row_bytes);
+                    next.k[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p));
+                    next.v[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p + a.page_size * row_bytes));
                 }
             }
         };

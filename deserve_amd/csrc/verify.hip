@@ -201,11 +201,29 @@ __device__ __forceinline__ void load_weights(const VerifyArgs &a, const SharedWa
     }
 }
 
+// Sums up to and with this lane's over a wave, by moves between lanes that do not go through LDS.
+template <int kCtrl, int kRows> __device__ __forceinline__ double lanes_below(double v)
+{
+    const uint64_t x = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, kCtrl, kRows, 0xf, true);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), kCtrl, kRows, 0xf, true);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_scan64(double v)
+{
+    v += lanes_below<0x111, 0xf>(v);       // row_shr 1, 2, 4, 8 within 16 lanes
+    v += lanes_below<0x112, 0xf>(v);
+    v += lanes_below<0x114, 0xf>(v);
+    v += lanes_below<0x118, 0xf>(v);
+    v += lanes_below<0x142, 0xa>(v);       // the last lane of rows 0 and 2 to rows 1 and 3
+    v += lanes_below<0x143, 0xc>(v);       // lane 31 to rows 2 and 3
+    return v;
+}
 __device__ __forceinline__ double wave_sum64(double v)
 {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+    const uint64_t x = __builtin_bit_cast(uint64_t, wave_scan64(v));
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)x, 63), hi = __builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), 63);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
 template <int DT> __global__ __launch_bounds__(kVerifyThreads) void verify_sums_kernel(VerifyArgs a)
@@ -264,27 +282,14 @@ template <int DT> __global__ __launch_bounds__(kVerifyThreads) void verify_sums_
     }
 }
 
-// Sums up to and with this lane's over a wave.
-__device__ __forceinline__ double wave_scan64(double v)
-{
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double x = __shfl_up(v, o);
-        if (lane >= o) v += x;
-    }
-    return v;
-}
-
 template <int DT> __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs a)
 {
     __shared__ SharedWalk s;
     __shared__ double of_wave[kVerifyThreads / 64];
-    __shared__ int drawn, last_with_mass;
+    __shared__ int hit_of[kVerifyThreads / 64], mass_of[kVerifyThreads / 64];
     const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     static_assert(sizeof(SharedWalk) % 4 == 0 && sizeof(SharedWalk) / 4 <= kVerifyThreads, "a word a thread");
     if (threadIdx.x < sizeof(SharedWalk) / 4) ((int *)&s)[threadIdx.x] = ((const int *)(a.walks + b))[threadIdx.x];
-    if (threadIdx.x == 0) drawn = 0x7fffffff, last_with_mass = -1;
     // sums of the parts, of w and of p, 64 at a time by every wave alike
     const double *of_w = a.sums + (long)b * a.parts, *of_p = of_w + (long)a.batch * a.parts;
     double first_w = lane < a.parts ? of_w[lane] : 0, first_p = lane < a.parts ? of_p[lane] : 0;
@@ -335,20 +340,31 @@ template <int DT> __global__ __launch_bounds__(kVerifyThreads) void verify_draw_
         for (int i = 0; i < kVerifyThreads / 64; i++)
             if (i < wave) cum += of_wave[i];
         const int e0 = threadIdx.x * kPerThread;
-        int hit = 0x7fffffff, mass = -1;
+        int hit = -1, mass = -1;               // first weight that passes the target; last with weight at all
 #pragma unroll
         for (int i = 0; i < kPerThread; i++) {
             cum += w[i];
             if (w[i] > 0) {
                 mass = e0 + i;
-                if (cum > target) hit = min(hit, e0 + i);
+                if (hit < 0 && cum > target) hit = e0 + i;
             }
         }
-        if (hit != 0x7fffffff) atomicMin(&drawn, hit);
-        if (mass >= 0) atomicMax(&last_with_mass, mass);
+        const unsigned long long hits = __ballot(hit >= 0), masses = __ballot(mass >= 0);
+        hit = __shfl(hit, hits ? __builtin_ctzll(hits) : 0);
+        mass = __shfl(mass, masses ? 63 - __builtin_clzll(masses) : 0);
+        if (lane == 0) {
+            hit_of[wave] = hits ? hit : -1;
+            mass_of[wave] = masses ? mass : -1;
+        }
         __syncthreads();
+        int drawn = -1, last = 0;
+#pragma unroll
+        for (int i = 0; i < kVerifyThreads / 64; i++) {
+            if (drawn < 0) drawn = hit_of[i];
+            last = max(last, mass_of[i]);
+        }
         // rounding may leave the sum of the part below what its whole sum promised
-        token = part * kPart + (drawn != 0x7fffffff ? drawn : max(last_with_mass, 0));
+        token = part * kPart + (drawn >= 0 ? drawn : last);
     }
     if (threadIdx.x == 0) a.out_tokens[s.first + s.count - 1] = token;
 }
