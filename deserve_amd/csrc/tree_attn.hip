@@ -267,6 +267,8 @@ extern "C" int dskv_tree_attn(const dskv_tree_step_t *s, void *out, const void *
         a.part_ml = a.part_o + slots_of(f, s->n_kv_heads) * s->head_dim;
         a.n_shares = f.shares;
         a.group = s->n_qo_heads / s->n_kv_heads;
+        a.page_shift = 31 + ilog2(s->page_size);
+        a.page_magic = (uint32_t)(((1ull << a.page_shift) + s->page_size - 1) / s->page_size);
         if (s->dtype == DSKV_F32) return launch_tree_dim<DSKV_F32>(a, f, st);
         if (s->dtype == DSKV_F16) return launch_tree_dim<DSKV_F16>(a, f, st);
         return launch_tree_dim<DSKV_BF16>(a, f, st);

@@ -29,7 +29,9 @@ struct TreeArgs {
     long q_stride, n_page_indices;        // q_stride in bytes
     int batch, nnz, max_rows, n_qo_heads, n_kv_heads, head_dim, page_size, num_pages;
     float scale;                          // sm_scale / log 2
-    // matrix form
+    // matrix forms
+    uint32_t page_magic;                  // ceil(2^page_shift / page_size): t / page_size = t * page_magic >> page_shift
+    int page_shift;
     float *part_o, *part_ml;              // (2 * n_shares, n_kv_heads, columns of a tile, head_dim | 2)
     int64_t *units_before;                // (batch + 1): units of the requests in front
     int n_shares, group;
@@ -166,17 +168,24 @@ __device__ __forceinline__ TreePlace tree_place(const TreeArgs &a, long share, i
     return at;
 }
 
-// Row of the pool (page * 2 P + place) of token t of a request, -1 if there is none.  K half; V lies P rows on.
-__device__ __forceinline__ int pool_row(const TreeArgs &a, const TreeRequest &r, long t, int &entry_id)
+// t / page_size for 0 <= t < 2^31: with s = 31 + ceil(log2 P) and M = ceil(2^s / P) < 2^32 the error of t M / 2^s is under
+// t / 2^s <= 1 / P.
+__device__ __forceinline__ int page_number(const TreeArgs &a, int t)
 {
-    const int page = entry_id;
-    return t < r.kv_len && page >= 0 && page < a.num_pages ? page * 2 * a.page_size + (int)(t % a.page_size) : -1;
+    return (int)((uint64_t)(uint32_t)t * a.page_magic >> a.page_shift);
 }
-__device__ __forceinline__ int page_of(const TreeArgs &a, const TreeRequest &r, long t)
+// Page of token t of a request, and its row of the pool (page * 2 P + place: K; V lies P rows on), -1 where there is none.
+__device__ __forceinline__ int page_of(const TreeArgs &a, const TreeRequest &r, int t)
 {
-    const long entry = r.page0 + t / a.page_size;
-    return t < r.kv_len && entry >= 0 && entry < a.n_page_indices ? a.kv_page_indices[entry] : -1;
+    const int entry = r.page0 + page_number(a, t);
+    return t < (int)r.kv_len && entry >= 0 && entry < (int)a.n_page_indices ? a.kv_page_indices[entry] : -1;
 }
+__device__ __forceinline__ int pool_row(const TreeArgs &a, int t, int page)
+{
+    return page >= 0 && page < a.num_pages ? page * 2 * a.page_size + t - page_number(a, t) * a.page_size : -1;
+}
+
+static __device__ const u32x4 kNoRow[32] = {};          // what a token that there is not reads as
 
 template <int DT, int kD, int kBlocks> struct TreeRegs {
     typedef TreeShape<DT, kD, kBlocks> S;
@@ -200,9 +209,11 @@ __global__ __launch_bounds__(kTreeThreads, kBlocks <= 2 ? 2 : 1) void tree_matri
     int b = place.b;
 
     char *const k_lds = lds + wave * S::kWaveLds, *const v_lds = k_lds + S::kSub * S::kKPitch;
-    const long row_bytes = (long)a.n_kv_heads * S::kRow;
+    const int row_bytes = a.n_kv_heads * S::kRow;
+    const long half_bytes = (long)a.page_size * row_bytes;
     const int load_row = lane / S::kChunks, load_chunk = lane % S::kChunks;
     const char *const pool = a.pages + head * S::kRow + load_chunk * 16;
+    const char *const none = reinterpret_cast<const char *>(kNoRow) + load_chunk * 16;
 
     while (unit < end) {
         const TreeRequest r = tree_request<S::kCols, S::kSub>(a, b);
@@ -216,8 +227,8 @@ __global__ __launch_bounds__(kTreeThreads, kBlocks <= 2 ? 2 : 1) void tree_matri
         const long item = base + (long)ct * r.subtiles;       // the item's first unit
         const int st0 = (int)(unit - item), st1 = (int)min(end - item, (long)r.subtiles);
         const int cols = min(r.n * a.group - ct * S::kCols, S::kCols);
-        const long prior = r.prior;
-        const int new_from = (int)(max(prior, 0L) / S::kSub);       // first subtile with new rows
+        const int prior = (int)max(r.prior, (long)-INT32_MAX);
+        const int new_from = max(prior, 0) / S::kSub;       // first subtile with new rows
 
         // ---- columns: q and what they see
         u32x4 q[kBlocks][S::kSteps];
@@ -236,7 +247,7 @@ __global__ __launch_bounds__(kTreeThreads, kBlocks <= 2 ? 2 : 1) void tree_matri
             }
             mask[k] = !a.masks ? ~0ull : there ? (unsigned long long)a.masks[r.first + i] : 0;
             // tokens from `limit` on are not seen whatever the mask says
-            const long lim = a.masks ? min(r.kv_len, prior + DSKV_MAX_TREE_ROWS) : min(r.kv_len, prior + i + 1);
+            const long lim = min(r.kv_len, (long)prior + (a.masks ? DSKV_MAX_TREE_ROWS : i + 1));
             limit[k] = there ? (int)max(lim, 0L) : 0;
         }
 
@@ -252,18 +263,19 @@ __global__ __launch_bounds__(kTreeThreads, kBlocks <= 2 ? 2 : 1) void tree_matri
 
         // ---- the wave's subtiles, one ahead in registers, the page ids another one ahead
         TreeRegs<DT, kD, kBlocks> next;
-        auto id_of = [&](int st) { return page_of(a, r, (long)st * S::kSub + (lane & (S::kSub - 1))); };
-        auto row_of = [&](int st, int id) { return pool_row(a, r, (long)st * S::kSub + (lane & (S::kSub - 1)), id); };
+        auto id_of = [&](int st) { return page_of(a, r, st * S::kSub + (lane & (S::kSub - 1))); };
+        auto row_of = [&](int st, int id) { return pool_row(a, st * S::kSub + (lane & (S::kSub - 1)), id); };
         auto request = [&](int rows) {
+            int row[S::kLoads];
+#pragma unroll
+            for (int i = 0; i < S::kLoads; i++) row[i] = __shfl(rows, load_row + S::kRowsPerLoad * i);
 #pragma unroll
             for (int i = 0; i < S::kLoads; i++) {
-                const int row = __shfl(rows, load_row + S::kRowsPerLoad * i);
-                next.k[i] = next.v[i] = u32x4{0, 0, 0, 0};
-                if (row >= 0) {
-                    const char *p = pool + (unsigned long)(unsigned)row * row_bytes;
-                    next.k[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p));
-                    next.v[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p + a.page_size * row_bytes));
-                }
+                const char *k = pool + (uint64_t)(uint32_t)row[i] * (uint32_t)row_bytes, *v = k + half_bytes;
+                k = row[i] >= 0 ? k : none;
+                v = row[i] >= 0 ? v : none;
+                next.k[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(k));
+                next.v[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(v));
             }
         };
         int rows_now = -1, id_next = -1;
@@ -272,6 +284,13 @@ __global__ __launch_bounds__(kTreeThreads, kBlocks <= 2 ? 2 : 1) void tree_matri
             request(rows_now);
         }
         if (st0 + wave + kTreeWaves < st1) id_next = id_of(st0 + wave + kTreeWaves);
+        // q and the masks are waited for here, in front of the loop
+#pragma unroll
+        for (int k = 0; k < kBlocks; k++) {
+#pragma unroll
+            for (int s = 0; s < S::kSteps; s++) asm volatile("" : "+v"(q[k][s]));
+            asm volatile("" : "+v"(mask[k]));
+        }
         for (int st = st0 + wave; st < st1; st += kTreeWaves) {
             const int t0 = st * S::kSub;
             const unsigned long long held = __ballot(rows_now >= 0);       // tokens that there are (lanes repeat)
@@ -340,8 +359,7 @@ __global__ __launch_bounds__(kTreeThreads, kBlocks <= 2 ? 2 : 1) void tree_matri
             // ---- weights
             u32x4 p[kBlocks];                                  // 16-bit: the operand; fp32: four floats
             auto sees = [&](int k, int token) {                // token of the subtile
-                const long at = t0 + token;
-                const long j = at - prior;
+                const int at = t0 + token, j = at - prior;
                 return at < limit[k] && ((held >> token) & 1) && (j < 0 || ((mask[k] >> (j & 63)) & 1));
             };
 #pragma unroll
@@ -411,12 +429,11 @@ __global__ __launch_bounds__(kTreeThreads, kBlocks <= 2 ? 2 : 1) void tree_matri
             while (__builtin_expect(bad != 0, 0)) {
                 const int token = __builtin_ctz(bad);
                 bad &= bad - 1;
-                const long t = (long)st * S::kSub + token;
-                int id = page_of(a, r, t);
-                const int row = pool_row(a, r, t, id);
+                const int t = st * S::kSub + token;
+                const int row = pool_row(a, t, page_of(a, r, t));
                 if (row < 0) continue;
-                const char *key = a.pages + (unsigned long)(unsigned)row * row_bytes + head * S::kRow;
-                const char *value = key + a.page_size * row_bytes;
+                const char *key = a.pages + (uint64_t)(uint32_t)row * (uint32_t)row_bytes + head * S::kRow;
+                const char *value = key + half_bytes;
 #pragma unroll
                 for (int k = 0; k < kBlocks; k++) {
                     float s = 0;

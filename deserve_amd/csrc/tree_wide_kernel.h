@@ -23,8 +23,6 @@ constexpr int kWideLeast = 8;               // units a share has at least: what 
 constexpr float kMostWeight = 256.f;
 constexpr int kBadBlocks = kTreeMostRows / kWideBlock + 2;       // that new rows reach into
 
-static __device__ const u32x4 kNoRow[16] = {};          // what a token that there is not reads as
-
 template <int kWaves> struct WideShape {
     static constexpr int kThreads = kWaves * 64;
     static constexpr int kCols = kWaves * 32;
@@ -118,8 +116,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
                 const int t = (st0 + x * W::kHalf) * kWideBlock + i;
                 int row = -1;
                 if (t < t_end) {
-                    int id = page_of(a, r, t);
-                    row = pool_row(a, r, t, id);
+                    row = pool_row(a, t, page_of(a, r, t));
                     if (row < 0) holes = 1;
                 }
                 const int at = (x & 1) * W::kHalf * kWideBlock + i;
@@ -349,8 +346,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
                 const int token = __builtin_ctz(bad);
                 bad &= bad - 1;
                 const int t = (st0 + j) * kWideBlock + token;
-                int id = page_of(a, r, t);
-                const int row = pool_row(a, r, t, id);
+                const int row = pool_row(a, t, page_of(a, r, t));
                 if (row < 0) continue;
                 const char *key = a.pages + (unsigned long)(unsigned)row * (unsigned)row_bytes + head * 256;
                 float s = 0;
