@@ -136,30 +136,30 @@ __global__ __launch_bounds__(kGenericWaves * 64) void tree_generic_kernel(TreeAr
 }
 
 // How a step is computed.  wide_waves > 0: tree_wide_kernel.h with so many waves; else the matrix form of tree_kernel.h with
-// tiles of `blocks` * 16 columns: few tiles, each as narrow as it can be.
+// tiles of `blocks` * 16 columns, up to tree_columns: few tiles, each as narrow as it can be.
 struct TreeForm {
     int wide_waves, blocks, cols, col_tiles, shares, least;
 };
 static bool matrix_form(int head_dim) { return head_dim == 64 || head_dim == 128; }
-static TreeForm tree_form(bool wide, int max_rows, int n_qo_heads, int n_kv_heads)
+static TreeForm tree_form(bool wide, int max_rows, int n_qo_heads, int n_kv_heads, int head_dim)
 {
     TreeForm f;
     const long cols = (long)max_rows * (n_qo_heads / n_kv_heads);
     f.wide_waves = !wide ? 0 : cols <= 128 ? 4 : 8;
-    const int widest = wide ? f.wide_waves * 32 : 64;
+    const int widest = wide ? f.wide_waves * 32 : tree_columns(head_dim);
     f.col_tiles = (int)((cols + widest - 1) / widest);
     f.blocks = wide ? 0 : (int)((cols + 16L * f.col_tiles - 1) / (16L * f.col_tiles));
     f.cols = wide ? widest : f.blocks * 16;
     f.least = wide ? kWideLeast : kTreeWaves;
     // two workgroups a compute unit where their registers and LDS allow it
-    const int resident = kTreeUnits * ((wide ? f.wide_waves == 4 : f.blocks <= 2) ? 2 : 1);
+    const int resident = kTreeUnits * (wide ? (f.wide_waves == 4 ? 2 : 1) : tree_workgroups(head_dim, f.blocks));
     f.shares = resident >= n_kv_heads ? resident / n_kv_heads : 1;
     if (f.shares > 8) f.shares = f.shares / 8 * 8;         // (see share_and_head)
     return f;
 }
 static bool wide_form(int max_rows, int n_qo_heads, int n_kv_heads, int head_dim, int dtype)
 {
-    return head_dim == 128 && dtype != DSKV_F32 && (long)max_rows * (n_qo_heads / n_kv_heads) > 64;
+    return head_dim == 128 && dtype != DSKV_F32 && (long)max_rows * (n_qo_heads / n_kv_heads) > tree_columns(head_dim);
 }
 static int64_t units_bytes(int batch) { return ((int64_t)batch + 2) / 2 * 16; }
 static int64_t slots_of(const TreeForm &f, int n_kv_heads) { return 2LL * f.shares * n_kv_heads * f.cols; }
@@ -203,7 +203,10 @@ template <int DT, int kD> static int launch_tree_blocks(const TreeArgs &a, const
     case 1: return launch_tree<DT, kD, 1>(a, f, stream);
     case 2: return launch_tree<DT, kD, 2>(a, f, stream);
     case 3: return launch_tree<DT, kD, 3>(a, f, stream);
-    default: return launch_tree<DT, kD, 4>(a, f, stream);
+    default:
+        if constexpr (tree_columns(kD) >= 64) return launch_tree<DT, kD, 4>(a, f, stream);
+        set_error("tree_attn: no form for %d columns", f.cols);
+        return DSKV_E_INVAL;
     }
 }
 template <int DT> static int launch_tree_dim(const TreeArgs &a, const TreeForm &f, hipStream_t stream)
@@ -218,9 +221,9 @@ extern "C" int64_t dskv_tree_attn_workspace(int32_t batch, int32_t nnz, int32_t 
 {
     using namespace dskv;
     if (batch <= 0 || nnz <= 0 || max_qo_len <= 0 || n_kv_heads <= 0 || n_qo_heads < n_kv_heads || !matrix_form(head_dim)) return 0;
-    const int64_t narrow = form_bytes(tree_form(false, max_qo_len, n_qo_heads, n_kv_heads), batch, n_kv_heads, head_dim);
+    const int64_t narrow = form_bytes(tree_form(false, max_qo_len, n_qo_heads, n_kv_heads, head_dim), batch, n_kv_heads, head_dim);
     if (!wide_form(max_qo_len, n_qo_heads, n_kv_heads, head_dim, dtype)) return narrow;
-    const int64_t wide = form_bytes(tree_form(true, max_qo_len, n_qo_heads, n_kv_heads), batch, n_kv_heads, head_dim);
+    const int64_t wide = form_bytes(tree_form(true, max_qo_len, n_qo_heads, n_kv_heads, head_dim), batch, n_kv_heads, head_dim);
     return narrow > wide ? narrow : wide;
 }
 
@@ -254,7 +257,7 @@ extern "C" int dskv_tree_attn(const dskv_tree_step_t *s, void *out, const void *
     if (matrix_form(s->head_dim) && (int64_t)s->num_pages * 2 * s->page_size < INT32_MAX &&
         s->n_page_indices < (1 << 30) / s->page_size && s->max_qo_len <= kTreeMostRows) {
         const TreeForm f = tree_form(s->sm_scale > 0 && wide_form(s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->head_dim, s->dtype),
-                                     s->max_qo_len, s->n_qo_heads, s->n_kv_heads);
+                                     s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->head_dim);
         const int64_t need = dskv_tree_attn_workspace(s->batch, s->nnz, s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->head_dim, s->dtype);
         if (!s->workspace || s->workspace_bytes < need) {
             set_error("tree_attn: workspace of %lld bytes, %lld are needed", (long long)s->workspace_bytes, (long long)need);

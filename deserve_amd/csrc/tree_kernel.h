@@ -19,6 +19,8 @@ namespace dskv {
 
 constexpr int kTreeWaves = 4;
 constexpr int kTreeThreads = kTreeWaves * 64;
+// The running maximum of a column is raised only when a subtile's (block's) weights under it sum to more than this in a lane.
+constexpr float kMostWeight = 256.f;
 constexpr int kTreeMostRows = 1024;         // of a request in the matrix forms; longer chunks are a prefill's
 
 struct TreeArgs {
@@ -36,6 +38,14 @@ struct TreeArgs {
     int64_t *units_before;                // (batch + 1): units of the requests in front
     int n_shares, group;
 };
+
+// Workgroups a compute unit: two where the registers allow it.
+constexpr int tree_workgroups(int dim, int blocks) { return dim == 64 && blocks <= 2 ? 2 : 1; }
+
+// Columns of a tile at most: what a wave's registers hold beside the K and V on their way.
+constexpr int tree_columns(int dim) { return dim == 64 ? 64 : 48; }
+// Subtiles a wave has in flight, in registers: two where there is room for them.
+constexpr int tree_depth(int dim, int blocks) { return dim == 64 || blocks <= 2 ? 2 : 1; }
 
 template <int DT, int kD, int kBlocks> struct TreeShape {
     static constexpr int kElt = DT == DSKV_F32 ? 4 : 2;
@@ -70,19 +80,21 @@ struct TreeRequest {
 // What the arrays say about request b, within the bounds of the tensors.
 template <int kCols, int kSub> __device__ __forceinline__ TreeRequest tree_request(const TreeArgs &a, int b)
 {
+    // (through the constant address space: scalar loads where b is uniform, also after the kernel has stored)
+    const const_i32_ptr qo = as_const(a.qo_indptr) + b, kv = as_const(a.kv_page_indptr) + b;
     TreeRequest r;
-    r.first = a.qo_indptr[b];
-    const long rows = (long)a.qo_indptr[b + 1] - r.first;
-    r.page0 = a.kv_page_indptr[b];
-    r.pages = a.kv_page_indptr[b + 1] - r.page0;
-    const int last = a.kv_last_page_lens[b];
+    r.first = qo[0];
+    const long rows = (long)qo[1] - r.first;
+    r.page0 = kv[0];
+    r.pages = kv[1] - r.page0;
+    const int last = as_const(a.kv_last_page_lens)[b];
     r.kv_len = r.pages > 0 ? max((long)(r.pages - 1) * a.page_size + min(last, a.page_size), 0L) : 0;
     r.n = r.first < 0 ? 0 : (int)max(min(min(rows, (long)a.max_rows), (long)a.nnz - r.first), 0L);
     r.prior = r.kv_len - rows;
     r.kv_len = max(min(r.kv_len, r.prior + (a.masks ? DSKV_MAX_TREE_ROWS : r.n)), 0L);
     r.col_tiles = (r.n * a.group + kCols - 1) / kCols;
     r.tile = kCols;
-    if (kCols > 64 && r.col_tiles > 1) r.tile = (r.n * a.group + 32 * r.col_tiles - 1) / (32 * r.col_tiles) * 32;
+    if (kCols > tree_columns(64) && r.col_tiles > 1) r.tile = (r.n * a.group + 32 * r.col_tiles - 1) / (32 * r.col_tiles) * 32;
     r.subtiles = max((int)((r.kv_len + kSub - 1) / kSub), 1);        // a row that sees nothing is written too
     return r;
 }
@@ -186,27 +198,76 @@ __device__ __forceinline__ int pool_row(const TreeArgs &a, int t, int page)
 }
 
 static __device__ const u32x4 kNoRow[32] = {};          // what a token that there is not reads as
+// (a pointer that may be to it or to the pool would be loaded from as a flat one, which waits for LDS, too)
+typedef const __attribute__((address_space(1))) u32x4 *global_chunk_ptr;
+
+// Which of the `count` <= 32 tokens from t on a column sees, as bits: `prior` tokens lie in front of the new ones, of which its
+// mask names some (all: no mask), and none from `limit` on.
+__device__ __forceinline__ uint32_t seen_bits(int t, int prior, int limit, unsigned long long mask, bool all)
+{
+    const int from = t - prior, left = limit - t;
+    uint32_t bits;
+    if (all || from <= -32) bits = ~0u;
+    else if (from >= 0) bits = from < 64 ? (uint32_t)(mask >> from) : 0u;
+    else bits = (uint32_t)(mask << -from) | ((1u << -from) - 1);
+    return left <= 0 ? 0u : left >= 32 ? bits : bits & ((1u << left) - 1);
+}
+
+// Whether some of 16 bytes of elements is infinite or no number: its exponent is all ones, and one more carries into the sign.
+template <int DT> __device__ __forceinline__ bool no_number(u32x4 x)
+{
+    constexpr uint32_t kExponent = DT == DSKV_F32 ? 0x7F800000u : DT == DSKV_BF16 ? 0x7F807F80u : 0x7C007C00u;
+    constexpr uint32_t kOne = DT == DSKV_F32 ? 0x00800000u : DT == DSKV_BF16 ? 0x00800080u : 0x04000400u;
+    constexpr uint32_t kSign = DT == DSKV_F32 ? 0x80000000u : 0x80008000u;
+    uint32_t any = 0;
+#pragma unroll
+    for (int w = 0; w < 4; w++) any |= (x[w] & kExponent) + kOne;
+    return (any & kSign) != 0;
+}
 
 template <int DT, int kD, int kBlocks> struct TreeRegs {
     typedef TreeShape<DT, kD, kBlocks> S;
     u32x4 k[S::kLoads], v[S::kLoads];
 };
 
+// A share's walk through its items; one item at a time.
+struct TreeItem {
+    TreeRequest r;
+    long base;           // units in front of request b
+    long next;           // the first unit behind the item's part
+    int b, ct, st0, st1; // column tile; subtiles of the part
+    bool first;          // of the share
+};
+template <int kCols, int kSub>
+__device__ __forceinline__ void open_item(const TreeArgs &a, long unit, long begin, long end, TreeItem &it)
+{
+    it.r = tree_request<kCols, kSub>(a, it.b);
+    while (unit >= it.base + it.r.units()) {                  // on to the next request that has rows
+        it.base += it.r.units();
+        it.b++;
+        it.r = tree_request<kCols, kSub>(a, it.b);
+    }
+    it.ct = (int)((unsigned)(unit - it.base) / (unsigned)it.r.subtiles);
+    const long item = it.base + (long)it.ct * it.r.subtiles;
+    it.st0 = (int)(unit - item);
+    it.st1 = (int)min(end - item, (long)it.r.subtiles);
+    it.next = item + it.st1;
+    it.first = unit == begin;
+}
+
 template <int DT, int kD, int kBlocks>
-__global__ __launch_bounds__(kTreeThreads, kBlocks <= 2 ? 2 : 1) void tree_matrix_kernel(TreeArgs a)
+__global__ __launch_bounds__(kTreeThreads, tree_workgroups(kD, kBlocks)) void tree_matrix_kernel(TreeArgs a)
 {
     typedef TreeShape<DT, kD, kBlocks> S;
     __shared__ __align__(16) char lds[S::kLds];
-    __shared__ unsigned bad_at[kTreeMostRows / S::kSub + 2];    // bit per token of a subtile with new rows: its V is no number
+    __shared__ unsigned bad_at[kTreeMostRows / S::kSub + 2 + 2 * kTreeWaves];    // bit per token of a subtile with new rows: its V is no number
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, c = lane & 15;
     int share, head;
     share_and_head(a, share, head);
-
-    TreePlace place = tree_place<S::kCols, S::kSub, kTreeThreads>(a, share, kTreeWaves);
+    const TreePlace place = tree_place<S::kCols, S::kSub, kTreeThreads>(a, share, kTreeWaves);
     const long begin = place.begin, end = place.end;
-    long unit = begin, base = place.base;
-    int b = place.b;
+    if (begin >= end) return;
 
     char *const k_lds = lds + wave * S::kWaveLds, *const v_lds = k_lds + S::kSub * S::kKPitch;
     const int row_bytes = a.n_kv_heads * S::kRow;
@@ -215,75 +276,102 @@ __global__ __launch_bounds__(kTreeThreads, kBlocks <= 2 ? 2 : 1) void tree_matri
     const char *const pool = a.pages + head * S::kRow + load_chunk * 16;
     const char *const none = reinterpret_cast<const char *>(kNoRow) + load_chunk * 16;
 
-    while (unit < end) {
-        const TreeRequest r = tree_request<S::kCols, S::kSub>(a, b);
-        const long r_units = r.units();
-        if (unit >= base + r_units) {                         // on to the next request that has rows
-            base += r_units;
-            b++;
-            continue;
-        }
-        const int ct = (int)((unit - base) / r.subtiles);
-        const long item = base + (long)ct * r.subtiles;       // the item's first unit
-        const int st0 = (int)(unit - item), st1 = (int)min(end - item, (long)r.subtiles);
-        const int cols = min(r.n * a.group - ct * S::kCols, S::kCols);
-        const int prior = (int)max(r.prior, (long)-INT32_MAX);
-        const int new_from = max(prior, 0) / S::kSub;       // first subtile with new rows
-
-        // ---- columns: q and what they see
-        u32x4 q[kBlocks][S::kSteps];
-        unsigned long long mask[kBlocks];
-        int limit[kBlocks];
-#pragma unroll
-        for (int k = 0; k < kBlocks; k++) {
-            const int col = ct * S::kCols + k * 16 + c;
-            const int i = col / a.group, hq = head * a.group + col - i * a.group;
-            const bool there = k * 16 + c < cols;
-            const char *row = a.q + (r.first + (there ? i : 0)) * a.q_stride + (there ? hq : 0) * S::kRow + g * 16;
-#pragma unroll
-            for (int s = 0; s < S::kSteps; s++) {
-                q[k][s] = u32x4{0, 0, 0, 0};
-                if (there) q[k][s] = *reinterpret_cast<const u32x4 *>(row + s * 64);
+    // ---- what is requested: the wave's subtiles through all items of the share, kDepth in flight, their page ids one step
+    // further ahead (a wave's loads return in order: an id that is requested in front of the rows before it does not wait for those)
+    TreeItem ahead;
+    ahead.b = place.b;
+    ahead.base = place.base;
+    open_item<S::kCols, S::kSub>(a, begin, begin, end, ahead);
+    // A wave takes a whole number of turns through its register sets per item, the last perhaps for subtiles that there are not: which set is
+    // whose turn is known at compile time then, and the waits for one leave the other on its way.
+    constexpr int kDepth = tree_depth(kD, kBlocks);
+    auto walk_end = [&](const TreeItem &x) {                    // of the wave's subtiles st0 + wave, + kTreeWaves ..
+        constexpr int kTurn = kDepth * kTreeWaves;
+        return x.st0 + wave + max((x.st1 - x.st0 - wave + kTurn - 1) / kTurn, 0) * kTurn;
+    };
+    int ahead_st = ahead.st0 + wave, ahead_end = walk_end(ahead);
+    bool more = true;
+    auto settle = [&]() {                                       // on to a subtile that there is
+        if (__builtin_expect(ahead_st < ahead_end, 1)) return;
+        while (more && ahead_st >= ahead_end) {
+            more = ahead.next < end;
+            if (more) {
+                open_item<S::kCols, S::kSub>(a, ahead.next, begin, end, ahead);
+                ahead_st = ahead.st0 + wave;
+                ahead_end = walk_end(ahead);
             }
-            mask[k] = !a.masks ? ~0ull : there ? (unsigned long long)a.masks[r.first + i] : 0;
-            // tokens from `limit` on are not seen whatever the mask says
-            const long lim = min(r.kv_len, (long)prior + (a.masks ? DSKV_MAX_TREE_ROWS : i + 1));
-            limit[k] = there ? (int)max(lim, 0L) : 0;
         }
+    };
+    struct Ids {
+        int page, t;
+    };
+    auto next_ids = [&]() {                                     // of the lane's token of the next subtile; moves on
+        settle();
+        Ids x;
+        x.t = ahead_st * S::kSub + (lane & (S::kSub - 1));
+        x.page = more && ahead_st < ahead.st1 ? page_of(a, ahead.r, x.t) : -1;
+        ahead_st += kTreeWaves;
+        return x;
+    };
+    TreeRegs<DT, kD, kBlocks> regs[kDepth];
+    unsigned long long held_of[kDepth];
+    auto request = [&](const Ids &x, TreeRegs<DT, kD, kBlocks> &to, unsigned long long &held) {
+        const int rows = pool_row(a, x.t, x.page);
+        held = __ballot(rows >= 0);                             // tokens that there are (lanes repeat)
+        int row[S::kLoads];
+#pragma unroll
+        for (int i = 0; i < S::kLoads; i++) row[i] = __shfl(rows, load_row + S::kRowsPerLoad * i);
+#pragma unroll
+        for (int i = 0; i < S::kLoads; i++) {
+            const char *k = pool + (uint64_t)(uint32_t)row[i] * (uint32_t)row_bytes, *v = k + half_bytes;
+            k = row[i] >= 0 ? k : none;
+            v = row[i] >= 0 ? v : none;
+            to.k[i] = __builtin_nontemporal_load((global_chunk_ptr)k);
+            to.v[i] = __builtin_nontemporal_load((global_chunk_ptr)v);
+        }
+    };
+    Ids ids = next_ids();
+#pragma unroll
+    for (int i = 0; i < kDepth; i++) {
+        const Ids ids_next = next_ids();
+        request(ids, regs[i], held_of[i]);
+        ids = ids_next;
+    }
 
-        f32x4 o[kBlocks][S::kDimTiles];
-        float m[kBlocks], l[kBlocks];
+    // ---- what is computed: one item after the other
+    TreeItem it;
+    it.b = place.b;
+    it.base = place.base;
+    int cols, prior, new_from, st;
+    u32x4 q[kBlocks][S::kSteps];
+    unsigned long long mask[kBlocks];
+    int limit[kBlocks];
+    f32x4 o[kBlocks][S::kDimTiles];
+    float m[kBlocks], l[kBlocks];
+    auto start_item = [&](long unit) {
+        open_item<S::kCols, S::kSub>(a, unit, begin, end, it);
+        cols = min(it.r.n * a.group - it.ct * S::kCols, S::kCols);
+        prior = (int)max(it.r.prior, (long)-INT32_MAX);
+        new_from = max(prior, 0) / S::kSub;                     // first subtile with new rows
+        st = it.st0 + wave;
 #pragma unroll
         for (int k = 0; k < kBlocks; k++) {
-            m[k] = -INFINITY;
+            const int col = it.ct * S::kCols + k * 16 + c;
+            const int i = (int)((unsigned)col / (unsigned)a.group), hq = head * a.group + col - i * a.group;
+            const bool there = k * 16 + c < cols;
+            const char *row = there ? a.q + (it.r.first + i) * a.q_stride + hq * S::kRow + g * 16
+                                    : reinterpret_cast<const char *>(kNoRow) + g * 16;
+#pragma unroll
+            for (int s = 0; s < S::kSteps; s++) q[k][s] = *(global_chunk_ptr)(row + s * 64);
+            mask[k] = !a.masks ? ~0ull : there ? (unsigned long long)a.masks[it.r.first + i] : 0;
+            // tokens from `limit` on are not seen whatever the mask says
+            const long lim = min(it.r.kv_len, (long)prior + (a.masks ? DSKV_MAX_TREE_ROWS : i + 1));
+            limit[k] = there ? (int)max(lim, 0L) : 0;
+            m[k] = -__FLT_MAX__;
             l[k] = 0;
 #pragma unroll
             for (int d = 0; d < S::kDimTiles; d++) o[k][d] = f32x4{0, 0, 0, 0};
         }
-
-        // ---- the wave's subtiles, one ahead in registers, the page ids another one ahead
-        TreeRegs<DT, kD, kBlocks> next;
-        auto id_of = [&](int st) { return page_of(a, r, st * S::kSub + (lane & (S::kSub - 1))); };
-        auto row_of = [&](int st, int id) { return pool_row(a, st * S::kSub + (lane & (S::kSub - 1)), id); };
-        auto request = [&](int rows) {
-            int row[S::kLoads];
-#pragma unroll
-            for (int i = 0; i < S::kLoads; i++) row[i] = __shfl(rows, load_row + S::kRowsPerLoad * i);
-#pragma unroll
-            for (int i = 0; i < S::kLoads; i++) {
-                const char *k = pool + (uint64_t)(uint32_t)row[i] * (uint32_t)row_bytes, *v = k + half_bytes;
-                k = row[i] >= 0 ? k : none;
-                v = row[i] >= 0 ? v : none;
-                next.k[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(k));
-                next.v[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(v));
-            }
-        };
-        int rows_now = -1, id_next = -1;
-        if (st0 + wave < st1) {
-            rows_now = row_of(st0 + wave, id_of(st0 + wave));
-            request(rows_now);
-        }
-        if (st0 + wave + kTreeWaves < st1) id_next = id_of(st0 + wave + kTreeWaves);
         // q and the masks are waited for here, in front of the loop
 #pragma unroll
         for (int k = 0; k < kBlocks; k++) {
@@ -291,146 +379,154 @@ __global__ __launch_bounds__(kTreeThreads, kBlocks <= 2 ? 2 : 1) void tree_matri
             for (int s = 0; s < S::kSteps; s++) asm volatile("" : "+v"(q[k][s]));
             asm volatile("" : "+v"(mask[k]));
         }
-        for (int st = st0 + wave; st < st1; st += kTreeWaves) {
-            const int t0 = st * S::kSub;
-            const unsigned long long held = __ballot(rows_now >= 0);       // tokens that there are (lanes repeat)
-            const bool whole = held == ~0ull && t0 + S::kSub <= prior + (a.masks ? 0 : 1);
-            __builtin_amdgcn_wave_barrier();
-            // A weight of 0 times a V that is no number would reach columns that do not see the token: such tokens among the
-            // new ones are taken out here and added behind the walk.
-            if (st >= new_from) {
-                unsigned bad = 0;
-#pragma unroll
-                for (int i = 0; i < S::kLoads; i++) {
-                    bool odd = false;
-#pragma unroll
-                    for (int w = 0; w < 4; w++) {
-                        const uint32_t x = next.v[i][w];
-                        if (DT == DSKV_F32) odd |= (x & 0x7F800000u) == 0x7F800000u;
-                        else if (DT == DSKV_BF16) odd |= (x & 0x7F80u) == 0x7F80u || (x & 0x7F800000u) == 0x7F800000u;
-                        else odd |= (x & 0x7C00u) == 0x7C00u || (x & 0x7C000000u) == 0x7C000000u;
-                    }
-                    const unsigned long long odd_lanes = __ballot(odd);
-#pragma unroll
-                    for (int j = 0; j < S::kRowsPerLoad; j++) {
-                        const unsigned long long of_row = (S::kChunks == 64 ? ~0ull : (1ull << S::kChunks) - 1) << (j * S::kChunks);
-                        if (odd_lanes & of_row) bad |= 1u << (j + S::kRowsPerLoad * i);
-                    }
-                    if ((bad >> (load_row + S::kRowsPerLoad * i)) & 1) next.v[i] = u32x4{0, 0, 0, 0};
-                }
-                if (lane == 0) bad_at[st - new_from] = bad;
-            }
+    };
+    auto subtile = [&](TreeRegs<DT, kD, kBlocks> &mine, unsigned long long &held_here) {
+        const unsigned long long held = held_here;
+        const bool whole = held == ~0ull && (st + 1) * S::kSub <= prior + (a.masks ? 0 : 1);
+        __builtin_amdgcn_wave_barrier();
+        // A weight of 0 times a V that is no number would reach columns that do not see the token: such tokens among the
+        // new ones are taken out here and added behind the walk.
+        if (st >= new_from) {
+            unsigned bad = 0;
+            bool odd[S::kLoads], any = false;
 #pragma unroll
             for (int i = 0; i < S::kLoads; i++) {
-                const int row = load_row + S::kRowsPerLoad * i;
-                *reinterpret_cast<u32x4 *>(k_lds + row * S::kKPitch + load_chunk * 16) = next.k[i];
-                *reinterpret_cast<u32x4 *>(v_lds + row * S::kVPitch + load_chunk * 16) = next.v[i];
+                odd[i] = no_number<DT>(mine.v[i]);
+                any |= odd[i];
             }
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            if (st + kTreeWaves < st1) {
-                rows_now = row_of(st + kTreeWaves, id_next);
-                request(rows_now);
-                if (st + 2 * kTreeWaves < st1) id_next = id_of(st + 2 * kTreeWaves);
+            if (__builtin_expect(__ballot(any) != 0, 0)) {
+#pragma unroll
+                for (int i = 0; i < S::kLoads; i++) {
+                    const unsigned long long odd_lanes = __ballot(odd[i]);
+#pragma unroll
+                    for (int j = 0; j < S::kRowsPerLoad; j++) {
+                        const unsigned long long of_row = ((1ull << S::kChunks) - 1) << (j * S::kChunks);
+                        if (odd_lanes & of_row) bad |= 1u << (j + S::kRowsPerLoad * i);
+                    }
+                    if ((bad >> (load_row + S::kRowsPerLoad * i)) & 1) mine.v[i] = u32x4{0, 0, 0, 0};
+                }
             }
+            if (lane == 0) bad_at[st - new_from] = bad;
+        }
+#pragma unroll
+        for (int i = 0; i < S::kLoads; i++) {
+            const int row = load_row + S::kRowsPerLoad * i;
+            *reinterpret_cast<u32x4 *>(k_lds + row * S::kKPitch + load_chunk * 16) = mine.k[i];
+            *reinterpret_cast<u32x4 *>(v_lds + row * S::kVPitch + load_chunk * 16) = mine.v[i];
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const Ids ids_next = next_ids();
+        request(ids, mine, held_here);
+        ids = ids_next;
+        if (st >= it.st1) {                                     // a turn without a subtile
+            st += kTreeWaves;
+            return;
+        }
 
-            // ---- scores
-            f32x4 s[kBlocks][S::kTiles];
+        // ---- scores
+        f32x4 s[kBlocks][S::kTiles];
 #pragma unroll
-            for (int t = 0; t < S::kTiles; t++) {
+        for (int t = 0; t < S::kTiles; t++) {
 #pragma unroll
-                for (int k = 0; k < kBlocks; k++) s[k][t] = f32x4{0, 0, 0, 0};
+            for (int k = 0; k < kBlocks; k++) s[k][t] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                for (int e = 0; e < S::kSteps; e++) {
-                    const u32x4 key = *reinterpret_cast<const u32x4 *>(k_lds + (t * 16 + c) * S::kKPitch + e * 64 + g * 16);
+            for (int e = 0; e < S::kSteps; e++) {
+                const u32x4 key = *reinterpret_cast<const u32x4 *>(k_lds + (t * 16 + c) * S::kKPitch + e * 64 + g * 16);
 #pragma unroll
-                    for (int k = 0; k < kBlocks; k++) {
-                        if constexpr (DT == DSKV_F32) {
-                            const f32x4 kf = __builtin_bit_cast(f32x4, key), qf = __builtin_bit_cast(f32x4, q[k][e]);
+                for (int k = 0; k < kBlocks; k++) {
+                    if constexpr (DT == DSKV_F32) {
+                        const f32x4 kf = __builtin_bit_cast(f32x4, key), qf = __builtin_bit_cast(f32x4, q[k][e]);
 #pragma unroll
-                            for (int j = 0; j < 4; j++)
-                                s[k][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j], qf[j], s[k][t], 0, 0, 0);
-                        } else {
-                            s[k][t] = Elt<DT>::mfma_k32(key, q[k][e], s[k][t]);
-                        }
+                        for (int j = 0; j < 4; j++)
+                            s[k][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j], qf[j], s[k][t], 0, 0, 0);
+                    } else {
+                        s[k][t] = Elt<DT>::mfma_k32(key, q[k][e], s[k][t]);
                     }
                 }
             }
-            // ---- weights
-            u32x4 p[kBlocks];                                  // 16-bit: the operand; fp32: four floats
-            auto sees = [&](int k, int token) {                // token of the subtile
-                const int at = t0 + token, j = at - prior;
-                return at < limit[k] && ((held >> token) & 1) && (j < 0 || ((mask[k] >> (j & 63)) & 1));
-            };
+        }
+        // ---- weights, under a maximum that is raised only where they ask for it
+        u32x4 p[kBlocks];                                  // 16-bit: the operand; fp32: four floats
 #pragma unroll
-            for (int k = 0; k < kBlocks; k++) {
-                float x[S::kTiles * 4];
+        for (int k = 0; k < kBlocks; k++) {
+            float x[S::kTiles * 4], w[S::kTiles * 4];
+#pragma unroll
+            for (int t = 0; t < S::kTiles; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[t * 4 + e] = s[k][t][e] * a.scale;
+            if (!whole) {
+                const uint32_t bits = ((uint32_t)held & seen_bits(st * S::kSub, prior, limit[k], mask[k], !a.masks)) >> (4 * g);
 #pragma unroll
                 for (int t = 0; t < S::kTiles; t++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) x[t * 4 + e] = s[k][t][e] * a.scale;
-                if (!whole) {
+                    for (int e = 0; e < 4; e++)
+                        if (!((bits >> (t * 16 + e)) & 1)) x[t * 4 + e] = -INFINITY;
+            }
+            float sum = 0;
 #pragma unroll
-                    for (int t = 0; t < S::kTiles; t++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            if (!sees(k, t * 16 + 4 * g + e)) x[t * 4 + e] = -INFINITY;
-                }
+            for (int e = 0; e < S::kTiles * 4; e++) {
+                w[e] = __builtin_amdgcn_exp2f(x[e] - m[k]);
+                sum += w[e];
+            }
+            if (__builtin_expect(__ballot(sum > kMostWeight) != 0, 0)) {
                 float top = x[0];
 #pragma unroll
                 for (int e = 1; e < S::kTiles * 4; e++) top = fmaxf(top, x[e]);
                 top = fmaxf(m[k], quad_rows_max(top));
-                const float from = top == -INFINITY ? 0.f : top;
-                const float keep = __builtin_amdgcn_exp2f(m[k] - from);
+                const float keep = __builtin_amdgcn_exp2f(m[k] - top);
                 m[k] = top;
-                float sum = 0;
-#pragma unroll
-                for (int e = 0; e < S::kTiles * 4; e++) {
-                    x[e] = __builtin_amdgcn_exp2f(x[e] - from);
-                    sum += x[e];
-                }
-                l[k] = l[k] * keep + sum;
+                l[k] *= keep;
 #pragma unroll
                 for (int d = 0; d < S::kDimTiles; d++) o[k][d] *= keep;
-                if constexpr (DT == DSKV_F32) {
-                    p[k] = __builtin_bit_cast(u32x4, f32x4{x[0], x[1], x[2], x[3]});
-                } else {
-                    // rounded to 16 bits for the matrix product: half a step of each weight
+                sum = 0;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) p[k][e] = Elt<DT>::pack2(x[2 * e], x[2 * e + 1]);
+                for (int e = 0; e < S::kTiles * 4; e++) {
+                    w[e] = __builtin_amdgcn_exp2f(x[e] - top);
+                    sum += w[e];
                 }
             }
-            // ---- output
+            l[k] += sum;
+            if constexpr (DT == DSKV_F32) {
+                p[k] = __builtin_bit_cast(u32x4, f32x4{w[0], w[1], w[2], w[3]});
+            } else {
+                // rounded to 16 bits for the matrix product: half a step of each weight
 #pragma unroll
-            for (int d = 0; d < S::kDimTiles; d++) {
-                if constexpr (DT == DSKV_F32) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float value = *reinterpret_cast<const float *>(v_lds + (4 * g + e) * S::kVPitch + (d * 16 + c) * 4);
-#pragma unroll
-                        for (int k = 0; k < kBlocks; k++)
-                            o[k][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                                value, __builtin_bit_cast(f32x4, p[k])[e], o[k][d], 0, 0, 0);
-                    }
-                } else {
-                    const char *at = v_lds + (4 * g + (c >> 2)) * S::kVPitch + d * 32 + (c & 3) * 8;
-                    const u32x2 lo = read_transposed(at), hi = read_transposed(at + 16 * S::kVPitch);
-                    const u32x4 value = {lo.x, lo.y, hi.x, hi.y};
-#pragma unroll
-                    for (int k = 0; k < kBlocks; k++) o[k][d] = Elt<DT>::mfma_k32(value, p[k], o[k][d]);
-                }
+                for (int e = 0; e < 4; e++) p[k][e] = Elt<DT>::pack2(w[2 * e], w[2 * e + 1]);
             }
         }
-
+        // ---- output
+#pragma unroll
+        for (int d = 0; d < S::kDimTiles; d++) {
+            if constexpr (DT == DSKV_F32) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float value = *reinterpret_cast<const float *>(v_lds + (4 * g + e) * S::kVPitch + (d * 16 + c) * 4);
+#pragma unroll
+                    for (int k = 0; k < kBlocks; k++)
+                        o[k][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                            value, __builtin_bit_cast(f32x4, p[k])[e], o[k][d], 0, 0, 0);
+                }
+            } else {
+                const char *at = v_lds + (4 * g + (c >> 2)) * S::kVPitch + d * 32 + (c & 3) * 8;
+                const u32x2 lo = read_transposed(at), hi = read_transposed(at + 16 * S::kVPitch);
+                const u32x4 value = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+                for (int k = 0; k < kBlocks; k++) o[k][d] = Elt<DT>::mfma_k32(value, p[k], o[k][d]);
+            }
+        }
+        st += kTreeWaves;
+    };
+    auto finish_item = [&]() {
         // ---- the wave's tokens that were taken out, for the columns that see them
-        for (int st = st0 + wave; st < st1; st += kTreeWaves) {
+        for (st = it.st0 + wave; st < it.st1; st += kTreeWaves) {
             if (st < new_from) continue;
             unsigned bad = __builtin_amdgcn_readfirstlane(bad_at[st - new_from]);
             while (__builtin_expect(bad != 0, 0)) {
                 const int token = __builtin_ctz(bad);
                 bad &= bad - 1;
                 const int t = st * S::kSub + token;
-                const int row = pool_row(a, t, page_of(a, r, t));
+                const int row = pool_row(a, t, page_of(a, it.r, t));
                 if (row < 0) continue;
                 const char *key = a.pages + (uint64_t)(uint32_t)row * (uint32_t)row_bytes + head * S::kRow;
                 const char *value = key + half_bytes;
@@ -446,8 +542,8 @@ __global__ __launch_bounds__(kTreeThreads, kBlocks <= 2 ? 2 : 1) void tree_matri
 #pragma unroll
                         for (int d = 0; d < E; d++) s = fmaf(x[d], y[d], s);
                     }
-                    const float weight = __builtin_amdgcn_exp2f(quad_rows_sum(s) * a.scale - (m[k] == -INFINITY ? 0.f : m[k]));
-                    if (t < limit[k] && (t < prior || ((mask[k] >> ((t - prior) & 63)) & 1))) {
+                    const float weight = __builtin_amdgcn_exp2f(quad_rows_sum(s) * a.scale - m[k]);
+                    if ((seen_bits(st * S::kSub, prior, limit[k], mask[k], !a.masks) >> token) & 1) {
 #pragma unroll
                         for (int d = 0; d < S::kDimTiles; d++)
 #pragma unroll
@@ -475,21 +571,20 @@ __global__ __launch_bounds__(kTreeThreads, kBlocks <= 2 ? 2 : 1) void tree_matri
                 *reinterpret_cast<f32x4 *>(o_lds + col * S::kOPitch + d * 16 + 4 * g) = o[k][d];
         }
         __syncthreads();
-        const bool cut = st0 > 0 || st1 < r.subtiles;
-        const long slot = 2L * share + (unit > begin ? 1 : 0);
+        const bool cut = it.st0 > 0 || it.st1 < it.r.subtiles;
+        const long slot = 2L * share + (it.first ? 0 : 1);
         const long part = (slot * a.n_kv_heads + head) * S::kCols;
         constexpr int kQuads = kD / 4;
         for (int x = threadIdx.x; x < cols * kQuads; x += kTreeThreads) {
             const int col = x / kQuads, quad = x % kQuads;
-            float top = -INFINITY;
+            float top = ml_lds[col * 2];
 #pragma unroll
-            for (int w = 0; w < kTreeWaves; w++) top = fmaxf(top, ml_lds[(w * S::kCols + col) * 2]);
-            const float from = top == -INFINITY ? 0.f : top;
+            for (int w = 1; w < kTreeWaves; w++) top = fmaxf(top, ml_lds[(w * S::kCols + col) * 2]);
             float sum = 0;
             f32x4 acc = {0, 0, 0, 0};
 #pragma unroll
             for (int w = 0; w < kTreeWaves; w++) {
-                const float weight = __builtin_amdgcn_exp2f(ml_lds[(w * S::kCols + col) * 2] - from);
+                const float weight = __builtin_amdgcn_exp2f(ml_lds[(w * S::kCols + col) * 2] - top);
                 sum += ml_lds[(w * S::kCols + col) * 2 + 1] * weight;
                 acc += *reinterpret_cast<const f32x4 *>(o_lds + (w * S::kCols + col) * S::kOPitch + quad * 4) * weight;
             }
@@ -500,15 +595,24 @@ __global__ __launch_bounds__(kTreeThreads, kBlocks <= 2 ? 2 : 1) void tree_matri
                     a.part_ml[(part + col) * 2 + 1] = sum;
                 }
             } else {
-                const int at = ct * S::kCols + col, i = at / a.group, hq = head * a.group + at - i * a.group;
+                const int at = it.ct * S::kCols + col, i = (int)((unsigned)at / (unsigned)a.group), hq = head * a.group + at - i * a.group;
                 const float inv = sum == 0 ? 0.f : 1.f / sum;
-                char *dst = a.out + ((r.first + i) * a.n_qo_heads + hq) * S::kRow + quad * 4 * S::kElt;
+                char *dst = a.out + ((it.r.first + i) * a.n_qo_heads + hq) * S::kRow + quad * 4 * S::kElt;
                 if constexpr (DT == DSKV_F32) *reinterpret_cast<f32x4 *>(dst) = acc * inv;
                 else *reinterpret_cast<u32x2 *>(dst) = u32x2{Elt<DT>::pack2(acc.x * inv, acc.y * inv), Elt<DT>::pack2(acc.z * inv, acc.w * inv)};
             }
         }
         __syncthreads();
-        unit = item + st1;
+    };
+    start_item(begin);
+    for (;;) {
+        while (st < it.st1) {
+#pragma unroll
+            for (int i = 0; i < kDepth; i++) subtile(regs[i], held_of[i]);
+        }
+        finish_item();
+        if (it.next >= end) return;
+        start_item(it.next);
     }
 }
 

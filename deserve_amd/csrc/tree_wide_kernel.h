@@ -20,7 +20,6 @@ constexpr int kWideBlock = 32;
 constexpr int kWideRegion = 1088;           // four rows, chunk by chunk ((4 c + row) * 16), and 64 bytes of padding
 constexpr int kWideStage = kWideBlock / 4 * kWideRegion;
 constexpr int kWideLeast = 8;               // units a share has at least: what fills the stages takes about as long
-constexpr float kMostWeight = 256.f;
 constexpr int kBadBlocks = kTreeMostRows / kWideBlock + 2;       // that new rows reach into
 
 template <int kWaves> struct WideShape {
@@ -173,19 +172,9 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
 #pragma unroll
             for (int s = 0; s < 8; s++) x = E::mfma_32x32(key[s], q[s], x);
         };
-        // Bits of block j's tokens that the column sees.
-        auto seen_of = [&](int j, uint32_t held) {
-            const int t = (st0 + j) * kWideBlock, from = t - prior;         // its first token among the new ones
-            uint32_t bits;
-            if (from >= 0) bits = from < 64 ? (uint32_t)(mask >> from) : a.masks ? 0u : ~0u;
-            else if (from > -32) bits = (uint32_t)(mask << -from) | ((1u << -from) - 1);
-            else bits = ~0u;
-            if (!a.masks) bits = ~0u;
-            const int left = limit - t;
-            bits &= left <= 0 ? 0u : left >= 32 ? ~0u : (1u << left) - 1;
-            return bits & held;
-        };
-        auto seen = [&](int j) { return j < blocks ? seen_of(j, held_at[j & (2 * W::kHalf - 1)]) : 0u; };
+        // bits of block j's tokens that the column sees
+        auto seen_of = [&](int j) { return seen_bits((st0 + j) * kWideBlock, prior, limit, mask, !a.masks); };
+        auto seen = [&](int j) { return j < blocks ? seen_of(j) & held_at[j & (2 * W::kHalf - 1)] : 0u; };
         auto mask_scores = [&](int j, f32x16 &x) {
             asm volatile("" : "+v"(x));                 // keeps this a branch that most blocks do not take
             uint32_t bits = seen(j) >> (4 * h);
@@ -226,12 +215,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
             for (int i = 0; i < W::kGroups; i++) {
                 const int region = wave * W::kGroups + i;
                 u32x4 *at = reinterpret_cast<u32x4 *>(v_stage(j & kLast) + region * kWideRegion + lane * 16);
-                const u32x4 x = *at;
-                bool odd = false;
-#pragma unroll
-                for (int w = 0; w < 4; w++)
-                    odd |= DT == DSKV_BF16 ? (x[w] & 0x7F80u) == 0x7F80u || (x[w] & 0x7F800000u) == 0x7F800000u
-                                           : (x[w] & 0x7C00u) == 0x7C00u || (x[w] & 0x7C000000u) == 0x7C000000u;
+                const bool odd = no_number<DT>(*at);
                 const unsigned long long lanes = __ballot(odd);
                 if (__builtin_expect(lanes != 0, 0)) {
                     uint32_t rows = 0;
@@ -341,7 +325,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
         for (int j = new_from; j < new_to; j++) {
             uint32_t bad = bad_at[j - new_from];
             if (__builtin_expect(bad == 0, 1)) continue;
-            const uint32_t bits = seen_of(j, ~0u);
+            const uint32_t bits = seen_of(j);
             while (bad) {
                 const int token = __builtin_ctz(bad);
                 bad &= bad - 1;
