@@ -138,7 +138,7 @@ __global__ __launch_bounds__(kGenericWaves * 64) void tree_generic_kernel(TreeAr
 // How a step is computed.  wide_waves > 0: tree_wide_kernel.h with so many waves; else the matrix form of tree_kernel.h with
 // tiles of `blocks` * 16 columns, up to tree_columns: few tiles, each as narrow as it can be.
 struct TreeForm {
-    int wide_waves, blocks, cols, col_tiles, shares, least;
+    int wide_waves, blocks, cols, col_tiles, shares, least, sides;
 };
 static bool matrix_form(int head_dim) { return head_dim == 64 || head_dim == 128; }
 static TreeForm tree_form(bool wide, int max_rows, int n_qo_heads, int n_kv_heads, int head_dim)
@@ -155,13 +155,14 @@ static TreeForm tree_form(bool wide, int max_rows, int n_qo_heads, int n_kv_head
     const int resident = kTreeUnits * (wide ? (f.wide_waves == 4 ? 2 : 1) : tree_workgroups(head_dim, f.blocks));
     f.shares = resident >= n_kv_heads ? resident / n_kv_heads : 1;
     if (f.shares > 8) f.shares = f.shares / 8 * 8;         // (see share_and_head)
+    f.sides = wide && f.col_tiles > 1 && f.shares % (8 * f.col_tiles) == 0 ? f.col_tiles : 1;
     return f;
 }
 static bool wide_form(int max_rows, int n_qo_heads, int n_kv_heads, int head_dim, int dtype)
 {
     return head_dim == 128 && dtype != DSKV_F32 && (long)max_rows * (n_qo_heads / n_kv_heads) > tree_columns(head_dim);
 }
-static int64_t units_bytes(int batch) { return ((int64_t)batch + 2) / 2 * 16; }
+static int64_t units_bytes(int batch) { return ((int64_t)batch + 3) / 2 * 16; }
 static int64_t slots_of(const TreeForm &f, int n_kv_heads) { return 2LL * f.shares * n_kv_heads * f.cols; }
 static int64_t form_bytes(const TreeForm &f, int batch, int n_kv_heads, int head_dim)
 {
@@ -269,6 +270,7 @@ extern "C" int dskv_tree_attn(const dskv_tree_step_t *s, void *out, const void *
         a.part_o = (float *)((char *)s->workspace + units_bytes(s->batch));
         a.part_ml = a.part_o + slots_of(f, s->n_kv_heads) * s->head_dim;
         a.n_shares = f.shares;
+        a.sides = f.sides;
         a.group = s->n_qo_heads / s->n_kv_heads;
         a.page_shift = 31 + ilog2(s->page_size);
         a.page_magic = (uint32_t)(((1ull << a.page_shift) + s->page_size - 1) / s->page_size);

@@ -35,8 +35,9 @@ struct TreeArgs {
     uint32_t page_magic;                  // ceil(2^page_shift / page_size): t / page_size = t * page_magic >> page_shift
     int page_shift;
     float *part_o, *part_ml;              // (2 * n_shares, n_kv_heads, columns of a tile, head_dim | 2)
-    int64_t *units_before;                // (batch + 1): units of the requests in front
+    int64_t *units_before;                // (batch + 2): units of the requests in front, and side_by_side
     int n_shares, group;
+    int sides;                            // see side_by_side
 };
 
 // Workgroups a compute unit: two where the registers allow it.
@@ -74,7 +75,6 @@ struct TreeRequest {
     int n;               // rows that are computed
     int col_tiles, subtiles;
     int tile;            // columns of a tile: its tiles are as even as 32 columns a wave allow
-    __device__ __forceinline__ long units() const { return (long)col_tiles * subtiles; }
 };
 
 // What the arrays say about request b, within the bounds of the tensors.
@@ -116,10 +116,42 @@ __device__ __forceinline__ void share_and_head(const TreeArgs &a, int &share, in
     }
 }
 
-// Shares that are in use: none has fewer than `least` units, if there are as many.
-__device__ __forceinline__ long shares_of(const TreeArgs &a, long units, int least)
+// Column tiles side by side.  Where (nearly) all requests have a.sides column tiles, their workgroups walk the same
+// tokens at the same time, on one XCD: K and V then come from its L2 for all but one of them.  Units are subtiles there, and
+// share (x + 8 j) takes column tile j % sides of span x + 8 (j / sides).  (n_shares is a multiple of 8 * sides.)
+__device__ __forceinline__ int share_of_span(int span, int side, int sides) { return span % 8 + 8 * (span / 8 * sides + side); }
+__device__ __forceinline__ bool side_by_side(const TreeArgs &a, long units, long spans)
 {
-    return max(min((long)a.n_shares, (units + least - 1) / least), 1L);
+    // idle workgroups cost what they save beyond a quarter
+    return a.sides > 1 && 4 * a.sides * spans <= 5 * units;
+}
+__device__ __forceinline__ long units_of(const TreeRequest &r, bool beside)
+{
+    return beside ? (r.col_tiles > 0 ? r.subtiles : 0) : (long)r.col_tiles * r.subtiles;
+}
+
+// Shares (spans) that are in use: none has fewer than `least` units, if there are as many.
+__device__ __forceinline__ long shares_of(long n_shares, long units, int least)
+{
+    return max(min(n_shares, (units + least - 1) / least), 1L);
+}
+
+// Sums up to and with this lane's over a wave, by moves between lanes that do not go through LDS.
+template <int kCtrl, int kRows> __device__ __forceinline__ long lanes_below(long v)
+{
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, kCtrl, kRows, 0xf, true);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)((uint64_t)v >> 32), kCtrl, kRows, 0xf, true);
+    return (long)((uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ long wave_scan(long v)
+{
+    v += lanes_below<0x111, 0xf>(v);       // row_shr 1, 2, 4, 8 within 16 lanes
+    v += lanes_below<0x112, 0xf>(v);
+    v += lanes_below<0x114, 0xf>(v);
+    v += lanes_below<0x118, 0xf>(v);
+    v += lanes_below<0x142, 0xa>(v);       // the last lane of rows 0 and 2 to rows 1 and 3
+    v += lanes_below<0x143, 0xc>(v);       // lane 31 to rows 2 and 3
+    return v;
 }
 
 // Where the workgroup's share begins and ends, by all of its kThreads threads; the first workgroup leaves the
@@ -128,56 +160,101 @@ struct TreePlace {
     long begin, end;     // units; equal: nothing to do
     long base;           // units in front of request b
     int b;
+    bool beside;
+    int side;
+    TreeRequest r;       // request b
 };
-template <int kCols, int kSub, int kThreads>
-__device__ __forceinline__ TreePlace tree_place(const TreeArgs &a, long share, int least)
+template <int kCols, int kSub, int kThreads, bool kSides>
+__device__ __forceinline__ void tree_place(const TreeArgs &a, int share, int least, TreePlace &at)
 {
-    __shared__ long scan[kThreads / 64], found[2];
+    __shared__ long scan[2][kThreads / 64], found_base;
+    __shared__ int found_b;
+    __shared__ TreeRequest found_r;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int per = (a.batch + kThreads - 1) / kThreads;
     const int b0 = threadIdx.x * per, b1 = min(b0 + per, a.batch);
-    long mine = 0;
-    for (int b = b0; b < b1; b++) mine += tree_request<kCols, kSub>(a, b).units();
-    long upto = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const long x = __shfl_up(upto, o);
-        if (lane >= o) upto += x;
+    long mine[2] = {0, 0}, upto[2];        // units; with column tiles side by side
+    TreeRequest r;
+    for (int b = b0; b < b1; b++) {
+        r = tree_request<kCols, kSub>(a, b);
+        mine[0] += units_of(r, false);
+        if (kSides) mine[1] += units_of(r, true);
     }
-    if (lane == 63) scan[wave] = upto;
+    long total[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < (kSides ? 2 : 1); i++) {
+        upto[i] = wave_scan(mine[i]);
+        if (lane == 63) scan[i][wave] = upto[i];
+    }
     __syncthreads();
-    long units = 0;
 #pragma unroll
-    for (int w = 0; w < kThreads / 64; w++) {
-        if (w == wave) upto += units;
-        units += scan[w];
+    for (int i = 0; i < (kSides ? 2 : 1); i++)
+#pragma unroll
+        for (int w = 0; w < kThreads / 64; w++) {
+            if (w == wave) upto[i] += total[i];
+            total[i] += scan[i][w];
+        }
+    at.beside = kSides && side_by_side(a, total[0], total[1]);
+    const int which = kSides && at.beside ? 1 : 0;
+    const long units = which ? total[1] : total[0];
+    long span = share, spans = a.n_shares;
+    at.side = 0;
+    if (which) {
+        const int j = share / 8;
+        at.side = j % a.sides;
+        span = share % 8 + 8 * (j / a.sides);
+        spans = a.n_shares / a.sides;
     }
-    TreePlace at = {0, 0, 0, 0};
-    const long shares = shares_of(a, units, least);
-    if (share < shares) {
-        at.begin = share_begin(share, units, shares);
-        at.end = share_begin(share + 1, units, shares);
+    const long used = shares_of(spans, units, least);
+    at.begin = at.end = 0;
+    if (span < used && units > 0) {
+        at.begin = share_begin(span, units, used);
+        at.end = share_begin(span + 1, units, used);
     }
-    long before = upto - mine;
+    long before = (which ? upto[1] : upto[0]) - (which ? mine[1] : mine[0]);
     const bool tells = blockIdx.x == 0;
-    if (tells || (before <= at.begin && at.begin < upto)) {
+    if (tells || (before <= at.begin && at.begin < (which ? upto[1] : upto[0]))) {
         for (int b = b0; b < b1; b++) {
-            const long u = tree_request<kCols, kSub>(a, b).units();
+            if (per > 1) r = tree_request<kCols, kSub>(a, b);
+            const long u = units_of(r, which);
             if (tells) a.units_before[b] = before;
             if (before <= at.begin && at.begin < before + u) {
-                found[0] = b;
-                found[1] = before;
+                found_b = b;
+                found_base = before;
+                found_r = r;
             }
             before += u;
         }
-        if (tells && b1 == a.batch) a.units_before[a.batch] = units;
+        if (tells && b1 == a.batch) {
+            a.units_before[a.batch] = units;
+            a.units_before[a.batch + 1] = which;
+        }
     }
     __syncthreads();
-    if (at.begin < at.end) {
-        at.b = __builtin_amdgcn_readfirstlane((int)found[0]);
-        at.base = found[1];
-    }
-    return at;
+    at.b = __builtin_amdgcn_readfirstlane(found_b);
+    at.base = found_base;
+    at.r = found_r;
+}
+// (LDS words are vectors for the compiler: an index that is the same for all lanes is said to be)
+__device__ __forceinline__ long uniform(long x)
+{
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)x), hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)((uint64_t)x >> 32));
+    return (long)((uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ void make_uniform(TreePlace &at)
+{
+    at.begin = uniform(at.begin);
+    at.end = uniform(at.end);
+    at.base = uniform(at.base);
+    at.r.first = uniform(at.r.first);
+    at.r.kv_len = uniform(at.r.kv_len);
+    at.r.prior = uniform(at.r.prior);
+    at.r.page0 = __builtin_amdgcn_readfirstlane(at.r.page0);
+    at.r.pages = __builtin_amdgcn_readfirstlane(at.r.pages);
+    at.r.n = __builtin_amdgcn_readfirstlane(at.r.n);
+    at.r.col_tiles = __builtin_amdgcn_readfirstlane(at.r.col_tiles);
+    at.r.subtiles = __builtin_amdgcn_readfirstlane(at.r.subtiles);
+    at.r.tile = __builtin_amdgcn_readfirstlane(at.r.tile);
 }
 
 // t / page_size for 0 <= t < 2^31: with s = 31 + ceil(log2 P) and M = ceil(2^s / P) < 2^32 the error of t M / 2^s is under
@@ -241,9 +318,8 @@ struct TreeItem {
 template <int kCols, int kSub>
 __device__ __forceinline__ void open_item(const TreeArgs &a, long unit, long begin, long end, TreeItem &it)
 {
-    it.r = tree_request<kCols, kSub>(a, it.b);
-    while (unit >= it.base + it.r.units()) {                  // on to the next request that has rows
-        it.base += it.r.units();
+    while (unit >= it.base + units_of(it.r, false)) {         // on to the next request that has rows
+        it.base += units_of(it.r, false);
         it.b++;
         it.r = tree_request<kCols, kSub>(a, it.b);
     }
@@ -265,7 +341,9 @@ __global__ __launch_bounds__(kTreeThreads, tree_workgroups(kD, kBlocks)) void tr
     const int g = lane >> 4, c = lane & 15;
     int share, head;
     share_and_head(a, share, head);
-    const TreePlace place = tree_place<S::kCols, S::kSub, kTreeThreads>(a, share, kTreeWaves);
+    TreePlace place;
+    tree_place<S::kCols, S::kSub, kTreeThreads, false>(a, share, kTreeWaves, place);
+    make_uniform(place);
     const long begin = place.begin, end = place.end;
     if (begin >= end) return;
 
@@ -281,6 +359,7 @@ __global__ __launch_bounds__(kTreeThreads, tree_workgroups(kD, kBlocks)) void tr
     TreeItem ahead;
     ahead.b = place.b;
     ahead.base = place.base;
+    ahead.r = place.r;
     open_item<S::kCols, S::kSub>(a, begin, begin, end, ahead);
     // A wave takes a whole number of turns through its register sets per item, the last perhaps for subtiles that there are not: which set is
     // whose turn is known at compile time then, and the waits for one leave the other on its way.
@@ -342,6 +421,7 @@ __global__ __launch_bounds__(kTreeThreads, tree_workgroups(kD, kBlocks)) void tr
     TreeItem it;
     it.b = place.b;
     it.base = place.base;
+    it.r = place.r;
     int cols, prior, new_from, st;
     u32x4 q[kBlocks][S::kSteps];
     unsigned long long mask[kBlocks];
@@ -627,12 +707,13 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int max_col
     const int quad = threadIdx.x % kQuads, column = threadIdx.x / kQuads % kColumns, group = threadIdx.x / (kQuads * kColumns);
     const TreeRequest r = tree_request<kCols, kSub>(a, b);
     const long before = a.units_before[b], units = a.units_before[a.batch];
+    const bool beside = a.units_before[a.batch + 1] != 0;
     const int col = blockIdx.z * kColumns + column;
     const int cols = min(r.n * a.group - ct * r.tile, r.tile);
     if (ct >= r.col_tiles || (int)blockIdx.z * kColumns >= cols) return;
-    const long shares = shares_of(a, units, least);
+    const long shares = shares_of(beside ? a.n_shares / a.sides : a.n_shares, units, least);
     const bool there = col < cols;
-    const long first = before + (long)ct * r.subtiles, last = first + r.subtiles - 1;
+    const long first = before + (beside ? 0 : (long)ct * r.subtiles), last = first + r.subtiles - 1;
     const long s0 = ((first + 1) * shares + units - 1) / units - 1, s1 = ((last + 1) * shares + units - 1) / units - 1;
     if (s0 == s1) return;
     float top = -INFINITY, sum = 0;
@@ -652,7 +733,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int max_col
 #pragma unroll
             for (int i = 0; i < kAhead; i++) {
                 const long si = min(s + i * kGroups, s1);
-                const long slot = 2 * si + (si == s0 && share_begin(si, units, shares) < first ? 1 : 0);
+                const long slot = 2 * (beside ? share_of_span((int)si, ct, a.sides) : si) + (si == s0 && share_begin(si, units, shares) < first ? 1 : 0);
                 const long part = (slot * a.n_kv_heads + head) * kCols + col;
                 pm[i] = a.part_ml[part * 2];
                 pl[i] = a.part_ml[part * 2 + 1];

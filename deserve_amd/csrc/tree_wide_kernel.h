@@ -45,10 +45,14 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
     const int g = lane >> 4, c = lane & 15, h = lane >> 5, r32 = lane & 31;
     int share, head;
     share_and_head(a, share, head);
-    TreePlace place = tree_place<W::kCols, kWideBlock, W::kThreads>(a, share, kWideLeast);
+    TreePlace place;
+    tree_place<W::kCols, kWideBlock, W::kThreads, true>(a, share, kWideLeast, place);
+    make_uniform(place);
     const long begin = place.begin, end = place.end;
+    const bool beside = place.beside;
     long unit = begin, base = place.base;
     int b = place.b;
+    TreeRequest r = place.r;
 
     auto k_stage = [&](int i) { return lds + i * kWideStage; };
     auto v_stage = [&](int i) { return lds + (W::kStages + i) * kWideStage; };
@@ -60,15 +64,19 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
     const char *const none = reinterpret_cast<const char *>(kNoRow) + (lane >> 2) * 16;
 
     while (unit < end) {
-        const TreeRequest r = tree_request<W::kCols, kWideBlock>(a, b);
-        if (unit >= base + r.units()) {
-            base += r.units();
+        if (unit >= base + units_of(r, beside)) {             // on to the next request that has rows
+            base += units_of(r, beside);
             b++;
+            r = tree_request<W::kCols, kWideBlock>(a, b);
             continue;
         }
-        const int ct = (int)((unit - base) / r.subtiles);
-        const long item = base + (long)ct * r.subtiles;
+        const int ct = beside ? place.side : (int)((unsigned)(unit - base) / (unsigned)r.subtiles);
+        const long item = base + (beside ? 0 : (long)ct * r.subtiles);
         const int st0 = (int)(unit - item), st1 = (int)min(end - item, (long)r.subtiles);
+        if (ct >= r.col_tiles) {                              // (beside: a request of fewer column tiles)
+            unit = item + st1;
+            continue;
+        }
         const int blocks = st1 - st0;
         const int cols = min(r.n * a.group - ct * r.tile, r.tile);
         const int prior = (int)max(r.prior, (long)-INT32_MAX);
