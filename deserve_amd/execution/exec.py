@@ -15,10 +15,11 @@ from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
-from deserve_amd.draft_ops import BatchTreeWithPagedKVCacheWrapper
+from deserve_amd.draft_ops import (MAX_TREE_ROWS, BatchTreeWithPagedKVCacheWrapper, Verdict, move_accepted_rows,
+                                   verify_drafts)
 from deserve_amd.execution.result import BatchResult
 from deserve_amd.kvcache.paged.kvcache import PagedKVCache
-from deserve_amd.model.context.flash import FlashDecodeCtx, FlashPrefillCtx
+from deserve_amd.model.context.flash import FlashDecodeCtx, FlashPrefillCtx, FlashTreeCtx
 from deserve_amd.paged_ops import (BatchDecodeWithPagedKVCacheWrapper,
                                    BatchPrefillWithPagedKVCacheWrapper)
 from deserve_amd.task import TaskData
@@ -142,3 +143,85 @@ class BatchPrefill(BatchExec):
             result = self.layer_storage.forward(self.xs, self.prefill_ctx)
             self.prefill_ctx.prefill_wrapper.end_forward()
             return self.post_process(result, ignore_eos)
+
+
+@dataclass
+class BatchVerify(BatchExec):
+    """A step of drafted tokens: the rows of a task are its last token and the drafts behind it, task.seqlen of them.
+    prepare() and step() run on every stage; the last one makes probabilities of what step() returns and calls
+    verify(); accept() with its verdict, on every stage, leaves the cache of the accepted rows in the order of the
+    sequence and task.seqlen as what the step has advanced by, for task.step().  No counterpart in the reference."""
+    tokens: Optional[torch.Tensor] = None      # int32, one a row; for verify()
+    parents: Optional[torch.Tensor] = None     # int32, one a row, within the task (build_step_tables); None: chains
+    tree_ctx: Optional[FlashTreeCtx] = None
+
+    @classmethod
+    def merge(cls, execs: Sequence["BatchVerify"]) -> "BatchVerify":
+        whole = super().merge(execs)
+        if any(e.tokens is not None for e in execs):
+            if any(e.tokens is None for e in execs):
+                raise ValueError("some of the steps have tokens, some have none")
+            whole.tokens = torch.cat([e.tokens for e in execs])
+        if any(e.parents is not None for e in execs):      # a chain is the tree in which each row follows the one in front
+            whole.parents = torch.cat([e._parents() for e in execs])
+        return whole
+
+    def _parents(self) -> torch.Tensor:
+        if self.parents is not None:
+            return self.parents
+        return torch.cat([torch.arange(-1, n - 1, dtype=torch.int32) for n in self.seqlens()]).to(self.xs.device)
+
+    def split(self) -> List["BatchVerify"]:
+        out, pos = super().split(), 0
+        for part in out:
+            rows = slice(pos, pos + part.total_seqlen())
+            part.tokens = None if self.tokens is None else self.tokens[rows]
+            part.parents = None if self.parents is None else self.parents[rows]
+            pos = rows.stop
+        return out
+
+    def pop(self) -> "BatchVerify":
+        begin = self.total_seqlen() - self.task_datas[-1].seqlen
+        tail = super().pop()
+        if self.tokens is not None:
+            self.tokens, tail.tokens = self.tokens[:begin], self.tokens[begin:]
+        if self.parents is not None:
+            self.parents, tail.parents = self.parents[:begin], self.parents[begin:]
+        return tail
+
+    def prepare(self) -> None:
+        with torch.inference_mode():
+            wrapper = get_tree_wrapper(self.kvcaches[0].pool.main_device)
+            self.tree_ctx = FlashTreeCtx.init_and_plan(self.task_datas, self.kvcaches, wrapper, parents=self.parents,
+                                                       **self._shape_kwargs())
+
+    def step(self, ignore_eos: bool = False) -> BatchResult:
+        """The rows of the stage's result; nothing is sampled here."""
+        with torch.inference_mode():
+            assert self.tree_ctx is not None
+            result = self.layer_storage.forward(self.xs, self.tree_ctx)
+            self.tree_ctx.tree_wrapper.end_forward()
+            ids = [t.task_id for t in self.task_datas]
+            return BatchResult(result, ids, result, list(ids), [], {})
+
+    def verify(self, target_probs: torch.Tensor, uniforms: torch.Tensor,
+               draft_probs: Optional[torch.Tensor] = None) -> Verdict:
+        """draft_ops.verify_drafts over the rows of the step."""
+        with torch.inference_mode():
+            assert self.tree_ctx is not None and self.tokens is not None
+            if max(self.seqlens()) > MAX_TREE_ROWS:
+                raise ValueError(f"a task has at most {MAX_TREE_ROWS} rows to verify")
+            return verify_drafts(target_probs, self.tokens, uniforms, self.tree_ctx.indptr, parents=self.parents,
+                                 draft_probs=draft_probs)
+
+    def accept(self, verdict: Verdict) -> List[int]:
+        """Tokens given to each task; waits for the verdict."""
+        with torch.inference_mode():
+            assert self.tree_ctx is not None
+            ctx = self.tree_ctx
+            if self.parents is not None:                    # the rows of an accepted chain are in place
+                move_accepted_rows(ctx.page_pool.pages, ctx.tables.slots, ctx.indptr, verdict.path, verdict.counts)
+            counts = verdict.counts.tolist()
+            for task, n in zip(self.task_datas, counts):
+                task.seqlen = n
+            return counts

@@ -15,12 +15,14 @@ kept (``host`` dict) so the attention planner never reads back from the device.
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import Dict, List, Sequence
+from typing import Dict, List, Optional, Sequence
 
 import numpy as np
 import torch
 
 from deserve_amd import staging
+from deserve_amd.draft_ops import (MAX_TREE_ROWS, BatchTreeWithPagedKVCacheWrapper, StepTables,
+                                   build_step_tables)
 from deserve_amd.kvcache.paged.kvcache import PagedKVCache
 from deserve_amd.kvcache.paged.page_pool import GpuPagePool
 from deserve_amd.model.context.forward import PagedForwardCtx
@@ -215,8 +217,11 @@ class FlashPrefillCtx(FlashForwardCtx):
     rope_layer: int = field(default=-1, repr=False)   # that asked last
     rope_device: int = field(default=-1, repr=False)
 
+    def _new_rope_table(self, nnz: int, head_dim: int, theta: float) -> torch.Tensor:
+        return rope_table(self.indptr, self.offsets, nnz, head_dim, theta)
+
     def rope_table(self, nnz: int, head_dim: int, theta: float) -> torch.Tensor:
-        """The step's cosines and sines (paged_ops.rope_table), built for the first layer that asks:
+        """The step's cosines and sines (one row per token), built for the first layer that asks:
         anew in every pass over the layers, since the offsets may have been written in between, on
         every stream that asks, since nothing orders one behind the other, and in every capture, which
         must hold the launch."""
@@ -229,7 +234,7 @@ class FlashPrefillCtx(FlashForwardCtx):
         self.rope_layer = self.layer_id
         table = self.rope_tables.get(key)
         if table is None:
-            table = self.rope_tables[key] = rope_table(self.indptr, self.offsets, nnz, head_dim, theta)
+            table = self.rope_tables[key] = self._new_rope_table(nnz, head_dim, theta)
         return table
 
     @classmethod
@@ -264,3 +269,53 @@ class FlashPrefillCtx(FlashForwardCtx):
                    offsets=v["offsets"], indptr=v["indptr"], kv_page_indices=v["kv_page_indices"],
                    kv_page_indptr=v["kv_page_indptr"], kv_last_page_lens=v["kv_last_page_lens"],
                    host=host, prefill_wrapper=wrapper)
+
+
+@dataclass
+class FlashTreeCtx(FlashForwardCtx):
+    """A step of drafted tokens: a task's seqlen rows are its last token and the drafts behind it (draft_ops).  No
+    counterpart in the reference."""
+    tree_wrapper: BatchTreeWithPagedKVCacheWrapper = None   # type: ignore[assignment]
+    tables: StepTables = None                               # type: ignore[assignment]
+    rope_tables: Dict[tuple, torch.Tensor] = field(default_factory=dict, repr=False)
+    rope_layer: int = field(default=-1, repr=False)
+    rope_device: int = field(default=-1, repr=False)
+
+    rope_table = FlashPrefillCtx.rope_table
+
+    def _new_rope_table(self, nnz: int, head_dim: int, theta: float) -> torch.Tensor:
+        return self.tables.rope_table(head_dim, theta)
+
+    @classmethod
+    def init_and_plan(cls, task_datas: List[TaskData], kvcaches: List[PagedKVCache[GpuPagePool]],
+                      wrapper: BatchTreeWithPagedKVCacheWrapper, num_qo_heads: int, num_kv_heads: int,
+                      head_dim: int, page_size: int, parents: Optional[torch.Tensor] = None) -> "FlashTreeCtx":
+        """Extends the caches by the tasks' rows, uploads lengths and block-table rows in one block and builds the step's
+        tables on the GPU.  parents: as build_step_tables takes them."""
+        pool = kvcaches[0].pool
+        if any(c.pool is not pool for c in kvcaches):
+            raise ValueError("a step of drafted tokens runs over one pool")
+        max_tokens = sum(t.seqlen for t in task_datas)
+        if parents is not None and max(t.seqlen for t in task_datas) > MAX_TREE_ROWS:
+            raise ValueError(f"a tree has at most {MAX_TREE_ROWS} rows")
+        if parents is not None and parents.numel() != max_tokens:
+            raise ValueError(f"parents holds {parents.numel()} entries for {max_tokens} rows")
+        meta = build_host_metadata(task_datas, kvcaches)
+        batch, exposed = len(task_datas), np.diff(meta["kv_page_indptr"])
+        width = int(exposed.max())
+        block = staging.take(batch * (2 + width))
+        words = block.tensor.numpy()
+        words[:batch] = meta["offsets"]
+        words[batch: 2 * batch] = meta["seqlens"]
+        table = words[2 * batch: batch * (2 + width)].reshape(batch, width)
+        table[np.arange(width)[None, :] < exposed[:, None]] = meta["kv_page_indices"]
+        dev = staging.to_device(block, batch * (2 + width), pool.main_device)
+        kv_lens, qo_lens = dev[:batch], dev[batch: 2 * batch]
+        tables = build_step_tables(dev[2 * batch:].view(batch, width), kv_lens, qo_lens, page_size,
+                                   max_tokens=max_tokens, max_pages=int(exposed.sum()), parents=parents)
+        wrapper.begin_forward(*tables.csr, num_qo_heads, num_kv_heads, head_dim, page_size,
+                              max_qo_len=int(meta["seqlens"].max()), masks=tables.masks)
+        return cls(bsz=batch, seqlens=qo_lens, layer_id=0, page_pool=pool, offsets=kv_lens, indptr=tables.qo_indptr,
+                   kv_page_indices=tables.kv_page_indices, kv_page_indptr=tables.kv_page_indptr,
+                   kv_last_page_lens=tables.kv_last_page_lens, host={f: torch.from_numpy(meta[f]) for f in _FIELDS},
+                   tree_wrapper=wrapper, tables=tables)

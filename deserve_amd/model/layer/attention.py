@@ -9,8 +9,9 @@ from typing import Optional
 
 import torch
 
+from deserve_amd.draft_ops import rope_append_slots
 from deserve_amd.kvcache.paged.page_pool import PagePool
-from deserve_amd.model.context.flash import FlashDecodeCtx, FlashForwardCtx, FlashPrefillCtx
+from deserve_amd.model.context.flash import FlashDecodeCtx, FlashForwardCtx, FlashPrefillCtx, FlashTreeCtx
 from deserve_amd.paged_ops import (BatchDecodeWithPagedKVCacheWrapper, BatchPrefillWithPagedKVCacheWrapper,
                                    append_paged_kv_cache, apply_rope, rope_append_paged_kv_cache)
 
@@ -84,6 +85,11 @@ class PagedAttentionCore:
         xk = self._rows(xk, self.n_local_kv_heads)
         xv = self._rows(xv, self.n_local_kv_heads)
         pages = ctx.page_pool.get_layered_pages(ctx.layer_id)
+        if isinstance(ctx, FlashTreeCtx):
+            # the rows' slots and positions are the step's tables
+            table = ctx.rope_table(xq.shape[0], self.head_dim, self.rope_theta) if self.use_rope else None
+            xq = rope_append_slots(xq, xk, xv, ctx.tables.slots, pages, table)
+            return ctx.tree_wrapper.forward(xq, pages, out=out).view(-1, self.dim)
         if (isinstance(ctx, FlashDecodeCtx) and self.fuse_decode_append and xk.shape[0] == ctx.bsz
                 and ctx.decode_wrapper.fused_append_supported(xq.dtype)):
             # a decode step: the attention launch rotates q and the new k and writes the new

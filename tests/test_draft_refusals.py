@@ -4,6 +4,12 @@ import ctypes
 import pytest
 import torch
 
+from deserve_amd.execution.exec import BatchVerify
+from deserve_amd.kvcache.paged.kvcache import PagedKVCache
+from deserve_amd.kvcache.paged.page_pool import PagePool
+from deserve_amd.kvcache.paged.page_table import PageTableAllocator
+from deserve_amd.model.context.flash import FlashTreeCtx
+from deserve_amd.task import TaskData
 from deserve_amd import _lib
 from deserve_amd.draft_ops import (BatchTreeWithPagedKVCacheWrapper, StepTables, build_step_tables, move_accepted_rows,
                                    rope_append_slots, verify_drafts)
@@ -182,3 +188,44 @@ def test_the_librarys_own_refusals():
     assert call(a10=0) == 0 and call(a2=0) == 0 and says(call(a10=-1), "negative") and says(call(a0=None), "null")
     assert says(call(a5=24), "16") and says(call(a0=24), "aligned") and says(call(a1=4096), "overlap") and says(call(a2=65536), "65535")
     assert says(call(a3=0), "page shape")
+
+
+def test_steps_of_a_stage():
+    pool = PagePool(1, 8, 16, torch.device("cpu"), torch.bfloat16, 2, 128)
+    table = PageTableAllocator(4, 256, 16, torch.device("cpu"))
+    caches = [PagedKVCache.empty(table, pool) for _ in range(2)]
+    tasks = [TaskData("a", 3, 1, 2, 3), TaskData("b", 0, 0, 65, 1)]
+    shape = dict(num_qo_heads=4, num_kv_heads=2, head_dim=128, page_size=16)
+    plan = lambda n, parents, of=caches: FlashTreeCtx.init_and_plan(tasks[:n], of[:n], None, parents=parents, **shape)
+    with pytest.raises(ValueError, match="at most 64 rows"):
+        plan(2, torch.zeros(67, dtype=torch.int32))
+    with pytest.raises(ValueError, match="parents holds 3 entries for 2 rows"):
+        plan(1, torch.zeros(3, dtype=torch.int32))
+    other = PagePool(1, 8, 16, torch.device("cpu"), torch.bfloat16, 2, 128)
+    with pytest.raises(ValueError, match="over one pool"):
+        plan(2, None, [caches[0], PagedKVCache.empty(table, other)])
+    assert pool.num_avails == 8                                       # nothing was reserved
+    steps = [BatchVerify(torch.zeros(t.seqlen, 1), None, [t], [c]) for t, c in zip(tasks, caches)]
+    steps[0].tokens = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="some have none"):
+        BatchVerify.merge(steps)
+    steps[1].tokens, steps[1].tree_ctx = torch.zeros(65, dtype=torch.int32), object()
+    with pytest.raises(ValueError, match="at most 64 rows"):
+        steps[1].verify(torch.zeros(65, 8), torch.zeros(65))
+
+
+def test_steps_regrouped():
+    """Chains and trees merged, split and popped keep their tokens and parents."""
+    tasks = [TaskData(str(i), 0, 0, n, n) for i, n in enumerate((2, 3, 1))]
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)
+    steps = [BatchVerify(torch.zeros(2, 1), None, tasks[:1], [0], i32(7, 8)),
+             BatchVerify(torch.ones(4, 1), None, tasks[1:], [1, 2], i32(4, 5, 6, 9), i32(-1, 0, 0, -1))]
+    whole = BatchVerify.merge(steps)
+    assert whole.tokens.tolist() == [7, 8, 4, 5, 6, 9] and whole.parents.tolist() == [-1, 0, -1, 0, 0, -1]
+    assert [(p.tokens.tolist(), p.parents.tolist()) for p in whole.split()] == \
+        [([7, 8], [-1, 0]), ([4, 5, 6], [-1, 0, 0]), ([9], [-1])]
+    tail = whole.pop()
+    assert (tail.tokens.tolist(), tail.parents.tolist()) == ([9], [-1])
+    assert (whole.tokens.tolist(), whole.parents.tolist()) == ([7, 8, 4, 5, 6], [-1, 0, -1, 0, 0])
+    chains = BatchVerify.merge([steps[0], BatchVerify(torch.ones(3, 1), None, [TaskData("x", 0, 0, 3, 3)], [1], i32(1, 2, 3))])
+    assert chains.parents is None and chains.pop().tokens.tolist() == [1, 2, 3]
