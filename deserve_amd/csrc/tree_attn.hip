@@ -138,7 +138,7 @@ __global__ __launch_bounds__(kGenericWaves * 64) void tree_generic_kernel(TreeAr
 // How a step is computed.  wide_waves > 0: tree_wide_kernel.h with so many waves; else the matrix form of tree_kernel.h with
 // tiles of `blocks` * 16 columns, up to tree_columns: few tiles, each as narrow as it can be.
 struct TreeForm {
-    int wide_waves, blocks, cols, col_tiles, shares, least, sides;
+    int wide_waves, blocks, cols, col_tiles, shares, sides;
 };
 static bool matrix_form(int head_dim) { return head_dim == 64 || head_dim == 128; }
 static TreeForm tree_form(bool wide, int max_rows, int n_qo_heads, int n_kv_heads, int head_dim)
@@ -150,7 +150,6 @@ static TreeForm tree_form(bool wide, int max_rows, int n_qo_heads, int n_kv_head
     f.col_tiles = (int)((cols + widest - 1) / widest);
     f.blocks = wide ? 0 : (int)((cols + 16L * f.col_tiles - 1) / (16L * f.col_tiles));
     f.cols = wide ? widest : f.blocks * 16;
-    f.least = wide ? kWideLeast : kTreeWaves;
     // two workgroups a compute unit where their registers and LDS allow it
     const int resident = kTreeUnits * (wide ? (f.wide_waves == 4 ? 2 : 1) : tree_workgroups(head_dim, f.blocks));
     f.shares = resident >= n_kv_heads ? resident / n_kv_heads : 1;
@@ -169,14 +168,14 @@ static int64_t form_bytes(const TreeForm &f, int batch, int n_kv_heads, int head
     return units_bytes(batch) + slots_of(f, n_kv_heads) * (head_dim + 2) * (int64_t)sizeof(float);
 }
 
-template <int DT, int kD, int kCols, int kSub> static int launch_tree_merge(const TreeArgs &a, const TreeForm &f, hipStream_t stream)
+template <int DT, int kD, int kCols, int kSub, int kLeast> static int launch_tree_merge(const TreeArgs &a, const TreeForm &f, hipStream_t stream)
 {
     // few items are cut into many parts each, many into few
     const bool many_parts = (long)a.batch * f.col_tiles * 4 < f.shares;
     const int columns = 256 / (kD / 4 * (many_parts ? 4 : 1));
     const dim3 grid((unsigned)(a.batch * f.col_tiles), (unsigned)a.n_kv_heads, (unsigned)((kCols + columns - 1) / columns));
-    if (many_parts) hipLaunchKernelGGL((tree_merge_kernel<DT, kD, kCols, kSub, 4>), grid, dim3(256), 0, stream, a, f.col_tiles, f.least);
-    else hipLaunchKernelGGL((tree_merge_kernel<DT, kD, kCols, kSub, 1>), grid, dim3(256), 0, stream, a, f.col_tiles, f.least);
+    if (many_parts) hipLaunchKernelGGL((tree_merge_kernel<DT, kD, kCols, kSub, kLeast, 4>), grid, dim3(256), 0, stream, a, f.col_tiles);
+    else hipLaunchKernelGGL((tree_merge_kernel<DT, kD, kCols, kSub, kLeast, 1>), grid, dim3(256), 0, stream, a, f.col_tiles);
     DSKV_LAUNCH_CHECK("tree_merge_kernel");
     return 0;
 }
@@ -186,13 +185,13 @@ template <int DT, int kD, int kBlocks> static int launch_tree(const TreeArgs &a,
     hipLaunchKernelGGL((tree_matrix_kernel<DT, kD, kBlocks>), dim3((unsigned)(f.shares * a.n_kv_heads)),
                        dim3(kTreeThreads), 0, stream, a);
     DSKV_LAUNCH_CHECK("tree_matrix_kernel");
-    return launch_tree_merge<DT, kD, S::kCols, S::kSub>(a, f, stream);
+    return launch_tree_merge<DT, kD, S::kCols, S::kSub, kTreeWaves>(a, f, stream);
 }
 template <int DT, int kWaves> static int launch_tree_wide(const TreeArgs &a, const TreeForm &f, hipStream_t stream)
 {
     hipLaunchKernelGGL((tree_wide_kernel<DT, kWaves>), dim3((unsigned)(f.shares * a.n_kv_heads)), dim3(kWaves * 64), 0, stream, a);
     DSKV_LAUNCH_CHECK("tree_wide_kernel");
-    return launch_tree_merge<DT, 128, kWaves * 32, kWideBlock>(a, f, stream);
+    return launch_tree_merge<DT, 128, kWaves * 32, kWideBlock, kWideLeast>(a, f, stream);
 }
 template <int DT, int kD> static int launch_tree_blocks(const TreeArgs &a, const TreeForm &f, hipStream_t stream)
 {

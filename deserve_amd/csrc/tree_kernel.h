@@ -99,7 +99,30 @@ template <int kCols, int kSub> __device__ __forceinline__ TreeRequest tree_reque
     return r;
 }
 
-__device__ __forceinline__ long share_begin(long s, long units, long shares) { return s * units / shares; }
+// Equal shares: `each` units, the first `longer` shares one more.  (Divisions of 64 bits cost a short call a microsecond.)
+struct Shares {
+    long each;
+    int longer, used;
+};
+__device__ __forceinline__ long quotient(long a, long b)        // 0 <= a, 0 < b
+{
+    return (a | b) >> 32 ? a / b : (long)((uint32_t)a / (uint32_t)b);
+}
+// None of the shares in use has fewer than `least` units, if there are as many.
+__device__ __forceinline__ Shares shares_of(int n_shares, long units, int least)
+{
+    Shares s;
+    s.used = (int)max(min((long)n_shares, (units + least - 1) / least), 1L);      // (`least`: a power of two)
+    s.each = quotient(units, s.used);
+    s.longer = (int)(units - s.each * s.used);
+    return s;
+}
+__device__ __forceinline__ long share_begin(const Shares &s, int share) { return share * s.each + min(share, s.longer); }
+__device__ __forceinline__ int share_with(const Shares &s, long unit)             // units > 0
+{
+    const long of_longer = s.longer * (s.each + 1);
+    return unit < of_longer ? (int)quotient(unit, s.each + 1) : s.longer + (int)quotient(unit - of_longer, s.each);
+}
 
 // Share and kv head of a workgroup.  Workgroups go round the eight XCDs in turn; the heads of a share belong on
 // one, since their rows of a token lie side by side: with a head per XCD every one of its L2s would be
@@ -130,12 +153,6 @@ __device__ __forceinline__ long units_of(const TreeRequest &r, bool beside)
     return beside ? (r.col_tiles > 0 ? r.subtiles : 0) : (long)r.col_tiles * r.subtiles;
 }
 
-// Shares (spans) that are in use: none has fewer than `least` units, if there are as many.
-__device__ __forceinline__ long shares_of(long n_shares, long units, int least)
-{
-    return max(min(n_shares, (units + least - 1) / least), 1L);
-}
-
 // Sums up to and with this lane's over a wave, by moves between lanes that do not go through LDS.
 template <int kCtrl, int kRows> __device__ __forceinline__ long lanes_below(long v)
 {
@@ -164,8 +181,8 @@ struct TreePlace {
     int side;
     TreeRequest r;       // request b
 };
-template <int kCols, int kSub, int kThreads, bool kSides>
-__device__ __forceinline__ void tree_place(const TreeArgs &a, int share, int least, TreePlace &at)
+template <int kCols, int kSub, int kThreads, bool kSides, int kLeast>
+__device__ __forceinline__ void tree_place(const TreeArgs &a, int share, TreePlace &at)
 {
     __shared__ long scan[2][kThreads / 64], found_base;
     __shared__ int found_b;
@@ -197,7 +214,7 @@ __device__ __forceinline__ void tree_place(const TreeArgs &a, int share, int lea
     at.beside = kSides && side_by_side(a, total[0], total[1]);
     const int which = kSides && at.beside ? 1 : 0;
     const long units = which ? total[1] : total[0];
-    long span = share, spans = a.n_shares;
+    int span = share, spans = a.n_shares;
     at.side = 0;
     if (which) {
         const int j = share / 8;
@@ -205,11 +222,11 @@ __device__ __forceinline__ void tree_place(const TreeArgs &a, int share, int lea
         span = share % 8 + 8 * (j / a.sides);
         spans = a.n_shares / a.sides;
     }
-    const long used = shares_of(spans, units, least);
+    const Shares shares = shares_of(spans, units, kLeast);
     at.begin = at.end = 0;
-    if (span < used && units > 0) {
-        at.begin = share_begin(span, units, used);
-        at.end = share_begin(span + 1, units, used);
+    if (span < shares.used) {
+        at.begin = share_begin(shares, span);
+        at.end = share_begin(shares, span + 1);
     }
     long before = (which ? upto[1] : upto[0]) - (which ? mine[1] : mine[0]);
     const bool tells = blockIdx.x == 0;
@@ -342,7 +359,7 @@ __global__ __launch_bounds__(kTreeThreads, tree_workgroups(kD, kBlocks)) void tr
     int share, head;
     share_and_head(a, share, head);
     TreePlace place;
-    tree_place<S::kCols, S::kSub, kTreeThreads, false>(a, share, kTreeWaves, place);
+    tree_place<S::kCols, S::kSub, kTreeThreads, false, kTreeWaves>(a, share, place);
     make_uniform(place);
     const long begin = place.begin, end = place.end;
     if (begin >= end) return;
@@ -698,8 +715,8 @@ __global__ __launch_bounds__(kTreeThreads, tree_workgroups(kD, kBlocks)) void tr
 
 // Items that were cut: a thread per (column, four dims) and group of parts.  kGroups > 1, for items in many parts: each takes
 // every kGroups-th part, and they meet in LDS.
-template <int DT, int kD, int kCols, int kSub, int kGroups>
-__global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int max_col_tiles, int least)
+template <int DT, int kD, int kCols, int kSub, int kLeast, int kGroups>
+__global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int max_col_tiles)
 {
     constexpr int kElt = DT == DSKV_F32 ? 4 : 2;
     constexpr int kQuads = kD / 4, kColumns = 256 / (kQuads * kGroups);
@@ -711,11 +728,12 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int max_col
     const int col = blockIdx.z * kColumns + column;
     const int cols = min(r.n * a.group - ct * r.tile, r.tile);
     if (ct >= r.col_tiles || (int)blockIdx.z * kColumns >= cols) return;
-    const long shares = shares_of(beside ? a.n_shares / a.sides : a.n_shares, units, least);
+    const Shares shares = shares_of(beside ? a.n_shares / a.sides : a.n_shares, units, kLeast);
     const bool there = col < cols;
     const long first = before + (beside ? 0 : (long)ct * r.subtiles), last = first + r.subtiles - 1;
-    const long s0 = ((first + 1) * shares + units - 1) / units - 1, s1 = ((last + 1) * shares + units - 1) / units - 1;
+    const int s0 = share_with(shares, first), s1 = share_with(shares, last);
     if (s0 == s1) return;
+    const bool second = share_begin(shares, s0) < first;       // in the first of its shares the item is the second
     float top = -INFINITY, sum = 0;
     f32x4 acc = {0, 0, 0, 0};
     auto add = [&](float pm, float pl, f32x4 po) {
@@ -727,13 +745,13 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int max_col
     };
     if (there) {
         constexpr int kAhead = 4;                  // parts requested together
-        for (long s = s0 + group; s <= s1; s += kAhead * kGroups) {
+        for (int s = s0 + group; s <= s1; s += kAhead * kGroups) {
             float pm[kAhead], pl[kAhead];
             f32x4 po[kAhead];
 #pragma unroll
             for (int i = 0; i < kAhead; i++) {
-                const long si = min(s + i * kGroups, s1);
-                const long slot = 2 * (beside ? share_of_span((int)si, ct, a.sides) : si) + (si == s0 && share_begin(si, units, shares) < first ? 1 : 0);
+                const int si = min(s + i * kGroups, s1);
+                const long slot = 2L * (beside ? share_of_span(si, ct, a.sides) : si) + (si == s0 && second ? 1 : 0);
                 const long part = (slot * a.n_kv_heads + head) * kCols + col;
                 pm[i] = a.part_ml[part * 2];
                 pl[i] = a.part_ml[part * 2 + 1];
