@@ -161,7 +161,7 @@ static bool wide_form(int max_rows, int n_qo_heads, int n_kv_heads, int head_dim
 {
     return head_dim == 128 && dtype != DSKV_F32 && (long)max_rows * (n_qo_heads / n_kv_heads) > tree_columns(head_dim);
 }
-static int64_t units_bytes(int batch) { return ((int64_t)batch + 3) / 2 * 16; }
+static int64_t units_bytes(int batch) { return ((int64_t)batch + 5) / 4 * 16; }
 static int64_t slots_of(const TreeForm &f, int n_kv_heads) { return 2LL * f.shares * n_kv_heads * f.cols; }
 static int64_t form_bytes(const TreeForm &f, int batch, int n_kv_heads, int head_dim)
 {
@@ -253,11 +253,12 @@ extern "C" int dskv_tree_attn(const dskv_tree_step_t *s, void *out, const void *
                   s->nnz, s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->head_dim, s->page_size, s->num_pages,
                   s->sm_scale * 1.4426950408889634f};
     hipStream_t st = (hipStream_t)stream;
-    // (rows of the pool and tokens of a request are numbered in 32 bits there)
+    const TreeForm f = tree_form(s->sm_scale > 0 && wide_form(s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->head_dim, s->dtype),
+                                 s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->head_dim);
+    // (rows of the pool, tokens of a request and units are numbered in 32 bits there)
     if (matrix_form(s->head_dim) && (int64_t)s->num_pages * 2 * s->page_size < INT32_MAX &&
-        s->n_page_indices < (1 << 30) / s->page_size && s->max_qo_len <= kTreeMostRows) {
-        const TreeForm f = tree_form(s->sm_scale > 0 && wide_form(s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->head_dim, s->dtype),
-                                     s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->head_dim);
+        s->n_page_indices < (1 << 30) / s->page_size && s->max_qo_len <= kTreeMostRows &&
+        (s->n_page_indices * s->page_size / 16 + 2LL * s->batch) * f.col_tiles < INT32_MAX) {
         const int64_t need = dskv_tree_attn_workspace(s->batch, s->nnz, s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->head_dim, s->dtype);
         if (!s->workspace || s->workspace_bytes < need) {
             set_error("tree_attn: workspace of %lld bytes, %lld are needed", (long long)s->workspace_bytes, (long long)need);
@@ -265,7 +266,7 @@ extern "C" int dskv_tree_attn(const dskv_tree_step_t *s, void *out, const void *
         }
         DSKV_REQUIRE((uintptr_t)s->workspace % 16 == 0, "tree_attn: the workspace must be 16-byte aligned");
         DSKV_REQUIRE((int64_t)s->batch * f.col_tiles < INT32_MAX && s->n_kv_heads <= 65535, "tree_attn: too large a batch");
-        a.units_before = (int64_t *)s->workspace;
+        a.units_before = (int32_t *)s->workspace;
         a.part_o = (float *)((char *)s->workspace + units_bytes(s->batch));
         a.part_ml = a.part_o + slots_of(f, s->n_kv_heads) * s->head_dim;
         a.n_shares = f.shares;

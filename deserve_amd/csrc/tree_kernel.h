@@ -35,7 +35,7 @@ struct TreeArgs {
     uint32_t page_magic;                  // ceil(2^page_shift / page_size): t / page_size = t * page_magic >> page_shift
     int page_shift;
     float *part_o, *part_ml;              // (2 * n_shares, n_kv_heads, columns of a tile, head_dim | 2)
-    int64_t *units_before;                // (batch + 2): units of the requests in front, and side_by_side
+    int32_t *units_before;                // (batch + 2): units of the requests in front, and side_by_side
     int n_shares, group;
     int sides;                            // see side_by_side
 };
@@ -86,7 +86,7 @@ template <int kCols, int kSub> __device__ __forceinline__ TreeRequest tree_reque
     r.first = qo[0];
     const long rows = (long)qo[1] - r.first;
     r.page0 = kv[0];
-    r.pages = kv[1] - r.page0;
+    r.pages = (int)min((long)kv[1] - r.page0, a.n_page_indices);
     const int last = as_const(a.kv_last_page_lens)[b];
     r.kv_len = r.pages > 0 ? max((long)(r.pages - 1) * a.page_size + min(last, a.page_size), 0L) : 0;
     r.n = r.first < 0 ? 0 : (int)max(min(min(rows, (long)a.max_rows), (long)a.nnz - r.first), 0L);
@@ -99,29 +99,27 @@ template <int kCols, int kSub> __device__ __forceinline__ TreeRequest tree_reque
     return r;
 }
 
-// Equal shares: `each` units, the first `longer` shares one more.  (Divisions of 64 bits cost a short call a microsecond.)
+// Equal shares: `each` units, the first `longer` shares one more.  Units are counted in 32 bits (what the arrays can hold fits; a
+// batch whose arrays contradict themselves so that it does not is left out): divisions of 64 bits cost a short call a
+// microsecond.
 struct Shares {
-    long each;
-    int longer, used;
+    int each, longer, used;
 };
-__device__ __forceinline__ long quotient(long a, long b)        // 0 <= a, 0 < b
-{
-    return (a | b) >> 32 ? a / b : (long)((uint32_t)a / (uint32_t)b);
-}
 // None of the shares in use has fewer than `least` units, if there are as many.
-__device__ __forceinline__ Shares shares_of(int n_shares, long units, int least)
+__device__ __forceinline__ Shares shares_of(int n_shares, int units, int least)
 {
     Shares s;
-    s.used = (int)max(min((long)n_shares, (units + least - 1) / least), 1L);      // (`least`: a power of two)
-    s.each = quotient(units, s.used);
-    s.longer = (int)(units - s.each * s.used);
+    s.used = max(min(n_shares, (int)(((unsigned)units + least - 1) / (unsigned)least)), 1);
+    s.each = (int)((unsigned)units / (unsigned)s.used);
+    s.longer = units - s.each * s.used;
     return s;
 }
-__device__ __forceinline__ long share_begin(const Shares &s, int share) { return share * s.each + min(share, s.longer); }
-__device__ __forceinline__ int share_with(const Shares &s, long unit)             // units > 0
+__device__ __forceinline__ int share_begin(const Shares &s, int share) { return share * s.each + min(share, s.longer); }
+__device__ __forceinline__ int share_with(const Shares &s, int unit)              // units > 0
 {
-    const long of_longer = s.longer * (s.each + 1);
-    return unit < of_longer ? (int)quotient(unit, s.each + 1) : s.longer + (int)quotient(unit - of_longer, s.each);
+    const int of_longer = s.longer * (s.each + 1);
+    return unit < of_longer ? (int)((unsigned)unit / (unsigned)(s.each + 1))
+                            : s.longer + (int)((unsigned)(unit - of_longer) / (unsigned)s.each);
 }
 
 // Share and kv head of a workgroup.  Workgroups go round the eight XCDs in turn; the heads of a share belong on
@@ -174,8 +172,8 @@ __device__ __forceinline__ long wave_scan(long v)
 // Where the workgroup's share begins and ends, by all of its kThreads threads; the first workgroup leaves the
 // sums for the merge launch.
 struct TreePlace {
-    long begin, end;     // units; equal: nothing to do
-    long base;           // units in front of request b
+    int begin, end;      // units; equal: nothing to do
+    int base;            // units in front of request b
     int b;
     bool beside;
     int side;
@@ -184,8 +182,8 @@ struct TreePlace {
 template <int kCols, int kSub, int kThreads, bool kSides, int kLeast>
 __device__ __forceinline__ void tree_place(const TreeArgs &a, int share, TreePlace &at)
 {
-    __shared__ long scan[2][kThreads / 64], found_base;
-    __shared__ int found_b;
+    __shared__ long scan[2][kThreads / 64];
+    __shared__ int found_base, found_b;
     __shared__ TreeRequest found_r;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int per = (a.batch + kThreads - 1) / kThreads;
@@ -213,7 +211,8 @@ __device__ __forceinline__ void tree_place(const TreeArgs &a, int share, TreePla
         }
     at.beside = kSides && side_by_side(a, total[0], total[1]);
     const int which = kSides && at.beside ? 1 : 0;
-    const long units = which ? total[1] : total[0];
+    const long sum = which ? total[1] : total[0];
+    const int units = sum <= INT32_MAX ? (int)sum : 0;
     int span = share, spans = a.n_shares;
     at.side = 0;
     if (which) {
@@ -228,12 +227,12 @@ __device__ __forceinline__ void tree_place(const TreeArgs &a, int share, TreePla
         at.begin = share_begin(shares, span);
         at.end = share_begin(shares, span + 1);
     }
-    long before = (which ? upto[1] : upto[0]) - (which ? mine[1] : mine[0]);
+    int before = (int)((which ? upto[1] : upto[0]) - (which ? mine[1] : mine[0]));
     const bool tells = blockIdx.x == 0;
-    if (tells || (before <= at.begin && at.begin < (which ? upto[1] : upto[0]))) {
+    if (tells || (before <= at.begin && at.begin < (int)(which ? upto[1] : upto[0]))) {
         for (int b = b0; b < b1; b++) {
             if (per > 1) r = tree_request<kCols, kSub>(a, b);
-            const long u = units_of(r, which);
+            const int u = (int)units_of(r, which);
             if (tells) a.units_before[b] = before;
             if (before <= at.begin && at.begin < before + u) {
                 found_b = b;
@@ -260,9 +259,9 @@ __device__ __forceinline__ long uniform(long x)
 }
 __device__ __forceinline__ void make_uniform(TreePlace &at)
 {
-    at.begin = uniform(at.begin);
-    at.end = uniform(at.end);
-    at.base = uniform(at.base);
+    at.begin = __builtin_amdgcn_readfirstlane(at.begin);
+    at.end = __builtin_amdgcn_readfirstlane(at.end);
+    at.base = __builtin_amdgcn_readfirstlane(at.base);
     at.r.first = uniform(at.r.first);
     at.r.kv_len = uniform(at.r.kv_len);
     at.r.prior = uniform(at.r.prior);
@@ -327,23 +326,23 @@ template <int DT, int kD, int kBlocks> struct TreeRegs {
 // A share's walk through its items; one item at a time.
 struct TreeItem {
     TreeRequest r;
-    long base;           // units in front of request b
-    long next;           // the first unit behind the item's part
+    int base;            // units in front of request b
+    int next;            // the first unit behind the item's part
     int b, ct, st0, st1; // column tile; subtiles of the part
     bool first;          // of the share
 };
 template <int kCols, int kSub>
-__device__ __forceinline__ void open_item(const TreeArgs &a, long unit, long begin, long end, TreeItem &it)
+__device__ __forceinline__ void open_item(const TreeArgs &a, int unit, int begin, int end, TreeItem &it)
 {
-    while (unit >= it.base + units_of(it.r, false)) {         // on to the next request that has rows
-        it.base += units_of(it.r, false);
+    while (unit >= it.base + (int)units_of(it.r, false)) {         // on to the next request that has rows
+        it.base += (int)units_of(it.r, false);
         it.b++;
         it.r = tree_request<kCols, kSub>(a, it.b);
     }
     it.ct = (int)((unsigned)(unit - it.base) / (unsigned)it.r.subtiles);
-    const long item = it.base + (long)it.ct * it.r.subtiles;
+    const int item = it.base + it.ct * it.r.subtiles;
     it.st0 = (int)(unit - item);
-    it.st1 = (int)min(end - item, (long)it.r.subtiles);
+    it.st1 = min(end - item, it.r.subtiles);
     it.next = item + it.st1;
     it.first = unit == begin;
 }
@@ -361,7 +360,7 @@ __global__ __launch_bounds__(kTreeThreads, tree_workgroups(kD, kBlocks)) void tr
     TreePlace place;
     tree_place<S::kCols, S::kSub, kTreeThreads, false, kTreeWaves>(a, share, place);
     make_uniform(place);
-    const long begin = place.begin, end = place.end;
+    const int begin = place.begin, end = place.end;
     if (begin >= end) return;
 
     char *const k_lds = lds + wave * S::kWaveLds, *const v_lds = k_lds + S::kSub * S::kKPitch;
@@ -445,7 +444,7 @@ __global__ __launch_bounds__(kTreeThreads, tree_workgroups(kD, kBlocks)) void tr
     int limit[kBlocks];
     f32x4 o[kBlocks][S::kDimTiles];
     float m[kBlocks], l[kBlocks];
-    auto start_item = [&](long unit) {
+    auto start_item = [&](int unit) {
         open_item<S::kCols, S::kSub>(a, unit, begin, end, it);
         cols = min(it.r.n * a.group - it.ct * S::kCols, S::kCols);
         prior = (int)max(it.r.prior, (long)-INT32_MAX);
@@ -723,14 +722,14 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int max_col
     const int b = blockIdx.x / max_col_tiles, ct = blockIdx.x % max_col_tiles, head = blockIdx.y;
     const int quad = threadIdx.x % kQuads, column = threadIdx.x / kQuads % kColumns, group = threadIdx.x / (kQuads * kColumns);
     const TreeRequest r = tree_request<kCols, kSub>(a, b);
-    const long before = a.units_before[b], units = a.units_before[a.batch];
+    const int before = a.units_before[b], units = a.units_before[a.batch];
     const bool beside = a.units_before[a.batch + 1] != 0;
     const int col = blockIdx.z * kColumns + column;
     const int cols = min(r.n * a.group - ct * r.tile, r.tile);
-    if (ct >= r.col_tiles || (int)blockIdx.z * kColumns >= cols) return;
+    if (ct >= r.col_tiles || (int)blockIdx.z * kColumns >= cols || units == 0) return;
     const Shares shares = shares_of(beside ? a.n_shares / a.sides : a.n_shares, units, kLeast);
     const bool there = col < cols;
-    const long first = before + (beside ? 0 : (long)ct * r.subtiles), last = first + r.subtiles - 1;
+    const int first = before + (beside ? 0 : ct * r.subtiles), last = first + r.subtiles - 1;
     const int s0 = share_with(shares, first), s1 = share_with(shares, last);
     if (s0 == s1) return;
     const bool second = share_begin(shares, s0) < first;       // in the first of its shares the item is the second

@@ -48,9 +48,9 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
     TreePlace place;
     tree_place<W::kCols, kWideBlock, W::kThreads, true, kWideLeast>(a, share, place);
     make_uniform(place);
-    const long begin = place.begin, end = place.end;
+    const int begin = place.begin, end = place.end;
     const bool beside = place.beside;
-    long unit = begin, base = place.base;
+    int unit = begin, base = place.base;
     int b = place.b;
     TreeRequest r = place.r;
 
@@ -64,15 +64,15 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
     const char *const none = reinterpret_cast<const char *>(kNoRow) + (lane >> 2) * 16;
 
     while (unit < end) {
-        if (unit >= base + units_of(r, beside)) {             // on to the next request that has rows
-            base += units_of(r, beside);
+        if (unit >= base + (int)units_of(r, beside)) {             // on to the next request that has rows
+            base += (int)units_of(r, beside);
             b++;
             r = tree_request<W::kCols, kWideBlock>(a, b);
             continue;
         }
         const int ct = beside ? place.side : (int)((unsigned)(unit - base) / (unsigned)r.subtiles);
-        const long item = base + (beside ? 0 : (long)ct * r.subtiles);
-        const int st0 = (int)(unit - item), st1 = (int)min(end - item, (long)r.subtiles);
+        const int item = base + (beside ? 0 : ct * r.subtiles);
+        const int st0 = unit - item, st1 = min(end - item, r.subtiles);
         if (ct >= r.col_tiles) {                              // (beside: a request of fewer column tiles)
             unit = item + st1;
             continue;
