@@ -161,7 +161,7 @@ static bool wide_form(int max_rows, int n_qo_heads, int n_kv_heads, int head_dim
 {
     return head_dim == 128 && dtype != DSKV_F32 && (long)max_rows * (n_qo_heads / n_kv_heads) > tree_columns(head_dim);
 }
-static int64_t units_bytes(int batch) { return ((int64_t)batch + 5) / 4 * 16; }
+static int64_t units_bytes(int batch) { return ((int64_t)batch + 6) / 4 * 16; }
 static int64_t slots_of(const TreeForm &f, int n_kv_heads) { return 2LL * f.shares * n_kv_heads * f.cols; }
 static int64_t form_bytes(const TreeForm &f, int batch, int n_kv_heads, int head_dim)
 {

@@ -35,7 +35,7 @@ struct TreeArgs {
     uint32_t page_magic;                  // ceil(2^page_shift / page_size): t / page_size = t * page_magic >> page_shift
     int page_shift;
     float *part_o, *part_ml;              // (2 * n_shares, n_kv_heads, columns of a tile, head_dim | 2)
-    int32_t *units_before;                // (batch + 2): units of the requests in front, and side_by_side
+    int32_t *units_before;                // (batch + 3): units (parts) of the requests in front; see tree_place
     int n_shares, group;
     int sides;                            // see side_by_side
 };
@@ -179,11 +179,16 @@ struct TreePlace {
     int side;
     TreeRequest r;       // request b
 };
-template <int kCols, int kSub, int kThreads, bool kSides, int kLeast>
+// A share that goes over from one item to another starts twice and joins its waves' results twice, which a small batch notices: if
+// parts of a common number of units, whole turns (kTurn) and at most two turns more than equal shares have, take no more
+// shares than there are, no part crosses an item's end.  Measured against equal shares (32 heads over 8, bf16): 3 requests of 5 rows over
+// 50 - 500 tokens 14.0 for 18.9 us, 8 over 1 - 4 K 26.7 for 31.7, 8 over 4 - 16 K 70.5 for 71.8, 8 trees of 64 rows over 1 - 4 K
+// 53.6 for 63.6; at 16 over 2 - 8 K they take too many shares.
+template <int kCols, int kSub, int kThreads, bool kSides, int kLeast, int kTurn>
 __device__ __forceinline__ void tree_place(const TreeArgs &a, int share, TreePlace &at)
 {
-    __shared__ long scan[2][kThreads / 64];
-    __shared__ int found_base, found_b;
+    __shared__ long scan[2][kThreads / 64], scan_parts[kThreads / 64];
+    __shared__ int found_base, found_b, found_begin, found_end;
     __shared__ TreeRequest found_r;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int per = (a.batch + kThreads - 1) / kThreads;
@@ -229,6 +234,52 @@ __device__ __forceinline__ void tree_place(const TreeArgs &a, int share, TreePla
     }
     int before = (int)((which ? upto[1] : upto[0]) - (which ? mine[1] : mine[0]));
     const bool tells = blockIdx.x == 0;
+    if constexpr (kTurn > 0) {
+        if (a.batch > 1 && a.batch <= spans / 2 && units > 0) {             // (a request per thread at most)
+            const int most = shares.each + (shares.longer > 0);
+            const int cut = most <= kLeast ? kLeast : (most + kTurn - 1) / kTurn * kTurn, cut_more = (cut + 2 * kTurn - 1) / kTurn * kTurn;
+            const int tiles = which ? (r.col_tiles > 0) : r.col_tiles;
+            long parts = 0;                                                 // of `cut` units and, in the upper half, a turn more
+            if (b0 < b1)
+                parts = (long)tiles * ((unsigned)(r.subtiles + cut - 1) / (unsigned)cut) |
+                        (long)tiles * ((unsigned)(r.subtiles + cut_more - 1) / (unsigned)cut_more) << 32;
+            long parts_upto = wave_scan(parts), parts_total = 0;
+            if (lane == 63) scan_parts[wave] = parts_upto;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < kThreads / 64; w++) {
+                if (w == wave) parts_upto += parts_total;
+                parts_total += scan_parts[w];
+            }
+            const bool fits = (int)parts_total <= spans;
+            const int half = fits ? 0 : 32, total_parts = (int)(parts_total >> half), part = fits ? cut : cut_more;
+            if (total_parts <= spans) {
+                const int p = (int)(parts >> half), first = (int)(parts_upto >> half) - p;
+                if (p > 0 && first <= span && span < first + p) {
+                    const int of_item = (int)((unsigned)p / (unsigned)tiles), ct = (span - first) / of_item;
+                    const int item = before + ct * r.subtiles;
+                    found_begin = item + (span - first - ct * of_item) * part;
+                    found_end = min(found_begin + part, item + r.subtiles);
+                    found_b = b0;
+                    found_base = before;
+                    found_r = r;
+                }
+                if (tells && b0 < b1) a.units_before[b0] = first;
+                if (tells && b1 == a.batch) {
+                    a.units_before[a.batch] = units;
+                    a.units_before[a.batch + 1] = which;
+                    a.units_before[a.batch + 2] = part;
+                }
+                __syncthreads();
+                at.begin = span < total_parts ? found_begin : 0;
+                at.end = span < total_parts ? found_end : 0;
+                at.b = __builtin_amdgcn_readfirstlane(found_b);
+                at.base = found_base;
+                at.r = found_r;
+                return;
+            }
+        }
+    }
     if (tells || (before <= at.begin && at.begin < (int)(which ? upto[1] : upto[0]))) {
         for (int b = b0; b < b1; b++) {
             if (per > 1) r = tree_request<kCols, kSub>(a, b);
@@ -244,6 +295,7 @@ __device__ __forceinline__ void tree_place(const TreeArgs &a, int share, TreePla
         if (tells && b1 == a.batch) {
             a.units_before[a.batch] = units;
             a.units_before[a.batch + 1] = which;
+            a.units_before[a.batch + 2] = 0;
         }
     }
     __syncthreads();
@@ -358,7 +410,7 @@ __global__ __launch_bounds__(kTreeThreads, tree_workgroups(kD, kBlocks)) void tr
     int share, head;
     share_and_head(a, share, head);
     TreePlace place;
-    tree_place<S::kCols, S::kSub, kTreeThreads, false, kTreeWaves>(a, share, place);
+    tree_place<S::kCols, S::kSub, kTreeThreads, false, kTreeWaves, kTreeWaves * tree_depth(kD, kBlocks)>(a, share, place);
     make_uniform(place);
     const int begin = place.begin, end = place.end;
     if (begin >= end) return;
@@ -724,15 +776,25 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int max_col
     const TreeRequest r = tree_request<kCols, kSub>(a, b);
     const int before = a.units_before[b], units = a.units_before[a.batch];
     const bool beside = a.units_before[a.batch + 1] != 0;
+    const int part_units = a.units_before[a.batch + 2];        // 0: equal shares
     const int col = blockIdx.z * kColumns + column;
     const int cols = min(r.n * a.group - ct * r.tile, r.tile);
     if (ct >= r.col_tiles || (int)blockIdx.z * kColumns >= cols || units == 0) return;
     const Shares shares = shares_of(beside ? a.n_shares / a.sides : a.n_shares, units, kLeast);
     const bool there = col < cols;
     const int first = before + (beside ? 0 : ct * r.subtiles), last = first + r.subtiles - 1;
-    const int s0 = share_with(shares, first), s1 = share_with(shares, last);
+    int s0, s1;
+    bool second = false;                                       // in the first of its shares the item is the second
+    if (part_units > 0) {
+        const int parts = (int)((unsigned)(r.subtiles + part_units - 1) / (unsigned)part_units);
+        s0 = before + (beside ? 0 : ct * parts);
+        s1 = s0 + parts - 1;
+    } else {
+        s0 = share_with(shares, first);
+        s1 = share_with(shares, last);
+        second = share_begin(shares, s0) < first;
+    }
     if (s0 == s1) return;
-    const bool second = share_begin(shares, s0) < first;       // in the first of its shares the item is the second
     float top = -INFINITY, sum = 0;
     f32x4 acc = {0, 0, 0, 0};
     auto add = [&](float pm, float pl, f32x4 po) {

@@ -46,7 +46,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
     int share, head;
     share_and_head(a, share, head);
     TreePlace place;
-    tree_place<W::kCols, kWideBlock, W::kThreads, true, kWideLeast>(a, share, place);
+    tree_place<W::kCols, kWideBlock, W::kThreads, true, kWideLeast, kWideLeast>(a, share, place);
     make_uniform(place);
     const int begin = place.begin, end = place.end;
     const bool beside = place.beside;

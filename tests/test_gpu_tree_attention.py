@@ -37,6 +37,10 @@ CASES = [
     ("wide_group7_page3", [70, 500], [30, 64], True, 3, 14, 2, 128, "bf16"),
     ("wide_segments", [2047, 2048, 1023, 1024, 4100], [20, 20, 33, 5, 64], True, 16, 16, 4, 128, "bf16"),
     ("wide_chains", [300, 20], [40, 64], False, 12, 32, 8, 128, "f16"),
+    ("wide_two_tiles", [900, 1500, 40, 333], [64, 50, 40, 33], True, 16, 16, 2, 128, "bf16"),
+    ("wide_two_tiles_or_one", [900, 1500, 140, 333, 700, 80], [64, 64, 64, 40, 64, 3], True, 16, 16, 1, 128, "f16"),
+    ("wide_two_tiles_many", [300 + 37 * i for i in range(11)], [64 - 3 * i for i in range(11)], True, 16, 64, 8, 128, "bf16"),
+    ("many_over_eight_heads", [31 * i for i in range(20)], [1 + i % 6 for i in range(20)], True, 16, 16, 8, 128, "bf16"),
     ("many_short", list(range(70)), [1 + i % 5 for i in range(70)], True, 8, 8, 2, 128, "bf16"),
     ("many_lengths", [int(x) for x in np.random.default_rng(1).integers(0, 900, 40)], [4] * 40, False, 16, 8, 2, 128, "bf16"),
 ]
