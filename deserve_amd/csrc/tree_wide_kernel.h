@@ -28,6 +28,7 @@ template <int kWaves> struct WideShape {
     static constexpr int kGroups = 8 / kWaves;           // regions of a block that a wave requests
     static constexpr int kHalf = kWaves == 8 ? 64 : 32;  // blocks that are looked up at a time; two such halves are kept
     static constexpr int kTokens = 2 * kHalf * kWideBlock;
+    static constexpr int kPair = kWaves == 8 ? 2 : 1;    // iterations between barriers
     static constexpr int kStages = kWaves == 8 ? 8 : 4;  // blocks of K, and of V, in LDS: as many as fit beside the other workgroup
 };
 
@@ -132,18 +133,15 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
                 if ((lane & 31) == 0) held_at[at / kWideBlock] = (uint32_t)(there64 >> (lane & 32));
             }
         };
-        // address of the lane's 16 bytes of K of block j (V: half_bytes on)
+        // rows of the pool that the lane requests 16 bytes of for block j
         struct Where {
-            const char *p[W::kGroups];
-            bool is[W::kGroups];
+            int row[W::kGroups];
         };
         auto where = [&](int j, Where &w) {
 #pragma unroll
             for (int i = 0; i < W::kGroups; i++) {
                 const int at = (j & (2 * W::kHalf - 1)) * kWideBlock + (wave * W::kGroups + i) * 4 + (lane & 3);
-                const int row = j < blocks ? row_at[at] : -1;      // (behind the walk nothing was looked up)
-                w.is[i] = row >= 0;
-                w.p[i] = row >= 0 ? pool + (unsigned long)(unsigned)row * (unsigned)row_bytes : none;
+                w.row[i] = j < blocks ? row_at[at] : -1;           // (behind the walk nothing was looked up)
             }
         };
         typedef __attribute__((address_space(3))) void *lds_ptr;
@@ -155,7 +153,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
 #pragma unroll
             for (int i = 0; i < W::kGroups; i++) {
                 const uint32_t to = (uint32_t)(uintptr_t)(lds_ptr)(stage + (wave * W::kGroups + i) * kWideRegion);
-                const char *p = w.is[i] ? w.p[i] + more : w.p[i];
+                const char *p = pool + (unsigned long)(unsigned)w.row[i] * (unsigned)row_bytes + more;
+                p = w.row[i] >= 0 ? p : none;
                 asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off"
                              :
                              : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(p)
@@ -249,21 +248,26 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
 #pragma unroll
         for (int s = 0; s < 8; s++) asm volatile("" : "+v"(q[s]));
         asm volatile("" : "+v"(mask));
-        Where at_v, at_between, at_k;                    // of blocks j + kStages - 2, - 1 and j + kStages
+        Where at_v[W::kPair], at_between, at_k[W::kPair];     // of the blocks that the next requests are for
         {
-            // as iterations -kStages .. -1 would request them
+            // as heads -kStages .. would request them
             Where w[W::kStages];
 #pragma unroll
             for (int i = 0; i < W::kStages; i++) where(i, w[i]);
 #pragma unroll
-            for (int i = 0; i < W::kStages; i++) {
-                request(w[i], k_stage(i), 0);
-                if (i >= 2) request(w[i - 2], v_stage(i - 2), half_bytes);
+            for (int i = 0; i < W::kStages; i += W::kPair) {
+#pragma unroll
+                for (int x = i; x < i + W::kPair; x++) request(w[x], k_stage(x), 0);
+#pragma unroll
+                for (int x = max(i - W::kPair - 1, 0); x < i - 1; x++) request(w[x], v_stage(x), half_bytes);
             }
-            at_v = w[W::kStages - 2];
+#pragma unroll
+            for (int x = 0; x < W::kPair; x++) {
+                at_v[x] = w[W::kStages - 1 - W::kPair + x];
+                where(W::kStages + x, at_k[x]);
+            }
             at_between = w[W::kStages - 1];
-            where(W::kStages, at_k);
-            DSKV_WAIT_VMEM(2 * (W::kStages - 2) * W::kGroups);              // K(0) and K(1)
+            DSKV_WAIT_VMEM((2 * W::kStages - 3 - W::kPair) * W::kGroups);              // K(0) and K(1)
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
@@ -274,20 +278,32 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
             if ((st0 + 1) * kWideBlock > mask_from) mask_scores(0, xs[0]);
             read_keys(k_stage(1));
         }
-        auto iteration = [&](int j, int phase) {         // phase = j % 4, a literal
+        // in front of iterations j .. j + kPair - 1; phase = j % 4, a literal
+        auto advance = [&](int j, int phase) {
             const int hi = W::kStages == 8 ? j & 4 : 0;  // stage of block j: phase + hi
-            // this wave's rows of K(j + 2) and V(j - 1) have landed
-            DSKV_WAIT_VMEM((2 * W::kStages - 5) * W::kGroups);
+            // this wave's rows of K(j + 2), V(j - 1) and, for a pair, K(j + 3) and V(j) have landed
+            DSKV_WAIT_VMEM((2 * W::kStages - 2 - 3 * W::kPair) * W::kGroups);
             asm volatile("" ::: "memory");
-            if (j > new_from && j <= new_to) set_aside(j - 1);
+#pragma unroll
+            for (int x = j - 1; x < j - 1 + W::kPair; x++)
+                if (x >= new_from && x < new_to) set_aside(x);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            request(at_k, k_stage(phase + hi), 0);                                  // K(j + kStages)
-            request(at_v, v_stage((phase + hi + kLast - 1) & kLast), half_bytes);   // V(j + kStages - 2)
-            at_v = at_between;
-            at_between = at_k;
-            where(j + W::kStages + 1, at_k);
+#pragma unroll
+            for (int x = 0; x < W::kPair; x++) request(at_k[x], k_stage(phase + x + hi), 0);                   // K(j + kStages + x)
+#pragma unroll
+            for (int x = 0; x < W::kPair; x++)                                           // V(j + kStages - 1 - kPair + x)
+                request(at_v[x], v_stage((phase + hi + kLast - W::kPair + x) & kLast), half_bytes);
+            at_v[0] = at_between;
+            if (W::kPair == 2) at_v[W::kPair - 1] = at_k[0];
+            at_between = at_k[W::kPair - 1];
+#pragma unroll
+            for (int x = 0; x < W::kPair; x++) where(j + W::kStages + W::kPair + x, at_k[x]);
+        };
+        auto iteration = [&](int j, int phase) {
+            const int hi = W::kStages == 8 ? j & 4 : 0;
+            if (W::kPair == 1 || (phase & 1) == 0) advance(j, phase);
             if (!works || j > blocks) return;
             const int cur = phase & 1, nxt = cur ^ 1;
             const char *rows = v_stage((phase + hi + kLast) & kLast) + v_off;                  // V(j - 1)
