@@ -8,8 +8,13 @@
 // workgroup per (share, kv head); its four waves take the share's subtiles in turn, each with a running maximum, sum and O of
 // its own, and meet in LDS where an item (request, column tile) ends.  An item that a share boundary cuts leaves
 // a partial (maximum, sum, O in fp32) that tree_merge_kernel adds up.
-// K and V go by whole rows through registers (one subtile ahead) and a wave's own LDS: rows of 256 bytes are what
+// K and V go by whole rows through registers and a wave's own LDS: rows of 256 bytes are what
 // HBM delivers best, and a row's page is looked up once per subtile, by lane, so pages may have any size.
+//
+// Bound by HBM where there is work enough: 64 requests of 5 rows over 256 - 4096 tokens (32 heads over 8, bf16, 0.6 GB) 119 us, of
+// which the launch for cut items takes 5: 4.9 TB/s; its loads alone run in 96.  In short calls by latency: one request over
+// 1.8 K tokens 14.4 us, 11.1 for the first launch (place of the share 2.6, page ids 3, K and V 2, products 3, waves meet 2).
+// fp32: the matrix instruction takes 64 products a cycle, a wave's subtile for 48 columns 3 us; 8 requests over 300 - 700 tokens 29.
 #pragma once
 
 #include "kv_tile.h"
@@ -46,6 +51,7 @@ constexpr int tree_workgroups(int dim, int blocks) { return dim == 64 && blocks 
 // Columns of a tile at most: what a wave's registers hold beside the K and V on their way.
 constexpr int tree_columns(int dim) { return dim == 64 ? 64 : 48; }
 // Subtiles a wave has in flight, in registers: two where there is room for them.
+// (64 requests of 5 rows over 256 - 4096 tokens: 121 us, with one set 140.)
 constexpr int tree_depth(int dim, int blocks) { return dim == 64 || blocks <= 2 ? 2 : 1; }
 
 template <int DT, int kD, int kBlocks> struct TreeShape {
@@ -138,7 +144,8 @@ __device__ __forceinline__ void share_and_head(const TreeArgs &a, int &share, in
 }
 
 // Column tiles side by side.  Where (nearly) all requests have a.sides column tiles, their workgroups walk the same
-// tokens at the same time, on one XCD: K and V then come from its L2 for all but one of them.  Units are subtiles there, and
+// tokens at the same time, on one XCD: K and V then come from its L2 for all but one of them (16 trees of 33 - 64 rows, two
+// tiles: 0.34 instead of 1.08 GB from HBM, 308 us instead of 320).  Units are subtiles there, and
 // share (x + 8 j) takes column tile j % sides of span x + 8 (j / sides).  (n_shares is a multiple of 8 * sides.)
 __device__ __forceinline__ int share_of_span(int span, int side, int sides) { return span % 8 + 8 * (span / 8 * sides + side); }
 __device__ __forceinline__ bool side_by_side(const TreeArgs &a, long units, long spans)

@@ -3,11 +3,17 @@
 // memory.  See tree_kernel.h for how the work is cut.  sm_scale is positive: a masked score is -infinity before it is
 // scaled.
 //
-// Bound by the matrix pipeline and the vector instructions beside it: 16 of 32x32x16 per block and wave, 16 exponentials a
-// lane.  Iteration j of a walk multiplies P(j - 1) into V(j - 1), turns S(j) into P(j) and computes S(j + 1), so that all of
+// Bound by the matrix pipeline and the vector instructions beside it: 16 of 32x32x16 per block and wave, 16 exponentials and some 75
+// other instructions.  16 requests over 1 - 16 K tokens, 64 heads over 8, bf16: with 64 rows each 316 us, 920 TFLOP/s; with 33
+// to 64 rows 295, 750 TFLOP/s, since a block lasts as long as its units with two busy waves, and columns come in
+// thirty-twos; of that 22 us are the launch for cut items (66 MB of partials).
+// Measured and left out: priority for the matrix instructions (281 for 276 us), exponentials free to move through the iteration (285).
+// Iteration j of a walk multiplies P(j - 1) into V(j - 1), turns S(j) into P(j) and computes S(j + 1), so that all of
 // its matrix instructions are independent of its exponentials.  Blocks lie in kStages stages of K and of V; iteration j
-// requests K(j + kStages) and V(j + kStages - 2) behind its only barrier, and reads the operands of K(j + 2) at its end.  The running maximum of a column is raised only when
-// a block's weights under it sum to more than kMostWeight in a lane.
+// requests K(j + kStages) and V(j + kStages - 2) behind its only barrier, and reads the operands of K(j + 2) at its end; with eight
+// stages there is room for two iterations to a barrier (276 us instead of 285 for 48 rows), V one block later.  The running maximum
+// of a column is raised only when a block's weights under it sum to more than kMostWeight in a lane.  Weights are rounded to 16
+// bits for the matrix product, half a step of each; sums, maxima and O stay in 32.
 // Where a token lies in the pool is looked up for some thousand tokens at a time and kept in LDS (row numbers, a bit per token that
 // there is), so that pages may have any size and the loop's loads wait for nothing but LDS.
 #pragma once

