@@ -266,7 +266,7 @@ __device__ __forceinline__ void tree_place(const TreeArgs &a, int share, TreePla
                     const int of_item = (int)((unsigned)p / (unsigned)tiles), ct = (span - first) / of_item;
                     const int item = before + ct * r.subtiles;
                     found_begin = item + (span - first - ct * of_item) * part;
-                    found_end = min(found_begin + part, item + r.subtiles);
+                    found_end = found_begin + min(part, item + r.subtiles - found_begin);
                     found_b = b0;
                     found_base = before;
                     found_r = r;

@@ -370,7 +370,7 @@ template <int DT> __global__ __launch_bounds__(kVerifyThreads) void verify_draw_
     if (threadIdx.x == 0) a.out_tokens[s.first + s.count - 1] = token;
 }
 
-static int verify_parts(int vocab) { return (vocab + kPart - 1) / kPart; }
+static int verify_parts(int vocab) { return (vocab - 1) / kPart + 1; }
 
 }  // namespace dskv
 

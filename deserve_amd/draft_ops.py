@@ -222,7 +222,11 @@ def rope_append_slots(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tenso
 class BatchTreeWithPagedKVCacheWrapper:
     """Attention of the rows of a step over the paged context and over the rows that they descend from, with the
     begin_forward / forward / end_forward protocol of paged_ops.  begin_forward plans nothing and reads nothing back: the kernel
-    takes lengths and tables from the device, so a captured step can be replayed with others."""
+    takes lengths and tables from the device, so a captured step can be replayed with others.
+    workspace_buffer: scratch of a forward while it runs (the 128 MiB of exec.get_wrappers hold every usual shape; one that needs
+    more is refused); forwards that may run at the same time, on two streams, need one each.
+    For requests of up to 1024 rows at head_dim 64 or 128; longer chunks and other dims are right, too, but read the context
+    once a row: prompts are the prefill wrapper's."""
 
     def __init__(self, workspace_buffer: torch.Tensor, kv_layout: str = "NHD") -> None:
         if kv_layout != "NHD":

@@ -191,7 +191,8 @@ class BatchVerify(BatchExec):
 
     def prepare(self) -> None:
         with torch.inference_mode():
-            wrapper = get_tree_wrapper(self.kvcaches[0].pool.main_device)
+            # a wrapper of its own, which costs nothing: a step prepared in between does not change this one
+            wrapper = BatchTreeWithPagedKVCacheWrapper(get_tree_wrapper(self.kvcaches[0].pool.main_device)._workspace)
             self.tree_ctx = FlashTreeCtx.init_and_plan(self.task_datas, self.kvcaches, wrapper, parents=self.parents,
                                                        **self._shape_kwargs())
 

@@ -126,6 +126,30 @@ def test_steps_leave_what_a_prefill_of_the_sequence_writes(kind, dtype, page):
                 assert (np.abs(off) <= bound[csr[0][b] + pos]).all(), (b, pos, layer)
 
 
+def test_steps_prepared_ahead_keep_their_own_tables():
+    dt = DTYPES["bf16"]
+    stage = PackedKVStage(StageArgs(HQ, HKV, HQ * DIM, 16, LAYERS, THETA))
+    pool, caches = _caches(2, 40, 16, dt)
+    tasks = [TaskData("a", 0, 0, 70, 70), TaskData("b", 0, 0, 20, 20)]
+    gen = torch.Generator().manual_seed(9)
+    randn = lambda n: torch.randn(n, LAYERS, HQ + 2 * HKV, DIM, generator=gen).to(dt).to(DEV)
+    _prefill(randn(90), tasks, caches)
+    for t, n in zip(tasks, (6, 3)):
+        t.step()
+        t.init(n)
+    xs = [randn(6), randn(3)]
+    steps = lambda: [BatchVerify(x, stage, [t], [c]) for x, t, c in zip(xs, tasks, caches)]
+    want = []
+    for s in steps():
+        s.prepare()
+        want.append(s.step().all_xs.clone())
+    ahead = steps()
+    for s in ahead:
+        s.prepare()
+    for s, w in zip(ahead, want):
+        assert torch.equal(s.step().all_xs, w)
+
+
 class _Program:
     """Buffers of a step, and the step over them: lengths stay on the device and go on by what was given."""
 
