@@ -178,10 +178,11 @@ template <int DT, int kD, int kCols, int kSub, int kLeast> static int launch_tre
     // few items are cut into many parts each, many into few: one request over 4 K tokens 16.8 us with four groups of parts and 20.1 with
     // one, 64 requests 189 with one and 196 with four
     const bool many_parts = (long)a.batch * f.col_tiles * 4 < f.shares;
-    const int columns = 256 / (kD / 4 * (many_parts ? 4 : 1));
+    constexpr int kEach = kCols >= 128 ? 4 : 1;
+    const int columns = 256 / (kD / 4) * (many_parts ? 1 : kEach) / (many_parts ? 4 : 1);
     const dim3 grid((unsigned)(a.batch * f.col_tiles), (unsigned)a.n_kv_heads, (unsigned)((kCols + columns - 1) / columns));
-    if (many_parts) hipLaunchKernelGGL((tree_merge_kernel<DT, kD, kCols, kSub, kLeast, 4>), grid, dim3(256), 0, stream, a, f.col_tiles);
-    else hipLaunchKernelGGL((tree_merge_kernel<DT, kD, kCols, kSub, kLeast, 1>), grid, dim3(256), 0, stream, a, f.col_tiles);
+    if (many_parts) hipLaunchKernelGGL((tree_merge_kernel<DT, kD, kCols, kSub, kLeast, 4, 1>), grid, dim3(256), 0, stream, a, f.col_tiles);
+    else hipLaunchKernelGGL((tree_merge_kernel<DT, kD, kCols, kSub, kLeast, 1, kEach>), grid, dim3(256), 0, stream, a, f.col_tiles);
     DSKV_LAUNCH_CHECK("tree_merge_kernel");
     return 0;
 }

@@ -772,8 +772,9 @@ __global__ __launch_bounds__(kTreeThreads, tree_workgroups(kD, kBlocks)) void tr
 }
 
 // Items that were cut: a thread per (column, four dims) and group of parts.  kGroups > 1, for items in many parts: each takes
-// every kGroups-th part, and they meet in LDS.
-template <int DT, int kD, int kCols, int kSub, int kLeast, int kGroups>
+// every kGroups-th part, and they meet in LDS.  kEach > 1, for many columns: columns that a thread takes at once (66
+// MB of partials, 16 trees of 33 - 64 rows: 16 us with four, 23 with one).
+template <int DT, int kD, int kCols, int kSub, int kLeast, int kGroups, int kEach>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int max_col_tiles)
 {
     constexpr int kElt = DT == DSKV_F32 ? 4 : 2;
@@ -784,11 +785,9 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int max_col
     const int before = a.units_before[b], units = a.units_before[a.batch];
     const bool beside = a.units_before[a.batch + 1] != 0;
     const int part_units = a.units_before[a.batch + 2];        // 0: equal shares
-    const int col = blockIdx.z * kColumns + column;
-    const int cols = min(r.n * a.group - ct * r.tile, r.tile);
-    if (ct >= r.col_tiles || (int)blockIdx.z * kColumns >= cols || units == 0) return;
+    const int cols = min(r.n * a.group - ct * r.tile, r.tile), col0 = (int)blockIdx.z * kColumns * kEach + column;
+    if (ct >= r.col_tiles || (int)blockIdx.z * kColumns * kEach >= cols || units == 0) return;
     const Shares shares = shares_of(beside ? a.n_shares / a.sides : a.n_shares, units, kLeast);
-    const bool there = col < cols;
     const int first = before + (beside ? 0 : ct * r.subtiles), last = first + r.subtiles - 1;
     int s0, s1;
     bool second = false;                                       // in the first of its shares the item is the second
@@ -802,53 +801,68 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int max_col
         second = share_begin(shares, s0) < first;
     }
     if (s0 == s1) return;
-    float top = -INFINITY, sum = 0;
-    f32x4 acc = {0, 0, 0, 0};
-    auto add = [&](float pm, float pl, f32x4 po) {
-        const float m = fmaxf(top, pm), from = m == -INFINITY ? 0.f : m;
-        const float w0 = __builtin_amdgcn_exp2f(top - from), w1 = __builtin_amdgcn_exp2f(pm - from);
-        top = m;
-        sum = sum * w0 + pl * w1;
-        acc = acc * w0 + po * w1;
+    float top[kEach], sum[kEach];
+    f32x4 acc[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; e++) {
+        top[e] = -INFINITY;
+        sum[e] = 0;
+        acc[e] = f32x4{0, 0, 0, 0};
+    }
+    auto add = [&](int e, float pm, float pl, f32x4 po) {
+        const float m = fmaxf(top[e], pm), from = m == -INFINITY ? 0.f : m;
+        const float w0 = __builtin_amdgcn_exp2f(top[e] - from), w1 = __builtin_amdgcn_exp2f(pm - from);
+        top[e] = m;
+        sum[e] = sum[e] * w0 + pl * w1;
+        acc[e] = acc[e] * w0 + po * w1;
     };
-    if (there) {
-        constexpr int kAhead = 4;                  // parts requested together
-        for (int s = s0 + group; s <= s1; s += kAhead * kGroups) {
-            float pm[kAhead], pl[kAhead];
-            f32x4 po[kAhead];
+    constexpr int kAhead = kEach > 1 ? 2 : 4;          // parts requested together
+    for (int s = s0 + group; s <= s1; s += kAhead * kGroups) {
+        float pm[kAhead][kEach], pl[kAhead][kEach];
+        f32x4 po[kAhead][kEach];
 #pragma unroll
-            for (int i = 0; i < kAhead; i++) {
-                const int si = min(s + i * kGroups, s1);
-                const long slot = 2L * (beside ? share_of_span(si, ct, a.sides) : si) + (si == s0 && second ? 1 : 0);
-                const long part = (slot * a.n_kv_heads + head) * kCols + col;
-                pm[i] = a.part_ml[part * 2];
-                pl[i] = a.part_ml[part * 2 + 1];
-                po[i] = *reinterpret_cast<const f32x4 *>(a.part_o + part * kD + quad * 4);
+        for (int i = 0; i < kAhead; i++) {
+            const int si = min(s + i * kGroups, s1);
+            const long slot = 2L * (beside ? share_of_span(si, ct, a.sides) : si) + (si == s0 && second ? 1 : 0);
+#pragma unroll
+            for (int e = 0; e < kEach; e++) {
+                const long part = (slot * a.n_kv_heads + head) * kCols + min(col0 + e * kColumns, cols - 1);
+                pm[i][e] = a.part_ml[part * 2];
+                pl[i][e] = a.part_ml[part * 2 + 1];
+                po[i][e] = *reinterpret_cast<const f32x4 *>(a.part_o + part * kD + quad * 4);
             }
-#pragma unroll
-            for (int i = 0; i < kAhead; i++)
-                if (s + i * kGroups <= s1) add(pm[i], pl[i], po[i]);
         }
+#pragma unroll
+        for (int i = 0; i < kAhead; i++)
+            if (s + i * kGroups <= s1) {
+#pragma unroll
+                for (int e = 0; e < kEach; e++) add(e, pm[i][e], pl[i][e], po[i][e]);
+            }
     }
     if constexpr (kGroups > 1) {
+        static_assert(kEach == 1, "the groups meet over one column a thread");
         __shared__ f32x4 acc_of[kGroups][kColumns * kQuads];
         __shared__ float ml_of[kGroups][kColumns][2];
-        acc_of[group][column * kQuads + quad] = acc;
+        acc_of[group][column * kQuads + quad] = acc[0];
         if (quad == 0) {
-            ml_of[group][column][0] = top;
-            ml_of[group][column][1] = sum;
+            ml_of[group][column][0] = top[0];
+            ml_of[group][column][1] = sum[0];
         }
         __syncthreads();
         if (group > 0) return;
 #pragma unroll
-        for (int w = 1; w < kGroups; w++) add(ml_of[w][column][0], ml_of[w][column][1], acc_of[w][column * kQuads + quad]);
+        for (int w = 1; w < kGroups; w++) add(0, ml_of[w][column][0], ml_of[w][column][1], acc_of[w][column * kQuads + quad]);
     }
-    if (!there) return;
-    const int at = ct * r.tile + col, i = at / a.group, hq = head * a.group + at - i * a.group;
-    const float inv = sum == 0 ? 0.f : 1.f / sum;
-    char *dst = a.out + (((r.first + i) * a.n_qo_heads + hq) * kD + quad * 4) * kElt;
-    if constexpr (DT == DSKV_F32) *reinterpret_cast<f32x4 *>(dst) = acc * inv;
-    else *reinterpret_cast<u32x2 *>(dst) = u32x2{Elt<DT>::pack2(acc.x * inv, acc.y * inv), Elt<DT>::pack2(acc.z * inv, acc.w * inv)};
+#pragma unroll
+    for (int e = 0; e < kEach; e++) {
+        const int col = col0 + e * kColumns;
+        if (col >= cols) break;
+        const int at = ct * r.tile + col, i = at / a.group, hq = head * a.group + at - i * a.group;
+        const float inv = sum[e] == 0 ? 0.f : 1.f / sum[e];
+        char *dst = a.out + (((r.first + i) * a.n_qo_heads + hq) * kD + quad * 4) * kElt;
+        if constexpr (DT == DSKV_F32) *reinterpret_cast<f32x4 *>(dst) = acc[e] * inv;
+        else *reinterpret_cast<u32x2 *>(dst) = u32x2{Elt<DT>::pack2(acc[e].x * inv, acc[e].y * inv), Elt<DT>::pack2(acc[e].z * inv, acc[e].w * inv)};
+    }
 }
 
 }  // namespace dskv

@@ -5,8 +5,8 @@
 //
 // Bound by the matrix pipeline and the vector instructions beside it: 16 of 32x32x16 per block and wave, 16 exponentials and some 75
 // other instructions.  16 requests over 1 - 16 K tokens, 64 heads over 8, bf16: with 64 rows each 316 us, 920 TFLOP/s; with 33
-// to 64 rows 295, 750 TFLOP/s, since a block lasts as long as its units with two busy waves, and columns come in
-// thirty-twos; of that 22 us are the launch for cut items (66 MB of partials).
+// to 64 rows 286, 777 TFLOP/s, since a block lasts as long as its units with two busy waves, and columns come in
+// thirty-twos; of that 16 us are the launch for cut items (66 MB of partials).
 // Measured and left out: priority for the matrix instructions (281 for 276 us), exponentials free to move through the iteration (285).
 // Iteration j of a walk multiplies P(j - 1) into V(j - 1), turns S(j) into P(j) and computes S(j + 1), so that all of
 // its matrix instructions are independent of its exponentials.  Blocks lie in kStages stages of K and of V; iteration j
