@@ -4,7 +4,7 @@
 // lanes that share lane % 16, so its maximum and sum never cross more than four lanes.
 // The work is cut without a host plan: request b has ct_b column tiles of kBlocks * 16 columns and st_b subtiles
 // of kSub tokens; all (request, column tile, subtile) units lie end to end, every workgroup takes the sums over the requests for
-// itself, and share s of n covers units [s U / n, (s + 1) U / n): equal to one unit, whatever the lengths.  One
+// itself, and takes one of n shares of them, equal to one unit whatever the lengths (see tree_place for small batches).  One
 // workgroup per (share, kv head); its four waves take the share's subtiles in turn, each with a running maximum, sum and O of
 // its own, and meet in LDS where an item (request, column tile) ends.  An item that a share boundary cuts leaves
 // a partial (maximum, sum, O in fp32) that tree_merge_kernel adds up.

@@ -81,7 +81,7 @@ class StepTables:
         # one allocation; the 64-bit arrays first
         words = [2 * max_tokens, 2 * max_tokens if tree else 0, batch + 1, batch + 1, max_pages, batch, max_tokens]
         slots, masks, qo_indptr, kv_indptr, indices, last, positions = \
-            torch.empty((sum(words),), dtype=torch.int32, device=device).split(words)
+            torch.empty((sum(words),), dtype=torch.int32, device=device).split_with_sizes(words)
         return cls(qo_indptr, kv_indptr, indices, last, positions, slots.view(torch.int64),
                    masks.view(torch.int64) if tree else None)
 
@@ -203,7 +203,7 @@ def rope_append_slots(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tenso
         if rope_table.dtype is not torch.float32 or len(table) != 2 or table[1] != dim or table[0] < nnz or not rope_table.is_contiguous() or rope_table.data_ptr() % 16:
             raise ValueError(f"rope_table must be a contiguous, 16-byte aligned float32 ({nnz}, {dim}) tensor")
         if out is None:
-            result = q.new_empty(q.shape)
+            result = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif out.shape != q.shape or out.dtype is not dtype or not out.is_contiguous():
             raise ValueError("out must be contiguous and of q's shape and dtype")
         else:
@@ -286,7 +286,7 @@ class BatchTreeWithPagedKVCacheWrapper:
         if masks is not None and masks.numel() < nnz:
             raise ValueError(f"masks hold {masks.numel()} rows, q has {nnz}")
         if out is None:
-            out = q.new_empty(q.shape)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif out.shape != q.shape or out.dtype is not dtype or not out.is_contiguous():
             raise ValueError("out must be contiguous and of q's shape and dtype")
         index = _on_device(q, paged_kv_data, out, self._held[0])
@@ -345,7 +345,7 @@ def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, uniforms: to
     lib = _lib.lib()
     need = lib.dskv_verify_workspace(batch, vocab)
     # workspace and results, from the caching allocator for every call: calls on several streams share nothing
-    workspace, counts, path, given = tokens.new_empty((need // 4 + batch + 2 * nnz,)).split((need // 4, batch, nnz, nnz))
+    workspace, counts, path, given = tokens.new_empty((need // 4 + batch + 2 * nnz,)).split_with_sizes((need // 4, batch, nnz, nnz))
     _call("verify_drafts", index, lib.dskv_verify_drafts, counts.data_ptr(), path.data_ptr(), given.data_ptr(),
           target_probs.data_ptr(), target_probs.stride(0) if nnz > 1 else vocab, _lib.ptr(draft_probs),
           0 if draft_probs is None else draft_probs.stride(0) if nnz > 1 else vocab, tokens.data_ptr(), uniforms.data_ptr(),
