@@ -571,6 +571,14 @@ __global__ __launch_bounds__(kTreeThreads, tree_workgroups(kD, kBlocks)) void tr
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
+        // LDS operands are read together and ahead: one wave a SIMD has nobody to wait for them in its place
+        u32x4 key[S::kTiles][S::kSteps];
+#pragma unroll
+        for (int t = 0; t < S::kTiles; t++)
+#pragma unroll
+            for (int e = 0; e < S::kSteps; e++)
+                key[t][e] = *reinterpret_cast<const u32x4 *>(k_lds + (t * 16 + c) * S::kKPitch + e * 64 + g * 16);
+        __builtin_amdgcn_sched_barrier(0);
         const Ids ids_next = next_ids();
         request(ids, mine, held_here);
         ids = ids_next;
@@ -587,20 +595,34 @@ __global__ __launch_bounds__(kTreeThreads, tree_workgroups(kD, kBlocks)) void tr
             for (int k = 0; k < kBlocks; k++) s[k][t] = f32x4{0, 0, 0, 0};
 #pragma unroll
             for (int e = 0; e < S::kSteps; e++) {
-                const u32x4 key = *reinterpret_cast<const u32x4 *>(k_lds + (t * 16 + c) * S::kKPitch + e * 64 + g * 16);
 #pragma unroll
                 for (int k = 0; k < kBlocks; k++) {
                     if constexpr (DT == DSKV_F32) {
-                        const f32x4 kf = __builtin_bit_cast(f32x4, key), qf = __builtin_bit_cast(f32x4, q[k][e]);
+                        const f32x4 kf = __builtin_bit_cast(f32x4, key[t][e]), qf = __builtin_bit_cast(f32x4, q[k][e]);
 #pragma unroll
                         for (int j = 0; j < 4; j++)
                             s[k][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j], qf[j], s[k][t], 0, 0, 0);
                     } else {
-                        s[k][t] = Elt<DT>::mfma_k32(key, q[k][e], s[k][t]);
+                        s[k][t] = Elt<DT>::mfma_k32(key[t][e], q[k][e], s[k][t]);
                     }
                 }
             }
         }
+        // V's operands: four of a lane along the tokens for every 16 dims
+        u32x4 value[S::kDimTiles];
+#pragma unroll
+        for (int d = 0; d < S::kDimTiles; d++) {
+            if constexpr (DT == DSKV_F32) {
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    value[d][e] = *reinterpret_cast<const uint32_t *>(v_lds + (4 * g + e) * S::kVPitch + (d * 16 + c) * 4);
+            } else {
+                const char *at = v_lds + (4 * g + (c >> 2)) * S::kVPitch + d * 32 + (c & 3) * 8;
+                const u32x2 lo = read_transposed(at), hi = read_transposed(at + 16 * S::kVPitch);
+                value[d] = u32x4{lo.x, lo.y, hi.x, hi.y};
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
         // ---- weights, under a maximum that is raised only where they ask for it
         u32x4 p[kBlocks];                                  // 16-bit: the operand; fp32: four floats
 #pragma unroll
@@ -652,24 +674,16 @@ __global__ __launch_bounds__(kTreeThreads, tree_workgroups(kD, kBlocks)) void tr
         }
         // ---- output
 #pragma unroll
-        for (int d = 0; d < S::kDimTiles; d++) {
-            if constexpr (DT == DSKV_F32) {
+        for (int d = 0; d < S::kDimTiles; d++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float value = *reinterpret_cast<const float *>(v_lds + (4 * g + e) * S::kVPitch + (d * 16 + c) * 4);
+            for (int e = 0; e < (DT == DSKV_F32 ? 4 : 1); e++)
 #pragma unroll
-                    for (int k = 0; k < kBlocks; k++)
-                        o[k][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                            value, __builtin_bit_cast(f32x4, p[k])[e], o[k][d], 0, 0, 0);
+                for (int k = 0; k < kBlocks; k++) {
+                    if constexpr (DT == DSKV_F32)
+                        o[k][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, value[d])[e],
+                                                                       __builtin_bit_cast(f32x4, p[k])[e], o[k][d], 0, 0, 0);
+                    else o[k][d] = Elt<DT>::mfma_k32(value[d], p[k], o[k][d]);
                 }
-            } else {
-                const char *at = v_lds + (4 * g + (c >> 2)) * S::kVPitch + d * 32 + (c & 3) * 8;
-                const u32x2 lo = read_transposed(at), hi = read_transposed(at + 16 * S::kVPitch);
-                const u32x4 value = {lo.x, lo.y, hi.x, hi.y};
-#pragma unroll
-                for (int k = 0; k < kBlocks; k++) o[k][d] = Elt<DT>::mfma_k32(value, p[k], o[k][d]);
-            }
-        }
         st += kTreeWaves;
     };
     auto finish_item = [&]() {
