@@ -32,7 +32,7 @@ __device__ __forceinline__ int request_of_row(const int32_t *indptr, int batch, 
 // Any type and head dim: one workgroup per (row, q head) whose waves take every kGenericWaves-th group of four
 // keys.  Lane (g, c) holds dims 8 c .. 8 c + 7 (and 128 more ..) of key g of the group.  Bound by the
 // latency of its loads: K and V are read once per row and q head, from the caches but for the first time (64 requests of 5 rows
-// over 4 K tokens, 128 dims, 1628 us where the matrix form takes 119): for head dims and sizes that the others do not take.
+// over 4 K tokens, 128 dims, 1628 us where the matrix form takes 118): for head dims and sizes that the others do not take.
 constexpr int kGenericWaves = 8;
 constexpr int kTreeUnits = 256;        // compute units
 
