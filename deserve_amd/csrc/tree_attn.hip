@@ -161,10 +161,11 @@ static TreeForm tree_form(bool wide, int max_rows, int n_qo_heads, int n_kv_head
 // More columns than a wave of the narrow form holds go to the wide one, which reads K and V once for all of them: 64
 // requests of 13 rows (52 columns) over 4 K tokens 219 us, narrow 373; of 12 rows 198 narrow, 218 wide (bf16, 32 heads over 8).
 // Up to 128 columns by four waves, two workgroups a unit: 64 requests of 16 rows 219 us, by eight waves 228; more by
-// eight: 16 trees of 48 rows over 1 - 16 K (64 heads) 272 us, by four waves 308.
+// eight: 16 trees of 48 rows over 1 - 16 K (64 heads) 272 us, by four waves 308.  With 64 dims 64 requests of 20 rows (80 columns)
+// 127 us, narrow 204; of 16 rows 109 narrow.
 static bool wide_form(int max_rows, int n_qo_heads, int n_kv_heads, int head_dim, int dtype)
 {
-    return head_dim == 128 && dtype != DSKV_F32 && (long)max_rows * (n_qo_heads / n_kv_heads) > tree_columns(head_dim);
+    return dtype != DSKV_F32 && (long)max_rows * (n_qo_heads / n_kv_heads) > tree_columns(head_dim);
 }
 static int64_t units_bytes(int batch) { return ((int64_t)batch + 6) / 4 * 16; }
 static int64_t slots_of(const TreeForm &f, int n_kv_heads) { return 2LL * f.shares * n_kv_heads * f.cols; }
@@ -194,17 +195,17 @@ template <int DT, int kD, int kBlocks> static int launch_tree(const TreeArgs &a,
     DSKV_LAUNCH_CHECK("tree_matrix_kernel");
     return launch_tree_merge<DT, kD, S::kCols, S::kSub, kTreeWaves>(a, f, stream);
 }
-template <int DT, int kWaves> static int launch_tree_wide(const TreeArgs &a, const TreeForm &f, hipStream_t stream)
+template <int DT, int kD, int kWaves> static int launch_tree_wide(const TreeArgs &a, const TreeForm &f, hipStream_t stream)
 {
-    hipLaunchKernelGGL((tree_wide_kernel<DT, kWaves>), dim3((unsigned)(f.shares * a.n_kv_heads)), dim3(kWaves * 64), 0, stream, a);
+    hipLaunchKernelGGL((tree_wide_kernel<DT, kD, kWaves>), dim3((unsigned)(f.shares * a.n_kv_heads)), dim3(kWaves * 64), 0, stream, a);
     DSKV_LAUNCH_CHECK("tree_wide_kernel");
-    return launch_tree_merge<DT, 128, kWaves * 32, kWideBlock, kWideLeast>(a, f, stream);
+    return launch_tree_merge<DT, kD, kWaves * 32, kWideBlock, kWideLeast>(a, f, stream);
 }
 template <int DT, int kD> static int launch_tree_blocks(const TreeArgs &a, const TreeForm &f, hipStream_t stream)
 {
-    if constexpr (DT != DSKV_F32 && kD == 128) {
-        if (f.wide_waves == 4) return launch_tree_wide<DT, 4>(a, f, stream);
-        if (f.wide_waves == 8) return launch_tree_wide<DT, 8>(a, f, stream);
+    if constexpr (DT != DSKV_F32) {
+        if (f.wide_waves == 4) return launch_tree_wide<DT, kD, 4>(a, f, stream);
+        if (f.wide_waves == 8) return launch_tree_wide<DT, kD, 8>(a, f, stream);
     }
     switch (f.blocks) {
     case 1: return launch_tree<DT, kD, 1>(a, f, stream);

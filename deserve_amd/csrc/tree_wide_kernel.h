@@ -1,13 +1,16 @@
-// The tree attention for more columns than fit a wave (head_dim 128, 16 bits): the columns are split over the waves of
+// The tree attention for more columns than fit a wave (head_dim 64 and 128, 16 bits): the columns are split over the waves of
 // a workgroup, 32 each, and all of them read the same 32-token blocks of K and V from LDS, which go there straight from
 // memory.  See tree_kernel.h for how the work is cut.  sm_scale is positive: a masked score is -infinity before it is
 // scaled.
 //
 // Bound by the matrix pipeline and the vector instructions beside it: 16 of 32x32x16 per block and wave, 16 exponentials and some 75
-// other instructions.  16 requests over 1 - 16 K tokens, 64 heads over 8, bf16: with 64 rows each 316 us, 920 TFLOP/s; with 33
+// other instructions (128 dims).  16 requests over 1 - 16 K tokens, 64 heads over 8, bf16: with 64 rows each 316 us, 920 TFLOP/s; with 33
 // to 64 rows 286, 777 TFLOP/s, since a block lasts as long as its units with two busy waves, and columns come in
 // thirty-twos; of that 16 us are the launch for cut items (66 MB of partials).
+// With 64 dims a stage holds two blocks side by side, so that a load fetches whole kilobytes there, too, and both sizes share one
+// layout of LDS: 16 requests of 48 rows, 64 heads, 175 us (the narrow form: 333).
 // Measured and left out: priority for the matrix instructions (281 for 276 us), exponentials free to move through the iteration (285).
+//
 // Iteration j of a walk multiplies P(j - 1) into V(j - 1), turns S(j) into P(j) and computes S(j + 1), so that all of
 // its matrix instructions are independent of its exponentials.  Blocks lie in kStages stages of K and of V; iteration j
 // requests K(j + kStages) and V(j + kStages - 2) behind its only barrier, and reads the operands of K(j + 2) at its end; with eight
@@ -23,26 +26,32 @@
 namespace dskv {
 
 constexpr int kWideBlock = 32;
-constexpr int kWideRegion = 1088;           // four rows, chunk by chunk ((4 c + row) * 16), and 64 bytes of padding
+constexpr int kWideRegion = 1088;           // 1 KB that a wave's load fetches, (4 chunk + row) * 16 of four rows, and 64 bytes of padding
 constexpr int kWideStage = kWideBlock / 4 * kWideRegion;
 constexpr int kWideLeast = 8;               // units a share has at least: what fills the stages takes about as long
 constexpr int kBadBlocks = kTreeMostRows / kWideBlock + 2;       // that new rows reach into
 
-template <int kWaves> struct WideShape {
+template <int kD, int kWaves> struct WideShape {
     static constexpr int kThreads = kWaves * 64;
     static constexpr int kCols = kWaves * 32;
-    static constexpr int kGroups = 8 / kWaves;           // regions of a block that a wave requests
+    static constexpr int kPack = 128 / kD;               // blocks of a stage: rows of 128 bytes lie side by side with the next block's
+    static constexpr int kChunks = kD / 8;               // 16-byte chunks of a row
+    static constexpr int kSteps = kD / 16, kDims = kD / 32;      // matrix instructions of a block's scores; 32-dim tiles of O
+    static constexpr int kGroups = 8 / kWaves;           // regions of a stage that a wave requests
     static constexpr int kHalf = kWaves == 8 ? 64 : 32;  // blocks that are looked up at a time; two such halves are kept
     static constexpr int kTokens = 2 * kHalf * kWideBlock;
-    static constexpr int kPair = kWaves == 8 ? 2 : 1;    // iterations between barriers
-    static constexpr int kStages = kWaves == 8 ? 8 : 4;  // blocks of K, and of V, in LDS: as many as fit beside the other workgroup
+    static constexpr int kPair = kWaves == 8 || kPack == 2 ? 2 : 1;      // iterations between barriers
+    static constexpr int kAsked = kPair / kPack;         // stages of K, and of V, that are requested there
+    static constexpr int kStages = kWaves == 8 && kPack == 1 ? 8 : 4;    // of K, and of V, in LDS: as many as fit beside the other workgroup
+    // a wave's loads that may be on their way behind a barrier's wait: all but those of K(j + 2) .., V(j - 1) ..
+    static constexpr int kInFlight = (2 * kStages - 2 - 3 * kAsked - (kPack - 1)) * kGroups;
 };
 
-template <int DT, int kWaves>
+template <int DT, int kD, int kWaves>
 __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
 {
     typedef Elt<DT> E;
-    typedef WideShape<kWaves> W;
+    typedef WideShape<kD, kWaves> W;
     __shared__ __align__(16) char lds[2 * W::kStages * kWideStage];
     __shared__ int32_t row_at[W::kTokens];               // row of the pool (page * 2 P + place), -1: none
     __shared__ uint32_t held_at[2 * W::kHalf];           // bit per token of a block: there is one
@@ -64,11 +73,16 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
     auto k_stage = [&](int i) { return lds + i * kWideStage; };
     auto v_stage = [&](int i) { return lds + (W::kStages + i) * kWideStage; };
     constexpr int kLast = W::kStages - 1;
-    const int row_bytes = a.n_kv_heads * 256;
+    // block j + n - j % 4 (of the walk, n a literal) in its stage of K or V
+    auto block_at = [&](auto &stage, int j, int n) -> char * {
+        if (W::kPack == 2) return stage((((j >> 2) << 1) + (n >> 1)) & kLast) + (n & 1) * 512;
+        return stage((n + (W::kStages == 8 ? j & 4 : 0)) & kLast);
+    };
+    const int row_bytes = a.n_kv_heads * kD * 2;
     const long half_bytes = (long)a.page_size * row_bytes;
     // lane p of a load fetches chunk p / 4 of row p % 4 of a region
-    const char *const pool = a.pages + head * 256 + (lane >> 2) * 16;
-    const char *const none = reinterpret_cast<const char *>(kNoRow) + (lane >> 2) * 16;
+    const char *const pool = a.pages + head * kD * 2 + (lane >> 2) % W::kChunks * 16;
+    const char *const none = reinterpret_cast<const char *>(kNoRow) + (lane >> 2) % W::kChunks * 16;
 
     while (unit < end) {
         if (unit >= base + (int)units_of(r, beside)) {             // on to the next request that has rows
@@ -102,11 +116,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
             const long lim = a.masks ? (long)prior + DSKV_MAX_TREE_ROWS : (long)prior + row_i + 1;
             limit = (int)max(min(lim, (long)t_end), 0L);
         }
-        u32x4 q[8];
+        u32x4 q[W::kSteps];
         {
-            const char *row = a.q + q_row * a.q_stride + hq * 256 + h * 16;
+            const char *row = a.q + q_row * a.q_stride + hq * kD * 2 + h * 16;
 #pragma unroll
-            for (int s = 0; s < 8; s++) {
+            for (int s = 0; s < W::kSteps; s++) {
                 q[s] = u32x4{0, 0, 0, 0};
                 if (there) q[s] = *reinterpret_cast<const u32x4 *>(row + s * 32);
             }
@@ -115,11 +129,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
         const int first_i = (ct * r.tile + wave * 32) / a.group;
         int mask_from = min(a.masks ? prior : prior + first_i + 1, t_end);
 
-        f32x16 acc[4], xs[2];
+        f32x16 acc[W::kDims], xs[2];
         float m_run = -__FLT_MAX__, l_run = 0;
         u32x4 pb[2][2];
 #pragma unroll
-        for (int d = 0; d < 4; d++)
+        for (int d = 0; d < W::kDims; d++)
 #pragma unroll
             for (int v = 0; v < 16; v++) acc[d][v] = 0;
         pb[1][0] = pb[1][1] = u32x4{0, 0, 0, 0};
@@ -139,11 +153,12 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
                 if ((lane & 31) == 0) held_at[at / kWideBlock] = (uint32_t)(there64 >> (lane & 32));
             }
         };
-        // rows of the pool that the lane requests 16 bytes of for block j
+        // rows of the pool that the lane requests 16 bytes of for stage u of the walk
         struct Where {
             int row[W::kGroups];
         };
-        auto where = [&](int j, Where &w) {
+        auto where = [&](int u, Where &w) {
+            const int j = W::kPack == 2 ? 2 * u + (lane >> 5) : u;
 #pragma unroll
             for (int i = 0; i < W::kGroups; i++) {
                 const int at = (j & (2 * W::kHalf - 1)) * kWideBlock + (wave * W::kGroups + i) * 4 + (lane & 3);
@@ -172,18 +187,18 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
 #define DSKV_WAIT_VMEM(n) __builtin_amdgcn_s_waitcnt(((n) & 15) | 0x70 | 0xF00 | (((n) >> 4) << 14))
 
         // ---- parts of an iteration
-        u32x4 key[8];                                    // K operand: token r32, dims 16 s + 8 h ..
+        u32x4 key[W::kSteps];                                    // K operand: token r32, dims 16 s + 8 h ..
         auto read_keys = [&](const char *stage) {
             // token r32 = row r32 & 3 of region r32 >> 2; chunk 2 s + h
             const char *rows = stage + (r32 >> 2) * kWideRegion + h * 64 + (r32 & 3) * 16;
 #pragma unroll
-            for (int s = 0; s < 8; s++) key[s] = *reinterpret_cast<const u32x4 *>(rows + s * 128);
+            for (int s = 0; s < W::kSteps; s++) key[s] = *reinterpret_cast<const u32x4 *>(rows + s * 128);
         };
         auto scores = [&](f32x16 &x) {
 #pragma unroll
             for (int v = 0; v < 16; v++) x[v] = 0;
 #pragma unroll
-            for (int s = 0; s < 8; s++) x = E::mfma_32x32(key[s], q[s], x);
+            for (int s = 0; s < W::kSteps; s++) x = E::mfma_32x32(key[s], q[s], x);
         };
         // bits of block j's tokens that the column sees
         auto seen_of = [&](int j) { return seen_bits((st0 + j) * kWideBlock, prior, limit, mask, !a.masks); };
@@ -217,26 +232,29 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
             m_run = m_new;
             l_run *= keep;
 #pragma unroll
-            for (int d = 0; d < 4; d++) acc[d] *= keep;
+            for (int d = 0; d < W::kDims; d++) acc[d] *= keep;
         };
         const int v_off = h * kWideRegion + (2 * (g & 1) + ((c & 3) >> 1)) * 64 + (c >> 2) * 16 + (c & 1) * 8;
         // A weight of 0 times a V that is no number would reach columns that do not see the token: such tokens among the new
         // ones are taken out of the block here, by the wave that requested them, and added behind the walk.
         const int new_from = max((max(prior, 0) >> 5) - st0, 0), new_to = min(((int)r.kv_len + 31) / 32 - st0, blocks);
-        auto set_aside = [&](int j) {
+        auto set_aside = [&](int u) {                    // of stage u
+            const int j = W::kPack == 2 ? 2 * u + (lane >> 5) : u;
+            const bool is_new = j >= new_from && j < new_to;
 #pragma unroll
             for (int i = 0; i < W::kGroups; i++) {
                 const int region = wave * W::kGroups + i;
-                u32x4 *at = reinterpret_cast<u32x4 *>(v_stage(j & kLast) + region * kWideRegion + lane * 16);
-                const bool odd = no_number<DT>(*at);
+                u32x4 *at = reinterpret_cast<u32x4 *>(v_stage(u & kLast) + region * kWideRegion + lane * 16);
+                const bool odd = is_new && no_number<DT>(*at);
                 const unsigned long long lanes = __ballot(odd);
                 if (__builtin_expect(lanes != 0, 0)) {
+                    const unsigned long long of_block = W::kPack == 1 ? lanes : lane < 32 ? lanes & 0xffffffff : lanes >> 32 << 32;
                     uint32_t rows = 0;
 #pragma unroll
                     for (int row = 0; row < 4; row++)
-                        if (lanes & (0x1111111111111111ull << row)) rows |= 1u << row;
+                        if (of_block & (0x1111111111111111ull << row)) rows |= 1u << row;
                     if ((rows >> (lane & 3)) & 1) *at = u32x4{0, 0, 0, 0};
-                    if (lane == 0) atomicOr(&bad_at[j - new_from], rows << (4 * region));
+                    if (rows != 0 && (W::kPack == 1 ? lane : lane & 31) == 0) atomicOr(&bad_at[j - new_from], rows << (4 * region));
                 }
             }
         };
@@ -252,70 +270,73 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
         if (holes) mask_from = 0;
         // q and the mask are waited for here: left to the loop, that would be a wait for all of its loads
 #pragma unroll
-        for (int s = 0; s < 8; s++) asm volatile("" : "+v"(q[s]));
+        for (int s = 0; s < W::kSteps; s++) asm volatile("" : "+v"(q[s]));
         asm volatile("" : "+v"(mask));
-        Where at_v[W::kPair], at_between, at_k[W::kPair];     // of the blocks that the next requests are for
+        Where at_v[W::kAsked], at_between, at_k[W::kAsked];     // of the stages that the next requests are for
         {
-            // as heads -kStages .. would request them
+            // as if there were iterations in front
             Where w[W::kStages];
 #pragma unroll
             for (int i = 0; i < W::kStages; i++) where(i, w[i]);
 #pragma unroll
-            for (int i = 0; i < W::kStages; i += W::kPair) {
+            for (int i = 0; i < W::kStages; i += W::kAsked) {
 #pragma unroll
-                for (int x = i; x < i + W::kPair; x++) request(w[x], k_stage(x), 0);
+                for (int x = i; x < i + W::kAsked; x++) request(w[x], k_stage(x), 0);
 #pragma unroll
-                for (int x = max(i - W::kPair - 1, 0); x < i - 1; x++) request(w[x], v_stage(x), half_bytes);
+                for (int x = max(i - W::kAsked - 1, 0); x < i - 1; x++) request(w[x], v_stage(x), half_bytes);
             }
 #pragma unroll
-            for (int x = 0; x < W::kPair; x++) {
-                at_v[x] = w[W::kStages - 1 - W::kPair + x];
+            for (int x = 0; x < W::kAsked; x++) {
+                at_v[x] = w[W::kStages - 1 - W::kAsked + x];
                 where(W::kStages + x, at_k[x]);
             }
             at_between = w[W::kStages - 1];
-            DSKV_WAIT_VMEM((2 * W::kStages - 3 - W::kPair) * W::kGroups);              // K(0) and K(1)
+            DSKV_WAIT_VMEM((2 * W::kStages - 3 - W::kAsked) * W::kGroups);              // the first two stages of K
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         if (works) {
-            read_keys(k_stage(0));
+            read_keys(block_at(k_stage, 0, 0));
             scores(xs[0]);
             if ((st0 + 1) * kWideBlock > mask_from) mask_scores(0, xs[0]);
-            read_keys(k_stage(1));
+            read_keys(block_at(k_stage, 0, 1));
         }
         // in front of iterations j .. j + kPair - 1; phase = j % 4, a literal
         auto advance = [&](int j, int phase) {
-            const int hi = W::kStages == 8 ? j & 4 : 0;  // stage of block j: phase + hi
+            const int u = j / W::kPack;                  // the stage that block j is in
             // this wave's rows of K(j + 2), V(j - 1) and, for a pair, K(j + 3) and V(j) have landed
-            DSKV_WAIT_VMEM((2 * W::kStages - 2 - 3 * W::kPair) * W::kGroups);
+            DSKV_WAIT_VMEM(W::kInFlight);
             asm volatile("" ::: "memory");
+            if (W::kPack == 2) {
+                if (j + 1 >= new_from && j < new_to) set_aside(u);
+            } else {
 #pragma unroll
-            for (int x = j - 1; x < j - 1 + W::kPair; x++)
-                if (x >= new_from && x < new_to) set_aside(x);
+                for (int x = u - 1; x < u - 1 + W::kPair; x++)
+                    if (x >= new_from && x < new_to) set_aside(x);
+            }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
 #pragma unroll
-            for (int x = 0; x < W::kPair; x++) request(at_k[x], k_stage(phase + x + hi), 0);                   // K(j + kStages + x)
+            for (int x = 0; x < W::kAsked; x++) request(at_k[x], block_at(k_stage, j, phase + x), 0);          // stage u + kStages + x of K
 #pragma unroll
-            for (int x = 0; x < W::kPair; x++)                                           // V(j + kStages - 1 - kPair + x)
-                request(at_v[x], v_stage((phase + hi + kLast - W::kPair + x) & kLast), half_bytes);
+            for (int x = 0; x < W::kAsked; x++)                                  // and u + kStages - 1 - kAsked + x of V
+                request(at_v[x], W::kPack == 2 ? v_stage((u + 2) & kLast) : block_at(v_stage, j, phase + kLast - W::kAsked + x), half_bytes);
             at_v[0] = at_between;
-            if (W::kPair == 2) at_v[W::kPair - 1] = at_k[0];
-            at_between = at_k[W::kPair - 1];
+            if (W::kAsked == 2) at_v[W::kAsked - 1] = at_k[0];
+            at_between = at_k[W::kAsked - 1];
 #pragma unroll
-            for (int x = 0; x < W::kPair; x++) where(j + W::kStages + W::kPair + x, at_k[x]);
+            for (int x = 0; x < W::kAsked; x++) where(u + W::kStages + W::kAsked + x, at_k[x]);
         };
         auto iteration = [&](int j, int phase) {
-            const int hi = W::kStages == 8 ? j & 4 : 0;
             if (W::kPair == 1 || (phase & 1) == 0) advance(j, phase);
             if (!works || j > blocks) return;
             const int cur = phase & 1, nxt = cur ^ 1;
-            const char *rows = v_stage((phase + hi + kLast) & kLast) + v_off;                  // V(j - 1)
-            u32x4 va[4][2];
+            const char *rows = block_at(v_stage, j, phase - 1) + v_off;                        // V(j - 1)
+            u32x4 va[W::kDims][2];
 #pragma unroll
-            for (int d = 0; d < 4; d++)
+            for (int d = 0; d < W::kDims; d++)
 #pragma unroll
                 for (int s = 0; s < 2; s++) {
                     const char *p = rows + s * 4 * kWideRegion + d * 256;
@@ -327,10 +348,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
             weights(xs[cur], 0, pb[cur][0], sum);
             if ((st0 + j + 2) * kWideBlock > mask_from) mask_scores(j + 1, xs[nxt]);
 #pragma unroll
-            for (int d = 0; d < 4; d++)
+            for (int d = 0; d < W::kDims; d++)
 #pragma unroll
                 for (int s = 0; s < 2; s++) acc[d] = E::mfma_32x32(va[d][s], pb[nxt][s], acc[d]);   // P(j - 1)
-            read_keys(k_stage((phase + hi + 2) & kLast));                                  // K(j + 2)
+            read_keys(block_at(k_stage, j, phase + 2));                                  // K(j + 2)
             weights(xs[cur], 1, pb[cur][1], sum);
             if (__builtin_expect(__builtin_amdgcn_ballot_w64(sum > kMostWeight) != 0, 0)) {
                 raise(xs[cur]);
@@ -362,14 +383,14 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
                 const int t = (st0 + j) * kWideBlock + token;
                 const int row = pool_row(a, t, page_of(a, r, t));
                 if (row < 0) continue;
-                const char *key = a.pages + (unsigned long)(unsigned)row * (unsigned)row_bytes + head * 256;
+                const char *key = a.pages + (unsigned long)(unsigned)row * (unsigned)row_bytes + head * kD * 2;
                 float s = 0;
-                for (int k = 0; k < 8; k++) {
+                for (int k = 0; k < W::kSteps; k++) {
                     float x[8], y[8];
                     Chunk<DT>::unpack(*reinterpret_cast<const u32x4 *>(key + k * 32 + h * 16), x);
                     u32x4 mine = q[0];
 #pragma unroll
-                    for (int i = 1; i < 8; i++) mine = k == i ? q[i] : mine;
+                    for (int i = 1; i < W::kSteps; i++) mine = k == i ? q[i] : mine;
                     Chunk<DT>::unpack(mine, y);
 #pragma unroll
                     for (int e = 0; e < 8; e++) s = fmaf(x[e], y[e], s);
@@ -379,7 +400,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
                 const float weight = __builtin_amdgcn_exp2f(fmaf(s + other, a.scale, -m_run));
                 if ((bits >> token) & 1)
 #pragma unroll
-                    for (int d = 0; d < 4; d++)
+                    for (int d = 0; d < W::kDims; d++)
 #pragma unroll
                         for (int v = 0; v < 16; v++)
                             acc[d][v] += weight * LoadElt<DT>::get(key + half_bytes, d * 32 + 8 * (v >> 2) + 4 * h + (v & 3));
@@ -395,10 +416,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
             const long slot = 2L * share + (unit > begin ? 1 : 0);
             const long part = (slot * a.n_kv_heads + head) * W::kCols + wave * 32 + r32;
 #pragma unroll
-            for (int d = 0; d < 4; d++)
+            for (int d = 0; d < W::kDims; d++)
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    *reinterpret_cast<f32x4 *>(a.part_o + part * 128 + d * 32 + 8 * i + 4 * h) =
+                    *reinterpret_cast<f32x4 *>(a.part_o + part * kD + d * 32 + 8 * i + 4 * h) =
                         f32x4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
             if (h == 0) {
                 a.part_ml[part * 2] = m_run;
@@ -406,9 +427,9 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
             }
         } else if (there) {
             const float inv = l == 0 ? 0.f : 1.f / l;
-            char *dst = a.out + ((q_row * a.n_qo_heads + hq) * 128 + 4 * h) * 2;
+            char *dst = a.out + ((q_row * a.n_qo_heads + hq) * kD + 4 * h) * 2;
 #pragma unroll
-            for (int d = 0; d < 4; d++)
+            for (int d = 0; d < W::kDims; d++)
 #pragma unroll
                 for (int i = 0; i < 4; i++)
                     *reinterpret_cast<u32x2 *>(dst + (d * 32 + 8 * i) * 2) =

@@ -40,6 +40,10 @@ CASES = [
     ("wide_two_tiles", [900, 1500, 40, 333], [64, 50, 40, 33], True, 16, 16, 2, 128, "bf16"),
     ("wide_two_tiles_or_one", [900, 1500, 140, 333, 700, 80], [64, 64, 64, 40, 64, 3], True, 16, 16, 1, 128, "f16"),
     ("wide_two_tiles_many", [300 + 37 * i for i in range(11)], [64 - 3 * i for i in range(11)], True, 16, 64, 8, 128, "bf16"),
+    ("wide_dim64", [0, 31, 32, 33, 63, 64, 65, 95, 96, 127, 128], [17, 33, 64, 20, 31, 32, 5, 18, 1, 40, 29], True, 16, 32, 8, 64, "bf16"),
+    ("wide_dim64_four_waves", [70, 1000, 5, 2047, 2048, 4100], [17, 20, 32, 32, 19, 30], True, 3, 16, 4, 64, "f16"),
+    ("wide_dim64_two_tiles", [900, 1500, 40, 333], [64, 50, 40, 33], True, 16, 16, 2, 64, "f16"),
+    ("wide_dim64_chains", [300, 20, 2111], [40, 64, 64], False, 12, 32, 8, 64, "bf16"),
     ("many_over_eight_heads", [31 * i for i in range(20)], [1 + i % 6 for i in range(20)], True, 16, 16, 8, 128, "bf16"),
     ("many_short", list(range(70)), [1 + i % 5 for i in range(70)], True, 8, 8, 2, 128, "bf16"),
     ("many_lengths", [int(x) for x in np.random.default_rng(1).integers(0, 900, 40)], [4] * 40, False, 16, 8, 2, 128, "bf16"),
@@ -117,7 +121,7 @@ def test_rows_that_see_nothing(dtype, dim):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dtype,dim,group", [("bf16", 128, 4), ("f16", 128, 1), ("f16", 128, 6), ("bf16", 128, 8), ("f16", 64, 8), ("fp32", 128, 4), ("fp32", 64, 2), ("bf16", 96, 4)])
+@pytest.mark.parametrize("dtype,dim,group", [("bf16", 128, 4), ("f16", 128, 1), ("f16", 128, 6), ("bf16", 128, 8), ("f16", 64, 8), ("bf16", 64, 2), ("fp32", 128, 4), ("fp32", 64, 2), ("bf16", 96, 4)])
 def test_infinities_and_nan_in_masked_places(dtype, dim, group):
     """A drafted row whose K and V are no numbers reaches the rows that descend from it and no other."""
     for value in (float("nan"), float("inf"), -float("inf")):
