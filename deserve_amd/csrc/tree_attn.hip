@@ -167,14 +167,14 @@ static bool wide_form(int max_rows, int n_qo_heads, int n_kv_heads, int head_dim
 {
     return dtype != DSKV_F32 && (long)max_rows * (n_qo_heads / n_kv_heads) > tree_columns(head_dim);
 }
-static int64_t units_bytes(int batch) { return ((int64_t)batch + 6) / 4 * 16; }
+static int64_t units_bytes(int batch) { return ((int64_t)batch + 7) / 4 * 16; }
 static int64_t slots_of(const TreeForm &f, int n_kv_heads) { return 2LL * f.shares * n_kv_heads * f.cols; }
 static int64_t form_bytes(const TreeForm &f, int batch, int n_kv_heads, int head_dim)
 {
     return units_bytes(batch) + slots_of(f, n_kv_heads) * (head_dim + 2) * (int64_t)sizeof(float);
 }
 
-template <int DT, int kD, int kCols, int kSub, int kLeast> static int launch_tree_merge(const TreeArgs &a, const TreeForm &f, hipStream_t stream)
+template <int DT, int kD, int kCols, int kSub> static int launch_tree_merge(const TreeArgs &a, const TreeForm &f, hipStream_t stream)
 {
     // few items are cut into many parts each, many into few: one request over 4 K tokens 16.8 us with four groups of parts and 20.1 with
     // one, 64 requests 189 with one and 196 with four
@@ -182,8 +182,8 @@ template <int DT, int kD, int kCols, int kSub, int kLeast> static int launch_tre
     constexpr int kEach = kCols >= 128 ? 4 : 1;
     const int columns = 256 / (kD / 4) * (many_parts ? 1 : kEach) / (many_parts ? 4 : 1);
     const dim3 grid((unsigned)(a.batch * f.col_tiles), (unsigned)a.n_kv_heads, (unsigned)((kCols + columns - 1) / columns));
-    if (many_parts) hipLaunchKernelGGL((tree_merge_kernel<DT, kD, kCols, kSub, kLeast, 4, 1>), grid, dim3(256), 0, stream, a, f.col_tiles);
-    else hipLaunchKernelGGL((tree_merge_kernel<DT, kD, kCols, kSub, kLeast, 1, kEach>), grid, dim3(256), 0, stream, a, f.col_tiles);
+    if (many_parts) hipLaunchKernelGGL((tree_merge_kernel<DT, kD, kCols, kSub, 4, 1>), grid, dim3(256), 0, stream, a, f.col_tiles);
+    else hipLaunchKernelGGL((tree_merge_kernel<DT, kD, kCols, kSub, 1, kEach>), grid, dim3(256), 0, stream, a, f.col_tiles);
     DSKV_LAUNCH_CHECK("tree_merge_kernel");
     return 0;
 }
@@ -193,13 +193,13 @@ template <int DT, int kD, int kBlocks> static int launch_tree(const TreeArgs &a,
     hipLaunchKernelGGL((tree_matrix_kernel<DT, kD, kBlocks>), dim3((unsigned)(f.shares * a.n_kv_heads)),
                        dim3(kTreeThreads), 0, stream, a);
     DSKV_LAUNCH_CHECK("tree_matrix_kernel");
-    return launch_tree_merge<DT, kD, S::kCols, S::kSub, kTreeWaves>(a, f, stream);
+    return launch_tree_merge<DT, kD, S::kCols, S::kSub>(a, f, stream);
 }
 template <int DT, int kD, int kWaves> static int launch_tree_wide(const TreeArgs &a, const TreeForm &f, hipStream_t stream)
 {
     hipLaunchKernelGGL((tree_wide_kernel<DT, kD, kWaves>), dim3((unsigned)(f.shares * a.n_kv_heads)), dim3(kWaves * 64), 0, stream, a);
     DSKV_LAUNCH_CHECK("tree_wide_kernel");
-    return launch_tree_merge<DT, kD, kWaves * 32, kWideBlock, kWideLeast>(a, f, stream);
+    return launch_tree_merge<DT, kD, kWaves * 32, kWideBlock>(a, f, stream);
 }
 template <int DT, int kD> static int launch_tree_blocks(const TreeArgs &a, const TreeForm &f, hipStream_t stream)
 {

@@ -41,7 +41,7 @@ struct TreeArgs {
     uint32_t page_magic;                  // ceil(2^page_shift / page_size): t / page_size = t * page_magic >> page_shift
     int page_shift;
     float *part_o, *part_ml;              // (2 * n_shares, n_kv_heads, columns of a tile, head_dim | 2)
-    int32_t *units_before;                // (batch + 3): units (parts) of the requests in front; see tree_place
+    int32_t *units_before;                // (batch + 4): units (parts) of the requests in front; see tree_place
     int n_shares, group;
     int sides;                            // see side_by_side
 };
@@ -113,17 +113,16 @@ template <int kCols, int kSub> __device__ __forceinline__ TreeRequest tree_reque
 struct Shares {
     int each, longer, used;
 };
-// None of the shares in use has fewer than `least` units, if there are as many.
-__device__ __forceinline__ Shares shares_of(int n_shares, int units, int least)
+__device__ __forceinline__ Shares shares_of(int units, int used)                  // used > 0
 {
     Shares s;
-    s.used = max(min(n_shares, (int)(((unsigned)units + least - 1) / (unsigned)least)), 1);
-    s.each = (int)((unsigned)units / (unsigned)s.used);
-    s.longer = units - s.each * s.used;
+    s.used = used;
+    s.each = (int)((unsigned)units / (unsigned)used);
+    s.longer = units - s.each * used;
     return s;
 }
 __device__ __forceinline__ int share_begin(const Shares &s, int share) { return share * s.each + min(share, s.longer); }
-__device__ __forceinline__ int share_with(const Shares &s, int unit)              // units > 0
+__device__ __forceinline__ int share_with(const Shares &s, int unit)              // units >= used
 {
     const int of_longer = s.longer * (s.each + 1);
     return unit < of_longer ? (int)((unsigned)unit / (unsigned)(s.each + 1))
@@ -197,6 +196,7 @@ template <int kCols, int kSub, int kThreads, bool kSides, int kLeast, int kTurn>
 __device__ __forceinline__ void tree_place(const TreeArgs &a, int share, TreePlace &at)
 {
     __shared__ long scan[2][kThreads / 64], scan_parts[kThreads / 64];
+    __shared__ int busy_of[kThreads / 64];
     __shared__ int found_base, found_b, found_begin, found_end;
     __shared__ TreeRequest found_r;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -210,6 +210,8 @@ __device__ __forceinline__ void tree_place(const TreeArgs &a, int share, TreePla
         if (kSides) mine[1] += units_of(r, true);
     }
     long total[2] = {0, 0};
+    const unsigned long long busy = __ballot(b0 < b1 && r.n > 0);
+    if (lane == 0) busy_of[wave] = __popcll(busy);
 #pragma unroll
     for (int i = 0; i < (kSides ? 2 : 1); i++) {
         upto[i] = wave_scan(mine[i]);
@@ -235,7 +237,13 @@ __device__ __forceinline__ void tree_place(const TreeArgs &a, int share, TreePla
         span = share % 8 + 8 * (j / a.sides);
         spans = a.n_shares / a.sides;
     }
-    const Shares shares = shares_of(spans, units, kLeast);
+    // Shares in use: of no fewer units than kLeast, but as many as there are requests with rows, if there are as many (17 requests
+    // of 8 rows over 3 - 21 tokens 14.4 us, with kLeast alone 33; 24 trees of 64 rows over 20 - 180 tokens 27 and 53).
+    int requests = per > 1 ? spans : 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; w++) requests += busy_of[w];
+    const int used = max(min(min(spans, units), max((int)(((unsigned)units + kLeast - 1) / kLeast), requests)), 1);
+    const Shares shares = shares_of(units, used);
     at.begin = at.end = 0;
     if (span < shares.used) {
         at.begin = share_begin(shares, span);
@@ -244,7 +252,7 @@ __device__ __forceinline__ void tree_place(const TreeArgs &a, int share, TreePla
     int before = (int)((which ? upto[1] : upto[0]) - (which ? mine[1] : mine[0]));
     const bool tells = blockIdx.x == 0;
     if constexpr (kTurn > 0) {
-        if (a.batch > 1 && a.batch <= spans / 2 && units > 0) {             // (a request per thread at most)
+        if (a.batch > 1 && a.batch <= spans && units > 0) {                 // (a request per thread at most)
             const int most = shares.each + (shares.longer > 0);
             const int cut = most <= kLeast ? kLeast : (most + kTurn - 1) / kTurn * kTurn, cut_more = (cut + 2 * kTurn - 1) / kTurn * kTurn;
             const int tiles = which ? (r.col_tiles > 0) : r.col_tiles;
@@ -305,6 +313,7 @@ __device__ __forceinline__ void tree_place(const TreeArgs &a, int share, TreePla
             a.units_before[a.batch] = units;
             a.units_before[a.batch + 1] = which;
             a.units_before[a.batch + 2] = 0;
+            a.units_before[a.batch + 3] = used;
         }
     }
     __syncthreads();
@@ -790,7 +799,7 @@ __global__ __launch_bounds__(kTreeThreads, tree_workgroups(kD, kBlocks)) void tr
 // Items that were cut: a thread per (column, four dims) and group of parts.  kGroups > 1, for items in many parts: each takes
 // every kGroups-th part, and they meet in LDS.  kEach > 1, for many columns: columns that a thread takes at once (66
 // MB of partials, 16 trees of 33 - 64 rows: 16 us with four, 23 with one).
-template <int DT, int kD, int kCols, int kSub, int kLeast, int kGroups, int kEach>
+template <int DT, int kD, int kCols, int kSub, int kGroups, int kEach>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int max_col_tiles)
 {
     constexpr int kElt = DT == DSKV_F32 ? 4 : 2;
@@ -803,7 +812,6 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int max_col
     const int part_units = a.units_before[a.batch + 2];        // 0: equal shares
     const int cols = min(r.n * a.group - ct * r.tile, r.tile), col0 = (int)blockIdx.z * kColumns * kEach + column;
     if (ct >= r.col_tiles || (int)blockIdx.z * kColumns * kEach >= cols || units == 0) return;
-    const Shares shares = shares_of(beside ? a.n_shares / a.sides : a.n_shares, units, kLeast);
     const int first = before + (beside ? 0 : ct * r.subtiles), last = first + r.subtiles - 1;
     int s0, s1;
     bool second = false;                                       // in the first of its shares the item is the second
@@ -812,6 +820,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int max_col
         s0 = before + (beside ? 0 : ct * parts);
         s1 = s0 + parts - 1;
     } else {
+        const Shares shares = shares_of(units, a.units_before[a.batch + 3]);
         s0 = share_with(shares, first);
         s1 = share_with(shares, last);
         second = share_begin(shares, s0) < first;
