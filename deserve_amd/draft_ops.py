@@ -13,7 +13,7 @@ yet; the others are drafted tokens that form a chain or a tree behind it, a row'
     move_accepted_rows(pool.pages, tables.slots, tables.qo_indptr, verdict.path, verdict.counts)
     kv_lens += verdict.counts
 
-Lengths, tables and verdicts stay on the device: nothing is planned on the host or read back, so the calls can be captured into
+A stage runs them through execution.exec.BatchVerify.  Lengths, tables and verdicts stay on the device: nothing is planned on the host or read back, so the calls can be captured into
 a graph and replayed with other lengths.  Work is enqueued on the current stream of the tensors' device.
 """
 from __future__ import annotations
