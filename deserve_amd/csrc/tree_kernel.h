@@ -496,12 +496,6 @@ __global__ __launch_bounds__(kTreeThreads, tree_workgroups(kD, kBlocks)) void tr
         }
     };
     Ids ids = next_ids();
-#pragma unroll
-    for (int i = 0; i < kDepth; i++) {
-        const Ids ids_next = next_ids();
-        request(ids, regs[i], held_of[i]);
-        ids = ids_next;
-    }
 
     // ---- what is computed: one item after the other
     TreeItem it;
@@ -538,7 +532,9 @@ __global__ __launch_bounds__(kTreeThreads, tree_workgroups(kD, kBlocks)) void tr
 #pragma unroll
             for (int d = 0; d < S::kDimTiles; d++) o[k][d] = f32x4{0, 0, 0, 0};
         }
-        // q and the masks are waited for here, in front of the loop
+    };
+    // q and the masks are waited for in front of the loop
+    auto settle_item = [&]() {
 #pragma unroll
         for (int k = 0; k < kBlocks; k++) {
 #pragma unroll
@@ -784,8 +780,15 @@ __global__ __launch_bounds__(kTreeThreads, tree_workgroups(kD, kBlocks)) void tr
         }
         __syncthreads();
     };
-    start_item(begin);
+    start_item(begin);                                          // (its loads in front of those that wait for page ids)
+#pragma unroll
+    for (int i = 0; i < kDepth; i++) {
+        const Ids ids_next = next_ids();
+        request(ids, regs[i], held_of[i]);
+        ids = ids_next;
+    }
     for (;;) {
+        settle_item();
         while (st < it.st1) {
 #pragma unroll
             for (int i = 0; i < kDepth; i++) subtile(regs[i], held_of[i]);
