@@ -545,51 +545,54 @@ __global__ __launch_bounds__(kTreeThreads, tree_workgroups(kD, kBlocks)) void tr
     auto subtile = [&](TreeRegs<DT, kD, kBlocks> &mine, unsigned long long &held_here) {
         const unsigned long long held = held_here;
         const bool whole = held == ~0ull && (st + 1) * S::kSub <= prior + (a.masks ? 0 : 1);
-        __builtin_amdgcn_wave_barrier();
-        // A weight of 0 times a V that is no number would reach columns that do not see the token: such tokens among the
-        // new ones are taken out here and added behind the walk.
-        if (st >= new_from) {
-            unsigned bad = 0;
-            bool odd[S::kLoads], any = false;
-#pragma unroll
-            for (int i = 0; i < S::kLoads; i++) {
-                odd[i] = no_number<DT>(mine.v[i]);
-                any |= odd[i];
-            }
-            if (__builtin_expect(__ballot(any) != 0, 0)) {
+        const bool there = st < it.st1;                         // (else a turn without a subtile)
+        u32x4 key[S::kTiles][S::kSteps];
+        if (there) {
+            __builtin_amdgcn_wave_barrier();
+            // A weight of 0 times a V that is no number would reach columns that do not see the token: such tokens among the
+            // new ones are taken out here and added behind the walk.
+            if (st >= new_from) {
+                unsigned bad = 0;
+                bool odd[S::kLoads], any = false;
 #pragma unroll
                 for (int i = 0; i < S::kLoads; i++) {
-                    const unsigned long long odd_lanes = __ballot(odd[i]);
-#pragma unroll
-                    for (int j = 0; j < S::kRowsPerLoad; j++) {
-                        const unsigned long long of_row = ((1ull << S::kChunks) - 1) << (j * S::kChunks);
-                        if (odd_lanes & of_row) bad |= 1u << (j + S::kRowsPerLoad * i);
-                    }
-                    if ((bad >> (load_row + S::kRowsPerLoad * i)) & 1) mine.v[i] = u32x4{0, 0, 0, 0};
+                    odd[i] = no_number<DT>(mine.v[i]);
+                    any |= odd[i];
                 }
+                if (__builtin_expect(__ballot(any) != 0, 0)) {
+#pragma unroll
+                    for (int i = 0; i < S::kLoads; i++) {
+                        const unsigned long long odd_lanes = __ballot(odd[i]);
+#pragma unroll
+                        for (int j = 0; j < S::kRowsPerLoad; j++) {
+                            const unsigned long long of_row = ((1ull << S::kChunks) - 1) << (j * S::kChunks);
+                            if (odd_lanes & of_row) bad |= 1u << (j + S::kRowsPerLoad * i);
+                        }
+                        if ((bad >> (load_row + S::kRowsPerLoad * i)) & 1) mine.v[i] = u32x4{0, 0, 0, 0};
+                    }
+                }
+                if (lane == 0) bad_at[st - new_from] = bad;
             }
-            if (lane == 0) bad_at[st - new_from] = bad;
+#pragma unroll
+            for (int i = 0; i < S::kLoads; i++) {
+                const int row = load_row + S::kRowsPerLoad * i;
+                *reinterpret_cast<u32x4 *>(k_lds + row * S::kKPitch + load_chunk * 16) = mine.k[i];
+                *reinterpret_cast<u32x4 *>(v_lds + row * S::kVPitch + load_chunk * 16) = mine.v[i];
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            // LDS operands are read together and ahead: one wave a SIMD has nobody to wait for them in its place
+#pragma unroll
+            for (int t = 0; t < S::kTiles; t++)
+#pragma unroll
+                for (int e = 0; e < S::kSteps; e++)
+                    key[t][e] = *reinterpret_cast<const u32x4 *>(k_lds + (t * 16 + c) * S::kKPitch + e * 64 + g * 16);
         }
-#pragma unroll
-        for (int i = 0; i < S::kLoads; i++) {
-            const int row = load_row + S::kRowsPerLoad * i;
-            *reinterpret_cast<u32x4 *>(k_lds + row * S::kKPitch + load_chunk * 16) = mine.k[i];
-            *reinterpret_cast<u32x4 *>(v_lds + row * S::kVPitch + load_chunk * 16) = mine.v[i];
-        }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        // LDS operands are read together and ahead: one wave a SIMD has nobody to wait for them in its place
-        u32x4 key[S::kTiles][S::kSteps];
-#pragma unroll
-        for (int t = 0; t < S::kTiles; t++)
-#pragma unroll
-            for (int e = 0; e < S::kSteps; e++)
-                key[t][e] = *reinterpret_cast<const u32x4 *>(k_lds + (t * 16 + c) * S::kKPitch + e * 64 + g * 16);
         __builtin_amdgcn_sched_barrier(0);
         const Ids ids_next = next_ids();
         request(ids, mine, held_here);
         ids = ids_next;
-        if (st >= it.st1) {                                     // a turn without a subtile
+        if (!there) {
             st += kTreeWaves;
             return;
         }
