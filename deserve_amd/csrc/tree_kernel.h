@@ -11,11 +11,11 @@
 // K and V go by whole rows through registers and a wave's own LDS: rows of 256 bytes are what
 // HBM delivers best, and a row's page is looked up once per subtile, by lane, so pages may have any size.
 //
-// Bound by HBM where there is work enough: 64 requests of 5 rows over 256 - 4096 tokens (32 heads over 8, bf16, 0.6 GB) 118 us, of
+// Bound by HBM where there is work enough: 64 requests of 5 rows over 256 - 4096 tokens (32 heads over 8, bf16, 0.6 GB) 117 us, of
 // which the launch for cut items takes 5: 5.0 TB/s; its loads alone run in 96.  In short calls by latency: one request over
-// 1.8 K tokens 13.9 us, 10.8 for the first launch (place of the share 2.6, page ids and requests 3, K and V 1.2, products 3, waves
+// 1.8 K tokens 13.4 us, 10.3 for the first launch (place of the share 2.6, page ids and requests 3, K and V 1.2, products 2, waves
 // meet 2).  fp32: the matrix instruction takes 32 products a cycle and SIMD, 3.2 of the 4.5 us of a wave's subtile for 48 columns; 8
-// requests over 300 - 700 tokens 30 us.
+// requests over 300 - 700 tokens 28 us.
 #pragma once
 
 #include "kv_tile.h"

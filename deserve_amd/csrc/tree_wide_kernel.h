@@ -5,7 +5,7 @@
 //
 // Bound by the matrix pipeline and the vector instructions beside it: 16 of 32x32x16 per block and wave, 16 exponentials and some 75
 // other instructions (128 dims).  16 requests over 1 - 16 K tokens, 64 heads over 8, bf16: with 64 rows each 316 us, 920 TFLOP/s; with 33
-// to 64 rows 286, 777 TFLOP/s, since a block lasts as long as its units with two busy waves, and columns come in
+// to 64 rows 281 - 296, 750 - 790 TFLOP/s, since a block lasts as long as its units with two busy waves, and columns come in
 // thirty-twos; of that 16 us are the launch for cut items (66 MB of partials).
 // With 64 dims a stage holds two blocks side by side, so that a load fetches whole kilobytes there, too, and both sizes share one
 // layout of LDS: 16 requests of 48 rows, 64 heads, 175 us (the narrow form: 333).
