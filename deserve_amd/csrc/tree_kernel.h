@@ -252,7 +252,7 @@ __device__ __forceinline__ void tree_place(const TreeArgs &a, int share, TreePla
     int before = (int)((which ? upto[1] : upto[0]) - (which ? mine[1] : mine[0]));
     const bool tells = blockIdx.x == 0;
     if constexpr (kTurn > 0) {
-        if (a.batch > 1 && a.batch <= spans && units > 0) {                 // (a request per thread at most)
+        if (a.batch > 1 && a.batch <= spans && per == 1 && units > 0) {     // (`parts` is of one request a thread)
             const int most = shares.each + (shares.longer > 0);
             const int cut = most <= kLeast ? kLeast : (most + kTurn - 1) / kTurn * kTurn, cut_more = (cut + 2 * kTurn - 1) / kTurn * kTurn;
             const int tiles = which ? (r.col_tiles > 0) : r.col_tiles;

@@ -46,6 +46,11 @@ CASES = [
     ("wide_dim64_chains", [300, 20, 2111], [40, 64, 64], False, 12, 32, 8, 64, "bf16"),
     ("many_over_eight_heads", [31 * i for i in range(20)], [1 + i % 6 for i in range(20)], True, 16, 16, 8, 128, "bf16"),
     ("many_short", list(range(70)), [1 + i % 5 for i in range(70)], True, 8, 8, 2, 128, "bf16"),
+    ("batch_300", [(7 * i) % 90 for i in range(300)], [i % 4 for i in range(300)], True, 16, 8, 2, 128, "bf16"),
+    ("batch_700_fp32", [(5 * i) % 40 for i in range(700)], [(i + 1) % 3 for i in range(700)], False, 8, 2, 1, 64, "fp32"),
+    ("batch_300_wide", [(11 * i) % 120 for i in range(300)], [(3 * i) % 25 for i in range(300)], True, 16, 4, 1, 128, "f16"),
+    ("batch_530_wide", [(13 * i) % 70 for i in range(530)], [(5 * i) % 41 for i in range(530)], True, 16, 4, 1, 128, "bf16"),
+    ("batch_530_wide_two_tiles", [(13 * i) % 70 for i in range(530)], [40 + i % 25 for i in range(530)], False, 16, 8, 1, 64, "bf16"),
     ("many_lengths", [int(x) for x in np.random.default_rng(1).integers(0, 900, 40)], [4] * 40, False, 16, 8, 2, 128, "bf16"),
 ]
 
