@@ -237,8 +237,8 @@ template <int DT> __global__ __launch_bounds__(kVerifyThreads) void verify_sums_
     if (tells && b >= a.batch - 1) {
         const long end = max((long)a.qo_indptr[a.batch], 0L);
         for (long t = end + threadIdx.x; t < a.nnz; t += kVerifyThreads) a.path[t] = a.out_tokens[t] = -1;
-        if (b >= a.batch) return;                                  // no requests at all
     }
+    if (b >= a.batch) return;                                      // no requests at all: no entry of theirs, no workspace
     if (wave == 0) {
         const Walk w = walk_drafts<DT>(a, b);
         share_walk(w, s, a.draft != nullptr);

@@ -144,3 +144,20 @@ def test_more_rows_than_a_tree_has_and_rows_behind_the_last():
     run(target, tokens, uniforms, np.array([0, 0, 64]), draft=draft)
     run(target[:0], tokens[:0], uniforms[:0], np.array([0, 0, 0]))
     run(target, tokens, uniforms, np.array([0]))
+
+
+@pytest.mark.parametrize("vocab", [300, 4097, 128000])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "f16"])
+@pytest.mark.parametrize("chain", [False, True])
+def test_rows_without_requests(vocab, dtype, chain):
+    """No requests and a vocabulary of several parts: what lies behind the only entry of qo_indptr is not the call's, and it has
+    no workspace.  Every row gets no token."""
+    from deserve_amd.draft_ops import verify_drafts
+
+    print("[case] rows without requests", vocab, dtype, chain, flush=True)
+    target, draft, _, uniforms = make(6, [9], vocab, dtype)
+    longer = dev([0, 5, 9])
+    got = verify_drafts(target, dev(np.arange(9)), dev(uniforms, np.float32), longer[:1], draft_probs=draft if chain else None)
+    assert got.counts.numel() == 0
+    assert got.path.tolist() == [-1] * 9 and got.tokens.tolist() == [-1] * 9
+    assert longer.tolist() == [0, 5, 9]
