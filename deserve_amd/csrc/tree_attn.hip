@@ -51,13 +51,13 @@ __global__ __launch_bounds__(kGenericWaves * 64) void tree_generic_kernel(TreeAr
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
     const int b = request_of_row(a.qo_indptr, a.batch, t);
     if (b < 0) return;
-    const int first = a.qo_indptr[b], n = a.qo_indptr[b + 1] - first, i = t - first;
+    const int first = a.qo_indptr[b], i = t - first;
     if (i < 0 || i >= a.max_rows) return;
-    const int page0 = a.kv_page_indptr[b], pages = a.kv_page_indptr[b + 1] - page0;
-    const long kv_len = pages > 0 ? (long)(pages - 1) * a.page_size + min(a.kv_last_page_lens[b], a.page_size) : 0;
-    const long prior = kv_len - n;
+    const int page0 = a.kv_page_indptr[b];
+    const TreeTokens tokens = tree_tokens(page0, a.kv_page_indptr[b + 1], a.kv_last_page_lens[b], a.page_size, a.n_page_indices);
+    const long prior = tokens.len - ((long)a.qo_indptr[b + 1] - first);
     const unsigned long long mask = a.masks ? (unsigned long long)a.masks[t] : 0;
-    const long seen = a.masks ? kv_len : min(kv_len, prior + i + 1);
+    const long seen = a.masks ? tokens.walk : min(tokens.walk, prior + i + 1);
     const int kv_head = h / (a.n_qo_heads / a.n_kv_heads);
     const long head_bytes = (long)a.head_dim * E, row_bytes = a.n_kv_heads * head_bytes;
     float q[kChunks][8], o[kChunks][8];

@@ -75,6 +75,21 @@ template <int DT, int kD, int kBlocks> struct TreeShape {
     static constexpr int kLds = kTreeWaves * kWaveLds > kMergeLds ? kTreeWaves * kWaveLds : kMergeLds;
 };
 
+// Tokens of a request by the index arrays.  Those may promise more than the tensors hold: an entry behind the last of kv_page_indices is
+// no page, and where a table begins in front of the first there is none either.
+struct TreeTokens {
+    long len;            // cached and new ones
+    long walk;           // from here on no token lies in a page
+};
+__device__ __forceinline__ TreeTokens tree_tokens(int page0, int page_end, int last, int page_size, long n_page_indices)
+{
+    const long pages = (long)page_end - page0, entries = page0 < 0 ? 0L : max(n_page_indices - page0, 0L);
+    TreeTokens x;
+    x.len = pages > 0 ? max((pages - 1) * page_size + min(last, page_size), 0L) : 0L;
+    x.walk = min(x.len, entries * page_size);
+    return x;
+}
+
 struct TreeRequest {
     long first;          // its first row
     long kv_len;         // tokens that its rows may see

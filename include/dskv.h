@@ -593,7 +593,8 @@ int dskv_rope_append_slots(void *q_out, void *pages_layer, int32_t num_pages, co
  * sees cached position j < kv_len_b - n_b, and new row j of its request where bit j of its mask is set (masks null:
  * where j <= i).  A row that sees nothing gets zeros.  K and V are in the pages (kv_len_b counts the new rows).
  * q rows are q_stride elements apart (heads contiguous), out is contiguous; rows behind qo_indptr[batch]
- * are left as they are.  A page id outside [0, num_pages) holds no tokens, nor does a table entry past n_page_indices.
+ * are left as they are.  A page id outside [0, num_pages) holds no tokens, nor does a table entry past n_page_indices, nor a table
+ * that begins in front of the first.
  * max_qo_len: no request has more rows (more: the further ones are left as they are); with masks at most
  * DSKV_MAX_TREE_ROWS.  head_dim: a multiple of 8 up to 256.
  * workspace (16-byte aligned): at least dskv_tree_attn_workspace(..) bytes, which do not depend on the lengths; used

@@ -197,6 +197,58 @@ def test_pages_outside_the_pool_hold_no_tokens(dtype, dim, hq):
     compare(run(step, on), *attention(Step_without(want_step, {1: [8 - int(step.kv_page_indptr[1]), 9 - int(step.kv_page_indptr[1])]})))
 
 
+SHORT = [  # cached tokens, rows, pages that the table has beyond its entries
+    ([100], [4], 2 ** 31 - 8), ([100, 9], [4, 3], 3), ([90], [20], 1), ([0], [7], 1), ([33, 40], [2, 30], 2)]
+
+
+def Step_short(step, beyond):
+    """The step whose last request's table claims `beyond` pages more than there are entries."""
+    last = len(step.kv) - 1
+
+    class Short(type(step)):
+        def claimed(self, b):
+            lo, hi, table, length = super().request(b)
+            return length + beyond * self.page if b == last else length
+
+        def request(self, b):
+            lo, hi, table, length = super().request(b)
+            return lo, hi, table, min(self.claimed(b), len(table) * self.page)
+
+        def sees(self, b):
+            lo, hi, _, held = self.request(b)
+            prior, out = self.claimed(b) - (hi - lo), np.ones((hi - lo, held), bool)
+            for i in range(hi - lo):
+                for j in range(prior, held):
+                    out[i, j] = j - prior <= i if self.masks is None else (int(self.masks[lo + i]) >> (j - prior)) & 1
+            return out
+    return Short(**vars(step))
+
+
+def short_tables(dtype, dim, hq, tree):
+    for kv, rows, beyond in SHORT:
+        step = make_step(12, kv, rows, tree, 16, hq, 2, dim, dtype)
+        on = step.on("cuda")
+        indptr = step.kv_page_indptr.astype(np.int64)
+        indptr[-1] += beyond
+        assert indptr[-1] < 2 ** 31
+        on["csr"] = (on["csr"][0], torch.from_numpy(indptr.astype(np.int32)).cuda(), *on["csr"][2:])
+        print("[case] short table", dtype, dim, hq, tree, kv, rows, beyond, flush=True)
+        compare(run(step, on), *attention(Step_short(step, beyond)))
+    # a table that begins behind the last entry, or in front of the first, has no pages
+    for begin in (len(step.kv_page_indices) + 5, 2 ** 31 - 9, -3):
+        on["csr"] = (on["csr"][0], torch.tensor([0, begin, max(begin, 0) + 4], dtype=torch.int32).cuda(), *on["csr"][2:])
+        assert not run(step, on)[int(step.qo_indptr[1]):].any(), begin
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dim,hq", [("f16", 96, 8), ("fp32", 200, 4), ("bf16", 8, 2)])
+@pytest.mark.parametrize("tree", [False, True])
+def test_tables_longer_than_their_entries(dtype, dim, hq, tree):
+    """Pages that a table promises behind the last entry hold no tokens, however many: those in front of them
+    stay cached ones."""
+    short_tables(dtype, dim, hq, tree)
+
+
 def Step_without(step, gone):
     """The step with the given pages of its requests unseen."""
     class Without(type(step)):
