@@ -265,7 +265,7 @@ extern "C" int dskv_tree_attn(const dskv_tree_step_t *s, void *out, const void *
                                  s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->head_dim);
     // (rows of the pool, tokens of a request and units are numbered in 32 bits there)
     if (matrix_form(s->head_dim) && (int64_t)s->num_pages * 2 * s->page_size < INT32_MAX &&
-        s->n_page_indices < (1 << 30) / s->page_size && s->max_qo_len <= kTreeMostRows &&
+        s->n_page_indices < kMostTokens / s->page_size && s->max_qo_len <= kTreeMostRows &&
         (s->n_page_indices * s->page_size / 16 + 2LL * s->batch) * f.col_tiles < INT32_MAX) {
         const int64_t need = dskv_tree_attn_workspace(s->batch, s->nnz, s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->head_dim, s->dtype);
         if (!s->workspace || s->workspace_bytes < need) {

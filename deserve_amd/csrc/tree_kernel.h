@@ -27,6 +27,7 @@ constexpr int kTreeWaves = 4;
 constexpr int kTreeThreads = kTreeWaves * 64;
 // The running maximum of a column is raised only when a subtile's (block's) weights under it sum to more than this in a lane.
 constexpr float kMostWeight = 256.f;
+constexpr int kMostTokens = 1 << 30;        // of a request in the matrix forms: what n_page_indices pages hold
 constexpr int kTreeMostRows = 1024;         // of a request in the matrix forms; longer chunks are a prefill's
 
 struct TreeArgs {
@@ -93,8 +94,8 @@ __device__ __forceinline__ TreeTokens tree_tokens(int page0, int page_end, int l
 struct TreeRequest {
     long first;          // its first row
     long kv_len;         // tokens that its rows may see
-    long prior;          // tokens in front of its rows
-    int page0, pages;
+    int prior;           // tokens in front of its rows
+    int page0;
     int n;               // rows that are computed
     int col_tiles, subtiles;
     int tile;            // columns of a tile: its tiles are as even as 32 columns a wave allow
@@ -109,12 +110,11 @@ template <int kCols, int kSub> __device__ __forceinline__ TreeRequest tree_reque
     r.first = qo[0];
     const long rows = (long)qo[1] - r.first;
     r.page0 = kv[0];
-    r.pages = (int)min((long)kv[1] - r.page0, a.n_page_indices);
-    const int last = as_const(a.kv_last_page_lens)[b];
-    r.kv_len = r.pages > 0 ? max((long)(r.pages - 1) * a.page_size + min(last, a.page_size), 0L) : 0;
+    const TreeTokens tokens = tree_tokens(kv[0], kv[1], as_const(a.kv_last_page_lens)[b], a.page_size, a.n_page_indices);
     r.n = r.first < 0 ? 0 : (int)max(min(min(rows, (long)a.max_rows), (long)a.nnz - r.first), 0L);
-    r.prior = r.kv_len - rows;
-    r.kv_len = max(min(r.kv_len, r.prior + (a.masks ? DSKV_MAX_TREE_ROWS : r.n)), 0L);
+    const long prior = tokens.len - rows;
+    r.kv_len = max(min(tokens.walk, prior + (a.masks ? DSKV_MAX_TREE_ROWS : r.n)), 0L);
+    r.prior = (int)max(min(prior, (long)kMostTokens), -(long)kMostTokens);       // (further off than any token that is walked)
     r.col_tiles = (r.n * a.group + kCols - 1) / kCols;
     r.tile = kCols;
     if (kCols > tree_columns(64) && r.col_tiles > 1) r.tile = (r.n * a.group + 32 * r.col_tiles - 1) / (32 * r.col_tiles) * 32;
@@ -349,9 +349,8 @@ __device__ __forceinline__ void make_uniform(TreePlace &at)
     at.base = __builtin_amdgcn_readfirstlane(at.base);
     at.r.first = uniform(at.r.first);
     at.r.kv_len = uniform(at.r.kv_len);
-    at.r.prior = uniform(at.r.prior);
+    at.r.prior = __builtin_amdgcn_readfirstlane(at.r.prior);
     at.r.page0 = __builtin_amdgcn_readfirstlane(at.r.page0);
-    at.r.pages = __builtin_amdgcn_readfirstlane(at.r.pages);
     at.r.n = __builtin_amdgcn_readfirstlane(at.r.n);
     at.r.col_tiles = __builtin_amdgcn_readfirstlane(at.r.col_tiles);
     at.r.subtiles = __builtin_amdgcn_readfirstlane(at.r.subtiles);
@@ -526,7 +525,7 @@ __global__ __launch_bounds__(kTreeThreads, tree_workgroups(kD, kBlocks)) void tr
     auto start_item = [&](int unit) {
         open_item<S::kCols, S::kSub>(a, unit, begin, end, it);
         cols = min(it.r.n * a.group - it.ct * S::kCols, S::kCols);
-        prior = (int)max(it.r.prior, (long)-INT32_MAX);
+        prior = it.r.prior;
         new_from = max(prior, 0) / S::kSub;                     // first subtile with new rows
         st = it.st0 + wave;
 #pragma unroll

@@ -100,7 +100,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
         }
         const int blocks = st1 - st0;
         const int cols = min(r.n * a.group - ct * r.tile, r.tile);
-        const int prior = (int)max(r.prior, (long)-INT32_MAX);
+        const int prior = r.prior;
         const int t_end = (int)min(r.kv_len, (long)st1 * kWideBlock);
         const bool works = wave * 32 < cols;
 

@@ -249,6 +249,13 @@ def test_tables_longer_than_their_entries(dtype, dim, hq, tree):
     short_tables(dtype, dim, hq, tree)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dim,hq", [("bf16", 128, 8), ("bf16", 128, 16), ("f16", 64, 4), ("f16", 64, 64), ("fp32", 128, 4)])
+@pytest.mark.parametrize("tree", [False, True])
+def test_tables_longer_than_their_entries_matrix_forms(dtype, dim, hq, tree):
+    short_tables(dtype, dim, hq, tree)
+
+
 def Step_without(step, gone):
     """The step with the given pages of its requests unseen."""
     class Without(type(step)):
