@@ -147,7 +147,8 @@ class BatchPrefill(BatchExec):
 
 @dataclass
 class BatchVerify(BatchExec):
-    """A step of drafted tokens: the rows of a task are its last token and the drafts behind it, task.seqlen of them.
+    """A step of drafted tokens: the rows of a task are its last token and the drafts behind it, task.seqlen of them,
+    MAX_TREE_ROWS at most.
     prepare() and step() run on every stage; the last one makes probabilities of what step() returns and calls
     verify(); accept() with its verdict, on every stage, leaves the cache of the accepted rows in the order of the
     sequence and task.seqlen as what the step has advanced by, for task.step().  No counterpart in the reference."""
@@ -190,6 +191,8 @@ class BatchVerify(BatchExec):
         return tail
 
     def prepare(self) -> None:
+        if max(self.seqlens()) > MAX_TREE_ROWS:            # on every stage, before a cache grows for rows that no verdict accepts
+            raise ValueError(f"a task has at most {MAX_TREE_ROWS} rows to verify")
         with torch.inference_mode():
             # a wrapper of its own, which costs nothing: a step prepared in between does not change this one
             wrapper = BatchTreeWithPagedKVCacheWrapper(get_tree_wrapper(self.kvcaches[0].pool.main_device)._workspace)

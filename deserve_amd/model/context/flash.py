@@ -298,6 +298,8 @@ class FlashTreeCtx(FlashForwardCtx):
         max_tokens = sum(t.seqlen for t in task_datas)
         if parents is not None and max(t.seqlen for t in task_datas) > MAX_TREE_ROWS:
             raise ValueError(f"a tree has at most {MAX_TREE_ROWS} rows")
+        if parents is not None and (parents.dtype is not torch.int32 or parents.dim() != 1 or not parents.is_contiguous()):
+            raise ValueError("parents must be a contiguous one-dimensional torch.int32 tensor")     # before the caches are extended
         if parents is not None and parents.numel() != max_tokens:
             raise ValueError(f"parents holds {parents.numel()} entries for {max_tokens} rows")
         meta = build_host_metadata(task_datas, kvcaches)

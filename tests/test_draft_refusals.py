@@ -229,3 +229,18 @@ def test_steps_regrouped():
     assert (whole.tokens.tolist(), whole.parents.tolist()) == ([7, 8, 4, 5, 6], [-1, 0, -1, 0, 0])
     chains = BatchVerify.merge([steps[0], BatchVerify(torch.ones(3, 1), None, [TaskData("x", 0, 0, 3, 3)], [1], i32(1, 2, 3))])
     assert chains.parents is None and chains.pop().tokens.tolist() == [1, 2, 3]
+
+
+def test_steps_that_cannot_be_verified_are_refused_before_they_begin():
+    """Chains of more rows than a verification takes, and parents of another form: no cache has grown."""
+    pool = PagePool(1, 8, 16, torch.device("cpu"), torch.bfloat16, 2, 128)
+    table = PageTableAllocator(4, 256, 16, torch.device("cpu"))
+    caches = [PagedKVCache.empty(table, pool) for _ in range(2)]
+    tasks = [TaskData("a", 3, 1, 2, 3), TaskData("b", 0, 0, 65, 1)]
+    for tokens in (None, torch.zeros(67, dtype=torch.int32)):
+        with pytest.raises(ValueError, match="at most 64 rows"):
+            BatchVerify(torch.zeros(67, 1), None, tasks, caches, tokens).prepare()
+    shape = dict(num_qo_heads=4, num_kv_heads=2, head_dim=128, page_size=16)
+    for parents in (torch.zeros(2).long(), torch.zeros((1, 2), dtype=torch.int32), torch.zeros(4, dtype=torch.int32)[::2]):
+        refused("parents must be", FlashTreeCtx.init_and_plan, tasks[:1], caches[:1], None, parents=parents, **shape)
+    assert pool.num_avails == 8 and caches[0].page_table.occupied == caches[1].page_table.occupied == 0
