@@ -158,6 +158,8 @@ class BatchVerify(BatchExec):
 
     @classmethod
     def merge(cls, execs: Sequence["BatchVerify"]) -> "BatchVerify":
+        """Chains merged with trees become trees: verify() takes no draft_probs for the step then, and their tokens are
+        proposals like the trees' - distributed as the target's all the same, though fewer of them are accepted."""
         whole = super().merge(execs)
         if any(e.tokens is not None for e in execs):
             if any(e.tokens is None for e in execs):
@@ -210,9 +212,11 @@ class BatchVerify(BatchExec):
 
     def verify(self, target_probs: torch.Tensor, uniforms: torch.Tensor,
                draft_probs: Optional[torch.Tensor] = None) -> Verdict:
-        """draft_ops.verify_drafts over the rows of the step."""
+        """draft_ops.verify_drafts over the rows of the step.  draft_probs: for steps of chains only (see merge)."""
         with torch.inference_mode():
             assert self.tree_ctx is not None and self.tokens is not None
+            if draft_probs is not None and self.parents is not None:
+                raise ValueError("draft_probs belong to chains: trees, and chains merged with trees are verified without")
             if max(self.seqlens()) > MAX_TREE_ROWS:
                 raise ValueError(f"a task has at most {MAX_TREE_ROWS} rows to verify")
             return verify_drafts(target_probs, self.tokens, uniforms, self.tree_ctx.indptr, parents=self.parents,

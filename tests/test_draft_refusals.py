@@ -244,3 +244,13 @@ def test_steps_that_cannot_be_verified_are_refused_before_they_begin():
     for parents in (torch.zeros(2).long(), torch.zeros((1, 2), dtype=torch.int32), torch.zeros(4, dtype=torch.int32)[::2]):
         refused("parents must be", FlashTreeCtx.init_and_plan, tasks[:1], caches[:1], None, parents=parents, **shape)
     assert pool.num_avails == 8 and caches[0].page_table.occupied == caches[1].page_table.occupied == 0
+
+
+def test_chains_merged_with_trees_are_verified_as_proposals():
+    """The draft's distributions are refused for the whole step, in words that say what is left to do."""
+    chain = BatchVerify(torch.zeros(2, 1), None, [TaskData("a", 0, 0, 2, 2)], [0], i32(7, 8))
+    tree = BatchVerify(torch.ones(3, 1), None, [TaskData("b", 0, 0, 3, 3)], [1], i32(4, 5, 6), i32(-1, 0, 0))
+    whole = BatchVerify.merge([chain, tree])
+    whole.tree_ctx = object()
+    probs = torch.rand((5, 8))
+    refused("merged with trees are verified without", whole.verify, probs, torch.rand(5), probs)
