@@ -25,8 +25,12 @@ namespace dskv {
 
 constexpr int kTreeWaves = 4;
 constexpr int kTreeThreads = kTreeWaves * 64;
-// The running maximum of a column is raised only when a subtile's (block's) weights under it sum to more than this in a lane.
-constexpr float kMostWeight = 256.f;
+// The running maximum of a column is raised only when a subtile's (block's) weights under it sum to more than most_weight in a lane.
+// It is set headroom under the largest score then: float16 has normal numbers from 2^-14 to 2^16 only, and weights of 2^8 to 2^15 at the
+// top leave those down to 2^-22 of the largest their eleven bits and are off by 2^-33 of it below.  (With 1 at the top, where a model parks its
+// attention on few keys without a V, the others at 2^-22 of their weight gave results 2 % off, and none at all under 2^-25.)
+constexpr float most_weight(int dtype) { return dtype == DSKV_F16 ? 32768.f : 256.f; }
+constexpr float headroom(int dtype) { return dtype == DSKV_F16 ? 8.f : 0.f; }
 constexpr int kMostTokens = 1 << 30;        // of a request in the matrix forms: what n_page_indices pages hold
 constexpr int kTreeMostRows = 1024;         // of a request in the matrix forms; longer chunks are a prefill's
 
@@ -670,11 +674,11 @@ __global__ __launch_bounds__(kTreeThreads, tree_workgroups(kD, kBlocks)) void tr
                 w[e] = __builtin_amdgcn_exp2f(x[e] - m[k]);
                 sum += w[e];
             }
-            if (__builtin_expect(__ballot(sum > kMostWeight) != 0, 0)) {
+            if (__builtin_expect(__ballot(sum > most_weight(DT)) != 0, 0)) {
                 float top = x[0];
 #pragma unroll
                 for (int e = 1; e < S::kTiles * 4; e++) top = fmaxf(top, x[e]);
-                top = fmaxf(m[k], quad_rows_max(top));
+                top = fmaxf(m[k], quad_rows_max(top) - headroom(DT));
                 const float keep = __builtin_amdgcn_exp2f(m[k] - top);
                 m[k] = top;
                 l[k] *= keep;
@@ -691,7 +695,7 @@ __global__ __launch_bounds__(kTreeThreads, tree_workgroups(kD, kBlocks)) void tr
             if constexpr (DT == DSKV_F32) {
                 p[k] = __builtin_bit_cast(u32x4, f32x4{w[0], w[1], w[2], w[3]});
             } else {
-                // rounded to 16 bits for the matrix product: half a step of each weight
+                // rounded to 16 bits for the matrix product: half a step of each weight (see headroom)
 #pragma unroll
                 for (int e = 0; e < 4; e++) p[k][e] = Elt<DT>::pack2(w[2 * e], w[2 * e + 1]);
             }

@@ -15,8 +15,8 @@
 // its matrix instructions are independent of its exponentials.  Blocks lie in kStages stages of K and of V; iteration j
 // requests K(j + kStages) and V(j + kStages - 2) behind its only barrier, and reads the operands of K(j + 2) at its end; with eight
 // stages there is room for two iterations to a barrier (276 us instead of 285 for 48 rows), V one block later.  The running maximum
-// of a column is raised only when a block's weights under it sum to more than kMostWeight in a lane.  Weights are rounded to 16
-// bits for the matrix product, half a step of each; sums, maxima and O stay in 32.
+// of a column is raised only when a block's weights under it sum to more than most_weight in a lane.  Weights are rounded to 16
+// bits for the matrix product, half a step of each (see headroom); sums, maxima and O stay in 32.
 // Where a token lies in the pool is looked up for some thousand tokens at a time and kept in LDS (row numbers, a bit per token that
 // there is), so that pages may have any size and the loop's loads wait for nothing but LDS.
 #pragma once
@@ -227,7 +227,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
             for (int v = 1; v < 16; v++) m = fmaxf(m, x[v] * a.scale);
             float other = m;
             swap_halves32(m, other);
-            const float m_new = fmaxf(m_run, fmaxf(m, other));
+            const float m_new = fmaxf(m_run, fmaxf(m, other) - headroom(DT));
             const float keep = __builtin_amdgcn_exp2f(m_run - m_new);
             m_run = m_new;
             l_run *= keep;
@@ -353,7 +353,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_wide_kernel(TreeArgs a)
                 for (int s = 0; s < 2; s++) acc[d] = E::mfma_32x32(va[d][s], pb[nxt][s], acc[d]);   // P(j - 1)
             read_keys(block_at(k_stage, j, phase + 2));                                  // K(j + 2)
             weights(xs[cur], 1, pb[cur][1], sum);
-            if (__builtin_expect(__builtin_amdgcn_ballot_w64(sum > kMostWeight) != 0, 0)) {
+            if (__builtin_expect(__builtin_amdgcn_ballot_w64(sum > most_weight(DT)) != 0, 0)) {
                 raise(xs[cur]);
                 __builtin_amdgcn_sched_barrier(0);
                 sum = 0;

@@ -306,3 +306,35 @@ def test_another_stream_and_replays_with_other_lengths():
         again = w.forward(q, pages, out=torch.full_like(out, 7))
         assert torch.equal(again, out)
         torch.cuda.synchronize()
+
+
+# Scores under a maximum: one key in sixteen is ahead of all the others by `bits` powers of two and its V is 0, so that the result is
+# the others' alone, as behind a token that a model parks its attention on.
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [14.3, 19.64, 21.9, 27.4])
+@pytest.mark.parametrize("dtype,dim,rows,hq", [("f16", 128, 5, 8), ("f16", 128, 40, 8), ("f16", 64, 5, 16), ("f16", 64, 48, 16), ("bf16", 128, 5, 8),
+                                               ("bf16", 128, 40, 8), ("fp32", 128, 5, 8), ("f16", 96, 5, 8)])
+@pytest.mark.parametrize("size", [1, 4096])
+def test_few_keys_far_ahead_of_all_others(dtype, dim, rows, hq, bits, size):
+    """The float16 forms hold weights of up to 2^8 to 2^15, so that one that is 2^-22 of a row's largest or more is a normal number,
+    and a smaller one off by at most half of float16's smallest step, 2^-25 of 2^8 and so 2^-33 of the largest: the definition's bound and that for every token.
+    Results are small here: float16 numbers under 2^-14 lie 2^-24 apart, so that rounding one is off by up to 2^-25, which half a
+    step of the value does not hold; with V of some thousands they are normal numbers."""
+    print("[case] far ahead", dtype, dim, rows, hq, bits, size, flush=True)
+    step = make_step(31, [3000], [rows], False, 16, hq, 2, dim, dtype)
+    step.q.zero_()
+    step.q[..., 0] = 8
+    step.pages[:, 0, :, :, 0] = 0
+    step.pages[:, 0, ::16, :, 0] = bits * np.log(2) * dim ** 0.5 / 8
+    step.pages[:, 1] = (step.pages[:, 1].abs() + 0.5) * size
+    step.pages[:, 1, ::16] = 0
+    want, bound = attention(step)
+    if dtype == "f16":
+        # weights over the largest: 1 for one token in 16, 2^-bits for the others
+        _, _, table, length = step.request(0)
+        first = np.arange(length) % 16 == 0
+        for i in range(rows):
+            seen = np.arange(length) <= step.kv[0] + i
+            total = (seen & first).sum() + (seen & ~first).sum() * 2.0 ** -(bits + 0.01)
+            bound[i] += (seen & ~first).sum() / total * 2.0 ** -33 * float(step.pages[:, 1].max()) + 2.0 ** -25
+    compare(run(step), want, bound)
