@@ -338,3 +338,47 @@ def test_few_keys_far_ahead_of_all_others(dtype, dim, rows, hq, bits, size):
             total = (seen & first).sum() + (seen & ~first).sum() * 2.0 ** -(bits + 0.01)
             bound[i] += (seen & ~first).sum() / total * 2.0 ** -33 * float(step.pages[:, 1].max()) + 2.0 ** -25
     compare(run(step), want, bound)
+
+
+SIDES = [  # name, cached tokens, rows, tree, page, Hq, Hkv, D, dtype: four and eight column tiles (of 256) that walk the same tokens
+    ("eight_tiles", [900, 40, 1700], [64, 64, 64], True, 16, 32, 1, 128, "bf16"),
+    ("eight_tiles_one_request", [2500], [64], True, 3, 32, 1, 128, "f16"),
+    ("eight_tiles_or_seven", [1500, 800, 33], [64, 64, 50], True, 16, 32, 1, 128, "f16"),
+    ("eight_tiles_two_heads", [300, 1111], [64, 64], False, 16, 64, 2, 128, "bf16"),
+    ("eight_tiles_many", [50 + 7 * i for i in range(36)], [64 - i % 3 for i in range(36)], True, 16, 32, 1, 128, "bf16"),
+    ("eight_tiles_dim64", [900, 40, 1700], [64, 64, 64], True, 16, 32, 1, 64, "bf16"),
+    ("four_tiles", [900, 40, 1700], [64, 64, 64], True, 16, 16, 1, 128, "f16"),
+    ("four_tiles_dim64", [2100, 64], [64, 60], True, 8, 32, 2, 64, "f16"),
+]
+
+
+def side_by_side(step):
+    """Column tiles of each request where those of all walk the same tokens, by the launch's rule; else 0."""
+    group, shares = step.hq // step.hkv, 256 // step.hkv
+    tiles = -(-step.rows * group // 256)
+    spans = -(-(step.kv + step.rows) // 32)
+    sides = int(tiles.max())
+    return sides if shares % (8 * sides) == 0 and 4 * sides * spans.sum() <= 5 * (tiles * spans).sum() else 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", SIDES, ids=lambda c: c[0])
+def test_four_and_eight_column_tiles_side_by_side(case):
+    print("[case] side by side", *case, flush=True)
+    step = case_step(case)
+    assert side_by_side(step) == (8 if "eight" in case[0] else 4)
+    on = step.on("cuda")
+    got = run(step, on)
+    compare(got, *attention(step))
+    assert torch.equal(got, run(step, on))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dim,rows,hq", [("bf16", 128, 40, 16), ("f16", 64, 64, 32), ("f16", 128, 33, 4), ("bf16", 64, 40, 4)])
+def test_scales_that_are_not_positive_with_many_columns(dtype, dim, rows, hq):
+    """More columns than a wave of the narrow form holds, and a scale under which the wide form's mask would be no mask."""
+    step = make_step(14, [130, 700, 0], [rows, 9, rows // 2], True, 16, hq, 2, dim, dtype)
+    on = step.on("cuda")
+    for scale in (0.0, -0.05, -0.3, 0.05):
+        print("[case] scale", dtype, dim, rows, hq, scale, flush=True)
+        compare(run(step, on, scale), *attention(step, scale))
