@@ -219,6 +219,8 @@ class BatchVerify(BatchExec):
                 raise ValueError("draft_probs belong to chains: trees, and chains merged with trees are verified without")
             if max(self.seqlens()) > MAX_TREE_ROWS:
                 raise ValueError(f"a task has at most {MAX_TREE_ROWS} rows to verify")
+            if target_probs.shape[0] < self.total_seqlen():      # (the tasks behind them would be given no token)
+                raise ValueError(f"{target_probs.shape[0]} rows of probabilities for {self.total_seqlen()} rows")
             return verify_drafts(target_probs, self.tokens, uniforms, self.tree_ctx.indptr, parents=self.parents,
                                  draft_probs=draft_probs)
 

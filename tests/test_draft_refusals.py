@@ -254,3 +254,15 @@ def test_chains_merged_with_trees_are_verified_as_proposals():
     whole.tree_ctx = object()
     probs = torch.rand((5, 8))
     refused("merged with trees are verified without", whole.verify, probs, torch.rand(5), probs)
+
+
+def test_a_step_is_verified_by_as_many_rows_as_it_has():
+    """Probabilities or tokens of fewer rows would give the tasks behind them no token, not even the target's own."""
+    step = BatchVerify(torch.zeros(5, 1), None, [TaskData("a", 0, 0, 2, 2), TaskData("b", 0, 0, 3, 3)], [0, 1], i32(7, 8, 4, 5, 6))
+    step.tree_ctx = type("Ctx", (), {"indptr": i32(0, 2, 5)})()
+    refused("2 rows of probabilities for 5 rows", step.verify, torch.rand((2, 8)), torch.rand(5))
+    refused("uniforms holds 4", step.verify, torch.rand((5, 8)), torch.rand(4))
+    step.tokens = step.tokens[:4]
+    refused("tokens holds 4", step.verify, torch.rand((5, 8)), torch.rand(5))
+    step.tokens = i32(7, 8, 4, 5, 6, 9, 9)                     # padded ones are taken
+    refused("on the GPU", step.verify, torch.rand((7, 8)), torch.rand(7))
