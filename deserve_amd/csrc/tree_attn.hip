@@ -32,7 +32,7 @@ __device__ __forceinline__ int request_of_row(const int32_t *indptr, int batch, 
 // Any type and head dim: one workgroup per (row, q head) whose waves take every kGenericWaves-th group of four
 // keys.  Lane (g, c) holds dims 8 c .. 8 c + 7 (and 128 more ..) of key g of the group.  Bound by the
 // latency of its loads: K and V are read once per row and q head, from the caches but for the first time (64 requests of 5 rows
-// over 4 K tokens, 128 dims, 1628 us where the matrix form takes 118): for head dims and sizes that the others do not take.
+// over 256 - 4096 tokens, 128 dims, 1625 us where the matrix form takes 117): for head dims and sizes that the others do not take.
 constexpr int kGenericWaves = 8;
 constexpr int kTreeUnits = 256;        // compute units
 
@@ -159,10 +159,10 @@ static TreeForm tree_form(bool wide, int max_rows, int n_qo_heads, int n_kv_head
     return f;
 }
 // More columns than a wave of the narrow form holds go to the wide one, which reads K and V once for all of them: 64
-// requests of 13 rows (52 columns) over 4 K tokens 219 us, narrow 373; of 12 rows 198 narrow, 218 wide (bf16, 32 heads over 8).
-// Up to 128 columns by four waves, two workgroups a unit: 64 requests of 16 rows 219 us, by eight waves 228; more by
-// eight: 16 trees of 48 rows over 1 - 16 K (64 heads) 272 us, by four waves 308.  With 64 dims 64 requests of 20 rows (80 columns)
-// 127 us, narrow 204; of 16 rows 109 narrow.
+// requests of 13 rows (52 columns) over 4 K tokens each 214 us, narrow 372; of 12 rows 199 narrow, 213 wide (bf16, 32 heads over 8).
+// Up to 128 columns by four waves, two workgroups a unit: 64 requests of 16 rows 214 us, by eight waves 218; more by
+// eight: 16 trees of 48 rows over 160 K tokens in all (64 heads) 324 us, by four waves 368.  With 64 dims 64 requests of 20 rows (80
+// columns) over 4 K tokens 130 us, narrow 211; of 16 rows 115 narrow, 129 wide.
 static bool wide_form(int max_rows, int n_qo_heads, int n_kv_heads, int head_dim, int dtype)
 {
     return dtype != DSKV_F32 && (long)max_rows * (n_qo_heads / n_kv_heads) > tree_columns(head_dim);
@@ -176,8 +176,8 @@ static int64_t form_bytes(const TreeForm &f, int batch, int n_kv_heads, int head
 
 template <int DT, int kD, int kCols, int kSub> static int launch_tree_merge(const TreeArgs &a, const TreeForm &f, hipStream_t stream)
 {
-    // few items are cut into many parts each, many into few: one request over 4 K tokens 16.8 us with four groups of parts and 20.1 with
-    // one, 64 requests 189 with one and 196 with four
+    // few items are cut into many parts each, many into few: one request over 4 K tokens 16.5 us with four groups of parts and 20.1 with
+    // one, 64 requests 183 with one and 190 with four
     const bool many_parts = (long)a.batch * f.col_tiles * 4 < f.shares;
     constexpr int kEach = kCols >= 128 ? 4 : 1;
     const int columns = 256 / (kD / 4) * (many_parts ? 1 : kEach) / (many_parts ? 4 : 1);

@@ -13,7 +13,7 @@
 //
 // Bound by HBM where there is work enough: 64 requests of 5 rows over 256 - 4096 tokens (32 heads over 8, bf16, 0.6 GB) 117 us, of
 // which the launch for cut items takes 5: 5.0 TB/s; its loads alone run in 96.  In short calls by latency: one request over
-// 1.8 K tokens 13.4 us, 10.3 for the first launch (place of the share 2.6, page ids and requests 3, K and V 1.2, products 2, waves
+// 1.8 K tokens 13.9 us, 10.3 - 11 for the first launch (place of the share 2.6, page ids and requests 3, K and V 1.2, products 2, waves
 // meet 2).  fp32: the matrix instruction takes 32 products a cycle and SIMD, 3.2 of the 4.5 us of a wave's subtile for 48 columns; 8
 // requests over 300 - 700 tokens 28 us.
 #pragma once
@@ -51,14 +51,16 @@ struct TreeArgs {
     int sides;                            // see side_by_side
 };
 
-// Workgroups a compute unit: two where the registers allow it.
+// Workgroups a compute unit: two where the registers allow it.  Else one, with one wave a SIMD: 128 dims take 256 VGPRs and 80 - 230
+// accumulation registers, 64 dims with 48 or 64 columns 256 and 80 - 140; 64 dims with fewer 175 - 228 in all.
 constexpr int tree_workgroups(int dim, int blocks) { return dim == 64 && blocks <= 2 ? 2 : 1; }
 
 // Columns of a tile at most: what a wave's registers hold beside the K and V on their way.
-// (64 of 128 dims spill: 64 requests of 16 rows over 4 K tokens 297 us, the wide form 209.)
+// (64 of 128 dims spill: 64 requests of 16 rows over 4 K tokens each 253 us, the wide form 214.)
 constexpr int tree_columns(int dim) { return dim == 64 ? 64 : 48; }
-// Subtiles a wave has in flight, in registers: two where there is room for them.
-// (64 requests of 5 rows over 256 - 4096 tokens: 121 us, with one set 140.)
+// Subtiles a wave has in flight, in registers: two where there is room for them.  64 requests over 256 - 4096 tokens, bf16, 32 heads
+// over 8: of 8 rows 121 us, with one set 122; 64 dims, of 12 rows 79 and 91.  With less to compute per subtile one set is no worse: of 5
+// rows 118 and 117, of one row 105 and 102; 64 dims, of 5 rows 72 and 67; one request over 1.8 K tokens 14.7 and 13.8.
 constexpr int tree_depth(int dim, int blocks) { return dim == 64 || blocks <= 2 ? 2 : 1; }
 
 template <int DT, int kD, int kBlocks> struct TreeShape {
@@ -165,7 +167,7 @@ __device__ __forceinline__ void share_and_head(const TreeArgs &a, int &share, in
 
 // Column tiles side by side.  Where (nearly) all requests have a.sides column tiles, their workgroups walk the same
 // tokens at the same time, on one XCD: K and V then come from its L2 for all but one of them (16 trees of 33 - 64 rows, two
-// tiles: 0.34 instead of 1.08 GB from HBM, 308 us instead of 320).  Units are subtiles there, and
+// tiles: 0.34 instead of 1.08 GB from HBM, 288 us instead of 305).  Units are subtiles there, and
 // share (x + 8 j) takes column tile j % sides of span x + 8 (j / sides).  (n_shares is a multiple of 8 * sides.)
 __device__ __forceinline__ int share_of_span(int span, int side, int sides) { return span % 8 + 8 * (span / 8 * sides + side); }
 __device__ __forceinline__ bool side_by_side(const TreeArgs &a, long units, long spans)
@@ -209,8 +211,8 @@ struct TreePlace {
 // A share that goes over from one item to another starts twice and joins its waves' results twice, which a small batch notices: if
 // parts of a common number of units, whole turns (kTurn) and at most two turns more than equal shares have, take no more
 // shares than there are, no part crosses an item's end.  Measured against equal shares (32 heads over 8, bf16): 3 requests of 5 rows over
-// 50 - 500 tokens 14.0 for 18.9 us, 8 over 1 - 4 K 26.7 for 31.7, 8 over 4 - 16 K 70.5 for 71.8, 8 trees of 64 rows over 1 - 4 K
-// 53.6 for 63.6; at 16 over 2 - 8 K they take too many shares.
+// 50 - 500 tokens 14.5 for 18.4 us, 8 over 1 - 4 K 26.6 for 29.5, 8 over 4 - 16 K 65.0 for 67.1, 8 trees of 64 rows over 1 - 4 K
+// 54 for 64.5; at 16 over 2 - 8 K they take too many shares.
 template <int kCols, int kSub, int kThreads, bool kSides, int kLeast, int kTurn>
 __device__ __forceinline__ void tree_place(const TreeArgs &a, int share, TreePlace &at)
 {
@@ -256,8 +258,9 @@ __device__ __forceinline__ void tree_place(const TreeArgs &a, int share, TreePla
         span = share % 8 + 8 * (j / a.sides);
         spans = a.n_shares / a.sides;
     }
-    // Shares in use: of no fewer units than kLeast, but as many as there are requests with rows, if there are as many (17 requests
-    // of 8 rows over 3 - 21 tokens 14.4 us, with kLeast alone 33; 24 trees of 64 rows over 20 - 180 tokens 27 and 53).
+    // Shares in use: of no fewer units than kLeast, but as many as there are requests with rows, if there are as many (40 requests of
+    // 8 rows over 3 - 21 tokens 21 us, with kLeast alone 33; 70 of 64 rows over 3 - 60 tokens 72 and 75, of 5 rows 33.5 and 32.5; where
+    // parts take no more shares than there are, these decide, and both are the same).
     int requests = per > 1 ? spans : 0;
 #pragma unroll
     for (int w = 0; w < kThreads / 64; w++) requests += busy_of[w];
@@ -695,7 +698,8 @@ __global__ __launch_bounds__(kTreeThreads, tree_workgroups(kD, kBlocks)) void tr
             if constexpr (DT == DSKV_F32) {
                 p[k] = __builtin_bit_cast(u32x4, f32x4{w[0], w[1], w[2], w[3]});
             } else {
-                // rounded to 16 bits for the matrix product: half a step of each weight (see headroom)
+                // rounded to 16 bits for the matrix product: half a step of each weight (see headroom); bf16 results are off by
+                // 0.0020 - 0.0023 of their norm, with weights in 32 bits by 0.0017, their own rounding
 #pragma unroll
                 for (int e = 0; e < 4; e++) p[k][e] = Elt<DT>::pack2(w[2 * e], w[2 * e + 1]);
             }
@@ -822,7 +826,7 @@ __global__ __launch_bounds__(kTreeThreads, tree_workgroups(kD, kBlocks)) void tr
 
 // Items that were cut: a thread per (column, four dims) and group of parts.  kGroups > 1, for items in many parts: each takes
 // every kGroups-th part, and they meet in LDS.  kEach > 1, for many columns: columns that a thread takes at once (66
-// MB of partials, 16 trees of 33 - 64 rows: 16 us with four, 23 with one).
+// MB of partials, 16 trees of 33 - 64 rows: 16 us with four, 24 with one).
 template <int DT, int kD, int kCols, int kSub, int kGroups, int kEach>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int max_col_tiles)
 {

@@ -4,17 +4,19 @@
 // scaled.
 //
 // Bound by the matrix pipeline and the vector instructions beside it: 16 of 32x32x16 per block and wave, 16 exponentials and some 75
-// other instructions (128 dims).  16 requests over 1 - 16 K tokens, 64 heads over 8, bf16: with 64 rows each 316 us, 920 TFLOP/s; with 33
-// to 64 rows 281 - 296, 750 - 790 TFLOP/s, since a block lasts as long as its units with two busy waves, and columns come in
-// thirty-twos; of that 16 us are the launch for cut items (66 MB of partials).
+// other instructions (128 dims).  16 requests over 1 - 16 K tokens, 64 heads over 8, bf16, when the board's power has settled: with 64 rows
+// each, over 160 K tokens in all, 370 us, 905 TFLOP/s; with 33 to 64 rows over 136 K 281 - 296, 750 - 790 TFLOP/s, since a block lasts as
+// long as its units with two busy waves, and columns come in thirty-twos; of that 15 us are the launch for cut items (66 MB of
+// partials).  The first thirty calls behind a pause take 330 - 340.
 // With 64 dims a stage holds two blocks side by side, so that a load fetches whole kilobytes there, too, and both sizes share one
-// layout of LDS: 16 requests of 48 rows, 64 heads, 175 us (the narrow form: 333).
-// Measured and left out: priority for the matrix instructions (281 for 276 us), exponentials free to move through the iteration (285).
+// layout of LDS: 16 requests of 48 rows, 64 heads, over 160 K tokens in all 205 us, 610 TFLOP/s (the narrow form: 396): half the
+// products of 128 dims for the same exponentials.
+// Measured and left out: priority for the matrix instructions (2 % slower), exponentials free to move through the iteration (3 %).
 //
 // Iteration j of a walk multiplies P(j - 1) into V(j - 1), turns S(j) into P(j) and computes S(j + 1), so that all of
 // its matrix instructions are independent of its exponentials.  Blocks lie in kStages stages of K and of V; iteration j
 // requests K(j + kStages) and V(j + kStages - 2) behind its only barrier, and reads the operands of K(j + 2) at its end; with eight
-// stages there is room for two iterations to a barrier (276 us instead of 285 for 48 rows), V one block later.  The running maximum
+// stages there is room for two iterations to a barrier (48 rows as above 324 us, with one 327), V one block later.  The running maximum
 // of a column is raised only when a block's weights under it sum to more than most_weight in a lane.  Weights are rounded to 16
 // bits for the matrix product, half a step of each (see headroom); sums, maxima and O stay in 32.
 // Where a token lies in the pool is looked up for some thousand tokens at a time and kept in LDS (row numbers, a bit per token that

@@ -311,7 +311,8 @@ class Verdict:
 
 def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Tensor, qo_indptr: torch.Tensor, *,
                   parents: Optional[torch.Tensor] = None, draft_probs: Optional[torch.Tensor] = None) -> Verdict:
-    """Accepts or refuses drafted tokens so that the tokens given are distributed as the target's own.
+    """Accepts or refuses drafted tokens so that the tokens given are distributed as the target's own - as its rows say,
+    if they sum to 1, the draft's too: R below starts at 1, not at a row's sum.  Rows of fewer bits are off by their rounding.
 
     target_probs (tokens, vocab): row t the target's probabilities of what follows row t.  tokens, uniforms (int32,
     float32): every row's token and its number from [0, 1); that of a request's row 0 is for the last draw.  From row 0 on the

@@ -622,6 +622,7 @@ int dskv_tree_attn(const dskv_tree_step_t *step, void *out, const void *q, int64
  *     uniform * q(x) < p(x);
  *   else: it passes if no earlier child refused there has token x and uniform * (1 - sum of p over the distinct tokens of those)
  *     < p(x).
+ * Tokens are distributed as the target's rows say where these, and the draft's, sum to 1, which nothing here checks or mends.
  * Where none passes (or there is none) the walk ends, and the request's last token is the first t with cumulated
  * w(0..t) > uniforms[row 0] * sum of w, where w = max(p - q, 0) if a child was refused with draft_probs, p with the refused
  * children's tokens at 0 without, and p if w has no mass (token 0 if p has none).  A last number below 0 counts as 0, one from 1 on
