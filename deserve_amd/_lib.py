@@ -67,6 +67,18 @@ class TreeStep(ctypes.Structure):
                                "num_pages", "dtype")] + [("sm_scale", c_float)]
 
 
+class QuantRows(ctypes.Structure):
+    """dskv_quant_rows_t of include/dskv.h."""
+    _fields_ = [(n, c_void_p) for n in ("qo_indptr", "kv_page_indices", "kv_page_indptr", "kv_last_page_lens")] + [
+        ("n_page_indices", c_int64)] + [
+        (n, c_int32) for n in ("batch", "nnz", "num_pages", "page_size", "n_kv_heads", "head_dim")]
+
+
+class QuantStep(ctypes.Structure):
+    """dskv_quant_step_t of include/dskv.h."""
+    _fields_ = [("step", TreeStep), ("min_qo_len", c_int32)]
+
+
 _lib: Optional[ctypes.CDLL] = None
 
 # name -> (restype, argtypes); mirrors include/dskv.h one to one
@@ -156,6 +168,12 @@ _SIGNATURES = {
                            [c_int32] * 4 + [c_void_p]),
     "dskv_move_rows": (c_int32, [c_void_p, c_int64, c_int32, c_int32, c_int32, c_int64] + [c_void_p] * 4 +
                        [c_int32, c_int32, c_void_p]),
+    "dskv_quant_page_bytes": (c_int64, [c_int32] * 3),
+    "dskv_rope_append_quant": (c_int32, [POINTER(QuantRows)] + [c_void_p] * 5 + [c_int64] * 3 +
+                               [c_void_p, c_int32, c_int32, c_void_p]),
+    "dskv_quant_attn_workspace": (c_int64, [c_int32] * 7),
+    "dskv_quant_attn": (c_int32, [POINTER(QuantStep), c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
+    "dskv_move_quant_rows": (c_int32, [POINTER(QuantRows), c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_void_p]),
     "dskv_swap_slice": (c_int32, [c_void_p, c_int64, c_int64, c_int32, c_void_p, c_void_p,
                                   c_void_p, c_void_p]),
     "dskv_swap_create": (c_int32, [POINTER(c_void_p), c_int64]),

@@ -92,6 +92,27 @@ int launch_append(void *pages_layer, int32_t num_pages, const void *k, const voi
                   int32_t n_kv_heads, int32_t head_dim, int32_t elt_bytes, const float *rope_table,
                   int32_t dtype, hipStream_t stream);
 
+// Largest b with qo_indptr[b] <= t < qo_indptr[b + 1], or -1; by a whole wave, 64 entries at a time.
+__device__ __forceinline__ int request_of_row(const int32_t *indptr, int batch, int t)
+{
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = batch;                 // entries lo .. lo + n hold the answer
+    while (n > 64) {
+        const int step = (n + 63) / 64;
+        const int at = lo + lane * step;
+        const unsigned long long le = __ballot(at < lo + n && indptr[min(at, batch)] <= t);
+        const int k = __popcll(le);
+        if (k == 0) return -1;
+        const int next = lo + (k - 1) * step;
+        n = min(step, lo + n - next);
+        lo = next;
+    }
+    const unsigned long long le = __ballot(lane < n && indptr[min(lo + lane, batch)] <= t);
+    if (le == 0) return -1;
+    const int b = lo + __popcll(le) - 1;
+    return t < indptr[b + 1] ? b : -1;
+}
+
 static inline bool is_pow2(int64_t x) { return x > 0 && (x & (x - 1)) == 0; }
 static inline int ilog2(int64_t x) {
     int s = 0;

@@ -1,0 +1,168 @@
+// Attention of a step's rows over pages of 8-bit K/V: what tree_attn.hip computes, with k_j = code * scale of its block and v_j alike.
+// A token that an append took for no number has K codes that are none: its score is none either, which reaches the rows that see it and, chosen
+// away by the mask, no others.  V codes are numbers.
+#include "quant.h"
+#include "tree_kernel.h"
+
+namespace dskv {
+
+struct QuantArgs : TreeArgs {
+    long head_bytes, half_bytes, page_bytes;      // see quant.h
+};
+
+// Any type and head dim: one workgroup per (row, q head) whose waves take every kQuantWaves-th group of four keys.  Lane
+// (g, c) holds dims 8 c .. 8 c + 7 (and 128 more ..) of key g of the group.
+constexpr int kQuantWaves = 8;
+
+template <int DT, int kChunks>
+__global__ __launch_bounds__(kQuantWaves * 64) void quant_generic_kernel(QuantArgs a)
+{
+    constexpr int E = DT == DSKV_F32 ? 4 : 2;                    // bytes of an element of q and out
+    const int t = blockIdx.x, h = blockIdx.y;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
+    const int b = request_of_row(a.qo_indptr, a.batch, t);
+    if (b < 0) return;
+    const int first = a.qo_indptr[b], i = t - first;
+    if (i < 0 || i >= a.max_rows) return;
+    const int page0 = a.kv_page_indptr[b];
+    const TreeTokens tokens = tree_tokens(page0, a.kv_page_indptr[b + 1], a.kv_last_page_lens[b], a.page_size, a.n_page_indices);
+    const long prior = tokens.len - ((long)a.qo_indptr[b + 1] - first);
+    const unsigned long long mask = a.masks ? (unsigned long long)a.masks[t] : 0;
+    const long seen = a.masks ? tokens.walk : min(tokens.walk, prior + i + 1);
+    const int kv_head = h / (a.n_qo_heads / a.n_kv_heads);
+    const char *const block = a.pages + kv_head * a.head_bytes, *const scales = a.pages + 2 * a.half_bytes + kv_head * 4;
+    float q[kChunks][8], o[kChunks][8];
+#pragma unroll
+    for (int k = 0; k < kChunks; k++)
+#pragma unroll
+        for (int d = 0; d < 8; d++) q[k][d] = o[k][d] = 0;
+#pragma unroll
+    for (int k = 0; k < kChunks; k++)
+        if (k * 128 + c * 8 < a.head_dim) {
+            const char *p = a.q + t * a.q_stride + ((long)h * a.head_dim + k * 128 + c * 8) * E;
+            Chunk<DT>::unpack(*reinterpret_cast<const u32x4 *>(p), q[k]);
+            if constexpr (E == 4) Chunk<DT>::unpack(*reinterpret_cast<const u32x4 *>(p + 16), q[k] + 4);
+        }
+    float m = -INFINITY, l = 0;
+    for (long j = wave * 4 + g; j - g < seen; j += kQuantWaves * 4) {
+        bool there = j < seen;
+        if (there && a.masks && j >= prior) there = j - prior < DSKV_MAX_TREE_ROWS && (mask >> (j - prior)) & 1;
+        long page = -1;
+        if (there) {
+            const long entry = page0 + j / a.page_size;
+            if (entry >= 0 && entry < a.n_page_indices) page = a.kv_page_indices[entry];
+        }
+        there = page >= 0 && page < a.num_pages;
+        const long record = (there ? page : 0) * a.page_bytes;
+        const char *key = block + record + (there ? j % a.page_size : 0) * a.head_dim;
+        float s = 0, v[kChunks][8];
+#pragma unroll
+        for (int k = 0; k < kChunks; k++) {
+#pragma unroll
+            for (int d = 0; d < 8; d++) v[k][d] = 0;
+            if (there && k * 128 + c * 8 < a.head_dim) {
+                float x[8];
+                decode8(*reinterpret_cast<const u32x2 *>(key + k * 128 + c * 8), x);
+                decode8(*reinterpret_cast<const u32x2 *>(key + a.half_bytes + k * 128 + c * 8), v[k]);
+#pragma unroll
+                for (int d = 0; d < 8; d++) s = fmaf(q[k][d], x[d], s);
+            }
+        }
+#pragma unroll
+        for (int x = 1; x < 16; x <<= 1) s += __shfl_xor(s, x);
+        if (there) {
+            const float *scale = reinterpret_cast<const float *>(scales + record);
+            s *= scale[0] * a.scale;
+            const float top = fmaxf(m, s);
+            const float base = top == -INFINITY ? 0.f : top;
+            const float keep = __builtin_amdgcn_exp2f(m - base), p = __builtin_amdgcn_exp2f(s - base), pv = p * scale[a.n_kv_heads];
+            m = top;
+            l = l * keep + p;
+#pragma unroll
+            for (int k = 0; k < kChunks; k++)
+#pragma unroll
+                for (int d = 0; d < 8; d++) o[k][d] = fmaf(o[k][d], keep, pv * v[k][d]);
+        }
+    }
+    // the 4 * kQuantWaves running sums meet in LDS
+    __shared__ float ms[kQuantWaves * 4], ls[kQuantWaves * 4];
+    __shared__ float os[kQuantWaves * 4][kChunks * 128 + 4];
+    const int part = wave * 4 + g;
+    if (c == 0) {
+        ms[part] = m;
+        ls[part] = l;
+    }
+#pragma unroll
+    for (int k = 0; k < kChunks; k++)
+#pragma unroll
+        for (int d = 0; d < 8; d++) os[part][k * 128 + c * 8 + d] = o[k][d];
+    __syncthreads();
+    float top = -INFINITY;
+    for (int p = 0; p < kQuantWaves * 4; p++) top = fmaxf(top, ms[p]);
+    const float base = top == -INFINITY ? 0.f : top;
+    for (int d = threadIdx.x; d < a.head_dim; d += kQuantWaves * 64) {
+        float sum = 0, acc = 0;
+        for (int p = 0; p < kQuantWaves * 4; p++) {
+            const float w = __builtin_amdgcn_exp2f(ms[p] - base);
+            sum += ls[p] * w;
+            acc += os[p][d] * w;
+        }
+        LoadElt<DT>::put(a.out, ((long)t * a.n_qo_heads + h) * a.head_dim + d, sum > 0 ? acc / sum : sum == 0 ? 0.f : NAN);
+    }
+}
+
+}  // namespace dskv
+
+extern "C" int64_t dskv_quant_attn_workspace(int32_t batch, int32_t nnz, int32_t max_qo_len, int32_t n_qo_heads,
+                                             int32_t n_kv_heads, int32_t head_dim, int32_t dtype)
+{
+    return 0;
+}
+
+extern "C" int dskv_quant_attn(const dskv_quant_step_t *step, void *out, const void *q, int64_t q_stride,
+                               const void *pages_layer, void *stream)
+{
+    using namespace dskv;
+    DSKV_REQUIRE(step, "quant_attn: null arguments");
+    const dskv_tree_step_t *s = &step->step;
+    DSKV_REQUIRE(s->batch >= 0 && s->nnz >= 0 && s->max_qo_len >= 0 && step->min_qo_len >= 0, "quant_attn: negative batch, nnz or rows");
+    DSKV_REQUIRE(s->dtype == DSKV_F32 || s->dtype == DSKV_F16 || s->dtype == DSKV_BF16, "quant_attn: unknown dtype %d", s->dtype);
+    DSKV_REQUIRE(s->n_kv_heads > 0 && s->n_qo_heads > 0 && s->n_qo_heads % s->n_kv_heads == 0,
+                 "quant_attn: n_qo_heads %d must be a multiple of n_kv_heads %d", s->n_qo_heads, s->n_kv_heads);
+    DSKV_REQUIRE(s->head_dim > 0 && s->head_dim % 8 == 0 && s->head_dim <= 256,
+                 "quant_attn: head_dim %d must be a multiple of 8 up to 256", s->head_dim);
+    DSKV_REQUIRE(s->page_size > 0 && s->num_pages > 0 && s->n_page_indices >= 0, "quant_attn: bad page shape");
+    DSKV_REQUIRE(s->sm_scale > 0, "quant_attn: sm_scale must be positive");
+    DSKV_REQUIRE(!s->masks || s->max_qo_len <= DSKV_MAX_TREE_ROWS, "quant_attn: masks hold %d rows a request, max_qo_len is %d",
+                 DSKV_MAX_TREE_ROWS, s->max_qo_len);
+    if (s->batch == 0 || s->nnz == 0 || s->max_qo_len == 0) return 0;
+    const int size = s->dtype == DSKV_F32 ? 4 : 2;
+    DSKV_REQUIRE(out && q && pages_layer && s->qo_indptr && s->kv_page_indptr && s->kv_last_page_lens &&
+                 (s->kv_page_indices || s->n_page_indices == 0), "quant_attn: null pointer argument");
+    DSKV_REQUIRE(q_stride >= (int64_t)s->n_qo_heads * s->head_dim, "quant_attn: rows of q overlap");
+    DSKV_REQUIRE(((uintptr_t)out | (uintptr_t)q | (uintptr_t)pages_layer) % 16 == 0 && q_stride * size % 16 == 0,
+                 "quant_attn: tensors and their rows must be 16-byte aligned");
+    const QuantShape shape = quant_shape(s->num_pages, s->page_size, s->n_kv_heads, s->head_dim);
+    QuantArgs a = {};
+    (TreeArgs &)a = {s->qo_indptr, s->kv_page_indptr, s->kv_page_indices, s->kv_last_page_lens, s->masks, (char *)out,
+                     (const char *)q, (const char *)pages_layer, (long)q_stride * size, (long)s->n_page_indices, s->batch,
+                     s->nnz, s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->head_dim, s->page_size, s->num_pages,
+                     s->sm_scale * 1.4426950408889634f};
+    a.head_bytes = shape.head_bytes;
+    a.half_bytes = shape.half_bytes;
+    a.page_bytes = shape.page_bytes;
+    hipStream_t st = (hipStream_t)stream;
+    DSKV_REQUIRE(s->n_qo_heads <= 65535, "quant_attn: at most 65535 heads");
+    const dim3 grid((unsigned)s->nnz, (unsigned)s->n_qo_heads), block(kQuantWaves * 64);
+#define DSKV_QUANT_GENERIC(DT)                                                                                 \
+    do {                                                                                                       \
+        if (s->head_dim <= 128) hipLaunchKernelGGL((quant_generic_kernel<DT, 1>), grid, block, 0, st, a);      \
+        else hipLaunchKernelGGL((quant_generic_kernel<DT, 2>), grid, block, 0, st, a);                         \
+    } while (0)
+    if (s->dtype == DSKV_F32) DSKV_QUANT_GENERIC(DSKV_F32);
+    else if (s->dtype == DSKV_F16) DSKV_QUANT_GENERIC(DSKV_F16);
+    else DSKV_QUANT_GENERIC(DSKV_BF16);
+#undef DSKV_QUANT_GENERIC
+    DSKV_LAUNCH_CHECK("quant_generic_kernel");
+    return 0;
+}

@@ -1,0 +1,403 @@
+// Rows of a step into pages of 8-bit K/V: the append of new rows, rotated on their way, and the move of accepted ones.
+#include "quant.h"
+#include "rope_math.h"
+
+namespace dskv {
+
+// Requests of a step: their rows' places, from the index arrays and within the bounds of the tensors.
+struct QuantRows {
+    const int32_t *qo_indptr, *kv_page_indices, *kv_page_indptr, *kv_last_page_lens;
+    long n_page_indices;
+    int batch, nnz;
+    QuantShape s;
+};
+
+// Request b: its rows and the tokens in front of them; n = 0 where the arrays contradict themselves.
+struct QuantRequest {
+    long first, n, prior;
+    int page0;
+};
+__device__ __forceinline__ QuantRequest quant_request(const QuantRows &a, int b)
+{
+    QuantRequest r;
+    r.first = a.qo_indptr[b];
+    r.n = (long)a.qo_indptr[b + 1] - r.first;
+    r.page0 = a.kv_page_indptr[b];
+    const long pages = (long)a.kv_page_indptr[b + 1] - r.page0;
+    const int last = a.kv_last_page_lens[b];
+    r.prior = (pages - 1) * a.s.page_size + last - r.n;
+    if (r.first < 0 || r.n < 0 || r.first + r.n > a.nnz || pages < 1 || last < 1 || last > a.s.page_size || r.prior < 0) r.n = 0;
+    return r;
+}
+// Page of the request's token t, -1 where there is none.
+__device__ __forceinline__ long quant_page(const QuantRows &a, const QuantRequest &r, long t)
+{
+    const long entry = r.page0 + t / a.s.page_size;
+    if (entry < 0 || entry >= a.n_page_indices) return -1;
+    const int page = a.kv_page_indices[entry];
+    return page >= 0 && page < a.s.num_pages ? page : -1;
+}
+
+// ---- append
+
+struct QuantAppend {
+    QuantRows r;
+    char *q_out, *pages;
+    const char *q, *k, *v;
+    long q_stride, k_stride, v_stride;   // bytes
+    const float *table;
+    int n_qo_heads, kv_blocks;
+    float most;                          // the largest value that code * scale may take in the type
+};
+
+// 8 elements of a row as floats, rotated by the row's angles (table null: not).
+template <int DT> struct Eight {
+    u32x4 raw[DT == DSKV_F32 ? 2 : 1];
+    __device__ __forceinline__ void load(const char *p)
+    {
+        raw[0] = *reinterpret_cast<const u32x4 *>(p);
+        if constexpr (DT == DSKV_F32) raw[1] = *reinterpret_cast<const u32x4 *>(p + 16);
+    }
+    __device__ __forceinline__ void unpack(float *f) const
+    {
+        Chunk<DT>::unpack(raw[0], f);
+        if constexpr (DT == DSKV_F32) Chunk<DT>::unpack(raw[1], f + 4);
+    }
+    __device__ __forceinline__ void store(char *p, const float *f) const
+    {
+        *reinterpret_cast<u32x4 *>(p) = Chunk<DT>::pack(f);
+        if constexpr (DT == DSKV_F32) *reinterpret_cast<u32x4 *>(p + 16) = Chunk<DT>::pack(f + 4);
+    }
+};
+__device__ __forceinline__ void rotate8(float *f, const float *table, long t, int col, int head_dim)
+{
+    const f32x4 c = *reinterpret_cast<const f32x4 *>(table + t * head_dim + col * 4);
+    const f32x4 s = *reinterpret_cast<const f32x4 *>(table + t * head_dim + head_dim / 2 + col * 4);
+    const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
+    rope_rotate<4>(f, cs, sn);
+}
+__device__ __forceinline__ float wave_max(float v)
+{
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    return v;
+}
+
+// Workgroups of the first kv_blocks rows of the grid: one wave per (row of the step, kv head).  The row that is the first of its
+// request in a page takes all of them there, and the block with them: their largest values, the scale, what the block holds already rounded anew
+// where that grows, and the codes.  The other rows' waves end at once.  Workgroups behind: q, a row each.
+// kLanes: lanes of a row, 8 elements each, a power of two.
+template <int DT, int kLanes>
+__global__ __launch_bounds__(256) void quant_append_kernel(QuantAppend a)
+{
+    constexpr int kElt = DT == DSKV_F32 ? 4 : 2, kRows = 64 / kLanes;
+    const QuantShape &s = a.r.s;
+    const int t = blockIdx.x, lane = threadIdx.x & 63, col = lane % kLanes, row = lane / kLanes;
+    const bool works = col * 8 < s.head_dim;
+    if ((int)blockIdx.y >= a.kv_blocks) {
+        for (int h = threadIdx.x / kLanes; h < a.n_qo_heads; h += 256 / kLanes) {
+            if (!works) continue;
+            Eight<DT> x;
+            float f[8];
+            x.load(a.q + t * a.q_stride + ((long)h * s.head_dim + col * 8) * kElt);
+            x.unpack(f);
+            rotate8(f, a.table, t, col, s.head_dim);
+            x.store(a.q_out + (((long)t * a.n_qo_heads + h) * s.head_dim + col * 8) * kElt, f);
+        }
+        return;
+    }
+    const int head = blockIdx.y * 4 + (threadIdx.x >> 6);
+    if (head >= s.n_kv_heads) return;
+    const int b = request_of_row(a.r.qo_indptr, a.r.batch, t);
+    if (b < 0) return;
+    const QuantRequest r = quant_request(a.r, b);
+    const long i = t - r.first, at = r.prior + i;
+    if (r.n == 0) return;
+    const int place = (int)(at % s.page_size);
+    if (i > 0 && place > 0) return;
+    const int count = (int)min((long)s.page_size - place, r.n - i);       // rows of the request in this page
+    const long page = quant_page(a.r, r, at);
+    if (page < 0) return;
+    char *const record = a.pages + page * s.page_bytes;
+    const long k_at = head * s.head_bytes, v_at = s.half_bytes + k_at;
+    uint32_t *const scales = reinterpret_cast<uint32_t *>(record + 2 * s.half_bytes);
+
+    const char *const k_rows = a.k + t * a.k_stride + ((long)head * s.head_dim + col * 8) * kElt;
+    const char *const v_rows = a.v + t * a.v_stride + ((long)head * s.head_dim + col * 8) * kElt;
+    // a token of which a value is no finite number: its K becomes no number, so that rows that see it get none and
+    // the others, whose weight of it is 0, are not touched by its V, which becomes 0
+    auto fetch = [&](int j, float *k, float *v) -> bool {
+#pragma unroll
+        for (int d = 0; d < 8; d++) k[d] = v[d] = 0;
+        if (works && j < count) {
+            Eight<DT> x, y;
+            x.load(k_rows + j * a.k_stride);
+            y.load(v_rows + j * a.v_stride);
+            x.unpack(k);
+            y.unpack(v);
+            if (a.table) rotate8(k, a.table, t + j, col, s.head_dim);
+        }
+        bool fine = true;
+#pragma unroll
+        for (int d = 0; d < 8; d++) fine = fine && fabsf(k[d]) <= __FLT_MAX__ && fabsf(v[d]) <= __FLT_MAX__;
+        const unsigned long long odd = __ballot(!fine) >> (row * kLanes);
+        return kLanes == 64 ? odd == 0 : (odd & ((1ull << kLanes) - 1)) == 0;
+    };
+    float k[8], v[8], k_most = 0, v_most = 0;
+    for (int j0 = 0; j0 < count; j0 += kRows)
+        if (fetch(j0 + row, k, v)) {
+#pragma unroll
+            for (int d = 0; d < 8; d++) {
+                k_most = fmaxf(k_most, fabsf(k[d]));
+                v_most = fmaxf(v_most, fabsf(v[d]));
+            }
+        }
+    const float most[2] = {fminf(wave_max(k_most), a.most), fminf(wave_max(v_most), a.most)};
+    uint32_t scale[2];
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+        uint32_t *const held = scales + x * s.n_kv_heads + head;
+        const uint32_t old = place > 0 ? stored_scale(*held) : 0u;
+        scale[x] = max(needed_scale(most[x]), old);
+        if (old != 0 && scale[x] > old) {
+            const float ratio = __builtin_bit_cast(float, old) * reciprocal_of(scale[x]);
+            for (int j = lane; j < place * s.head_dim / 8; j += 64) {
+                u32x2 *const codes = reinterpret_cast<u32x2 *>(record + (x ? v_at : k_at)) + j;
+                float f[8];
+                decode8(*codes, f);
+#pragma unroll
+                for (int d = 0; d < 8; d++) f[d] *= ratio;
+                *codes = encode8(f);
+            }
+        }
+        if (lane == 0) *held = scale[x];
+    }
+    const float k_by = reciprocal_of(scale[0]), v_by = reciprocal_of(scale[1]);
+    for (int j0 = 0; j0 < count; j0 += kRows) {
+        const int j = j0 + row;
+        const bool fine = fetch(j, k, v);
+        if (!works || j >= count) continue;
+#pragma unroll
+        for (int d = 0; d < 8; d++) {
+            k[d] = fminf(fmaxf(k[d], -a.most), a.most) * k_by;
+            v[d] = fminf(fmaxf(v[d], -a.most), a.most) * v_by;
+        }
+        const uint32_t none = kNoNumberCode * 0x01010101u;
+        const long to = (long)(place + j) * s.head_dim + col * 8;
+        *reinterpret_cast<u32x2 *>(record + k_at + to) = fine ? encode8(k) : u32x2{none, none};
+        *reinterpret_cast<u32x2 *>(record + v_at + to) = fine ? encode8(v) : u32x2{0, 0};
+    }
+}
+
+// ---- move
+
+struct QuantMove {
+    QuantRows r;
+    char *pages;
+    long layer_stride;
+    const int32_t *path, *counts;
+};
+
+// One wave per (request, half and head, layer).  All rows that move are read first; then the pages that they go to are taken one by
+// one: the scale that the rows need there, what else the block holds rounded anew where it grows, and the rows.
+// Lane j keeps row j of the walk; kLanes: lanes of a row's codes, 8 each.
+template <int kLanes>
+__global__ __launch_bounds__(256) void quant_move_kernel(QuantMove a)
+{
+    constexpr int kRows = 64 / kLanes, kPasses = DSKV_MAX_TREE_ROWS / kRows;
+    const QuantShape &s = a.r.s;
+    const int b = blockIdx.x, lane = threadIdx.x & 63, col = lane % kLanes, row = lane / kLanes;
+    const int block = blockIdx.y * 4 + (threadIdx.x >> 6);                 // half and head
+    if (block >= 2 * s.n_kv_heads) return;
+    const QuantRequest r = quant_request(a.r, b);
+    const int count = (int)min((long)a.counts[b], r.n);
+    if (count < 2 || count > DSKV_MAX_TREE_ROWS) return;
+    char *const layer = a.pages + blockIdx.z * a.layer_stride;
+    const long block_at = block * s.head_bytes, scale_at = 2 * s.half_bytes + block * 4L;
+
+    const int p = lane < count ? a.path[r.first + lane] : -1;
+    const int before = __shfl_up(p, 1);
+    const bool goes = lane > 0 && lane < count && p > lane && p < r.n && p > before;
+    long from = -1, to = -1;                                              // pages
+    if (goes) {
+        from = quant_page(a.r, r, r.prior + p);
+        to = quant_page(a.r, r, r.prior + lane);
+    }
+    const bool moves = from >= 0 && to >= 0;
+    const unsigned long long moving = __ballot(moves);
+    if (moving == 0) return;
+    const long from_at = from * s.page_bytes + block_at + (r.prior + p) % s.page_size * s.head_dim;
+    const int place = (int)((r.prior + lane) % s.page_size);
+    const float from_scale = moves ? *reinterpret_cast<const float *>(layer + from * s.page_bytes + scale_at) : 0.f;
+
+    u32x2 codes[kPasses];
+    float most = 0;                                                       // of row `lane`
+#pragma unroll
+    for (int i = 0; i < kPasses; i++) {
+        const int j = i * kRows + row;
+        const long at = __shfl(from_at, j);
+        codes[i] = u32x2{0, 0};
+        if ((moving >> j) & 1 && col * 8 < s.head_dim) codes[i] = *reinterpret_cast<const u32x2 *>(layer + at + col * 8);
+    }
+#pragma unroll
+    for (int i = 0; i < kPasses; i++) {
+        // (codes without their sign are ordered as their values; 0x7F is none)
+        uint32_t top = 0;
+#pragma unroll
+        for (int w = 0; w < 2; w++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t c = codes[i][w] >> (8 * e) & 0x7F;
+                top = c == kNoNumberCode ? top : max(top, c);
+            }
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+        const uint32_t mine = (uint32_t)__shfl((int)top, lane % kRows * kLanes);      // row i * kRows + lane % kRows
+        if (lane / kRows == i) most = __builtin_amdgcn_cvt_f32_fp8((int)mine, 0) * from_scale;
+    }
+    uint32_t scale = 0;                                                   // of the page that row `lane` goes to
+    const long length = r.prior + r.n;
+    for (int j = 1; j < count;) {
+        const long begin = (r.prior + j) / s.page_size * s.page_size;     // the page's first token
+        const int end = (int)min((long)count, begin + s.page_size - r.prior);
+        const long page = quant_page(a.r, r, r.prior + j);
+        const bool here = lane >= j && lane < end && moves;
+        const float top = wave_max(here ? most : 0.f);
+        if (__ballot(here) != 0) {
+            char *const record = layer + page * s.page_bytes;
+            uint32_t *const held = reinterpret_cast<uint32_t *>(record + scale_at);
+            const uint32_t old = stored_scale(*held), now = top > 0 ? max(needed_scale(top), old) : old;
+            if (old != 0 && now > old) {
+                const float ratio = __builtin_bit_cast(float, old) * reciprocal_of(now);
+                const int rows = (int)min((long)s.page_size, length - begin);
+                for (int x = lane; x < rows * s.head_dim / 8; x += 64) {
+                    u32x2 *const at = reinterpret_cast<u32x2 *>(record + block_at) + x;
+                    float f[8];
+                    decode8(*at, f);
+#pragma unroll
+                    for (int d = 0; d < 8; d++) f[d] *= ratio;
+                    *at = encode8(f);
+                }
+            }
+            if (lane == 0 && now != old) *held = now;
+            if (here) scale = now;
+        }
+        j = end;
+    }
+    __builtin_amdgcn_s_waitcnt(0);                                        // the blocks have been rounded anew
+    asm volatile("" ::: "memory");
+    const float by = moves && scale != 0 ? from_scale * reciprocal_of(scale) : 0.f;
+    const long to_at = to * s.page_bytes + block_at + (long)place * s.head_dim;
+#pragma unroll
+    for (int i = 0; i < kPasses; i++) {
+        const int j = i * kRows + row;
+        const long at = __shfl(to_at, j);
+        const float ratio = __shfl(by, j);
+        if ((moving >> j) & 1 && col * 8 < s.head_dim) {
+            float f[8];
+            decode8(codes[i], f);
+#pragma unroll
+            for (int d = 0; d < 8; d++) f[d] *= ratio;
+            *reinterpret_cast<u32x2 *>(layer + at + col * 8) = encode8(f);
+        }
+    }
+}
+
+static int lanes_of(int head_dim)
+{
+    int lanes = 1;
+    while (lanes * 8 < head_dim) lanes *= 2;
+    return lanes;
+}
+static int check_rows(const dskv_quant_rows_t *r, const char *what)
+{
+    DSKV_REQUIRE(r, "%s: null arguments", what);
+    DSKV_REQUIRE(r->batch >= 0 && r->nnz >= 0 && r->n_page_indices >= 0, "%s: negative batch, nnz or table", what);
+    DSKV_REQUIRE(r->num_pages > 0 && r->page_size > 0 && r->n_kv_heads > 0, "%s: bad page shape", what);
+    DSKV_REQUIRE(r->head_dim > 0 && r->head_dim % 8 == 0 && r->head_dim <= 256,
+                 "%s: head_dim %d must be a multiple of 8 up to 256", what, r->head_dim);
+    DSKV_REQUIRE((int64_t)r->page_size * r->head_dim < INT32_MAX && r->n_kv_heads <= 65535, "%s: too large a page", what);
+    if (r->batch == 0 || r->nnz == 0) return 0;
+    DSKV_REQUIRE(r->qo_indptr && r->kv_page_indptr && r->kv_last_page_lens && (r->kv_page_indices || r->n_page_indices == 0),
+                 "%s: null pointer argument", what);
+    return 0;
+}
+static QuantRows rows_of(const dskv_quant_rows_t *r)
+{
+    return {r->qo_indptr, r->kv_page_indices, r->kv_page_indptr, r->kv_last_page_lens, (long)r->n_page_indices, r->batch, r->nnz,
+            quant_shape(r->num_pages, r->page_size, r->n_kv_heads, r->head_dim)};
+}
+template <int DT> static int launch_quant_append(const QuantAppend &a, hipStream_t stream)
+{
+    const dim3 grid((unsigned)a.r.nnz, (unsigned)(a.kv_blocks + (a.table ? 1 : 0))), block(256);
+    switch (lanes_of(a.r.s.head_dim)) {
+    case 1: hipLaunchKernelGGL((quant_append_kernel<DT, 1>), grid, block, 0, stream, a); break;
+    case 2: hipLaunchKernelGGL((quant_append_kernel<DT, 2>), grid, block, 0, stream, a); break;
+    case 4: hipLaunchKernelGGL((quant_append_kernel<DT, 4>), grid, block, 0, stream, a); break;
+    case 8: hipLaunchKernelGGL((quant_append_kernel<DT, 8>), grid, block, 0, stream, a); break;
+    case 16: hipLaunchKernelGGL((quant_append_kernel<DT, 16>), grid, block, 0, stream, a); break;
+    default: hipLaunchKernelGGL((quant_append_kernel<DT, 32>), grid, block, 0, stream, a); break;
+    }
+    DSKV_LAUNCH_CHECK("quant_append_kernel");
+    return 0;
+}
+
+}  // namespace dskv
+
+extern "C" int64_t dskv_quant_page_bytes(int32_t page_size, int32_t n_kv_heads, int32_t head_dim)
+{
+    return page_size > 0 && n_kv_heads > 0 && head_dim > 0 ? dskv::quant_page_bytes(page_size, n_kv_heads, head_dim) : 0;
+}
+
+extern "C" int dskv_rope_append_quant(const dskv_quant_rows_t *rows, void *q_out, void *pages_layer, const void *q, const void *k,
+                                      const void *v, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                                      const float *rope_table, int32_t n_qo_heads, int32_t dtype, void *stream)
+{
+    using namespace dskv;
+    if (int rc = check_rows(rows, "rope_append_quant")) return rc;
+    DSKV_REQUIRE(dtype == DSKV_F32 || dtype == DSKV_F16 || dtype == DSKV_BF16, "rope_append_quant: unknown dtype %d", dtype);
+    if (rows->batch == 0 || rows->nnz == 0) return 0;
+    DSKV_REQUIRE(pages_layer && k && v && (!rope_table || (q && q_out)), "rope_append_quant: null pointer argument");
+    const int size = dtype == DSKV_F32 ? 4 : 2;
+    const int64_t kv_row = (int64_t)rows->n_kv_heads * rows->head_dim;
+    DSKV_REQUIRE(!rope_table || n_qo_heads > 0, "rope_append_quant: n_qo_heads %d", n_qo_heads);
+    DSKV_REQUIRE((!rope_table || q_stride >= (int64_t)n_qo_heads * rows->head_dim) && k_stride >= kv_row && v_stride >= kv_row,
+                 "rope_append_quant: rows overlap");
+    DSKV_REQUIRE((((uintptr_t)q_out | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)pages_layer | (uintptr_t)rope_table) % 16 == 0) &&
+                 ((rope_table ? q_stride : 0) | k_stride | v_stride) * size % 16 == 0,
+                 "rope_append_quant: tensors and their rows must be 16-byte aligned");
+    QuantAppend a = {rows_of(rows), (char *)q_out, (char *)pages_layer, (const char *)q, (const char *)k, (const char *)v,
+                     (long)q_stride * size, (long)k_stride * size, (long)v_stride * size, rope_table, n_qo_heads,
+                     (rows->n_kv_heads + 3) / 4,
+                     // 240 * 2^8, 240 * 2^120: the code above, 256, would make an infinity of the type with that scale
+                     dtype == DSKV_F16 ? 61440.f : 3.1901472e38f};
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == DSKV_F32) return launch_quant_append<DSKV_F32>(a, st);
+    if (dtype == DSKV_F16) return launch_quant_append<DSKV_F16>(a, st);
+    return launch_quant_append<DSKV_BF16>(a, st);
+}
+
+extern "C" int dskv_move_quant_rows(const dskv_quant_rows_t *rows, void *pages, int64_t layer_stride_bytes, int32_t n_layers,
+                                    const int32_t *path, const int32_t *counts, void *stream)
+{
+    using namespace dskv;
+    if (int rc = check_rows(rows, "move_quant_rows")) return rc;
+    DSKV_REQUIRE(n_layers >= 0 && n_layers <= 65535, "move_quant_rows: %d layers", n_layers);
+    if (rows->batch == 0 || rows->nnz == 0 || n_layers == 0) return 0;
+    DSKV_REQUIRE(pages && path && counts, "move_quant_rows: null pointer argument");
+    DSKV_REQUIRE((uintptr_t)pages % 16 == 0 && layer_stride_bytes % 16 == 0, "move_quant_rows: pages must be 16-byte aligned");
+    QuantMove a = {rows_of(rows), (char *)pages, (long)layer_stride_bytes, path, counts};
+    DSKV_REQUIRE(n_layers == 1 || layer_stride_bytes >= rows->num_pages * a.r.s.page_bytes, "move_quant_rows: layers overlap");
+    const dim3 grid((unsigned)rows->batch, (unsigned)((2 * rows->n_kv_heads + 3) / 4), (unsigned)n_layers), block(256);
+    hipStream_t st = (hipStream_t)stream;
+    switch (lanes_of(rows->head_dim)) {
+    case 1: hipLaunchKernelGGL((quant_move_kernel<1>), grid, block, 0, st, a); break;
+    case 2: hipLaunchKernelGGL((quant_move_kernel<2>), grid, block, 0, st, a); break;
+    case 4: hipLaunchKernelGGL((quant_move_kernel<4>), grid, block, 0, st, a); break;
+    case 8: hipLaunchKernelGGL((quant_move_kernel<8>), grid, block, 0, st, a); break;
+    case 16: hipLaunchKernelGGL((quant_move_kernel<16>), grid, block, 0, st, a); break;
+    default: hipLaunchKernelGGL((quant_move_kernel<32>), grid, block, 0, st, a); break;
+    }
+    DSKV_LAUNCH_CHECK("quant_move_kernel");
+    return 0;
+}

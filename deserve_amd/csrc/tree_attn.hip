@@ -8,27 +8,6 @@
 
 namespace dskv {
 
-// Largest b with qo_indptr[b] <= t < qo_indptr[b + 1], or -1; by a whole wave, 64 entries at a time.
-__device__ __forceinline__ int request_of_row(const int32_t *indptr, int batch, int t)
-{
-    const int lane = threadIdx.x & 63;
-    int lo = 0, n = batch;                 // entries lo .. lo + n hold the answer
-    while (n > 64) {
-        const int step = (n + 63) / 64;
-        const int at = lo + lane * step;
-        const unsigned long long le = __ballot(at < lo + n && indptr[min(at, batch)] <= t);
-        const int k = __popcll(le);
-        if (k == 0) return -1;
-        const int next = lo + (k - 1) * step;
-        n = min(step, lo + n - next);
-        lo = next;
-    }
-    const unsigned long long le = __ballot(lane < n && indptr[min(lo + lane, batch)] <= t);
-    if (le == 0) return -1;
-    const int b = lo + __popcll(le) - 1;
-    return t < indptr[b + 1] ? b : -1;
-}
-
 // Any type and head dim: one workgroup per (row, q head) whose waves take every kGenericWaves-th group of four
 // keys.  Lane (g, c) holds dims 8 c .. 8 c + 7 (and 128 more ..) of key g of the group.  Bound by the
 // latency of its loads: K and V are read once per row and q head, from the caches but for the first time (64 requests of 5 rows

@@ -22,6 +22,7 @@ from deserve_amd.kvcache.paged.kvcache import PagedKVCache
 from deserve_amd.model.context.flash import FlashDecodeCtx, FlashPrefillCtx, FlashTreeCtx
 from deserve_amd.paged_ops import (BatchDecodeWithPagedKVCacheWrapper,
                                    BatchPrefillWithPagedKVCacheWrapper)
+from deserve_amd.quant_ops import BatchQuantizedWithPagedKVCacheWrapper
 from deserve_amd.task import TaskData
 
 WORKSPACE_BYTES = 128 * 1024 * 1024
@@ -48,6 +49,17 @@ def get_tree_wrapper(device: torch.device) -> BatchTreeWithPagedKVCacheWrapper:
     if device not in _tree_wrappers:
         _tree_wrappers[device] = BatchTreeWithPagedKVCacheWrapper(get_wrappers(device)[0]._workspace)
     return _tree_wrappers[device]
+
+
+_quantized_wrappers: Dict[torch.device, BatchQuantizedWithPagedKVCacheWrapper] = {}
+
+
+def get_quantized_wrapper(device: torch.device) -> BatchQuantizedWithPagedKVCacheWrapper:
+    """The wrapper for steps over 8-bit pages, over the workspace of get_wrappers."""
+    device = torch.device(device)
+    if device not in _quantized_wrappers:
+        _quantized_wrappers[device] = BatchQuantizedWithPagedKVCacheWrapper(get_wrappers(device)[0]._workspace)
+    return _quantized_wrappers[device]
 
 
 @dataclass

@@ -649,6 +649,58 @@ int dskv_move_rows(void *pages, int64_t layer_stride_bytes, int32_t n_layers, in
                    int64_t row_bytes, const int64_t *slots, const int32_t *qo_indptr, const int32_t *path,
                    const int32_t *counts, int32_t batch, int32_t nnz, void *stream);
 
+/*
+ * A K/V cache in 8 bits (no counterpart in the reference).  A page of a layer is a record of dskv_quant_page_bytes(..) bytes: the
+ * codes of K, then of V, (2, n_kv_heads, page_size, head_dim) in e4m3 (OCP), then one fp32 scale for each half and head, (2, n_kv_heads), and
+ * padding to a multiple of 128.  A value is code * scale of its block, the tokens of one page and head; scales are powers of two from 2^-126 on.
+ * Records are moved by the calls above as pages of so many bytes.  Lengths and tables are on the device and nothing is planned
+ * on the host, so the calls below can be captured into a graph and replayed with other lengths.
+ */
+int64_t dskv_quant_page_bytes(int32_t page_size, int32_t n_kv_heads, int32_t head_dim);
+typedef struct dskv_quant_rows {
+    const int32_t *qo_indptr, *kv_page_indices, *kv_page_indptr, *kv_last_page_lens;
+    int64_t n_page_indices;
+    int32_t batch, nnz, num_pages, page_size, n_kv_heads, head_dim;
+} dskv_quant_rows_t;
+
+/*
+ * New rows into such pages: row i of the n_b of request b becomes its token kv_len_b - n_b + i (kv_len_b counts the new rows).
+ * rope_table, q, k, v, their strides and q_out: as in dskv_rope_append_slots; k is rotated in 32 bits and rounded once, to its code.
+ * A block that gets rows: scale = the least power of two that the largest of their magnitudes takes to 448 or less, and
+ * no less than the block's scale where tokens in front of them stay; those are rounded anew where it is more.  Codes are rounded to nearest,
+ * ties to even.  A token of which a value of k (rotated) or v is no finite number counts in no scale, and its codes of that
+ * head are no number in K and 0 in V: rows that see it get no number, others nothing of it.  Values that code * scale could only take to an
+ * infinity of the type (over 61440 in f16, 240 * 2^120 else) are stored as that.
+ * A request whose arrays contradict themselves, a page id outside [0, num_pages) and a table entry past n_page_indices take
+ * no rows; q is rotated in every row.  No page takes rows of two requests.  head_dim: a multiple of 8 up to 256.
+ */
+int dskv_rope_append_quant(const dskv_quant_rows_t *rows, void *q_out, void *pages_layer, const void *q, const void *k,
+                           const void *v, int64_t q_stride, int64_t k_stride, int64_t v_stride, const float *rope_table,
+                           int32_t n_qo_heads, int32_t dtype, void *stream);
+
+/*
+ * dskv_tree_attn over such pages: same arguments and result, with sm_scale > 0 and dtype that of q and out.
+ * min_qo_len: no request has fewer rows (a hint: what does not hold costs time, not results; 0 is always right).
+ */
+typedef struct dskv_quant_step {
+    dskv_tree_step_t step;
+    int32_t min_qo_len;
+} dskv_quant_step_t;
+int64_t dskv_quant_attn_workspace(int32_t batch, int32_t nnz, int32_t max_qo_len, int32_t n_qo_heads, int32_t n_kv_heads,
+                                  int32_t head_dim, int32_t dtype);
+int dskv_quant_attn(const dskv_quant_step_t *step, void *out, const void *q, int64_t q_stride, const void *pages_layer,
+                    void *stream);
+
+/*
+ * dskv_move_rows for such pages: row j >= 1 of every request's walk from token prior_b + path[j] to token prior_b + j, with
+ * prior_b = kv_len_b - n_b, in all layers, from the values as they were before the call.  The scale of a block that rows move into is raised to
+ * the least power of two that takes their largest magnitude to 448 or less, if it is under that; what the block holds of the request's tokens is
+ * rounded anew then.  path rises, as dskv_verify_drafts writes it; entries that do not, or lie outside their request, move nothing, nor
+ * do walks of more than DSKV_MAX_TREE_ROWS rows.
+ */
+int dskv_move_quant_rows(const dskv_quant_rows_t *rows, void *pages, int64_t layer_stride_bytes, int32_t n_layers,
+                         const int32_t *path, const int32_t *counts, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
