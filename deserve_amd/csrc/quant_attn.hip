@@ -1,14 +1,9 @@
 // Attention of a step's rows over pages of 8-bit K/V: what tree_attn.hip computes, with k_j = code * scale of its block and v_j alike.
 // A token that an append took for no number has K codes that are none: its score is none either, which reaches the rows that see it and, chosen
 // away by the mask, no others.  V codes are numbers.
-#include "quant.h"
-#include "tree_kernel.h"
+#include "quant_kernel.h"
 
 namespace dskv {
-
-struct QuantArgs : TreeArgs {
-    long head_bytes, half_bytes, page_bytes;      // see quant.h
-};
 
 // Any type and head dim: one workgroup per (row, q head) whose waves take every kQuantWaves-th group of four keys.  Lane
 // (g, c) holds dims 8 c .. 8 c + 7 (and 128 more ..) of key g of the group.
@@ -111,12 +106,74 @@ __global__ __launch_bounds__(kQuantWaves * 64) void quant_generic_kernel(QuantAr
     }
 }
 
+// How a step is computed: tiles of `blocks` * 16 columns, few and each as narrow as it can be.
+struct QuantForm {
+    int blocks, cols, col_tiles, shares;
+};
+constexpr int kQuantUnits = 256;        // compute units
+static bool quant_matrix_form(int head_dim) { return head_dim == 64 || head_dim == 128; }
+static QuantForm quant_form(int max_rows, int n_qo_heads, int n_kv_heads, int dtype)
+{
+    QuantForm f;
+    const long cols = (long)max_rows * (n_qo_heads / n_kv_heads);
+    const int widest = quant_columns(dtype);
+    f.col_tiles = (int)((cols + widest - 1) / widest);
+    f.blocks = (int)((cols + 16L * f.col_tiles - 1) / (16L * f.col_tiles));
+    f.cols = f.blocks * 16;
+    const int resident = kQuantUnits * quant_workgroups(dtype, f.blocks);
+    f.shares = resident >= n_kv_heads ? resident / n_kv_heads : 1;
+    if (f.shares > 8) f.shares = f.shares / 8 * 8;         // (see share_and_head)
+    return f;
+}
+static int64_t units_bytes(int batch) { return ((int64_t)batch + 7) / 4 * 16; }
+static int64_t slots_of(const QuantForm &f, int n_kv_heads) { return 2LL * f.shares * n_kv_heads * f.cols; }
+static int64_t form_bytes(const QuantForm &f, int batch, int n_kv_heads, int head_dim)
+{
+    return units_bytes(batch) + slots_of(f, n_kv_heads) * (head_dim + 2) * (int64_t)sizeof(float);
+}
+
+template <int DT, int kD, int kCols, int kSub> static int launch_quant_merge(const QuantArgs &a, const QuantForm &f, hipStream_t stream)
+{
+    const bool many_parts = (long)a.batch * f.col_tiles * 4 < f.shares;
+    constexpr int kEach = kCols >= 128 ? 4 : 1;
+    const int columns = 256 / (kD / 4) * (many_parts ? 1 : kEach) / (many_parts ? 4 : 1);
+    const dim3 grid((unsigned)(a.batch * f.col_tiles), (unsigned)a.n_kv_heads, (unsigned)((kCols + columns - 1) / columns));
+    if (many_parts) hipLaunchKernelGGL((tree_merge_kernel<DT, kD, kCols, kSub, 4, 1, QuantArgs>), grid, dim3(256), 0, stream, a, f.col_tiles);
+    else hipLaunchKernelGGL((tree_merge_kernel<DT, kD, kCols, kSub, 1, kEach, QuantArgs>), grid, dim3(256), 0, stream, a, f.col_tiles);
+    DSKV_LAUNCH_CHECK("tree_merge_kernel");
+    return 0;
+}
+template <int DT, int kD, int kBlocks> static int launch_quant(const QuantArgs &a, const QuantForm &f, hipStream_t stream)
+{
+    typedef QuantTile<DT, kD, kBlocks> S;
+    hipLaunchKernelGGL((quant_matrix_kernel<DT, kD, kBlocks>), dim3((unsigned)(f.shares * a.n_kv_heads)), dim3(kTreeThreads), 0, stream, a);
+    DSKV_LAUNCH_CHECK("quant_matrix_kernel");
+    return launch_quant_merge<DT, kD, S::kCols, S::kSub>(a, f, stream);
+}
+template <int DT, int kD> static int launch_quant_blocks(const QuantArgs &a, const QuantForm &f, hipStream_t stream)
+{
+    switch (f.blocks) {
+    case 1: return launch_quant<DT, kD, 1>(a, f, stream);
+    case 2: return launch_quant<DT, kD, 2>(a, f, stream);
+    default:
+        if constexpr (quant_columns(DT) >= 48) return launch_quant<DT, kD, 3>(a, f, stream);
+        set_error("quant_attn: no form for %d columns", f.cols);
+        return DSKV_E_INVAL;
+    }
+}
+template <int DT> static int launch_quant_dim(const QuantArgs &a, const QuantForm &f, hipStream_t stream)
+{
+    return a.head_dim == 64 ? launch_quant_blocks<DT, 64>(a, f, stream) : launch_quant_blocks<DT, 128>(a, f, stream);
+}
+
 }  // namespace dskv
 
 extern "C" int64_t dskv_quant_attn_workspace(int32_t batch, int32_t nnz, int32_t max_qo_len, int32_t n_qo_heads,
                                              int32_t n_kv_heads, int32_t head_dim, int32_t dtype)
 {
-    return 0;
+    using namespace dskv;
+    if (batch <= 0 || nnz <= 0 || max_qo_len <= 0 || n_kv_heads <= 0 || n_qo_heads < n_kv_heads || !quant_matrix_form(head_dim)) return 0;
+    return form_bytes(quant_form(max_qo_len, n_qo_heads, n_kv_heads, dtype), batch, n_kv_heads, head_dim);
 }
 
 extern "C" int dskv_quant_attn(const dskv_quant_step_t *step, void *out, const void *q, int64_t q_stride,
@@ -152,6 +209,34 @@ extern "C" int dskv_quant_attn(const dskv_quant_step_t *step, void *out, const v
     a.half_bytes = shape.half_bytes;
     a.page_bytes = shape.page_bytes;
     hipStream_t st = (hipStream_t)stream;
+    const QuantForm f = quant_form(s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->dtype);
+    // (places in the pool, tokens of a request and units are numbered in 32 bits there)
+    if (quant_matrix_form(s->head_dim) && s->num_pages * (shape.page_bytes / 16) < UINT32_MAX &&
+        s->n_page_indices < kMostTokens / s->page_size &&
+        (s->n_page_indices * s->page_size / 16 + 2LL * s->batch) * f.col_tiles < INT32_MAX) {
+        const int64_t need = dskv_quant_attn_workspace(s->batch, s->nnz, s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->head_dim, s->dtype);
+        if (!s->workspace || s->workspace_bytes < need) {
+            set_error("quant_attn: workspace of %lld bytes, %lld are needed", (long long)s->workspace_bytes, (long long)need);
+            return DSKV_E_NOMEM;
+        }
+        DSKV_REQUIRE((uintptr_t)s->workspace % 16 == 0, "quant_attn: the workspace must be 16-byte aligned");
+        DSKV_REQUIRE((int64_t)s->batch * f.col_tiles < INT32_MAX && s->n_kv_heads <= 65535, "quant_attn: too large a batch");
+        a.units_before = (int32_t *)s->workspace;
+        a.part_o = (float *)((char *)s->workspace + units_bytes(s->batch));
+        a.part_ml = a.part_o + slots_of(f, s->n_kv_heads) * s->head_dim;
+        a.n_shares = f.shares;
+        a.sides = 1;
+        a.group = s->n_qo_heads / s->n_kv_heads;
+        a.page_shift = 31 + ilog2(s->page_size);
+        a.page_magic = (uint32_t)(((1ull << a.page_shift) + s->page_size - 1) / s->page_size);
+        a.page16 = (uint32_t)(shape.page_bytes / 16);
+        a.row16 = (uint32_t)(s->head_dim / 16);
+        a.rows_from = 0;
+        a.rows_to = INT32_MAX;
+        if (s->dtype == DSKV_F32) return launch_quant_dim<DSKV_F32>(a, f, st);
+        if (s->dtype == DSKV_F16) return launch_quant_dim<DSKV_F16>(a, f, st);
+        return launch_quant_dim<DSKV_BF16>(a, f, st);
+    }
     DSKV_REQUIRE(s->n_qo_heads <= 65535, "quant_attn: at most 65535 heads");
     const dim3 grid((unsigned)s->nnz, (unsigned)s->n_qo_heads), block(kQuantWaves * 64);
 #define DSKV_QUANT_GENERIC(DT)                                                                                 \

@@ -1,0 +1,422 @@
+// The attention over 8-bit pages for few columns (head_dim 64 and 128, all three types): one row per request, drafted tokens, short
+// chunks.  Work is cut as in tree_kernel.h - columns of a kv head, subtiles of 32 tokens, equal shares, one workgroup per (share, kv head), a wave
+// per subtile -, and what differs is what a wave does with a subtile:
+// codes go by whole rows through registers and the wave's LDS as they are; the matrix instructions' operands are made of them behind LDS,
+// two codes an instruction, exactly: every code is a number of bf16 and of f16.  K's scales multiply the scores and V's the weights, in 32 bits,
+// token by token, so that pages may end anywhere in a subtile.
+// Weights times V's scale span more than f16 holds: the second product is in bf16 for all types.  A weight is rounded to bf16 for bf16
+// results (2^-9 of it, half of what the result's own rounding is), to two bf16 terms for f16 (2^-17) and to three, that is to 32
+// bits, for fp32, whose q is three terms as well.
+#pragma once
+
+#include "quant.h"
+#include "tree_kernel.h"
+
+namespace dskv {
+
+struct QuantArgs : TreeArgs {
+    long head_bytes, half_bytes, page_bytes;      // see quant.h
+    uint32_t page16, row16;                       // bytes of a page and of a token's row, in sixteens
+    int rows_from, rows_to;                       // rows of a request that this launch computes, 0 of any other's
+};
+__device__ __forceinline__ int rows_taken(const QuantArgs &a, int n) { return n >= a.rows_from && n <= a.rows_to ? n : 0; }
+
+constexpr uint32_t kNoQuantRow = 0xFFFFFFFFu;
+// Where token t's K lies in the head's part of the pool, in sixteens of bytes.
+__device__ __forceinline__ uint32_t quant_row(const QuantArgs &a, int t, int page)
+{
+    return page >= 0 && page < a.num_pages ? (uint32_t)page * a.page16 + (uint32_t)(t - page_number(a, t) * a.page_size) * a.row16
+                                           : kNoQuantRow;
+}
+
+// 8 codes as a matrix operand of type T
+template <int T> __device__ __forceinline__ u32x4 operand_of(u32x2 codes)
+{
+    u32x4 x;
+#pragma unroll
+    for (int w = 0; w < 2; w++) {
+        if constexpr (T == DSKV_F16) {
+            x[2 * w] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[w], 1.0f, false));
+            x[2 * w + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[w], 1.0f, true));
+        } else {
+            x[2 * w] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[w], 1.0f, false));
+            x[2 * w + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[w], 1.0f, true));
+        }
+    }
+    return x;
+}
+// Eight floats as kTerms operands of bf16 that add up to them; what is left is rounded away.
+template <int kTerms> __device__ __forceinline__ void split8(const float *f, u32x4 *terms)
+{
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        float a = f[2 * w], b = f[2 * w + 1];
+#pragma unroll
+        for (int i = 0; i < kTerms; i++) {
+            const uint32_t pair = Elt<DSKV_BF16>::pack2(a, b);
+            terms[i][w] = pair;
+            if (i + 1 < kTerms) {
+                float x, y;
+                Elt<DSKV_BF16>::unpack2(pair, x, y);
+                a -= x;
+                b -= y;
+            }
+        }
+    }
+}
+
+template <int DT, int kD, int kBlocks> struct QuantTile {
+    static constexpr int kElt = DT == DSKV_F32 ? 4 : 2;
+    static constexpr int kSub = 32;                                  // tokens of a subtile
+    static constexpr int kTiles = 2;
+    static constexpr int kChunks = kD / 16;                          // 16-byte chunks of a row
+    static constexpr int kRowsPerLoad = 64 / kChunks;
+    static constexpr int kLoads = kSub / kRowsPerLoad;
+    static constexpr int kSteps = kD / 32;                           // matrix instructions of a tile's scores
+    static constexpr int kDimTiles = kD / 16;
+    static constexpr int kCols = kBlocks * 16;
+    static constexpr int kQTerms = DT == DSKV_F32 ? 3 : 1, kPTerms = DT == DSKV_BF16 ? 1 : DT == DSKV_F16 ? 2 : 3;
+    static constexpr int kKeyType = DT == DSKV_F16 ? DSKV_F16 : DSKV_BF16;
+    static constexpr int kPitch = kD + 16;                           // bytes; 16 rows' chunks at one offset meet no bank twice
+    static constexpr int kWaveLds = 2 * kSub * kPitch + 2 * kSub * 4;      // K, V, their scales
+    static constexpr int kOPitch = kD + 4;                           // floats
+    static constexpr int kMergeLds = kTreeWaves * kCols * (kOPitch + 2) * 4;
+    static constexpr int kLds = kTreeWaves * kWaveLds > kMergeLds ? kTreeWaves * kWaveLds : kMergeLds;
+    static constexpr int kWorkgroups = DT != DSKV_F32 && kBlocks <= 2 ? 2 : 1;      // of a compute unit
+    static constexpr int kDepth = 2;                                 // subtiles a wave has in flight
+};
+constexpr int quant_workgroups(int dtype, int blocks) { return dtype != DSKV_F32 && blocks <= 2 ? 2 : 1; }
+constexpr int quant_columns(int dtype) { return dtype == DSKV_F32 ? 32 : 48; }
+
+template <int DT, int kD, int kBlocks>
+__global__ __launch_bounds__(kTreeThreads, (QuantTile<DT, kD, kBlocks>::kWorkgroups)) void quant_matrix_kernel(QuantArgs a)
+{
+    typedef QuantTile<DT, kD, kBlocks> S;
+    __shared__ __align__(16) char lds[S::kLds];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, c = lane & 15;
+    int share, head;
+    share_and_head(a, share, head);
+    TreePlace place;
+    tree_place<S::kCols, S::kSub, kTreeThreads, false, kTreeWaves, kTreeWaves * S::kDepth>(a, share, place);
+    make_uniform(place);
+    const int begin = place.begin, end = place.end;
+    if (begin >= end) return;
+
+    char *const k_lds = lds + wave * S::kWaveLds, *const v_lds = k_lds + S::kSub * S::kPitch;
+    float *const scale_lds = reinterpret_cast<float *>(v_lds + S::kSub * S::kPitch);
+    const int load_row = lane / S::kChunks, load_chunk = lane % S::kChunks;
+    const char *const pool = a.pages + head * a.head_bytes + load_chunk * 16;
+    // lanes 0 .. 31 fetch the scales of K, the others those of V
+    const char *const scales = a.pages + 2 * a.half_bytes + ((lane >> 5) * a.n_kv_heads + head) * 4;
+    const char *const none = reinterpret_cast<const char *>(kNoRow) + load_chunk * 16;
+
+    // ---- what is requested: the wave's subtiles through all items of the share, kDepth in flight, their page ids one step
+    // further ahead (see tree_kernel.h)
+    TreeItem ahead;
+    ahead.b = place.b;
+    ahead.base = place.base;
+    ahead.r = place.r;
+    open_item<S::kCols, S::kSub>(a, begin, begin, end, ahead);
+    auto walk_end = [&](const TreeItem &x) {                    // of the wave's subtiles st0 + wave, + kTreeWaves ..; whole turns of kDepth
+        constexpr int kTurn = S::kDepth * kTreeWaves;
+        return x.st0 + wave + max((x.st1 - x.st0 - wave + kTurn - 1) / kTurn, 0) * kTurn;
+    };
+    int ahead_st = ahead.st0 + wave, ahead_end = walk_end(ahead);
+    bool more = true;
+    auto settle = [&]() {                                       // on to a subtile that there is
+        if (__builtin_expect(ahead_st < ahead_end, 1)) return;
+        while (more && ahead_st >= ahead_end) {
+            more = ahead.next < end;
+            if (more) {
+                open_item<S::kCols, S::kSub>(a, ahead.next, begin, end, ahead);
+                ahead_st = ahead.st0 + wave;
+                ahead_end = walk_end(ahead);
+            }
+        }
+    };
+    struct Ids {
+        int page, t;
+    };
+    auto next_ids = [&]() {                                     // of the lane's token of the next subtile; moves on
+        settle();
+        Ids x;
+        x.t = ahead_st * S::kSub + (lane & (S::kSub - 1));
+        x.page = more && ahead_st < ahead.st1 ? page_of(a, ahead.r, x.t) : -1;
+        ahead_st += kTreeWaves;
+        return x;
+    };
+    struct Held {
+        u32x4 k[S::kLoads], v[S::kLoads];
+        float scale;
+        uint32_t there;                                         // bit per token: there is one
+    };
+    Held held[S::kDepth];
+    auto request = [&](const Ids &x, Held &to) {
+        const uint32_t mine = quant_row(a, x.t, x.page);
+        to.there = (uint32_t)__ballot(mine != kNoQuantRow);     // (lanes repeat)
+        uint32_t row[S::kLoads];
+#pragma unroll
+        for (int i = 0; i < S::kLoads; i++) row[i] = (uint32_t)__shfl((int)mine, load_row + S::kRowsPerLoad * i);
+        const char *s = mine != kNoQuantRow ? scales + x.page * a.page_bytes : reinterpret_cast<const char *>(kNoRow);
+        to.scale = *(const __attribute__((address_space(1))) float *)s;
+#pragma unroll
+        for (int i = 0; i < S::kLoads; i++) {
+            const char *k = pool + (uint64_t)row[i] * 16, *v = k + a.half_bytes;
+            k = row[i] != kNoQuantRow ? k : none;
+            v = row[i] != kNoQuantRow ? v : none;
+            to.k[i] = __builtin_nontemporal_load((global_chunk_ptr)k);
+            to.v[i] = __builtin_nontemporal_load((global_chunk_ptr)v);
+        }
+    };
+    Ids ids = next_ids();
+
+    // ---- what is computed: one item after the other
+    TreeItem it;
+    it.b = place.b;
+    it.base = place.base;
+    it.r = place.r;
+    int cols, prior, st;
+    u32x4 q[kBlocks][S::kSteps][S::kQTerms];                    // step 2 h + s: dims 64 h + 16 g + 8 s .. of the column
+    unsigned long long mask[kBlocks];
+    int limit[kBlocks];
+    f32x4 o[kBlocks][S::kDimTiles];
+    float m[kBlocks], l[kBlocks];
+    auto start_item = [&](int unit) {
+        open_item<S::kCols, S::kSub>(a, unit, begin, end, it);
+        cols = min(it.r.n * a.group - it.ct * S::kCols, S::kCols);
+        prior = it.r.prior;
+        st = it.st0 + wave;
+#pragma unroll
+        for (int k = 0; k < kBlocks; k++) {
+            const int col = it.ct * S::kCols + k * 16 + c;
+            const int i = (int)((unsigned)col / (unsigned)a.group), hq = head * a.group + col - i * a.group;
+            const bool there = k * 16 + c < cols;
+            const char *row = there ? a.q + (it.r.first + i) * a.q_stride + hq * kD * S::kElt + g * 16 * S::kElt
+                                    : reinterpret_cast<const char *>(kNoRow);
+            const int apart = there ? 1 : 0;
+#pragma unroll
+            for (int e = 0; e < S::kSteps; e++) {
+                const char *at = row + apart * ((e >> 1) * 64 + (e & 1) * 8) * S::kElt;
+                q[k][e][0] = *(global_chunk_ptr)at;
+                if constexpr (DT == DSKV_F32) q[k][e][1] = *(global_chunk_ptr)(at + 16);
+            }
+            mask[k] = !a.masks ? ~0ull : there ? (unsigned long long)a.masks[it.r.first + i] : 0;
+            // tokens from `limit` on are not seen whatever the mask says
+            const long lim = min(it.r.kv_len, (long)prior + (a.masks ? DSKV_MAX_TREE_ROWS : i + 1));
+            limit[k] = there ? (int)max(lim, 0L) : 0;
+            m[k] = -__FLT_MAX__;
+            l[k] = 0;
+#pragma unroll
+            for (int d = 0; d < S::kDimTiles; d++) o[k][d] = f32x4{0, 0, 0, 0};
+        }
+    };
+    // q and the masks are waited for in front of the loop
+    auto settle_item = [&]() {
+#pragma unroll
+        for (int k = 0; k < kBlocks; k++) {
+#pragma unroll
+            for (int e = 0; e < S::kSteps; e++) {
+                if constexpr (DT == DSKV_F32) {
+                    float f[8];
+                    Chunk<DSKV_F32>::unpack(q[k][e][0], f);
+                    Chunk<DSKV_F32>::unpack(q[k][e][1], f + 4);
+                    split8<3>(f, q[k][e]);
+                }
+                asm volatile("" : "+v"(q[k][e][0]));
+            }
+            asm volatile("" : "+v"(mask[k]));
+        }
+    };
+    auto subtile = [&](Held &mine) {
+        const bool there = st < it.st1;                         // (else a turn without a subtile)
+        const uint32_t there_bits = mine.there;
+        const bool whole = there_bits == ~0u && (st + 1) * S::kSub <= prior + (a.masks ? 0 : 1);
+        u32x4 key[S::kTiles][kD / 64];
+        f32x4 k_scale[S::kTiles], v_scale[S::kTiles];
+        if (there) {
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int i = 0; i < S::kLoads; i++) {
+                const int row = load_row + S::kRowsPerLoad * i;
+                *reinterpret_cast<u32x4 *>(k_lds + row * S::kPitch + load_chunk * 16) = mine.k[i];
+                *reinterpret_cast<u32x4 *>(v_lds + row * S::kPitch + load_chunk * 16) = mine.v[i];
+            }
+            scale_lds[lane] = lane < 32 ? mine.scale * a.scale : mine.scale;
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            // LDS operands are read together and ahead
+#pragma unroll
+            for (int t = 0; t < S::kTiles; t++) {
+#pragma unroll
+                for (int h = 0; h < kD / 64; h++)
+                    key[t][h] = *reinterpret_cast<const u32x4 *>(k_lds + (t * 16 + c) * S::kPitch + h * 64 + g * 16);
+                k_scale[t] = *reinterpret_cast<const f32x4 *>(scale_lds + t * 16 + 4 * g);
+                v_scale[t] = *reinterpret_cast<const f32x4 *>(scale_lds + 32 + t * 16 + 4 * g);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        const Ids ids_next = next_ids();
+        request(ids, mine);
+        ids = ids_next;
+        if (!there) {
+            st += kTreeWaves;
+            return;
+        }
+
+        // ---- scores
+        f32x4 s[kBlocks][S::kTiles];
+#pragma unroll
+        for (int t = 0; t < S::kTiles; t++) {
+#pragma unroll
+            for (int k = 0; k < kBlocks; k++) s[k][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int e = 0; e < S::kSteps; e++) {
+                const u32x4 chunk = key[t][e >> 1];
+                const u32x4 x = operand_of<S::kKeyType>((e & 1) ? u32x2{chunk.z, chunk.w} : u32x2{chunk.x, chunk.y});
+#pragma unroll
+                for (int k = 0; k < kBlocks; k++)
+#pragma unroll
+                    for (int i = 0; i < S::kQTerms; i++) s[k][t] = Elt<S::kKeyType>::mfma_k32(x, q[k][e][i], s[k][t]);
+            }
+        }
+        // V's codes: eight of a lane along the tokens for every 16 dims, in the order that the scores have them: 4 g .. 4 g + 3 and
+        // 16 more.  Lane (g, x) supplies dims 8 (x % 2) .. of the x / 2-th of these.
+        u32x2 value[S::kDimTiles];
+        {
+            typedef int lds_i32x2 __attribute__((ext_vector_type(2)));
+            const int j = c >> 1, token = 4 * g + (j & 3) + (j >> 2) * 16;
+            const char *at = v_lds + token * S::kPitch + (c & 1) * 8;
+#pragma unroll
+            for (int d = 0; d < S::kDimTiles; d++)
+                value[d] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                                                         (__attribute__((address_space(3))) lds_i32x2 *)(at + d * 16)));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        // ---- weights, under a maximum that is raised only where they ask for it
+        u32x4 p[kBlocks][S::kPTerms];
+#pragma unroll
+        for (int k = 0; k < kBlocks; k++) {
+            float x[8], w[8];
+#pragma unroll
+            for (int t = 0; t < S::kTiles; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[t * 4 + e] = s[k][t][e] * k_scale[t][e];
+            if (!whole) {
+                const uint32_t bits = (there_bits & seen_bits(st * S::kSub, prior, limit[k], mask[k], !a.masks)) >> (4 * g);
+#pragma unroll
+                for (int t = 0; t < S::kTiles; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (!((bits >> (t * 16 + e)) & 1)) x[t * 4 + e] = -INFINITY;
+            }
+            float sum = 0;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                w[e] = __builtin_amdgcn_exp2f(x[e] - m[k]);
+                sum += w[e];
+            }
+            if (__builtin_expect(__ballot(sum > most_weight(DSKV_BF16)) != 0, 0)) {
+                float top = x[0];
+#pragma unroll
+                for (int e = 1; e < 8; e++) top = fmaxf(top, x[e]);
+                top = fmaxf(m[k], quad_rows_max(top));
+                const float keep = __builtin_amdgcn_exp2f(m[k] - top);
+                m[k] = top;
+                l[k] *= keep;
+#pragma unroll
+                for (int d = 0; d < S::kDimTiles; d++) o[k][d] *= keep;
+                sum = 0;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    w[e] = __builtin_amdgcn_exp2f(x[e] - top);
+                    sum += w[e];
+                }
+            }
+            l[k] += sum;
+#pragma unroll
+            for (int e = 0; e < 8; e++) w[e] *= v_scale[e >> 2][e & 3];
+            split8<S::kPTerms>(w, p[k]);
+        }
+        // ---- output
+#pragma unroll
+        for (int d = 0; d < S::kDimTiles; d++) {
+            const u32x4 x = operand_of<DSKV_BF16>(value[d]);
+#pragma unroll
+            for (int k = 0; k < kBlocks; k++)
+#pragma unroll
+                for (int i = 0; i < S::kPTerms; i++) o[k][d] = Elt<DSKV_BF16>::mfma_k32(x, p[k][i], o[k][d]);
+        }
+        st += kTreeWaves;
+    };
+    auto finish_item = [&]() {
+        // the waves' results meet
+        float *const o_lds = reinterpret_cast<float *>(lds);
+        float *const ml_lds = o_lds + kTreeWaves * S::kCols * S::kOPitch;
+        __syncthreads();                                       // all waves are through with their K and V
+#pragma unroll
+        for (int k = 0; k < kBlocks; k++) {
+            l[k] = quad_rows_sum(l[k]);
+            const int col = wave * S::kCols + k * 16 + c;
+            if (g == 0) {
+                ml_lds[col * 2] = m[k];
+                ml_lds[col * 2 + 1] = l[k];
+            }
+#pragma unroll
+            for (int d = 0; d < S::kDimTiles; d++)
+                *reinterpret_cast<f32x4 *>(o_lds + col * S::kOPitch + d * 16 + 4 * g) = o[k][d];
+        }
+        __syncthreads();
+        const bool cut = it.st0 > 0 || it.st1 < it.r.subtiles;
+        const long slot = 2L * share + (it.first ? 0 : 1);
+        const long part = (slot * a.n_kv_heads + head) * S::kCols;
+        constexpr int kQuads = kD / 4;
+        for (int x = threadIdx.x; x < cols * kQuads; x += kTreeThreads) {
+            const int col = x / kQuads, quad = x % kQuads;
+            float top = ml_lds[col * 2];
+#pragma unroll
+            for (int w = 1; w < kTreeWaves; w++) top = fmaxf(top, ml_lds[(w * S::kCols + col) * 2]);
+            float sum = 0;
+            f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+            for (int w = 0; w < kTreeWaves; w++) {
+                const float weight = __builtin_amdgcn_exp2f(ml_lds[(w * S::kCols + col) * 2] - top);
+                sum += ml_lds[(w * S::kCols + col) * 2 + 1] * weight;
+                acc += *reinterpret_cast<const f32x4 *>(o_lds + (w * S::kCols + col) * S::kOPitch + quad * 4) * weight;
+            }
+            if (cut) {
+                *reinterpret_cast<f32x4 *>(a.part_o + (part + col) * kD + quad * 4) = acc;
+                if (quad == 0) {
+                    a.part_ml[(part + col) * 2] = top;
+                    a.part_ml[(part + col) * 2 + 1] = sum;
+                }
+            } else {
+                const int at = it.ct * S::kCols + col, i = (int)((unsigned)at / (unsigned)a.group), hq = head * a.group + at - i * a.group;
+                const float inv = sum == 0 ? 0.f : 1.f / sum;
+                char *dst = a.out + (((it.r.first + i) * a.n_qo_heads + hq) * kD + quad * 4) * S::kElt;
+                if constexpr (DT == DSKV_F32) *reinterpret_cast<f32x4 *>(dst) = acc * inv;
+                else *reinterpret_cast<u32x2 *>(dst) = u32x2{Elt<DT>::pack2(acc.x * inv, acc.y * inv), Elt<DT>::pack2(acc.z * inv, acc.w * inv)};
+            }
+        }
+        __syncthreads();
+    };
+    start_item(begin);                                          // (its loads in front of those that wait for page ids)
+#pragma unroll
+    for (int i = 0; i < S::kDepth; i++) {
+        const Ids ids_next = next_ids();
+        request(ids, held[i]);
+        ids = ids_next;
+    }
+    for (;;) {
+        settle_item();
+        while (st < it.st1) {
+#pragma unroll
+            for (int i = 0; i < S::kDepth; i++) subtile(held[i]);
+        }
+        finish_item();
+        if (it.next >= end) return;
+        start_item(it.next);
+    }
+}
+
+}  // namespace dskv

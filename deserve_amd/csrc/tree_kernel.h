@@ -107,8 +107,11 @@ struct TreeRequest {
     int tile;            // columns of a tile: its tiles are as even as 32 columns a wave allow
 };
 
+// Of a request's n rows those that a launch computes: here all of them.
+__device__ __forceinline__ int rows_taken(const TreeArgs &, int n) { return n; }
+
 // What the arrays say about request b, within the bounds of the tensors.
-template <int kCols, int kSub> __device__ __forceinline__ TreeRequest tree_request(const TreeArgs &a, int b)
+template <int kCols, int kSub, typename A> __device__ __forceinline__ TreeRequest tree_request(const A &a, int b)
 {
     // (through the constant address space: scalar loads where b is uniform, also after the kernel has stored)
     const const_i32_ptr qo = as_const(a.qo_indptr) + b, kv = as_const(a.kv_page_indptr) + b;
@@ -117,7 +120,7 @@ template <int kCols, int kSub> __device__ __forceinline__ TreeRequest tree_reque
     const long rows = (long)qo[1] - r.first;
     r.page0 = kv[0];
     const TreeTokens tokens = tree_tokens(kv[0], kv[1], as_const(a.kv_last_page_lens)[b], a.page_size, a.n_page_indices);
-    r.n = r.first < 0 ? 0 : (int)max(min(min(rows, (long)a.max_rows), (long)a.nnz - r.first), 0L);
+    r.n = rows_taken(a, r.first < 0 ? 0 : (int)max(min(min(rows, (long)a.max_rows), (long)a.nnz - r.first), 0L));
     const long prior = tokens.len - rows;
     r.kv_len = max(min(tokens.walk, prior + (a.masks ? DSKV_MAX_TREE_ROWS : r.n)), 0L);
     r.prior = (int)max(min(prior, (long)kMostTokens), -(long)kMostTokens);       // (further off than any token that is walked)
@@ -213,8 +216,8 @@ struct TreePlace {
 // shares than there are, no part crosses an item's end.  Measured against equal shares (32 heads over 8, bf16): 3 requests of 5 rows over
 // 50 - 500 tokens 14.5 for 18.4 us, 8 over 1 - 4 K 26.6 for 29.5, 8 over 4 - 16 K 65.0 for 67.1, 8 trees of 64 rows over 1 - 4 K
 // 54 for 64.5; at 16 over 2 - 8 K they take too many shares.
-template <int kCols, int kSub, int kThreads, bool kSides, int kLeast, int kTurn>
-__device__ __forceinline__ void tree_place(const TreeArgs &a, int share, TreePlace &at)
+template <int kCols, int kSub, int kThreads, bool kSides, int kLeast, int kTurn, typename A>
+__device__ __forceinline__ void tree_place(const A &a, int share, TreePlace &at)
 {
     __shared__ long scan[2][kThreads / 64], scan_parts[kThreads / 64];
     __shared__ int busy_of[kThreads / 64];
@@ -422,8 +425,8 @@ struct TreeItem {
     int b, ct, st0, st1; // column tile; subtiles of the part
     bool first;          // of the share
 };
-template <int kCols, int kSub>
-__device__ __forceinline__ void open_item(const TreeArgs &a, int unit, int begin, int end, TreeItem &it)
+template <int kCols, int kSub, typename A>
+__device__ __forceinline__ void open_item(const A &a, int unit, int begin, int end, TreeItem &it)
 {
     while (unit >= it.base + (int)units_of(it.r, false)) {         // on to the next request that has rows
         it.base += (int)units_of(it.r, false);
@@ -827,8 +830,8 @@ __global__ __launch_bounds__(kTreeThreads, tree_workgroups(kD, kBlocks)) void tr
 // Items that were cut: a thread per (column, four dims) and group of parts.  kGroups > 1, for items in many parts: each takes
 // every kGroups-th part, and they meet in LDS.  kEach > 1, for many columns: columns that a thread takes at once (66
 // MB of partials, 16 trees of 33 - 64 rows: 16 us with four, 24 with one).
-template <int DT, int kD, int kCols, int kSub, int kGroups, int kEach>
-__global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int max_col_tiles)
+template <int DT, int kD, int kCols, int kSub, int kGroups, int kEach, typename A>
+__global__ __launch_bounds__(256) void tree_merge_kernel(A a, int max_col_tiles)
 {
     constexpr int kElt = DT == DSKV_F32 ? 4 : 2;
     constexpr int kQuads = kD / 4, kColumns = 256 / (kQuads * kGroups);
