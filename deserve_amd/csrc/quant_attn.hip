@@ -1,7 +1,7 @@
 // Attention of a step's rows over pages of 8-bit K/V: what tree_attn.hip computes, with k_j = code * scale of its block and v_j alike.
 // A token that an append took for no number has K codes that are none: its score is none either, which reaches the rows that see it and, chosen
 // away by the mask, no others.  V codes are numbers.
-#include "quant_kernel.h"
+#include "quant_wide_kernel.h"
 
 namespace dskv {
 
@@ -106,24 +106,35 @@ __global__ __launch_bounds__(kQuantWaves * 64) void quant_generic_kernel(QuantAr
     }
 }
 
-// How a step is computed: tiles of `blocks` * 16 columns, few and each as narrow as it can be.
+// How rows of a step are computed.  wide_waves > 0: quant_wide_kernel.h with so many waves; else quant_kernel.h with tiles of
+// `blocks` * 16 columns, few and each as narrow as it can be.
 struct QuantForm {
-    int blocks, cols, col_tiles, shares;
+    int wide_waves, blocks, cols, col_tiles, shares, sides;
 };
 constexpr int kQuantUnits = 256;        // compute units
 static bool quant_matrix_form(int head_dim) { return head_dim == 64 || head_dim == 128; }
-static QuantForm quant_form(int max_rows, int n_qo_heads, int n_kv_heads, int dtype)
+static QuantForm quant_form(bool wide, int max_rows, int n_qo_heads, int n_kv_heads, int dtype)
 {
     QuantForm f;
     const long cols = (long)max_rows * (n_qo_heads / n_kv_heads);
-    const int widest = quant_columns(dtype);
+    f.wide_waves = !wide ? 0 : cols <= 128 ? 4 : 8;
+    const int widest = wide ? f.wide_waves * 32 : quant_columns(dtype);
     f.col_tiles = (int)((cols + widest - 1) / widest);
-    f.blocks = (int)((cols + 16L * f.col_tiles - 1) / (16L * f.col_tiles));
-    f.cols = f.blocks * 16;
-    const int resident = kQuantUnits * quant_workgroups(dtype, f.blocks);
+    f.blocks = wide ? 0 : (int)((cols + 16L * f.col_tiles - 1) / (16L * f.col_tiles));
+    f.cols = wide ? widest : f.blocks * 16;
+    const int resident = kQuantUnits * (wide ? (f.wide_waves == 4 ? 2 : 1) : quant_workgroups(dtype, f.blocks));
     f.shares = resident >= n_kv_heads ? resident / n_kv_heads : 1;
     if (f.shares > 8) f.shares = f.shares / 8 * 8;         // (see share_and_head)
+    f.sides = wide && f.col_tiles > 1 && f.shares % (8 * f.col_tiles) == 0 ? f.col_tiles : 1;
     return f;
+}
+// Requests of so many rows and fewer are the narrow form's, the others the wide one's, which reads K and V once for all columns
+// (never fewer than one: a request of more columns a row than the narrow form's tiles hold is in several of these).
+static int narrow_rows(int n_qo_heads, int n_kv_heads, int dtype)
+{
+    if (dtype == DSKV_F32) return INT32_MAX;
+    const int rows = quant_columns(dtype) / (n_qo_heads / n_kv_heads);
+    return rows > 1 ? rows : 1;
 }
 static int64_t units_bytes(int batch) { return ((int64_t)batch + 7) / 4 * 16; }
 static int64_t slots_of(const QuantForm &f, int n_kv_heads) { return 2LL * f.shares * n_kv_heads * f.cols; }
@@ -150,8 +161,18 @@ template <int DT, int kD, int kBlocks> static int launch_quant(const QuantArgs &
     DSKV_LAUNCH_CHECK("quant_matrix_kernel");
     return launch_quant_merge<DT, kD, S::kCols, S::kSub>(a, f, stream);
 }
+template <int DT, int kD, int kWaves> static int launch_quant_wide(const QuantArgs &a, const QuantForm &f, hipStream_t stream)
+{
+    hipLaunchKernelGGL((quant_wide_kernel<DT, kD, kWaves>), dim3((unsigned)(f.shares * a.n_kv_heads)), dim3(kWaves * 64), 0, stream, a);
+    DSKV_LAUNCH_CHECK("quant_wide_kernel");
+    return launch_quant_merge<DT, kD, kWaves * 32, kWideBlock>(a, f, stream);
+}
 template <int DT, int kD> static int launch_quant_blocks(const QuantArgs &a, const QuantForm &f, hipStream_t stream)
 {
+    if constexpr (DT != DSKV_F32) {
+        if (f.wide_waves == 4) return launch_quant_wide<DT, kD, 4>(a, f, stream);
+        if (f.wide_waves == 8) return launch_quant_wide<DT, kD, 8>(a, f, stream);
+    }
     switch (f.blocks) {
     case 1: return launch_quant<DT, kD, 1>(a, f, stream);
     case 2: return launch_quant<DT, kD, 2>(a, f, stream);
@@ -165,6 +186,20 @@ template <int DT> static int launch_quant_dim(const QuantArgs &a, const QuantFor
 {
     return a.head_dim == 64 ? launch_quant_blocks<DT, 64>(a, f, stream) : launch_quant_blocks<DT, 128>(a, f, stream);
 }
+// The requests of rows_from .. rows_to rows, in form f.
+static int launch_quant_form(QuantArgs a, const QuantForm &f, int dtype, int rows_from, int rows_to, void *workspace, hipStream_t stream)
+{
+    a.units_before = (int32_t *)workspace;
+    a.part_o = (float *)((char *)workspace + units_bytes(a.batch));
+    a.part_ml = a.part_o + slots_of(f, a.n_kv_heads) * a.head_dim;
+    a.n_shares = f.shares;
+    a.sides = f.sides;
+    a.rows_from = rows_from;
+    a.rows_to = rows_to;
+    if (dtype == DSKV_F32) return launch_quant_dim<DSKV_F32>(a, f, stream);
+    if (dtype == DSKV_F16) return launch_quant_dim<DSKV_F16>(a, f, stream);
+    return launch_quant_dim<DSKV_BF16>(a, f, stream);
+}
 
 }  // namespace dskv
 
@@ -173,7 +208,12 @@ extern "C" int64_t dskv_quant_attn_workspace(int32_t batch, int32_t nnz, int32_t
 {
     using namespace dskv;
     if (batch <= 0 || nnz <= 0 || max_qo_len <= 0 || n_kv_heads <= 0 || n_qo_heads < n_kv_heads || !quant_matrix_form(head_dim)) return 0;
-    return form_bytes(quant_form(max_qo_len, n_qo_heads, n_kv_heads, dtype), batch, n_kv_heads, head_dim);
+    const int narrow_most = narrow_rows(n_qo_heads, n_kv_heads, dtype);
+    const int64_t narrow = form_bytes(quant_form(false, max_qo_len < narrow_most ? max_qo_len : narrow_most, n_qo_heads, n_kv_heads, dtype),
+                                      batch, n_kv_heads, head_dim);
+    if (max_qo_len <= narrow_most) return narrow;
+    const int64_t wide = form_bytes(quant_form(true, max_qo_len, n_qo_heads, n_kv_heads, dtype), batch, n_kv_heads, head_dim);
+    return narrow > wide ? narrow : wide;
 }
 
 extern "C" int dskv_quant_attn(const dskv_quant_step_t *step, void *out, const void *q, int64_t q_stride,
@@ -209,33 +249,31 @@ extern "C" int dskv_quant_attn(const dskv_quant_step_t *step, void *out, const v
     a.half_bytes = shape.half_bytes;
     a.page_bytes = shape.page_bytes;
     hipStream_t st = (hipStream_t)stream;
-    const QuantForm f = quant_form(s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->dtype);
+    // two launches where some requests have few rows and others many, one after the other over the same workspace
+    const int narrow_most = narrow_rows(s->n_qo_heads, s->n_kv_heads, s->dtype);
+    const bool some_narrow = step->min_qo_len <= narrow_most, some_wide = s->max_qo_len > narrow_most;
+    const QuantForm narrow = quant_form(false, some_wide ? narrow_most : s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->dtype);
+    const QuantForm wide = quant_form(true, s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->dtype);
+    const int64_t col_tiles = some_wide && wide.col_tiles > narrow.col_tiles ? wide.col_tiles : narrow.col_tiles;
     // (places in the pool, tokens of a request and units are numbered in 32 bits there)
     if (quant_matrix_form(s->head_dim) && s->num_pages * (shape.page_bytes / 16) < UINT32_MAX &&
         s->n_page_indices < kMostTokens / s->page_size &&
-        (s->n_page_indices * s->page_size / 16 + 2LL * s->batch) * f.col_tiles < INT32_MAX) {
+        (s->n_page_indices * s->page_size / 32 + 2LL * s->batch) * col_tiles < INT32_MAX) {
         const int64_t need = dskv_quant_attn_workspace(s->batch, s->nnz, s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->head_dim, s->dtype);
         if (!s->workspace || s->workspace_bytes < need) {
             set_error("quant_attn: workspace of %lld bytes, %lld are needed", (long long)s->workspace_bytes, (long long)need);
             return DSKV_E_NOMEM;
         }
         DSKV_REQUIRE((uintptr_t)s->workspace % 16 == 0, "quant_attn: the workspace must be 16-byte aligned");
-        DSKV_REQUIRE((int64_t)s->batch * f.col_tiles < INT32_MAX && s->n_kv_heads <= 65535, "quant_attn: too large a batch");
-        a.units_before = (int32_t *)s->workspace;
-        a.part_o = (float *)((char *)s->workspace + units_bytes(s->batch));
-        a.part_ml = a.part_o + slots_of(f, s->n_kv_heads) * s->head_dim;
-        a.n_shares = f.shares;
-        a.sides = 1;
+        DSKV_REQUIRE((int64_t)s->batch * col_tiles < INT32_MAX && s->n_kv_heads <= 65535, "quant_attn: too large a batch");
         a.group = s->n_qo_heads / s->n_kv_heads;
         a.page_shift = 31 + ilog2(s->page_size);
         a.page_magic = (uint32_t)(((1ull << a.page_shift) + s->page_size - 1) / s->page_size);
         a.page16 = (uint32_t)(shape.page_bytes / 16);
         a.row16 = (uint32_t)(s->head_dim / 16);
-        a.rows_from = 0;
-        a.rows_to = INT32_MAX;
-        if (s->dtype == DSKV_F32) return launch_quant_dim<DSKV_F32>(a, f, st);
-        if (s->dtype == DSKV_F16) return launch_quant_dim<DSKV_F16>(a, f, st);
-        return launch_quant_dim<DSKV_BF16>(a, f, st);
+        if (some_narrow || !some_wide)
+            if (int rc = launch_quant_form(a, narrow, s->dtype, 0, some_wide ? narrow_most : INT32_MAX, s->workspace, st)) return rc;
+        return some_wide ? launch_quant_form(a, wide, s->dtype, some_narrow ? narrow_most + 1 : 0, INT32_MAX, s->workspace, st) : 0;
     }
     DSKV_REQUIRE(s->n_qo_heads <= 65535, "quant_attn: at most 65535 heads");
     const dim3 grid((unsigned)s->nnz, (unsigned)s->n_qo_heads), block(kQuantWaves * 64);

@@ -1,0 +1,358 @@
+// The attention over 8-bit pages for more columns than fit a wave (head_dim 64 and 128, 16-bit types): the columns are split over the
+// waves of a workgroup, 32 each, and all of them read the same 32-token blocks of K and V from LDS, where these lie in the type of q,
+// multiplied by their scales.  See tree_kernel.h for how the work is cut.  A wave fetches its part of a block in codes, 8
+// bytes a lane and row, some blocks ahead, makes 8 numbers of them - two an instruction, which applies the scale; exact in bf16, in f16 but for
+// what f16 itself does not hold - and writes them to LDS, so that every code is converted once a workgroup.
+//
+// Iteration j of a walk multiplies P(j - 1) into V(j - 1), turns S(j) into P(j) and computes S(j + 1), so that all of
+// its matrix instructions are independent of its exponentials.  Behind its only barrier K(j + 3) and V(j) are written to LDS, K(j + 5) and V(j + 2)
+// requested, and at its end the operands of K(j + 2) read; with 64 dims a stage holds two blocks side by side, and so it is once in two iterations.  The running maximum of a column is raised only when a block's weights under it
+// sum to more than most_weight in a lane.  Weights are rounded to 16 bits for the matrix product, half a step of each (see headroom).
+// Where a token lies in the pool, and its scales, are looked up for some thousand tokens at a time and kept in LDS, so that pages may
+// have any size.
+#pragma once
+
+#include "quant_kernel.h"
+
+namespace dskv {
+
+constexpr int kWideBlock = 32;
+constexpr int kWideRegion = 1088;           // 64 lanes' 16 bytes, (4 chunk + row) * 16 of four rows, and 64 bytes of padding
+constexpr int kWideStage = kWideBlock / 4 * kWideRegion;
+constexpr int kWideLeast = 8;               // units a share has at least: what fills the stages takes about as long
+
+template <int kD, int kWaves> struct QuantWide {
+    static constexpr int kThreads = kWaves * 64;
+    static constexpr int kCols = kWaves * 32;
+    static constexpr int kPack = 128 / kD;               // blocks of a stage: rows of 64 dims lie side by side with the next block's
+    static constexpr int kChunks = kD / 8;               // 8-code chunks of a row
+    static constexpr int kSteps = kD / 16, kDims = kD / 32;      // matrix instructions of a block's scores; 32-dim tiles of O
+    static constexpr int kGroups = 8 / kWaves;           // regions of a stage that a wave fetches
+    static constexpr int kHalf = kWaves == 8 ? 64 : 32;  // blocks that are looked up at a time; two such halves are kept
+    static constexpr int kTokens = 2 * kHalf * kWideBlock;
+    static constexpr int kKStages = kPack == 2 ? 2 : 4, kVStages = kPack == 2 ? 4 : 2;      // in LDS
+    static constexpr int kAhead = 2;                     // stages of K, and of V, on their way in registers
+    // what turn u (in front of the iterations of stage u) writes: K(u + kFirst) and V(u + kBehind)
+    static constexpr int kFirst = kPack == 2 ? 2 : 3, kBehind = kPack - 1;
+};
+
+template <int DT, int kD, int kWaves>
+__global__ __launch_bounds__(kWaves * 64, 2) void quant_wide_kernel(QuantArgs a)
+{
+    typedef Elt<DT> E;
+    typedef QuantWide<kD, kWaves> W;
+    __shared__ __align__(16) char lds[(W::kKStages + W::kVStages) * kWideStage];
+    __shared__ uint32_t row_at[W::kTokens];              // where a token's K lies (see quant_row)
+    __shared__ uint16_t scale_at[W::kTokens];            // exponents of its scales, V's in the upper byte
+    __shared__ uint32_t held_at[2 * W::kHalf];           // bit per token of a block: there is one
+    __shared__ int holes;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, c = lane & 15, h = lane >> 5, r32 = lane & 31;
+    int share, head;
+    share_and_head(a, share, head);
+    TreePlace place;
+    tree_place<W::kCols, kWideBlock, W::kThreads, true, kWideLeast, kWideLeast>(a, share, place);
+    make_uniform(place);
+    const int begin = place.begin, end = place.end;
+    const bool beside = place.beside;
+    int unit = begin, base = place.base;
+    int b = place.b;
+    TreeRequest r = place.r;
+
+    auto k_stage = [&](int i) { return lds + (i & (W::kKStages - 1)) * kWideStage; };
+    auto v_stage = [&](int i) { return lds + (W::kKStages + (i & (W::kVStages - 1))) * kWideStage; };
+    // block j in its stage of K or V
+    auto block_at = [&](auto &stage, int j) -> char * { return W::kPack == 2 ? stage(j >> 1) + (j & 1) * 512 : stage(j); };
+    // lane p of a wave fetches chunk p / 4 of row p % 4 of a region
+    const char *const pool = a.pages + head * a.head_bytes + (lane >> 2) % W::kChunks * 8;
+    const char *const none = reinterpret_cast<const char *>(kNoRow);
+    const char *const scales = a.pages + 2 * a.half_bytes + head * 4;
+
+    while (unit < end) {
+        if (unit >= base + (int)units_of(r, beside)) {             // on to the next request that has rows
+            base += (int)units_of(r, beside);
+            b++;
+            r = tree_request<W::kCols, kWideBlock>(a, b);
+            continue;
+        }
+        const int ct = beside ? place.side : (int)((unsigned)(unit - base) / (unsigned)r.subtiles);
+        const int item = base + (beside ? 0 : ct * r.subtiles);
+        const int st0 = unit - item, st1 = min(end - item, r.subtiles);
+        if (ct >= r.col_tiles) {                              // (beside: a request of fewer column tiles)
+            unit = item + st1;
+            continue;
+        }
+        const int cols = min(r.n * a.group - ct * r.tile, r.tile);
+        const int prior = r.prior;
+        // (what lies behind the tile's last row is not walked, though it was counted)
+        const long last_seen = a.masks ? r.kv_len : min(r.kv_len, (long)prior + (ct * r.tile + cols - 1) / a.group + 1);
+        const int t_end = (int)max(min(last_seen, (long)st1 * kWideBlock), 0L);
+        const int blocks = max((t_end + kWideBlock - 1) / kWideBlock - st0, 0);
+        const bool works = wave * 32 < cols;
+
+        // ---- the column
+        const int col = ct * r.tile + wave * 32 + r32, row_i = col / a.group;
+        const bool there = wave * 32 + r32 < cols;
+        const long q_row = r.first + (there ? row_i : 0);
+        const int hq = head * a.group + (there ? col - row_i * a.group : 0);
+        unsigned long long mask = ~0ull;
+        int limit = 0;                                  // tokens from here on are not seen
+        if (there) {
+            if (a.masks) mask = (unsigned long long)a.masks[q_row];
+            const long lim = a.masks ? (long)prior + DSKV_MAX_TREE_ROWS : (long)prior + row_i + 1;
+            limit = (int)max(min(lim, (long)t_end), 0L);
+        }
+        u32x4 q[W::kSteps];
+        {
+            const char *row = a.q + q_row * a.q_stride + hq * kD * 2 + h * 16;
+#pragma unroll
+            for (int s = 0; s < W::kSteps; s++) {
+                q[s] = u32x4{0, 0, 0, 0};
+                if (there) q[s] = *reinterpret_cast<const u32x4 *>(row + s * 32);
+            }
+        }
+        // blocks that reach behind here need their scores masked
+        const int first_i = (ct * r.tile + wave * 32) / a.group;
+        int mask_from = min(a.masks ? prior : prior + first_i + 1, t_end);
+
+        f32x16 acc[W::kDims], xs[2];
+        float m_run = -__FLT_MAX__, l_run = 0;
+        u32x4 pb[2][2];
+#pragma unroll
+        for (int d = 0; d < W::kDims; d++)
+#pragma unroll
+            for (int v = 0; v < 16; v++) acc[d][v] = 0;
+        pb[1][0] = pb[1][1] = u32x4{0, 0, 0, 0};
+
+        // ---- places in the pool, kHalf blocks at a time: half x of the walk into half x % 2
+        auto look_up = [&](int x) {
+            for (int i = threadIdx.x; i < W::kHalf * kWideBlock; i += W::kThreads) {
+                const int t = (st0 + x * W::kHalf) * kWideBlock + i;
+                uint32_t row = kNoQuantRow;
+                uint32_t exponents = 0;
+                if (t < t_end) {
+                    const int page = page_of(a, r, t);
+                    row = quant_row(a, t, page);
+                    if (row == kNoQuantRow) holes = 1;
+                    else {
+                        const uint32_t *s = reinterpret_cast<const uint32_t *>(scales + page * a.page_bytes);
+                        exponents = (s[0] >> 23 & 0xFF) | (s[a.n_kv_heads] >> 15 & 0xFF00);
+                    }
+                }
+                const int at = (x & 1) * W::kHalf * kWideBlock + i;
+                row_at[at] = row;
+                scale_at[at] = (uint16_t)exponents;
+                const unsigned long long there64 = __ballot(row != kNoQuantRow);
+                if ((lane & 31) == 0) held_at[at / kWideBlock] = (uint32_t)(there64 >> (lane & 32));
+            }
+        };
+        // token of the walk, as the tables have it, that the lane fetches of region i of stage u; its block
+        auto block_of = [&](int u) { return W::kPack == 2 ? 2 * u + (lane >> 5) : u; };
+        auto token_of = [&](int u, int i) {
+            return (block_of(u) & (2 * W::kHalf - 1)) * kWideBlock + (wave * W::kGroups + i) * 4 + (lane & 3);
+        };
+        u32x2 k_codes[W::kAhead][W::kGroups], v_codes[W::kAhead][W::kGroups];
+        auto request = [&](int u, u32x2 (&codes)[W::kGroups], long more) {
+#pragma unroll
+            for (int i = 0; i < W::kGroups; i++) {
+                const uint32_t row = block_of(u) < blocks ? row_at[token_of(u, i)] : kNoQuantRow;
+                const char *p = pool + (uint64_t)row * 16 + more;
+                p = row != kNoQuantRow ? p : none;
+                codes[i] = *(const __attribute__((address_space(1))) u32x2 *)p;
+            }
+        };
+        auto write = [&](const u32x2 (&codes)[W::kGroups], int u, char *stage, int shift) {
+#pragma unroll
+            for (int i = 0; i < W::kGroups; i++) {
+                // (behind the walk nothing was looked up, and the codes are zeros)
+                const uint32_t exponent = block_of(u) < blocks ? (uint32_t)scale_at[token_of(u, i)] >> shift & 0xFF : 127u;
+                const float scale = __builtin_bit_cast(float, exponent << 23);
+                u32x4 x;
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                    if constexpr (DT == DSKV_F16) {
+                        x[2 * w] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[i][w], scale, false));
+                        x[2 * w + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[i][w], scale, true));
+                    } else {
+                        x[2 * w] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[i][w], scale, false));
+                        x[2 * w + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[i][w], scale, true));
+                    }
+                }
+                *reinterpret_cast<u32x4 *>(stage + (wave * W::kGroups + i) * kWideRegion + lane * 16) = x;
+            }
+        };
+
+        // ---- parts of an iteration
+        u32x4 key[W::kSteps];                                    // K operand: token r32, dims 16 s + 8 h ..
+        auto read_keys = [&](const char *stage) {
+            // token r32 = row r32 & 3 of region r32 >> 2; chunk 2 s + h
+            const char *rows = stage + (r32 >> 2) * kWideRegion + h * 64 + (r32 & 3) * 16;
+#pragma unroll
+            for (int s = 0; s < W::kSteps; s++) key[s] = *reinterpret_cast<const u32x4 *>(rows + s * 128);
+        };
+        auto scores = [&](f32x16 &x) {
+#pragma unroll
+            for (int v = 0; v < 16; v++) x[v] = 0;
+#pragma unroll
+            for (int s = 0; s < W::kSteps; s++) x = E::mfma_32x32(key[s], q[s], x);
+        };
+        // bits of block j's tokens that the column sees
+        auto seen = [&](int j) {
+            return j < blocks ? seen_bits((st0 + j) * kWideBlock, prior, limit, mask, !a.masks) & held_at[j & (2 * W::kHalf - 1)] : 0u;
+        };
+        auto mask_scores = [&](int j, f32x16 &x) {
+            asm volatile("" : "+v"(x));                 // keeps this a branch that most blocks do not take
+            uint32_t bits = seen(j) >> (4 * h);
+            asm volatile("" : "+v"(bits));
+#pragma unroll
+            for (int v = 0; v < 16; v++)
+                if (!((bits >> (8 * (v >> 2) + (v & 3))) & 1)) x[v] = -INFINITY;
+        };
+        auto weights = [&](const f32x16 &x, int s, u32x4 &out, float &sum) {
+            float p[8];
+#pragma unroll
+            for (int v = 0; v < 8; v++) {
+                p[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * s + v], a.scale, -m_run));
+                sum += p[v];
+            }
+            out = u32x4{E::pack2(p[0], p[1]), E::pack2(p[2], p[3]), E::pack2(p[4], p[5]), E::pack2(p[6], p[7])};
+            asm volatile("" ::"v"(out), "v"(sum));      // keeps them in their half of the iteration
+        };
+        auto raise = [&](const f32x16 &x) {
+            float m = x[0] * a.scale;
+#pragma unroll
+            for (int v = 1; v < 16; v++) m = fmaxf(m, x[v] * a.scale);
+            float other = m;
+            swap_halves32(m, other);
+            const float m_new = fmaxf(m_run, fmaxf(m, other) - headroom(DT));
+            const float keep = __builtin_amdgcn_exp2f(m_run - m_new);
+            m_run = m_new;
+            l_run *= keep;
+#pragma unroll
+            for (int d = 0; d < W::kDims; d++) acc[d] *= keep;
+        };
+        const int v_off = h * kWideRegion + (2 * (g & 1) + ((c & 3) >> 1)) * 64 + (c >> 2) * 16 + (c & 1) * 8;
+        // ---- the walk
+        __syncthreads();                                 // the item before is through with LDS
+        if (threadIdx.x == 0) holes = 0;
+        __syncthreads();
+        look_up(0);
+        for (int i = threadIdx.x; i < kWideStage / 16; i += W::kThreads)
+            reinterpret_cast<u32x4 *>(v_stage(-1))[i] = u32x4{0, 0, 0, 0};     // V(-1), which P(-1) = 0 is multiplied by
+        __syncthreads();
+        if (holes) mask_from = 0;
+        // q and the mask are waited for here: left to the loop, that would be a wait for its loads
+#pragma unroll
+        for (int s = 0; s < W::kSteps; s++) asm volatile("" : "+v"(q[s]));
+        asm volatile("" : "+v"(mask));
+        // as if there were turns in front
+#pragma unroll
+        for (int i = 0; i < W::kAhead; i++) {
+            request(i, k_codes[i], 0);
+            request(i, v_codes[i], a.half_bytes);
+        }
+#pragma unroll
+        for (int i = 0; i < W::kFirst; i++) {
+            write(k_codes[i % W::kAhead], i, k_stage(i), 0);
+            request(W::kAhead + i, k_codes[i % W::kAhead], 0);
+        }
+#pragma unroll
+        for (int i = 0; i < W::kBehind; i++) {
+            write(v_codes[i], i, v_stage(i), 8);
+            request(W::kAhead + i, v_codes[i], a.half_bytes);
+        }
+        __syncthreads();
+        if (works) {
+            read_keys(block_at(k_stage, 0));
+            scores(xs[0]);
+            if ((st0 + 1) * kWideBlock > mask_from) mask_scores(0, xs[0]);
+            read_keys(block_at(k_stage, 1));
+        }
+        // phase: u up to a multiple of kAhead, a literal
+        auto turn = [&](int u, int phase) {
+            constexpr int kMask = W::kAhead - 1;
+            const int k_at = (phase + W::kFirst) & kMask, v_at = (phase + W::kBehind) & kMask;
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            write(k_codes[k_at], u + W::kFirst, k_stage(u + W::kFirst), 0);
+            write(v_codes[v_at], u + W::kBehind, v_stage(u + W::kBehind), 8);
+            request(u + W::kFirst + W::kAhead, k_codes[k_at], 0);
+            request(u + W::kBehind + W::kAhead, v_codes[v_at], a.half_bytes);
+        };
+        auto iteration = [&](int j, int phase) {
+            if (W::kPack == 1 || (phase & 1) == 0) turn(j / W::kPack, phase / W::kPack);
+            if (!works || j > blocks) return;
+            const int cur = phase & 1, nxt = cur ^ 1;
+            const char *rows = block_at(v_stage, j - 1) + v_off;                        // V(j - 1)
+            u32x4 va[W::kDims][2];
+#pragma unroll
+            for (int d = 0; d < W::kDims; d++)
+#pragma unroll
+                for (int s = 0; s < 2; s++) {
+                    const char *p = rows + s * 4 * kWideRegion + d * 256;
+                    const u32x2 lo = read_transposed(p), hi = read_transposed(p + 2 * kWideRegion);
+                    va[d][s] = u32x4{lo.x, lo.y, hi.x, hi.y};
+                }
+            scores(xs[nxt]);                                                        // S(j + 1)
+            float sum = 0;
+            weights(xs[cur], 0, pb[cur][0], sum);
+            if ((st0 + j + 2) * kWideBlock > mask_from) mask_scores(j + 1, xs[nxt]);
+#pragma unroll
+            for (int d = 0; d < W::kDims; d++)
+#pragma unroll
+                for (int s = 0; s < 2; s++) acc[d] = E::mfma_32x32(va[d][s], pb[nxt][s], acc[d]);   // P(j - 1)
+            read_keys(block_at(k_stage, j + 2));                                         // K(j + 2)
+            weights(xs[cur], 1, pb[cur][1], sum);
+            if (__builtin_expect(__builtin_amdgcn_ballot_w64(sum > most_weight(DT)) != 0, 0)) {
+                raise(xs[cur]);
+                __builtin_amdgcn_sched_barrier(0);
+                sum = 0;
+                weights(xs[cur], 0, pb[cur][0], sum);
+                weights(xs[cur], 1, pb[cur][1], sum);
+            }
+            l_run += sum;
+        };
+        for (int j = 0; j <= blocks; j += 4) {
+            if (j % W::kHalf == W::kHalf / 2 && j + W::kHalf / 2 < blocks) look_up(j / W::kHalf + 1);
+            iteration(j, 0);
+            if (holes) mask_from = 0;
+            iteration(j + 1, 1);
+            iteration(j + 2, 2);
+            iteration(j + 3, 3);
+        }
+
+        // ---- the item's result
+        float l_other = l_run;
+        swap_halves32(l_run, l_other);
+        const float l = l_run + l_other;
+        const bool cut = st0 > 0 || st1 < r.subtiles;
+        if (there && cut) {
+            const long slot = 2L * share + (unit > begin ? 1 : 0);
+            const long part = (slot * a.n_kv_heads + head) * W::kCols + wave * 32 + r32;
+#pragma unroll
+            for (int d = 0; d < W::kDims; d++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    *reinterpret_cast<f32x4 *>(a.part_o + part * kD + d * 32 + 8 * i + 4 * h) =
+                        f32x4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+            if (h == 0) {
+                a.part_ml[part * 2] = m_run;
+                a.part_ml[part * 2 + 1] = l;
+            }
+        } else if (there) {
+            const float inv = l == 0 ? 0.f : 1.f / l;
+            char *dst = a.out + ((q_row * a.n_qo_heads + hq) * kD + 4 * h) * 2;
+#pragma unroll
+            for (int d = 0; d < W::kDims; d++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    *reinterpret_cast<u32x2 *>(dst + (d * 32 + 8 * i) * 2) =
+                        u32x2{E::pack2(acc[d][4 * i] * inv, acc[d][4 * i + 1] * inv),
+                              E::pack2(acc[d][4 * i + 2] * inv, acc[d][4 * i + 3] * inv)};
+        }
+        unit = item + st1;
+    }
+}
+
+}  // namespace dskv

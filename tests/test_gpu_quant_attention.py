@@ -181,7 +181,7 @@ def test_replayed_with_other_lengths(n):
            torch.zeros(100, dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")]
     q, k, v = (torch.zeros((total, h, 128), dtype=torch.bfloat16, device="cuda") for h in (8, 2, 2))
     out = torch.zeros_like(q)
-    w = BatchQuantizedWithPagedKVCacheWrapper(torch.empty(64 << 20, dtype=torch.uint8, device="cuda"))
+    w = BatchQuantizedWithPagedKVCacheWrapper(torch.empty(128 << 20, dtype=torch.uint8, device="cuda"))
     w.begin_forward(*csr, 8, 2, 128, 16, max_qo_len=n)
 
     def step():
