@@ -11,7 +11,7 @@ pair become lazily created per-device singletons.
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Dict, List, Optional, Sequence, Tuple
+from typing import Dict, List, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -19,10 +19,10 @@ from deserve_amd.draft_ops import (MAX_TREE_ROWS, BatchTreeWithPagedKVCacheWrapp
                                    verify_drafts)
 from deserve_amd.execution.result import BatchResult
 from deserve_amd.kvcache.paged.kvcache import PagedKVCache
-from deserve_amd.model.context.flash import FlashDecodeCtx, FlashPrefillCtx, FlashTreeCtx
+from deserve_amd.model.context.flash import FlashDecodeCtx, FlashPrefillCtx, FlashQuantCtx, FlashTreeCtx
 from deserve_amd.paged_ops import (BatchDecodeWithPagedKVCacheWrapper,
                                    BatchPrefillWithPagedKVCacheWrapper)
-from deserve_amd.quant_ops import BatchQuantizedWithPagedKVCacheWrapper
+from deserve_amd.quant_ops import BatchQuantizedWithPagedKVCacheWrapper, move_accepted_quantized_rows
 from deserve_amd.task import TaskData
 
 WORKSPACE_BYTES = 128 * 1024 * 1024
@@ -111,6 +111,14 @@ class BatchExec:
                            [t.task_id for t in all_datas], [t.task_id for t in done],
                            {t.task_id: p for t, p in probs})
 
+    def _quantized(self) -> Optional[BatchQuantizedWithPagedKVCacheWrapper]:
+        """For a step over 8-bit pages a wrapper of its own, which costs nothing: a step prepared in between does not
+        change this one.  None for pages of the model's type."""
+        pool = self.kvcaches[0].pool
+        if getattr(pool, "record", None) is None:
+            return None
+        return BatchQuantizedWithPagedKVCacheWrapper(get_quantized_wrapper(pool.main_device)._workspace)
+
     def _shape_kwargs(self) -> dict:
         a = self.layer_storage.model_args
         n_kv = a.n_heads if a.n_kv_heads is None else a.n_kv_heads
@@ -120,10 +128,14 @@ class BatchExec:
 
 @dataclass
 class BatchDecode(BatchExec):
-    decode_ctx: Optional[FlashDecodeCtx] = None
+    decode_ctx: Optional[Union[FlashDecodeCtx, FlashQuantCtx]] = None
 
     def prepare(self) -> None:
         with torch.inference_mode():
+            quantized = self._quantized()
+            if quantized is not None:
+                self.decode_ctx = FlashQuantCtx.init_and_plan(self.task_datas, self.kvcaches, quantized, **self._shape_kwargs())
+                return
             wrapper, _ = get_wrappers(self.kvcaches[0].pool.main_device)
             # the context's index arrays and the attention work list go up in one kernel
             ctx = FlashDecodeCtx.init_and_plan(self.task_datas, self.kvcaches, wrapper,
@@ -140,10 +152,14 @@ class BatchDecode(BatchExec):
 
 @dataclass
 class BatchPrefill(BatchExec):
-    prefill_ctx: Optional[FlashPrefillCtx] = None
+    prefill_ctx: Optional[Union[FlashPrefillCtx, FlashQuantCtx]] = None
 
     def prepare(self) -> None:
         with torch.inference_mode():
+            quantized = self._quantized()
+            if quantized is not None:
+                self.prefill_ctx = FlashQuantCtx.init_and_plan(self.task_datas, self.kvcaches, quantized, **self._shape_kwargs())
+                return
             _, wrapper = get_wrappers(self.kvcaches[0].pool.main_device)
             # metadata and plan in one pinned block, one upload kernel
             self.prefill_ctx = FlashPrefillCtx.init_and_plan(self.task_datas, self.kvcaches, wrapper,
@@ -209,7 +225,8 @@ class BatchVerify(BatchExec):
             raise ValueError(f"a task has at most {MAX_TREE_ROWS} rows to verify")
         with torch.inference_mode():
             # a wrapper of its own, which costs nothing: a step prepared in between does not change this one
-            wrapper = BatchTreeWithPagedKVCacheWrapper(get_tree_wrapper(self.kvcaches[0].pool.main_device)._workspace)
+            wrapper = self._quantized() or BatchTreeWithPagedKVCacheWrapper(
+                get_tree_wrapper(self.kvcaches[0].pool.main_device)._workspace)
             self.tree_ctx = FlashTreeCtx.init_and_plan(self.task_datas, self.kvcaches, wrapper, parents=self.parents,
                                                        **self._shape_kwargs())
 
@@ -241,8 +258,14 @@ class BatchVerify(BatchExec):
         with torch.inference_mode():
             assert self.tree_ctx is not None
             ctx = self.tree_ctx
-            if self.parents is not None:                    # the rows of an accepted chain are in place
-                move_accepted_rows(ctx.page_pool.pages, ctx.tables.slots, ctx.indptr, verdict.path, verdict.counts)
+            pool = ctx.page_pool
+            if self.parents is None:                        # the rows of an accepted chain are in place
+                pass
+            elif pool.record is not None:
+                move_accepted_quantized_rows(pool.pages, ctx.indptr, ctx.kv_page_indices, ctx.kv_page_indptr, ctx.kv_last_page_lens,
+                                             verdict.path, verdict.counts, pool.page_size, pool.n_kv_heads, pool.head_dim)
+            else:
+                move_accepted_rows(pool.pages, ctx.tables.slots, ctx.indptr, verdict.path, verdict.counts)
             counts = verdict.counts.tolist()
             for task, n in zip(self.task_datas, counts):
                 task.seqlen = n

@@ -11,6 +11,9 @@ alternates between batch sizes replays instead of capturing again.  The workgrou
 of small 16-bit batches does not follow the requests' lengths (their plans are filled up
 with empty workgroups): a size needs a capture for whole requests and one where some are cut.
 
+Over 8-bit pages (a BatchQuantizedWithPagedKVCacheWrapper) nothing is planned: lengths and tables are read on the
+device, and a batch size needs one capture.
+
 Nothing that is captured clears memory with a memset node, and the library
 calls allocate nothing; the outputs of the captured forward live in the graph's
 own memory pool and are overwritten by every replay.
@@ -18,19 +21,20 @@ own memory pool and are overwritten by every replay.
 from __future__ import annotations
 
 from collections import OrderedDict
-from typing import List, Sequence
+from typing import List, Sequence, Union
 
 import torch
 
 from deserve_amd import _lib
 from deserve_amd.kvcache.paged.kvcache import PagedKVCache
-from deserve_amd.model.context.flash import FlashDecodeCtx, MetadataBuffers, StagedUpload
+from deserve_amd.model.context.flash import FlashDecodeCtx, FlashQuantCtx, MetadataBuffers, StagedUpload
 from deserve_amd.paged_ops import BatchDecodeWithPagedKVCacheWrapper
+from deserve_amd.quant_ops import BatchQuantizedWithPagedKVCacheWrapper
 from deserve_amd.task import TaskData
 
 
 class GraphedDecodeStep:
-    def __init__(self, layer_storage, wrapper: BatchDecodeWithPagedKVCacheWrapper, max_batch: int,
+    def __init__(self, layer_storage, wrapper: Union[BatchDecodeWithPagedKVCacheWrapper, BatchQuantizedWithPagedKVCacheWrapper], max_batch: int,
                  max_pages: int, device: torch.device, num_qo_heads: int, num_kv_heads: int,
                  head_dim: int, page_size: int, target_workgroups: int = 0, max_graphs: int = 8) -> None:
         self.layer_storage, self.wrapper = layer_storage, wrapper
@@ -38,7 +42,8 @@ class GraphedDecodeStep:
                           page_size=page_size)
         self.target_workgroups = target_workgroups
         self.meta = MetadataBuffers(max_batch, max_pages, device)
-        words = int(_lib.lib().dskv_decode_plan_bound(max_batch, max_pages * page_size))
+        self.quantized = isinstance(wrapper, BatchQuantizedWithPagedKVCacheWrapper)
+        words = 0 if self.quantized else int(_lib.lib().dskv_decode_plan_bound(max_batch, max_pages * page_size))
         self.plan = StagedUpload(words, device)
         self.max_graphs = max_graphs
         self._graphs: "OrderedDict[tuple, tuple]" = OrderedDict()   # key -> (graph, inputs, output)
@@ -47,7 +52,13 @@ class GraphedDecodeStep:
         self._output = None
         self.captures = 0
 
-    def _prepare(self, task_datas: Sequence[TaskData], kvcaches: Sequence[PagedKVCache]) -> FlashDecodeCtx:
+    def _prepare(self, task_datas: Sequence[TaskData], kvcaches: Sequence[PagedKVCache]) -> Union[FlashDecodeCtx, FlashQuantCtx]:
+        if any((c.pool.record is not None) != self.quantized for c in kvcaches):
+            raise ValueError("the wrapper is for pages of the model's type, the caches' are in 8 bits, or the other way round")
+        if self.quantized:
+            if any(t.seqlen != 1 for t in task_datas):
+                raise ValueError("a captured decode step has one row for every request")
+            return FlashQuantCtx.init_and_plan(list(task_datas), list(kvcaches), self.wrapper, **self.shape, buffers=self.meta)
         ctx = FlashDecodeCtx.init_paged_decode_ctx(list(task_datas), list(kvcaches), self.wrapper, self.meta)
         self.wrapper.begin_forward(indptr=ctx.kv_page_indptr, indices=ctx.kv_page_indices,
                                    last_page_len=ctx.kv_last_page_lens,
@@ -81,8 +92,11 @@ class GraphedDecodeStep:
         tensors = list(xs) if isinstance(xs, (tuple, list)) else [xs]
         ctx = self._prepare(task_datas, kvcaches)
         w = self.wrapper
-        key = self.graph_key(len(task_datas), w._n_workgroups, w._n_items, tensors,
-                             w.fused_append_supported(tensors[0].dtype))
+        if self.quantized:
+            key = self.graph_key(len(task_datas), 0, 0, tensors, True)
+        else:
+            key = self.graph_key(len(task_datas), w._n_workgroups, w._n_items, tensors,
+                                 w.fused_append_supported(tensors[0].dtype))
         held = self._graphs.get(key)
         if held is None:
             inputs = [t.clone() for t in tensors]

@@ -12,6 +12,7 @@ import torch
 
 from deserve_amd.kvcache._alloc import BuddyIndex
 from deserve_amd.kvcache.pinned.pinned_memory import pinned_empty
+from deserve_amd.quant_ops import CODE_DTYPE, PageRecord
 
 
 @dataclass
@@ -54,6 +55,8 @@ class ChunkPool:
         self.main_device, self.main_dtype = torch.device(main_device), main_dtype
         self.mutex = threading.Lock()
         self.per_token_shape = (2, page_size, n_kv_heads, head_dim)
+        if main_dtype is CODE_DTYPE:        # records of 8-bit pages (see page_pool)
+            self.per_token_shape, main_dtype = (PageRecord(page_size, n_kv_heads, head_dim).page_bytes,), torch.uint8
         self.chunks = pinned_empty(((1 << (height - 1)) * num_layers,) + self.per_token_shape,
                                    main_dtype)
         self._buddy = BuddyIndex(height)

@@ -4,6 +4,9 @@
 n_kv_heads, head_dim) on ``main_device``.  Allocation state is the host-side
 ``FreePageIndex``; the reference's attribute names (``page_bitmap``,
 ``page_buffer``, ``num_avails``) are views of it.
+
+A pool of main_dtype torch.float8_e4m3fn holds its pages in 8 bits: ``pages`` is (num_layers, num_pages, page_bytes) uint8
+then, records of codes and scales (``record``, quant_ops.PageRecord).
 """
 from __future__ import annotations
 
@@ -14,6 +17,7 @@ import numpy as np
 import torch
 
 from deserve_amd.kvcache._alloc import FreePageIndex
+from deserve_amd.quant_ops import CODE_DTYPE, PageRecord
 
 
 def _ids_to_numpy(ids: torch.Tensor) -> np.ndarray:
@@ -29,8 +33,13 @@ class PagePool:
         self.n_kv_heads, self.head_dim = n_kv_heads, head_dim
         self.mutex = threading.Lock()
         self._index = FreePageIndex(num_pages)
-        self.pages = torch.empty((num_layers, num_pages, 2, page_size, n_kv_heads, head_dim),
-                                 device=self.main_device, dtype=main_dtype)
+        self.record = PageRecord(page_size, n_kv_heads, head_dim) if main_dtype is CODE_DTYPE else None
+        if self.record is not None:
+            self.pages = torch.empty((num_layers, num_pages, self.record.page_bytes), device=self.main_device,
+                                     dtype=torch.uint8)
+        else:
+            self.pages = torch.empty((num_layers, num_pages, 2, page_size, n_kv_heads, head_dim),
+                                     device=self.main_device, dtype=main_dtype)
 
     # ---- reference attribute names, backed by the host index
     @property
@@ -91,7 +100,8 @@ class PagePool:
             self._index.give(_ids_to_numpy(blocks))
 
     def retrieve(self, indices: torch.Tensor) -> torch.Tensor:
-        """Copy of pages[:, indices] -> (L, n, 2, P, Hkv, D) (page_pool.py:78-79)."""
+        """Copy of pages[:, indices] -> (L, n, 2, P, Hkv, D) (page_pool.py:78-79); of 8-bit pages their records,
+        (L, n, page_bytes), which record.values() reads."""
         from deserve_amd.kvcache import _native
 
         return _native.gather_pages(self, indices)

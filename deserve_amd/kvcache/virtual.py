@@ -107,6 +107,8 @@ class VirtualPagePool(GpuPagePool):
 
     def calc_swap_size(self) -> int:
         """Elements of one microbatch's pinned image."""
+        if self.record is not None:
+            return self.num_layers * self.num_pages_swap * self.record.page_bytes
         return (self.num_layers * self.num_pages_swap * 2 * self.page_size * self.n_kv_heads *
                 self.head_dim)
 

@@ -15,7 +15,7 @@ kept (``host`` dict) so the attention planner never reads back from the device.
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import Dict, List, Optional, Sequence
+from typing import Dict, List, Optional, Sequence, Union
 
 import numpy as np
 import torch
@@ -28,6 +28,7 @@ from deserve_amd.kvcache.paged.page_pool import GpuPagePool
 from deserve_amd.model.context.forward import PagedForwardCtx
 from deserve_amd.paged_ops import (BatchDecodeWithPagedKVCacheWrapper,
                                    BatchPrefillWithPagedKVCacheWrapper, rope_table)
+from deserve_amd.quant_ops import BatchQuantizedWithPagedKVCacheWrapper
 from deserve_amd.task import TaskData
 
 _FIELDS = ("indptr", "kv_page_indptr", "kv_last_page_lens", "offsets", "seqlens",
@@ -272,10 +273,46 @@ class FlashPrefillCtx(FlashForwardCtx):
 
 
 @dataclass
+class FlashQuantCtx(FlashForwardCtx):
+    """A decode, prefill or mixed step over 8-bit pages (quant_ops): one kind of step, since the kernels tell from the rows of
+    a request how to compute it.  No counterpart in the reference."""
+    quant_wrapper: BatchQuantizedWithPagedKVCacheWrapper = None   # type: ignore[assignment]
+    rope_tables: Dict[tuple, torch.Tensor] = field(default_factory=dict, repr=False)
+    rope_layer: int = field(default=-1, repr=False)
+    rope_device: int = field(default=-1, repr=False)
+
+    rope_table = FlashPrefillCtx.rope_table
+    _new_rope_table = FlashPrefillCtx._new_rope_table
+
+    @property
+    def decode_wrapper(self) -> BatchQuantizedWithPagedKVCacheWrapper:
+        return self.quant_wrapper
+
+    prefill_wrapper = decode_wrapper
+
+    @classmethod
+    def init_and_plan(cls, task_datas: List[TaskData], kvcaches: List[PagedKVCache[GpuPagePool]],
+                      wrapper: BatchQuantizedWithPagedKVCacheWrapper, num_qo_heads: int, num_kv_heads: int,
+                      head_dim: int, page_size: int, buffers: "MetadataBuffers | None" = None) -> "FlashQuantCtx":
+        """Extends the caches, uploads the step's index arrays in one block; nothing is planned.  buffers: where they go, for
+        callers that replay captured launches: the block tables may then be as long as the buffers are."""
+        pool = kvcaches[0].pool
+        if any(c.pool is not pool for c in kvcaches):
+            raise ValueError("a step over 8-bit pages runs over one pool")
+        ctx = cls.init_paged_forward_ctx(task_datas, kvcaches, buffers, quant_wrapper=wrapper)
+        indices, seqlens = ctx.kv_page_indices, ctx.host["seqlens"]
+        if buffers is not None:
+            ctx.kv_page_indices = indices = buffers.dev[indices.storage_offset() - buffers.dev.storage_offset():]
+        wrapper.begin_forward(ctx.indptr, ctx.kv_page_indptr, indices, ctx.kv_last_page_lens, num_qo_heads, num_kv_heads,
+                              head_dim, page_size, max_qo_len=int(seqlens.max()), min_qo_len=int(seqlens.min()))
+        return ctx
+
+
+@dataclass
 class FlashTreeCtx(FlashForwardCtx):
-    """A step of drafted tokens: a task's seqlen rows are its last token and the drafts behind it (draft_ops).  No
-    counterpart in the reference."""
-    tree_wrapper: BatchTreeWithPagedKVCacheWrapper = None   # type: ignore[assignment]
+    """A step of drafted tokens: a task's seqlen rows are its last token and the drafts behind it (draft_ops).  Over
+    8-bit pages tree_wrapper is theirs.  No counterpart in the reference."""
+    tree_wrapper: Union[BatchTreeWithPagedKVCacheWrapper, BatchQuantizedWithPagedKVCacheWrapper] = None   # type: ignore[assignment]
     tables: StepTables = None                               # type: ignore[assignment]
     rope_tables: Dict[tuple, torch.Tensor] = field(default_factory=dict, repr=False)
     rope_layer: int = field(default=-1, repr=False)
@@ -288,8 +325,8 @@ class FlashTreeCtx(FlashForwardCtx):
 
     @classmethod
     def init_and_plan(cls, task_datas: List[TaskData], kvcaches: List[PagedKVCache[GpuPagePool]],
-                      wrapper: BatchTreeWithPagedKVCacheWrapper, num_qo_heads: int, num_kv_heads: int,
-                      head_dim: int, page_size: int, parents: Optional[torch.Tensor] = None) -> "FlashTreeCtx":
+                      wrapper: Union[BatchTreeWithPagedKVCacheWrapper, BatchQuantizedWithPagedKVCacheWrapper],
+                      num_qo_heads: int, num_kv_heads: int, head_dim: int, page_size: int, parents: Optional[torch.Tensor] = None) -> "FlashTreeCtx":
         """Extends the caches by the tasks' rows, uploads lengths and block-table rows in one block and builds the step's
         tables on the GPU.  parents: as build_step_tables takes them."""
         pool = kvcaches[0].pool

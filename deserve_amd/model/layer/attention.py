@@ -11,9 +11,10 @@ import torch
 
 from deserve_amd.draft_ops import rope_append_slots
 from deserve_amd.kvcache.paged.page_pool import PagePool
-from deserve_amd.model.context.flash import FlashDecodeCtx, FlashForwardCtx, FlashPrefillCtx, FlashTreeCtx
+from deserve_amd.model.context.flash import FlashDecodeCtx, FlashForwardCtx, FlashPrefillCtx, FlashQuantCtx, FlashTreeCtx
 from deserve_amd.paged_ops import (BatchDecodeWithPagedKVCacheWrapper, BatchPrefillWithPagedKVCacheWrapper,
                                    append_paged_kv_cache, apply_rope, rope_append_paged_kv_cache)
+from deserve_amd.quant_ops import BatchQuantizedWithPagedKVCacheWrapper, rope_append_quantized
 
 
 class PagedAttentionCore:
@@ -85,6 +86,14 @@ class PagedAttentionCore:
         xk = self._rows(xk, self.n_local_kv_heads)
         xv = self._rows(xv, self.n_local_kv_heads)
         pages = ctx.page_pool.get_layered_pages(ctx.layer_id)
+        quantized = ctx.quant_wrapper if isinstance(ctx, FlashQuantCtx) else \
+            ctx.tree_wrapper if isinstance(ctx, FlashTreeCtx) else None
+        if isinstance(quantized, BatchQuantizedWithPagedKVCacheWrapper):
+            # 8-bit pages: every kind of step is an append that makes codes, and one attention
+            table = ctx.rope_table(xq.shape[0], self.head_dim, self.rope_theta) if self.use_rope else None
+            xq = rope_append_quantized(xq, xk, xv, ctx.indptr, pages, ctx.kv_page_indices, ctx.kv_page_indptr,
+                                       ctx.kv_last_page_lens, ctx.page_pool.page_size, table)
+            return quantized.forward(xq, pages, out=out).view(-1, self.dim)
         if isinstance(ctx, FlashTreeCtx):
             # the rows' slots and positions are the step's tables
             table = ctx.rope_table(xq.shape[0], self.head_dim, self.rope_theta) if self.use_rope else None
