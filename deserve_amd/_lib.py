@@ -76,7 +76,7 @@ class QuantRows(ctypes.Structure):
 
 class QuantStep(ctypes.Structure):
     """dskv_quant_step_t of include/dskv.h."""
-    _fields_ = [("step", TreeStep), ("min_qo_len", c_int32)]
+    _fields_ = [("step", TreeStep), ("counters", c_void_p), ("n_counters", c_int64), ("min_qo_len", c_int32)]
 
 
 _lib: Optional[ctypes.CDLL] = None
@@ -172,6 +172,7 @@ _SIGNATURES = {
     "dskv_rope_append_quant": (c_int32, [POINTER(QuantRows)] + [c_void_p] * 5 + [c_int64] * 3 +
                                [c_void_p, c_int32, c_int32, c_void_p]),
     "dskv_quant_attn_workspace": (c_int64, [c_int32] * 7),
+    "dskv_quant_attn_counters": (c_int64, [c_int32]),
     "dskv_quant_attn": (c_int32, [POINTER(QuantStep), c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
     "dskv_move_quant_rows": (c_int32, [POINTER(QuantRows), c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_void_p]),
     "dskv_swap_slice": (c_int32, [c_void_p, c_int64, c_int64, c_int32, c_void_p, c_void_p,

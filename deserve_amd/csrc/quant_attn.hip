@@ -3,6 +3,8 @@
 // away by the mask, no others.  V codes are numbers.
 #include "quant_wide_kernel.h"
 
+#include <algorithm>
+
 namespace dskv {
 
 // Any type and head dim: one workgroup per (row, q head) whose waves take every kQuantWaves-th group of four keys.  Lane
@@ -128,44 +130,38 @@ static QuantForm quant_form(bool wide, int max_rows, int n_qo_heads, int n_kv_he
     f.sides = wide && f.col_tiles > 1 && f.shares % (8 * f.col_tiles) == 0 ? f.col_tiles : 1;
     return f;
 }
-// Requests of so many rows and fewer are the narrow form's, the others the wide one's, which reads K and V once for all columns
-// (never fewer than one: a request of more columns a row than the narrow form's tiles hold is in several of these).
-static int narrow_rows(int n_qo_heads, int n_kv_heads, int dtype)
+// Requests of so many rows and fewer are the narrow form's (never fewer than one: a request of more columns a row than its tiles
+// hold is in several of them), the others the wide one's, which reads K and V once for all columns.  Where a step has both, those for one block of
+// 16 columns: beside a chunk they are decode rows, which would be padded to three.
+static int narrow_rows(int max_rows, int n_qo_heads, int n_kv_heads, int dtype)
 {
     if (dtype == DSKV_F32) return INT32_MAX;
-    const int rows = quant_columns(dtype) / (n_qo_heads / n_kv_heads);
-    return rows > 1 ? rows : 1;
+    const int group = n_qo_heads / n_kv_heads, all = std::max(quant_columns(dtype) / group, 1);
+    return max_rows <= all ? all : std::max(16 / group, 1);
 }
 static int64_t units_bytes(int batch) { return ((int64_t)batch + 7) / 4 * 16; }
 static int64_t slots_of(const QuantForm &f, int n_kv_heads) { return 2LL * f.shares * n_kv_heads * f.cols; }
+static int64_t cuts_bytes(const QuantForm &f) { return (2LL * f.shares * (int64_t)sizeof(QuantCut) + 15) / 16 * 16; }
 static int64_t form_bytes(const QuantForm &f, int batch, int n_kv_heads, int head_dim)
 {
-    return units_bytes(batch) + slots_of(f, n_kv_heads) * (head_dim + 2) * (int64_t)sizeof(float);
+    return units_bytes(batch) + cuts_bytes(f) + slots_of(f, n_kv_heads) * (head_dim + 2) * (int64_t)sizeof(float);
 }
 
-template <int DT, int kD, int kCols, int kSub> static int launch_quant_merge(const QuantArgs &a, const QuantForm &f, hipStream_t stream)
-{
-    const bool many_parts = (long)a.batch * f.col_tiles * 4 < f.shares;
-    constexpr int kEach = kCols >= 128 ? 4 : 1;
-    const int columns = 256 / (kD / 4) * (many_parts ? 1 : kEach) / (many_parts ? 4 : 1);
-    const dim3 grid((unsigned)(a.batch * f.col_tiles), (unsigned)a.n_kv_heads, (unsigned)((kCols + columns - 1) / columns));
-    if (many_parts) hipLaunchKernelGGL((tree_merge_kernel<DT, kD, kCols, kSub, 4, 1, QuantArgs>), grid, dim3(256), 0, stream, a, f.col_tiles);
-    else hipLaunchKernelGGL((tree_merge_kernel<DT, kD, kCols, kSub, 1, kEach, QuantArgs>), grid, dim3(256), 0, stream, a, f.col_tiles);
-    DSKV_LAUNCH_CHECK("tree_merge_kernel");
-    return 0;
-}
 template <int DT, int kD, int kBlocks> static int launch_quant(const QuantArgs &a, const QuantForm &f, hipStream_t stream)
 {
-    typedef QuantTile<DT, kD, kBlocks> S;
     hipLaunchKernelGGL((quant_matrix_kernel<DT, kD, kBlocks>), dim3((unsigned)(f.shares * a.n_kv_heads)), dim3(kTreeThreads), 0, stream, a);
     DSKV_LAUNCH_CHECK("quant_matrix_kernel");
-    return launch_quant_merge<DT, kD, S::kCols, S::kSub>(a, f, stream);
+    return 0;
 }
 template <int DT, int kD, int kWaves> static int launch_quant_wide(const QuantArgs &a, const QuantForm &f, hipStream_t stream)
 {
     hipLaunchKernelGGL((quant_wide_kernel<DT, kD, kWaves>), dim3((unsigned)(f.shares * a.n_kv_heads)), dim3(kWaves * 64), 0, stream, a);
     DSKV_LAUNCH_CHECK("quant_wide_kernel");
-    return launch_quant_merge<DT, kD, kWaves * 32, kWideBlock>(a, f, stream);
+    constexpr int kColumns = 256 / (kD / 4) * kMergeEach;                // of a workgroup
+    const dim3 grid((unsigned)(2 * f.shares), (unsigned)a.n_kv_heads, (unsigned)((kWaves * 32 + kColumns - 1) / kColumns));
+    hipLaunchKernelGGL((quant_merge_kernel<DT, kD, kWaves * 32>), grid, dim3(256), 0, stream, a);
+    DSKV_LAUNCH_CHECK("quant_merge_kernel");
+    return 0;
 }
 template <int DT, int kD> static int launch_quant_blocks(const QuantArgs &a, const QuantForm &f, hipStream_t stream)
 {
@@ -190,7 +186,8 @@ template <int DT> static int launch_quant_dim(const QuantArgs &a, const QuantFor
 static int launch_quant_form(QuantArgs a, const QuantForm &f, int dtype, int rows_from, int rows_to, void *workspace, hipStream_t stream)
 {
     a.units_before = (int32_t *)workspace;
-    a.part_o = (float *)((char *)workspace + units_bytes(a.batch));
+    a.cuts = (QuantCut *)((char *)workspace + units_bytes(a.batch));
+    a.part_o = (float *)((char *)a.cuts + cuts_bytes(f));
     a.part_ml = a.part_o + slots_of(f, a.n_kv_heads) * a.head_dim;
     a.n_shares = f.shares;
     a.sides = f.sides;
@@ -208,12 +205,18 @@ extern "C" int64_t dskv_quant_attn_workspace(int32_t batch, int32_t nnz, int32_t
 {
     using namespace dskv;
     if (batch <= 0 || nnz <= 0 || max_qo_len <= 0 || n_kv_heads <= 0 || n_qo_heads < n_kv_heads || !quant_matrix_form(head_dim)) return 0;
-    const int narrow_most = narrow_rows(n_qo_heads, n_kv_heads, dtype);
+    const int narrow_most = narrow_rows(max_qo_len, n_qo_heads, n_kv_heads, dtype);
     const int64_t narrow = form_bytes(quant_form(false, max_qo_len < narrow_most ? max_qo_len : narrow_most, n_qo_heads, n_kv_heads, dtype),
                                       batch, n_kv_heads, head_dim);
     if (max_qo_len <= narrow_most) return narrow;
     const int64_t wide = form_bytes(quant_form(true, max_qo_len, n_qo_heads, n_kv_heads, dtype), batch, n_kv_heads, head_dim);
     return narrow > wide ? narrow : wide;
+}
+
+// two for each share and kv head: workgroups are two a compute unit at most, or one for each head
+extern "C" int64_t dskv_quant_attn_counters(int32_t n_kv_heads)
+{
+    return n_kv_heads <= 0 ? 0 : 2 * (int64_t)std::max(2 * dskv::kQuantUnits, (int)n_kv_heads);
 }
 
 extern "C" int dskv_quant_attn(const dskv_quant_step_t *step, void *out, const void *q, int64_t q_stride,
@@ -250,7 +253,7 @@ extern "C" int dskv_quant_attn(const dskv_quant_step_t *step, void *out, const v
     a.page_bytes = shape.page_bytes;
     hipStream_t st = (hipStream_t)stream;
     // two launches where some requests have few rows and others many, one after the other over the same workspace
-    const int narrow_most = narrow_rows(s->n_qo_heads, s->n_kv_heads, s->dtype);
+    const int narrow_most = narrow_rows(s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->dtype);
     const bool some_narrow = step->min_qo_len <= narrow_most, some_wide = s->max_qo_len > narrow_most;
     const QuantForm narrow = quant_form(false, some_wide ? narrow_most : s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->dtype);
     const QuantForm wide = quant_form(true, s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->dtype);
@@ -266,6 +269,12 @@ extern "C" int dskv_quant_attn(const dskv_quant_step_t *step, void *out, const v
         }
         DSKV_REQUIRE((uintptr_t)s->workspace % 16 == 0, "quant_attn: the workspace must be 16-byte aligned");
         DSKV_REQUIRE((int64_t)s->batch * col_tiles < INT32_MAX && s->n_kv_heads <= 65535, "quant_attn: too large a batch");
+        if (!step->counters || step->n_counters < dskv_quant_attn_counters(s->n_kv_heads)) {
+            set_error("quant_attn: %lld counters, %lld are needed", (long long)step->n_counters, (long long)dskv_quant_attn_counters(s->n_kv_heads));
+            return DSKV_E_NOMEM;
+        }
+        DSKV_REQUIRE((uintptr_t)step->counters % 4 == 0, "quant_attn: the counters must be 4-byte aligned");
+        a.counters = step->counters;
         a.group = s->n_qo_heads / s->n_kv_heads;
         a.page_shift = 31 + ilog2(s->page_size);
         a.page_magic = (uint32_t)(((1ull << a.page_shift) + s->page_size - 1) / s->page_size);

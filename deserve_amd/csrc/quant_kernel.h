@@ -17,6 +17,8 @@ namespace dskv {
 struct QuantArgs : TreeArgs {
     long head_bytes, half_bytes, page_bytes;      // see quant.h
     uint32_t page16, row16;                       // bytes of a page and of a token's row, in sixteens
+    uint32_t *counters;                           // narrow form: one for each partial and kv head; zero between launches
+    struct QuantCut *cuts;                        // wide form: two for each share
     int rows_from, rows_to;                       // rows of a request that this launch computes, 0 of any other's
 };
 __device__ __forceinline__ int rows_taken(const QuantArgs &a, int n) { return n >= a.rows_from && n <= a.rows_to ? n : 0; }
@@ -27,6 +29,122 @@ __device__ __forceinline__ uint32_t quant_row(const QuantArgs &a, int t, int pag
 {
     return page >= 0 && page < a.num_pages ? (uint32_t)page * a.page16 + (uint32_t)(t - page_number(a, t) * a.page_size) * a.row16
                                            : kNoQuantRow;
+}
+
+// ---- Items that share boundaries cut leave a partial (maximum, sum, O in fp32, for every column) for each part.
+struct QuantParts {
+    int first, n;        // shares (spans) that hold a part; n == 1: not cut
+    bool second;         // in the first of them the item is the second
+    uint32_t slot;       // of the first
+};
+__device__ __forceinline__ uint32_t part_slot(const QuantArgs &a, const TreePlace &place, const QuantParts &p, int ct, int i)
+{
+    const int span = p.first + i, share = place.beside ? share_of_span(span, ct, a.sides) : span;
+    return 2u * (uint32_t)share + (i == 0 && p.second ? 1u : 0u);
+}
+// item: its first unit, of `units`.
+__device__ __forceinline__ QuantParts parts_of(const QuantArgs &a, const TreePlace &place, int item, int units, int ct)
+{
+    QuantParts p = {place.first_part, place.n_parts, false, 0};
+    if (p.n == 0) {
+        Shares s = place.shares;
+        s.each = __builtin_amdgcn_readfirstlane(s.each);
+        s.longer = __builtin_amdgcn_readfirstlane(s.longer);
+        p.first = share_with(s, item);
+        p.n = share_with(s, item + units - 1) - p.first + 1;
+        p.second = share_begin(s, p.first) < item;
+    }
+    p.slot = part_slot(a, place, p, ct, 0);
+    return p;
+}
+// The narrow form's parts are merged in the launch: partials are stored with device scope, a part whose stores are acknowledged counts itself
+// in, and the one that completes the count reads all of them, past its XCD's L2, and writes the rows.  The order of the sums does not depend on
+// which that is.  (A launch of its own: one request over 1.8 K tokens 15.0 us, so 12.3.  With the wide form's 133 KB a part that is too much for one
+// workgroup: 16 chunks 983 us, with a launch of its own 941.)
+constexpr int kDeviceScope = 16;                                   // cache policy of the buffer instructions: sc1
+template <int kCols, int kD> struct PartSlot {
+    __amdgpu_buffer_rsrc_t o, ml;
+    __device__ __forceinline__ PartSlot(const QuantArgs &a, int head, uint32_t slot)
+    {
+        const long part = ((long)slot * a.n_kv_heads + head) * kCols;
+        o = __builtin_amdgcn_make_buffer_rsrc(a.part_o + part * kD, 0, kCols * kD * 4, kBufferFlags);
+        ml = __builtin_amdgcn_make_buffer_rsrc(a.part_ml + part * 2, 0, kCols * 8, kBufferFlags);
+    }
+    __device__ __forceinline__ void put_o(int col, int dim, f32x4 v) const
+    {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), o, (col * kD + dim) * 4, 0, kDeviceScope);
+    }
+    __device__ __forceinline__ void put_ml(int col, float m, float l) const
+    {
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, f32x2{m, l}), ml, col * 8, 0, kDeviceScope);
+    }
+    __device__ __forceinline__ f32x4 get_o(int col, int dim) const
+    {
+        return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(o, (col * kD + dim) * 4, 0, kDeviceScope));
+    }
+    __device__ __forceinline__ f32x2 get_ml(int col) const
+    {
+        return __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(ml, col * 8, 0, kDeviceScope));
+    }
+};
+// Four dims of a column's row.
+template <int DT, int kD>
+__device__ __forceinline__ void put_result(const QuantArgs &a, const TreeRequest &r, int head, int at, int dim, f32x4 acc, float sum)
+{
+    constexpr int kElt = DT == DSKV_F32 ? 4 : 2;
+    const int i = (int)((unsigned)at / (unsigned)a.group), hq = head * a.group + at - i * a.group;
+    const float inv = sum == 0 ? 0.f : 1.f / sum;
+    char *dst = a.out + (((r.first + i) * a.n_qo_heads + hq) * kD + dim) * kElt;
+    if constexpr (DT == DSKV_F32) *reinterpret_cast<f32x4 *>(dst) = acc * inv;
+    else *reinterpret_cast<u32x2 *>(dst) = u32x2{Elt<DT>::pack2(acc.x * inv, acc.y * inv), Elt<DT>::pack2(acc.z * inv, acc.w * inv)};
+}
+// By all threads of a workgroup, behind its stores of a part's partial.  last: a word of LDS.
+template <int DT, int kD, int kCols, int kThreads, int kAtOnce>
+__device__ __forceinline__ void join_parts(const QuantArgs &a, const TreePlace &place, const TreeRequest &r, const QuantParts &p,
+                                           int head, int ct, int col0, int cols, int *last)
+{
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");               // the partial is where other XCDs see it
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        uint32_t *const counter = a.counters + (long)p.slot * a.n_kv_heads + head;
+        const uint32_t before = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *last = before + 1 == (uint32_t)p.n;
+        if (before + 1 == (uint32_t)p.n) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!*last) return;
+    asm volatile("" ::: "memory");
+    constexpr int kQuads = kD / 4;
+    for (int x = threadIdx.x; x < cols * kQuads; x += kThreads) {
+        const int col = x / kQuads, dim = x % kQuads * 4;
+        float top = -INFINITY, sum = 0;
+        f32x4 acc = {0, 0, 0, 0};
+        for (int i0 = 0; i0 < p.n; i0 += kAtOnce) {
+            f32x4 o[kAtOnce];
+            f32x2 ml[kAtOnce];
+#pragma unroll
+            for (int i = 0; i < kAtOnce; i++) {
+                const PartSlot<kCols, kD> part(a, head, part_slot(a, place, p, ct, min(i0 + i, p.n - 1)));
+                ml[i] = part.get_ml(col);
+                o[i] = part.get_o(col, dim);
+            }
+            float m = top;
+#pragma unroll
+            for (int i = 0; i < kAtOnce; i++) m = fmaxf(m, ml[i].x);
+            const float from = m == -INFINITY ? 0.f : m, keep = __builtin_amdgcn_exp2f(top - from);
+            top = m;
+            sum *= keep;
+            acc *= keep;
+#pragma unroll
+            for (int i = 0; i < kAtOnce; i++)
+                if (i0 + i < p.n) {
+                    const float w = __builtin_amdgcn_exp2f(ml[i].x - from);
+                    sum += ml[i].y * w;
+                    acc += o[i] * w;
+                }
+        }
+        put_result<DT, kD>(a, r, head, col0 + col, dim, acc, sum);
+    }
 }
 
 // 8 codes as a matrix operand of type T
@@ -93,6 +211,7 @@ __global__ __launch_bounds__(kTreeThreads, (QuantTile<DT, kD, kBlocks>::kWorkgro
 {
     typedef QuantTile<DT, kD, kBlocks> S;
     __shared__ __align__(16) char lds[S::kLds];
+    __shared__ int last_part;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, c = lane & 15;
     int share, head;
@@ -368,8 +487,7 @@ __global__ __launch_bounds__(kTreeThreads, (QuantTile<DT, kD, kBlocks>::kWorkgro
         }
         __syncthreads();
         const bool cut = it.st0 > 0 || it.st1 < it.r.subtiles;
-        const long slot = 2L * share + (it.first ? 0 : 1);
-        const long part = (slot * a.n_kv_heads + head) * S::kCols;
+        const PartSlot<S::kCols, kD> part(a, head, 2u * (uint32_t)share + (it.first ? 0u : 1u));
         constexpr int kQuads = kD / 4;
         for (int x = threadIdx.x; x < cols * kQuads; x += kTreeThreads) {
             const int col = x / kQuads, quad = x % kQuads;
@@ -385,18 +503,16 @@ __global__ __launch_bounds__(kTreeThreads, (QuantTile<DT, kD, kBlocks>::kWorkgro
                 acc += *reinterpret_cast<const f32x4 *>(o_lds + (w * S::kCols + col) * S::kOPitch + quad * 4) * weight;
             }
             if (cut) {
-                *reinterpret_cast<f32x4 *>(a.part_o + (part + col) * kD + quad * 4) = acc;
-                if (quad == 0) {
-                    a.part_ml[(part + col) * 2] = top;
-                    a.part_ml[(part + col) * 2 + 1] = sum;
-                }
+                part.put_o(col, quad * 4, acc);
+                if (quad == 0) part.put_ml(col, top, sum);
             } else {
-                const int at = it.ct * S::kCols + col, i = (int)((unsigned)at / (unsigned)a.group), hq = head * a.group + at - i * a.group;
-                const float inv = sum == 0 ? 0.f : 1.f / sum;
-                char *dst = a.out + (((it.r.first + i) * a.n_qo_heads + hq) * kD + quad * 4) * S::kElt;
-                if constexpr (DT == DSKV_F32) *reinterpret_cast<f32x4 *>(dst) = acc * inv;
-                else *reinterpret_cast<u32x2 *>(dst) = u32x2{Elt<DT>::pack2(acc.x * inv, acc.y * inv), Elt<DT>::pack2(acc.z * inv, acc.w * inv)};
+                put_result<DT, kD>(a, it.r, head, it.ct * S::kCols + col, quad * 4, acc, sum);
             }
+        }
+        if (cut) {
+            const int item = it.base + it.ct * it.r.subtiles;
+            join_parts<DT, kD, S::kCols, kTreeThreads, 8>(a, place, it.r, parts_of(a, place, item, it.r.subtiles, it.ct), head, it.ct,
+                                                          it.ct * S::kCols, cols, &last_part);
         }
         __syncthreads();
     };

@@ -16,6 +16,7 @@
 
 namespace dskv {
 
+constexpr int kMergeEach = 4;                // columns that a thread of the merge launch takes
 constexpr int kWideBlock = 32;
 constexpr int kWideRegion = 1088;           // 64 lanes' 16 bytes, (4 chunk + row) * 16 of four rows, and 64 bytes of padding
 constexpr int kWideStage = kWideBlock / 4 * kWideRegion;
@@ -34,6 +35,12 @@ template <int kD, int kWaves> struct QuantWide {
     static constexpr int kAhead = 2;                     // stages of K, and of V, on their way in registers
     // what turn u (in front of the iterations of stage u) writes: K(u + kFirst) and V(u + kBehind)
     static constexpr int kFirst = kPack == 2 ? 2 : 3, kBehind = kPack - 1;
+};
+
+// An item that begins in a share and ends in another.
+struct QuantCut {
+    int b, ct;
+    QuantParts parts;    // n < 2: none
 };
 
 template <int DT, int kD, int kWaves>
@@ -58,6 +65,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void quant_wide_kernel(QuantArgs a)
     int unit = begin, base = place.base;
     int b = place.b;
     TreeRequest r = place.r;
+    if (head == 0 && threadIdx.x < 2) a.cuts[2 * share + threadIdx.x].parts.n = 0;
 
     auto k_stage = [&](int i) { return lds + (i & (W::kKStages - 1)) * kWideStage; };
     auto v_stage = [&](int i) { return lds + (W::kKStages + (i & (W::kVStages - 1))) * kWideStage; };
@@ -152,33 +160,39 @@ __global__ __launch_bounds__(kWaves * 64, 2) void quant_wide_kernel(QuantArgs a)
             return (block_of(u) & (2 * W::kHalf - 1)) * kWideBlock + (wave * W::kGroups + i) * 4 + (lane & 3);
         };
         u32x2 k_codes[W::kAhead][W::kGroups], v_codes[W::kAhead][W::kGroups];
-        auto request = [&](int u, u32x2 (&codes)[W::kGroups], long more) {
-#pragma unroll
-            for (int i = 0; i < W::kGroups; i++) {
-                const uint32_t row = block_of(u) < blocks ? row_at[token_of(u, i)] : kNoQuantRow;
-                const char *p = pool + (uint64_t)row * 16 + more;
-                p = row != kNoQuantRow ? p : none;
-                codes[i] = *(const __attribute__((address_space(1))) u32x2 *)p;
-            }
+        auto request = [&](uint32_t row, u32x2 &codes, long more) {
+            const char *p = pool + (uint64_t)row * 16 + more;
+            p = row != kNoQuantRow ? p : none;
+            codes = *(const __attribute__((address_space(1))) u32x2 *)p;
         };
-        auto write = [&](const u32x2 (&codes)[W::kGroups], int u, char *stage, int shift) {
+        auto write = [&](u32x2 codes, uint32_t exponent, int i, char *stage) {
+            const float scale = __builtin_bit_cast(float, exponent << 23);
+            u32x4 x;
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+                if constexpr (DT == DSKV_F16) {
+                    x[2 * w] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[w], scale, false));
+                    x[2 * w + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[w], scale, true));
+                } else {
+                    x[2 * w] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[w], scale, false));
+                    x[2 * w + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[w], scale, true));
+                }
+            }
+            *reinterpret_cast<u32x4 *>(stage + (wave * W::kGroups + i) * kWideRegion + lane * 16) = x;
+        };
+        // what turn u needs of the tables: exponents of what it writes, places of what it requests
+        struct Known {
+            uint8_t k_exponent[W::kGroups], v_exponent[W::kGroups];
+            uint32_t k_row[W::kGroups], v_row[W::kGroups];
+        };
+        const uint8_t *const exponent_at = reinterpret_cast<const uint8_t *>(scale_at);
+        auto know = [&](int u, Known &x) {
 #pragma unroll
             for (int i = 0; i < W::kGroups; i++) {
-                // (behind the walk nothing was looked up, and the codes are zeros)
-                const uint32_t exponent = block_of(u) < blocks ? (uint32_t)scale_at[token_of(u, i)] >> shift & 0xFF : 127u;
-                const float scale = __builtin_bit_cast(float, exponent << 23);
-                u32x4 x;
-#pragma unroll
-                for (int w = 0; w < 2; w++) {
-                    if constexpr (DT == DSKV_F16) {
-                        x[2 * w] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[i][w], scale, false));
-                        x[2 * w + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[i][w], scale, true));
-                    } else {
-                        x[2 * w] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[i][w], scale, false));
-                        x[2 * w + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[i][w], scale, true));
-                    }
-                }
-                *reinterpret_cast<u32x4 *>(stage + (wave * W::kGroups + i) * kWideRegion + lane * 16) = x;
+                x.k_exponent[i] = exponent_at[2 * token_of(u + W::kFirst, i)];
+                x.v_exponent[i] = exponent_at[2 * token_of(u + W::kBehind, i) + 1];
+                x.k_row[i] = row_at[token_of(u + W::kFirst + W::kAhead, i)];
+                x.v_row[i] = row_at[token_of(u + W::kBehind + W::kAhead, i)];
             }
         };
 
@@ -247,20 +261,29 @@ __global__ __launch_bounds__(kWaves * 64, 2) void quant_wide_kernel(QuantArgs a)
         asm volatile("" : "+v"(mask));
         // as if there were turns in front
 #pragma unroll
-        for (int i = 0; i < W::kAhead; i++) {
-            request(i, k_codes[i], 0);
-            request(i, v_codes[i], a.half_bytes);
-        }
+        for (int u = 0; u < W::kAhead; u++)
 #pragma unroll
-        for (int i = 0; i < W::kFirst; i++) {
-            write(k_codes[i % W::kAhead], i, k_stage(i), 0);
-            request(W::kAhead + i, k_codes[i % W::kAhead], 0);
-        }
+            for (int i = 0; i < W::kGroups; i++) {
+                const uint32_t row = row_at[token_of(u, i)];
+                request(row, k_codes[u][i], 0);
+                request(row, v_codes[u][i], a.half_bytes);
+            }
 #pragma unroll
-        for (int i = 0; i < W::kBehind; i++) {
-            write(v_codes[i], i, v_stage(i), 8);
-            request(W::kAhead + i, v_codes[i], a.half_bytes);
-        }
+        for (int u = 0; u < W::kFirst; u++)
+#pragma unroll
+            for (int i = 0; i < W::kGroups; i++) {
+                write(k_codes[u % W::kAhead][i], exponent_at[2 * token_of(u, i)], i, k_stage(u));
+                request(row_at[token_of(u + W::kAhead, i)], k_codes[u % W::kAhead][i], 0);
+            }
+#pragma unroll
+        for (int u = 0; u < W::kBehind; u++)
+#pragma unroll
+            for (int i = 0; i < W::kGroups; i++) {
+                write(v_codes[u][i], exponent_at[2 * token_of(u, i) + 1], i, v_stage(u));
+                request(row_at[token_of(u + W::kAhead, i)], v_codes[u][i], a.half_bytes);
+            }
+        Known known;
+        know(0, known);
         __syncthreads();
         if (works) {
             read_keys(block_at(k_stage, 0));
@@ -272,17 +295,26 @@ __global__ __launch_bounds__(kWaves * 64, 2) void quant_wide_kernel(QuantArgs a)
         auto turn = [&](int u, int phase) {
             constexpr int kMask = W::kAhead - 1;
             const int k_at = (phase + W::kFirst) & kMask, v_at = (phase + W::kBehind) & kMask;
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
-            write(k_codes[k_at], u + W::kFirst, k_stage(u + W::kFirst), 0);
-            write(v_codes[v_at], u + W::kBehind, v_stage(u + W::kBehind), 8);
-            request(u + W::kFirst + W::kAhead, k_codes[k_at], 0);
-            request(u + W::kBehind + W::kAhead, v_codes[v_at], a.half_bytes);
+#pragma unroll
+            for (int i = 0; i < W::kGroups; i++) {
+                write(k_codes[k_at][i], known.k_exponent[i], i, k_stage(u + W::kFirst));
+                write(v_codes[v_at][i], known.v_exponent[i], i, v_stage(u + W::kBehind));
+                request(known.k_row[i], k_codes[k_at][i], 0);
+                request(known.v_row[i], v_codes[v_at][i], a.half_bytes);
+            }
+            know(u + 1, known);
+        };
+        auto meet = [&](int phase) {
+            const bool turns = W::kPack == 1 || (phase & 1) == 0;
+            if (turns) {
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+            }
+            return turns;
         };
         auto iteration = [&](int j, int phase) {
-            if (W::kPack == 1 || (phase & 1) == 0) turn(j / W::kPack, phase / W::kPack);
-            if (!works || j > blocks) return;
+            const bool turns = meet(phase);
             const int cur = phase & 1, nxt = cur ^ 1;
             const char *rows = block_at(v_stage, j - 1) + v_off;                        // V(j - 1)
             u32x4 va[W::kDims][2];
@@ -295,6 +327,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void quant_wide_kernel(QuantArgs a)
                     va[d][s] = u32x4{lo.x, lo.y, hi.x, hi.y};
                 }
             scores(xs[nxt]);                                                        // S(j + 1)
+            if (turns) turn(j / W::kPack, phase / W::kPack);
             float sum = 0;
             weights(xs[cur], 0, pb[cur][0], sum);
             if ((st0 + j + 2) * kWideBlock > mask_from) mask_scores(j + 1, xs[nxt]);
@@ -313,13 +346,32 @@ __global__ __launch_bounds__(kWaves * 64, 2) void quant_wide_kernel(QuantArgs a)
             }
             l_run += sum;
         };
-        for (int j = 0; j <= blocks; j += 4) {
-            if (j % W::kHalf == W::kHalf / 2 && j + W::kHalf / 2 < blocks) look_up(j / W::kHalf + 1);
-            iteration(j, 0);
-            if (holes) mask_from = 0;
-            iteration(j + 1, 1);
-            iteration(j + 2, 2);
-            iteration(j + 3, 3);
+        auto look_ahead = [&](int j) {                   // (the turns look up to 12 blocks behind the last one, too)
+            if (j % W::kHalf == W::kHalf / 2 && j + W::kHalf / 2 < blocks + 16) look_up(j / W::kHalf + 1);
+        };
+        if (works) {
+            for (int j = 0;; j += 4) {
+                look_ahead(j);
+                iteration(j, 0);
+                if (holes) mask_from = 0;
+                if (j >= blocks) break;
+                iteration(j + 1, 1);
+                if (j + 1 >= blocks) break;
+                iteration(j + 2, 2);
+                if (j + 2 >= blocks) break;
+                iteration(j + 3, 3);
+                if (j + 3 >= blocks) break;
+            }
+        } else {
+            // a wave without columns only fetches
+            auto passes = [&](int j, int phase) {
+                if (meet(phase)) turn(j / W::kPack, phase / W::kPack);
+                return j >= blocks;
+            };
+            for (int j = 0;; j += 4) {
+                look_ahead(j);
+                if (passes(j, 0) || passes(j + 1, 1) || passes(j + 2, 2) || passes(j + 3, 3)) break;
+            }
         }
 
         // ---- the item's result
@@ -328,18 +380,14 @@ __global__ __launch_bounds__(kWaves * 64, 2) void quant_wide_kernel(QuantArgs a)
         const float l = l_run + l_other;
         const bool cut = st0 > 0 || st1 < r.subtiles;
         if (there && cut) {
-            const long slot = 2L * share + (unit > begin ? 1 : 0);
-            const long part = (slot * a.n_kv_heads + head) * W::kCols + wave * 32 + r32;
+            const long part = ((2L * share + (unit > begin ? 1 : 0)) * a.n_kv_heads + head) * W::kCols + wave * 32 + r32;
 #pragma unroll
             for (int d = 0; d < W::kDims; d++)
 #pragma unroll
                 for (int i = 0; i < 4; i++)
                     *reinterpret_cast<f32x4 *>(a.part_o + part * kD + d * 32 + 8 * i + 4 * h) =
                         f32x4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
-            if (h == 0) {
-                a.part_ml[part * 2] = m_run;
-                a.part_ml[part * 2 + 1] = l;
-            }
+            if (h == 0) *reinterpret_cast<f32x2 *>(a.part_ml + part * 2) = f32x2{m_run, l};
         } else if (there) {
             const float inv = l == 0 ? 0.f : 1.f / l;
             char *dst = a.out + ((q_row * a.n_qo_heads + hq) * kD + 4 * h) * 2;
@@ -351,8 +399,74 @@ __global__ __launch_bounds__(kWaves * 64, 2) void quant_wide_kernel(QuantArgs a)
                         u32x2{E::pack2(acc[d][4 * i] * inv, acc[d][4 * i + 1] * inv),
                               E::pack2(acc[d][4 * i + 2] * inv, acc[d][4 * i + 3] * inv)};
         }
+        // an item that goes on in another share is the merge launch's
+        if (cut && st0 == 0 && head == 0 && threadIdx.x == 0) a.cuts[2 * share + (unit > begin ? 1 : 0)] = {b, ct, parts_of(a, place, item, r.subtiles, ct)};
         unit = item + st1;
     }
+}
+
+// Items that were cut, two for each share that they begin in: a thread per four dims of kEach columns, workgroups along the columns.
+template <int DT, int kD, int kCols>
+__global__ __launch_bounds__(256) void quant_merge_kernel(QuantArgs a)
+{
+    constexpr int kQuads = kD / 4, kColumns = 256 / kQuads, kEach = kMergeEach, kAhead = 2;       // columns side by side, a thread's, parts requested together
+    const QuantCut cut = a.cuts[blockIdx.x];
+    if (cut.parts.n < 2) return;
+    const int head = blockIdx.y, quad = threadIdx.x % kQuads, column = threadIdx.x / kQuads;
+    const TreeRequest r = tree_request<kCols, kWideBlock>(a, cut.b);
+    const int cols = min(r.n * a.group - cut.ct * r.tile, r.tile), col0 = (int)blockIdx.z * kColumns * kEach + column;
+    if ((int)blockIdx.z * kColumns * kEach >= cols) return;
+    const bool beside = a.units_before[a.batch + 1] != 0;
+    TreePlace place;
+    place.beside = beside;
+    float top[kEach], sum[kEach];
+    f32x4 acc[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; e++) {
+        top[e] = -INFINITY;
+        sum[e] = 0;
+        acc[e] = f32x4{0, 0, 0, 0};
+    }
+    for (int i0 = 0; i0 < cut.parts.n; i0 += kAhead) {
+        f32x4 o[kAhead][kEach];
+        f32x2 ml[kAhead][kEach];
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) {
+#pragma unroll
+            for (int e = 0; e < kEach; e++) {
+                ml[i][e] = f32x2{-INFINITY, 0};
+                o[i][e] = f32x4{0, 0, 0, 0};
+            }
+            if (i0 + i >= cut.parts.n) continue;
+            const long slot = part_slot(a, place, cut.parts, cut.ct, i0 + i);
+#pragma unroll
+            for (int e = 0; e < kEach; e++) {
+                const long part = (slot * a.n_kv_heads + head) * kCols + min(col0 + e * kColumns, cols - 1);
+                ml[i][e] = *reinterpret_cast<const f32x2 *>(a.part_ml + part * 2);
+                o[i][e] = *reinterpret_cast<const f32x4 *>(a.part_o + part * kD + quad * 4);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < kEach; e++) {
+            float m = top[e];
+#pragma unroll
+            for (int i = 0; i < kAhead; i++) m = fmaxf(m, ml[i][e].x);
+            const float keep = __builtin_amdgcn_exp2f(top[e] - m);
+            top[e] = m;
+            sum[e] *= keep;
+            acc[e] *= keep;
+#pragma unroll
+            for (int i = 0; i < kAhead; i++)
+                if (i0 + i < cut.parts.n) {
+                    const float w = __builtin_amdgcn_exp2f(ml[i][e].x - m);
+                    sum[e] += ml[i][e].y * w;
+                    acc[e] += o[i][e] * w;
+                }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < kEach; e++)
+        if (col0 + e * kColumns < cols) put_result<DT, kD>(a, r, head, cut.ct * r.tile + col0 + e * kColumns, quad * 4, acc[e], sum[e]);
 }
 
 }  // namespace dskv

@@ -161,8 +161,8 @@ template <int DT, int kD, int kCols, int kSub> static int launch_tree_merge(cons
     constexpr int kEach = kCols >= 128 ? 4 : 1;
     const int columns = 256 / (kD / 4) * (many_parts ? 1 : kEach) / (many_parts ? 4 : 1);
     const dim3 grid((unsigned)(a.batch * f.col_tiles), (unsigned)a.n_kv_heads, (unsigned)((kCols + columns - 1) / columns));
-    if (many_parts) hipLaunchKernelGGL((tree_merge_kernel<DT, kD, kCols, kSub, 4, 1, TreeArgs>), grid, dim3(256), 0, stream, a, f.col_tiles);
-    else hipLaunchKernelGGL((tree_merge_kernel<DT, kD, kCols, kSub, 1, kEach, TreeArgs>), grid, dim3(256), 0, stream, a, f.col_tiles);
+    if (many_parts) hipLaunchKernelGGL((tree_merge_kernel<DT, kD, kCols, kSub, 4, 1>), grid, dim3(256), 0, stream, a, f.col_tiles);
+    else hipLaunchKernelGGL((tree_merge_kernel<DT, kD, kCols, kSub, 1, kEach>), grid, dim3(256), 0, stream, a, f.col_tiles);
     DSKV_LAUNCH_CHECK("tree_merge_kernel");
     return 0;
 }

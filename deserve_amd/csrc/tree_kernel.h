@@ -210,6 +210,8 @@ struct TreePlace {
     bool beside;
     int side;
     TreeRequest r;       // request b
+    Shares shares;       // equal ones; else the share is one of n_parts parts of an item, in the shares from first_part on
+    int first_part, n_parts;
 };
 // A share that goes over from one item to another starts twice and joins its waves' results twice, which a small batch notices: if
 // parts of a common number of units, whole turns (kTurn) and at most two turns more than equal shares have, take no more
@@ -221,7 +223,7 @@ __device__ __forceinline__ void tree_place(const A &a, int share, TreePlace &at)
 {
     __shared__ long scan[2][kThreads / 64], scan_parts[kThreads / 64];
     __shared__ int busy_of[kThreads / 64];
-    __shared__ int found_base, found_b, found_begin, found_end;
+    __shared__ int found_base, found_b, found_begin, found_end, found_part, found_parts;
     __shared__ TreeRequest found_r;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int per = (a.batch + kThreads - 1) / kThreads;
@@ -270,6 +272,8 @@ __device__ __forceinline__ void tree_place(const A &a, int share, TreePlace &at)
     const int used = max(min(min(spans, units), max((int)(((unsigned)units + kLeast - 1) / kLeast), requests)), 1);
     const Shares shares = shares_of(units, used);
     at.begin = at.end = 0;
+    at.shares = shares;
+    at.first_part = at.n_parts = 0;
     if (span < shares.used) {
         at.begin = share_begin(shares, span);
         at.end = share_begin(shares, span + 1);
@@ -305,6 +309,8 @@ __device__ __forceinline__ void tree_place(const A &a, int share, TreePlace &at)
                     found_b = b0;
                     found_base = before;
                     found_r = r;
+                    found_part = first + ct * of_item;
+                    found_parts = of_item;
                 }
                 if (tells && b0 < b1) a.units_before[b0] = first;
                 if (tells && b1 == a.batch) {
@@ -318,6 +324,8 @@ __device__ __forceinline__ void tree_place(const A &a, int share, TreePlace &at)
                 at.b = __builtin_amdgcn_readfirstlane(found_b);
                 at.base = found_base;
                 at.r = found_r;
+                at.first_part = found_part;
+                at.n_parts = found_parts;
                 return;
             }
         }
@@ -357,6 +365,8 @@ __device__ __forceinline__ void make_uniform(TreePlace &at)
     at.begin = __builtin_amdgcn_readfirstlane(at.begin);
     at.end = __builtin_amdgcn_readfirstlane(at.end);
     at.base = __builtin_amdgcn_readfirstlane(at.base);
+    at.first_part = __builtin_amdgcn_readfirstlane(at.first_part);
+    at.n_parts = __builtin_amdgcn_readfirstlane(at.n_parts);
     at.r.first = uniform(at.r.first);
     at.r.kv_len = uniform(at.r.kv_len);
     at.r.prior = __builtin_amdgcn_readfirstlane(at.r.prior);
@@ -830,8 +840,8 @@ __global__ __launch_bounds__(kTreeThreads, tree_workgroups(kD, kBlocks)) void tr
 // Items that were cut: a thread per (column, four dims) and group of parts.  kGroups > 1, for items in many parts: each takes
 // every kGroups-th part, and they meet in LDS.  kEach > 1, for many columns: columns that a thread takes at once (66
 // MB of partials, 16 trees of 33 - 64 rows: 16 us with four, 24 with one).
-template <int DT, int kD, int kCols, int kSub, int kGroups, int kEach, typename A>
-__global__ __launch_bounds__(256) void tree_merge_kernel(A a, int max_col_tiles)
+template <int DT, int kD, int kCols, int kSub, int kGroups, int kEach>
+__global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int max_col_tiles)
 {
     constexpr int kElt = DT == DSKV_F32 ? 4 : 2;
     constexpr int kQuads = kD / 4, kColumns = 256 / (kQuads * kGroups);

@@ -117,7 +117,7 @@ class BatchExec:
         pool = self.kvcaches[0].pool
         if getattr(pool, "record", None) is None:
             return None
-        return BatchQuantizedWithPagedKVCacheWrapper(get_quantized_wrapper(pool.main_device)._workspace)
+        return get_quantized_wrapper(pool.main_device).another()
 
     def _shape_kwargs(self) -> dict:
         a = self.layer_storage.model_args

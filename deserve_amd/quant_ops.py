@@ -143,14 +143,34 @@ class BatchQuantizedWithPagedKVCacheWrapper:
     """Attention of a step's rows over pages of 8-bit K/V, with the begin_forward / forward / end_forward protocol of paged_ops:
     one row per request (decode), chains or trees of drafted tokens, chunks of prompts, or all of them together.  begin_forward plans
     nothing and reads nothing back: the kernels take lengths and tables from the device, so a captured step can be replayed with others.
-    workspace_buffer: scratch of a forward while it runs; forwards that may run at the same time, on two streams, need one each."""
+    workspace_buffer: scratch of a forward while it runs; forwards that may run at the same time, on two streams, need a wrapper over
+    a workspace of its own each.  Making one waits for the device's current stream, once, and is not for a capture."""
 
     def __init__(self, workspace_buffer: torch.Tensor, kv_layout: str = "HND") -> None:
         if kv_layout != "HND":
             raise ValueError("8-bit pages hold their tokens by head: only the HND layout is implemented")
         self._workspace = workspace_buffer
+        # what the parts of a request count themselves in with: zero between launches, kept for good (captured ones hold its address)
+        self._counters = self._zeros(_lib.lib().dskv_quant_attn_counters(1))
         self._step: Optional[_lib.QuantStep] = None
         self._held: tuple = ()
+
+    def _zeros(self, n: int) -> torch.Tensor:
+        device = self._workspace.device
+        if device.type != "cuda":
+            return torch.zeros((n,), dtype=torch.int32)
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a wrapper for 8-bit pages is made, or first given so many kv heads, outside of a capture")
+        with torch.cuda.device(device):
+            zeros = torch.zeros((n,), dtype=torch.int32, device=device)
+            torch.cuda.current_stream().synchronize()        # whatever stream uses them first
+        return zeros
+
+    def another(self) -> "BatchQuantizedWithPagedKVCacheWrapper":
+        """For a step planned beside this wrapper's, over the same workspace; costs nothing."""
+        other = object.__new__(type(self))
+        other.__dict__.update(self.__dict__, _step=None, _held=())
+        return other
 
     def begin_forward(self, qo_indptr: torch.Tensor, paged_kv_indptr: torch.Tensor, paged_kv_indices: torch.Tensor,
                       paged_kv_last_page_len: torch.Tensor, num_qo_heads: int, num_kv_heads: int, head_dim: int,
@@ -171,13 +191,16 @@ class BatchQuantizedWithPagedKVCacheWrapper:
         if max_qo_len < 0 or min_qo_len < 0:
             raise ValueError("max_qo_len and min_qo_len must not be negative")
         _on_device(qo_indptr, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len, masks, self._workspace)
-        self._held = (qo_indptr, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len, masks, record.page_bytes)
+        if num_kv_heads > 512 and self._counters.numel() < _lib.lib().dskv_quant_attn_counters(num_kv_heads):
+            self._counters = self._zeros(_lib.lib().dskv_quant_attn_counters(num_kv_heads))
+        counters = self._counters
+        self._held = (qo_indptr, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len, masks, record.page_bytes, counters)
         step = _lib.TreeStep(
             qo_indptr.data_ptr(), paged_kv_indptr.data_ptr(), paged_kv_indices.data_ptr(),
             paged_kv_last_page_len.data_ptr(), _lib.ptr(masks), self._workspace.data_ptr(),
             self._workspace.numel() * self._workspace.element_size(), paged_kv_indices.numel(), batch, 0, max_qo_len,
             num_qo_heads, num_kv_heads, head_dim, page_size)
-        self._step = _lib.QuantStep(step, min_qo_len)
+        self._step = _lib.QuantStep(step, counters.data_ptr(), counters.numel(), min_qo_len)
 
     def forward(self, q: torch.Tensor, pages: torch.Tensor, sm_scale: Optional[float] = None, *,
                 out: Optional[torch.Tensor] = None) -> torch.Tensor:

@@ -681,11 +681,16 @@ int dskv_rope_append_quant(const dskv_quant_rows_t *rows, void *q_out, void *pag
 /*
  * dskv_tree_attn over such pages: same arguments and result, with sm_scale > 0 and dtype that of q and out.
  * min_qo_len: no request has fewer rows (a hint: what does not hold costs time, not results; 0 is always right).
+ * counters: dskv_quant_attn_counters(n_kv_heads) words on the device that are zero before the first call that is given them and
+ * used by one call at a time, like the workspace; every call leaves them zero.
  */
 typedef struct dskv_quant_step {
     dskv_tree_step_t step;
+    uint32_t *counters;
+    int64_t n_counters;
     int32_t min_qo_len;
 } dskv_quant_step_t;
+int64_t dskv_quant_attn_counters(int32_t n_kv_heads);
 int64_t dskv_quant_attn_workspace(int32_t batch, int32_t nnz, int32_t max_qo_len, int32_t n_qo_heads, int32_t n_kv_heads,
                                   int32_t head_dim, int32_t dtype);
 int dskv_quant_attn(const dskv_quant_step_t *step, void *out, const void *q, int64_t q_stride, const void *pages_layer,

@@ -127,7 +127,7 @@ def test_c_entries():
                 dtype=_lib.BF16, sm_scale=0.1)
 
     def attend(out=16, q=16, stride=4096, pages=16, min_qo_len=0, **kw):
-        step = _lib.QuantStep(_lib.TreeStep(**{**base, **kw}), min_qo_len)
+        step = _lib.QuantStep(_lib.TreeStep(**{**base, **kw}), None, 0, min_qo_len)
         return lib.dskv_quant_attn(ctypes.byref(step), out, q, stride, pages, None), _lib.last_error()
     for want, kw in (("negative", dict(batch=-1)), ("negative", dict(min_qo_len=-1)), ("dtype", dict(dtype=5)), ("multiple", dict(n_qo_heads=30)),
                      ("head_dim", dict(head_dim=100)), ("page shape", dict(num_pages=0)), ("sm_scale", dict(sm_scale=0.0)),
@@ -137,4 +137,13 @@ def test_c_entries():
         assert rc == _lib.E_INVAL and want in said, (want, rc, said)
     for kw in (dict(batch=0), dict(nnz=0), dict(max_qo_len=0)):
         assert attend(**kw)[0] == 0
+    rc, said = attend()
+    assert rc == _lib.E_NOMEM and "workspace of 0" in said
+    need = lib.dskv_quant_attn_workspace(1, 2, 2, 32, 8, 128, _lib.BF16)
+    rc, said = attend(workspace=16, workspace_bytes=need)
+    assert rc == _lib.E_NOMEM and "0 counters" in said
+    rc, said = attend(workspace=24, workspace_bytes=need)
+    assert rc == _lib.E_INVAL and "workspace must be 16-byte aligned" in said
+    assert lib.dskv_quant_attn_workspace(0, 2, 2, 32, 8, 128, 2) == 0 == lib.dskv_quant_attn_workspace(1, 2, 2, 32, 8, 80, 2)
+    assert lib.dskv_quant_attn_counters(8) == 1024 and lib.dskv_quant_attn_counters(1000) == 2000 and lib.dskv_quant_attn_counters(0) == 0
     assert lib.dskv_quant_attn(None, 16, 16, 4096, 16, None) == _lib.E_INVAL
