@@ -45,7 +45,7 @@ struct QuantAppend {
     const char *q, *k, *v;
     long q_stride, k_stride, v_stride;   // bytes
     const float *table;
-    int n_qo_heads, kv_blocks;
+    int n_qo_heads, kv_blocks, rows_each;
     float most;                          // the largest value that code * scale may take in the type
 };
 
@@ -68,13 +68,19 @@ template <int DT> struct Eight {
         if constexpr (DT == DSKV_F32) *reinterpret_cast<u32x4 *>(p + 16) = Chunk<DT>::pack(f + 4);
     }
 };
-__device__ __forceinline__ void rotate8(float *f, const float *table, long t, int col, int head_dim)
-{
-    const f32x4 c = *reinterpret_cast<const f32x4 *>(table + t * head_dim + col * 4);
-    const f32x4 s = *reinterpret_cast<const f32x4 *>(table + t * head_dim + head_dim / 2 + col * 4);
-    const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
-    rope_rotate<4>(f, cs, sn);
-}
+struct Angles {
+    float cs[4], sn[4];
+    __device__ __forceinline__ Angles(const float *table, long t, int col, int head_dim)
+    {
+        const f32x4 c = *reinterpret_cast<const f32x4 *>(table + t * head_dim + col * 4);
+        const f32x4 s = *reinterpret_cast<const f32x4 *>(table + t * head_dim + head_dim / 2 + col * 4);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            cs[i] = c[i];
+            sn[i] = s[i];
+        }
+    }
+};
 __device__ __forceinline__ float wave_max(float v)
 {
 #pragma unroll
@@ -82,109 +88,159 @@ __device__ __forceinline__ float wave_max(float v)
     return v;
 }
 
-// Workgroups of the first kv_blocks rows of the grid: one wave per (row of the step, kv head).  The row that is the first of its
-// request in a page takes all of them there, and the block with them: their largest values, the scale, what the block holds already rounded anew
-// where that grows, and the codes.  The other rows' waves end at once.  Workgroups behind: q, a row each.
+// Workgroups of the first kv_blocks rows of the grid: one wave per (rows_each rows of the step, kv head).  Of these it takes every one that is the first of
+// its request in a page, and all rows of the request there with it, and so the whole block: their largest values, the scale, what the
+// block holds already rounded anew where that grows, and the codes.  Workgroups behind: q, rows_each rows each.
 // kLanes: lanes of a row, 8 elements each, a power of two.
+// Bound by HBM where there are many rows: what is read a second time comes from the caches.  (More rows held in registers: 180 of these instead of 89,
+// 80 us for the 62 below.)
 template <int DT, int kLanes>
-__global__ __launch_bounds__(256) void quant_append_kernel(QuantAppend a)
+__global__ __launch_bounds__(256, 4) void quant_append_kernel(QuantAppend a)
 {
     constexpr int kElt = DT == DSKV_F32 ? 4 : 2, kRows = 64 / kLanes;
     const QuantShape &s = a.r.s;
-    const int t = blockIdx.x, lane = threadIdx.x & 63, col = lane % kLanes, row = lane / kLanes;
+    const int t0 = blockIdx.x * a.rows_each, t1 = min(t0 + a.rows_each, a.r.nnz);
+    const int lane = threadIdx.x & 63, col = lane % kLanes, row = lane / kLanes;
     const bool works = col * 8 < s.head_dim;
     if ((int)blockIdx.y >= a.kv_blocks) {
-        for (int h = threadIdx.x / kLanes; h < a.n_qo_heads; h += 256 / kLanes) {
+        constexpr int kHeads = 256 / kLanes, kAtOnce = 4;
+        for (int t = t0; t < t1; t++) {
             if (!works) continue;
-            Eight<DT> x;
-            float f[8];
-            x.load(a.q + t * a.q_stride + ((long)h * s.head_dim + col * 8) * kElt);
-            x.unpack(f);
-            rotate8(f, a.table, t, col, s.head_dim);
-            x.store(a.q_out + (((long)t * a.n_qo_heads + h) * s.head_dim + col * 8) * kElt, f);
+            const Angles angles(a.table, t, col, s.head_dim);
+            for (int h0 = threadIdx.x / kLanes; h0 < a.n_qo_heads; h0 += kAtOnce * kHeads) {
+                Eight<DT> x[kAtOnce];
+#pragma unroll
+                for (int i = 0; i < kAtOnce; i++)
+                    if (h0 + i * kHeads < a.n_qo_heads)
+                        x[i].load(a.q + t * a.q_stride + ((long)(h0 + i * kHeads) * s.head_dim + col * 8) * kElt);
+#pragma unroll
+                for (int i = 0; i < kAtOnce; i++)
+                    if (h0 + i * kHeads < a.n_qo_heads) {
+                        float f[8];
+                        x[i].unpack(f);
+                        rope_rotate<4>(f, angles.cs, angles.sn);
+                        x[i].store(a.q_out + (((long)t * a.n_qo_heads + h0 + i * kHeads) * s.head_dim + col * 8) * kElt, f);
+                    }
+            }
         }
         return;
     }
     const int head = blockIdx.y * 4 + (threadIdx.x >> 6);
     if (head >= s.n_kv_heads) return;
-    const int b = request_of_row(a.r.qo_indptr, a.r.batch, t);
+    int b = request_of_row(a.r.qo_indptr, a.r.batch, t0);
     if (b < 0) return;
-    const QuantRequest r = quant_request(a.r, b);
-    if (r.n == 0) return;
-    const int i = t - r.first, at = r.prior + i;
-    const int place = (int)((unsigned)at % (unsigned)s.page_size);
-    if (i > 0 && place > 0) return;
-    const int count = min(s.page_size - place, r.n - i);                  // rows of the request in this page
-    const long page = quant_page(a.r, r, at);
-    if (page < 0) return;
-    char *const record = a.pages + page * s.page_bytes;
-    const long k_at = head * s.head_bytes, v_at = s.half_bytes + k_at;
-    uint32_t *const scales = reinterpret_cast<uint32_t *>(record + 2 * s.half_bytes);
-
-    const char *const k_rows = a.k + t * a.k_stride + ((long)head * s.head_dim + col * 8) * kElt;
-    const char *const v_rows = a.v + t * a.v_stride + ((long)head * s.head_dim + col * 8) * kElt;
-    // a token of which a value is no finite number: its K becomes no number, so that rows that see it get none and
-    // the others, whose weight of it is 0, are not touched by its V, which becomes 0
-    auto fetch = [&](int j, float *k, float *v) -> bool {
-#pragma unroll
-        for (int d = 0; d < 8; d++) k[d] = v[d] = 0;
-        if (works && j < count) {
-            Eight<DT> x, y;
-            x.load(k_rows + j * a.k_stride);
-            y.load(v_rows + j * a.v_stride);
-            x.unpack(k);
-            y.unpack(v);
-            if (a.table) rotate8(k, a.table, t + j, col, s.head_dim);
+    for (int t = t0; t < t1;) {
+        while (b < a.r.batch && a.r.qo_indptr[b + 1] <= t) b++;           // on to the request of row t
+        if (b == a.r.batch) return;
+        const QuantRequest r = quant_request(a.r, b);
+        if (r.n == 0) {                                                   // its arrays contradict themselves
+            const int next = a.r.qo_indptr[b + 1];
+            if (next <= t) return;
+            t = next;
+            continue;
         }
-        bool fine = true;
+        const int i = t - r.first, at = r.prior + i;
+        const int place = (int)((unsigned)at % (unsigned)s.page_size);
+        const int count = min(s.page_size - place, r.n - i);              // rows of the request in this page from t on
+        const int begin = t;
+        t += count;
+        if (i > 0 && place > 0) continue;                                 // another wave's
+        const char *const k_rows = a.k + begin * a.k_stride + ((long)head * s.head_dim + col * 8) * kElt;
+        const char *const v_rows = a.v + begin * a.v_stride + ((long)head * s.head_dim + col * 8) * kElt;
+        struct Pass {
+            float k[8], v[8];
+            bool fine;
+        };
+        float k_most = 0, v_most = 0;
+        // a token of which a value is no finite number: its K becomes no number, so that rows that see it get none and
+        // the others, whose weight of it is 0, are not touched by its V, which becomes 0
+        auto fetch = [&](int j, Pass &p) {
 #pragma unroll
-        for (int d = 0; d < 8; d++) fine = fine && fabsf(k[d]) <= __FLT_MAX__ && fabsf(v[d]) <= __FLT_MAX__;
-        const unsigned long long odd = __ballot(!fine) >> (row * kLanes);
-        return kLanes == 64 ? odd == 0 : (odd & ((1ull << kLanes) - 1)) == 0;
-    };
-    float k[8], v[8], k_most = 0, v_most = 0;
-    for (int j0 = 0; j0 < count; j0 += kRows)
-        if (fetch(j0 + row, k, v)) {
+            for (int d = 0; d < 8; d++) p.k[d] = p.v[d] = 0;
+            if (works && j < count) {
+                Eight<DT> x, y;
+                x.load(k_rows + j * a.k_stride);
+                y.load(v_rows + j * a.v_stride);
+                x.unpack(p.k);
+                y.unpack(p.v);
+                if (a.table) {
+                    const Angles angles(a.table, begin + j, col, s.head_dim);
+                    rope_rotate<4>(p.k, angles.cs, angles.sn);
+                }
+            }
+        };
+        auto measure = [&](Pass &p) {
+            float k_top = 0, v_top = 0, zero = 0;
 #pragma unroll
             for (int d = 0; d < 8; d++) {
-                k_most = fmaxf(k_most, fabsf(k[d]));
-                v_most = fmaxf(v_most, fabsf(v[d]));
+                k_top = fmaxf(k_top, fabsf(p.k[d]));
+                v_top = fmaxf(v_top, fabsf(p.v[d]));
+                zero = fmaf(p.k[d], 0.f, fmaf(p.v[d], 0.f, zero));        // no number if one of them is infinite or none
+            }
+            const unsigned long long odd = __ballot(zero != 0.f) >> (row * kLanes);
+            p.fine = (odd & ((1ull << kLanes) - 1)) == 0;
+            k_most = fmaxf(k_most, p.fine ? k_top : 0.f);
+            v_most = fmaxf(v_most, p.fine ? v_top : 0.f);
+        };
+        // rows of one pass stay in registers; of more, what the second reading needs is in the L2
+        Pass first;
+        fetch(row, first);
+        const int page = quant_page(a.r, r, at);
+        if (page < 0) continue;
+        char *const record = a.pages + page * s.page_bytes;
+        char *const k_block = record + head * s.head_bytes, *const v_block = k_block + s.half_bytes;
+        uint32_t *const scales = reinterpret_cast<uint32_t *>(record + 2 * s.half_bytes) + head;
+        uint32_t scale[2] = {0, 0};                                       // of the rows that stay
+        if (place > 0) {
+            scale[0] = stored_scale(scales[0]);
+            scale[1] = stored_scale(scales[s.n_kv_heads]);
+        }
+        measure(first);
+#pragma unroll 1
+        for (int j = kRows; j < count; j += kRows) {
+            Pass p;
+            fetch(j + row, p);
+            measure(p);
+        }
+        const float most[2] = {fminf(wave_max(k_most), a.most), fminf(wave_max(v_most), a.most)};
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            const uint32_t old = scale[x];
+            scale[x] = max(needed_scale(most[x]), old);
+            if (old != 0 && scale[x] > old) {
+                const float ratio = __builtin_bit_cast(float, old) * reciprocal_of(scale[x]);
+                for (int j = lane; j < place * s.head_dim / 8; j += 64) {
+                    u32x2 *const codes = reinterpret_cast<u32x2 *>(x ? v_block : k_block) + j;
+                    float f[8];
+                    decode8(*codes, f);
+#pragma unroll
+                    for (int d = 0; d < 8; d++) f[d] *= ratio;
+                    *codes = encode8(f);
+                }
             }
         }
-    const float most[2] = {fminf(wave_max(k_most), a.most), fminf(wave_max(v_most), a.most)};
-    uint32_t scale[2];
+        if (lane < 2) scales[lane * s.n_kv_heads] = lane ? scale[1] : scale[0];
+        const float k_by = reciprocal_of(scale[0]), v_by = reciprocal_of(scale[1]);
+        auto put = [&](int j, Pass &p) {
+            if (!works || j >= count) return;
 #pragma unroll
-    for (int x = 0; x < 2; x++) {
-        uint32_t *const held = scales + x * s.n_kv_heads + head;
-        const uint32_t old = place > 0 ? stored_scale(*held) : 0u;
-        scale[x] = max(needed_scale(most[x]), old);
-        if (old != 0 && scale[x] > old) {
-            const float ratio = __builtin_bit_cast(float, old) * reciprocal_of(scale[x]);
-            for (int j = lane; j < place * s.head_dim / 8; j += 64) {
-                u32x2 *const codes = reinterpret_cast<u32x2 *>(record + (x ? v_at : k_at)) + j;
-                float f[8];
-                decode8(*codes, f);
-#pragma unroll
-                for (int d = 0; d < 8; d++) f[d] *= ratio;
-                *codes = encode8(f);
+            for (int d = 0; d < 8; d++) {
+                p.k[d] = fminf(fmaxf(p.k[d], -a.most), a.most) * k_by;
+                p.v[d] = fminf(fmaxf(p.v[d], -a.most), a.most) * v_by;
             }
+            const uint32_t none = kNoNumberCode * 0x01010101u;
+            const long to = (long)(place + j) * s.head_dim + col * 8;
+            *reinterpret_cast<u32x2 *>(k_block + to) = p.fine ? encode8(p.k) : u32x2{none, none};
+            *reinterpret_cast<u32x2 *>(v_block + to) = p.fine ? encode8(p.v) : u32x2{0, 0};
+        };
+        put(row, first);
+#pragma unroll 1
+        for (int j = kRows; j < count; j += kRows) {
+            Pass p;
+            fetch(j + row, p);
+            measure(p);                                                   // (for p.fine)
+            put(j + row, p);
         }
-        if (lane == 0) *held = scale[x];
-    }
-    const float k_by = reciprocal_of(scale[0]), v_by = reciprocal_of(scale[1]);
-    for (int j0 = 0; j0 < count; j0 += kRows) {
-        const int j = j0 + row;
-        const bool fine = fetch(j, k, v);
-        if (!works || j >= count) continue;
-#pragma unroll
-        for (int d = 0; d < 8; d++) {
-            k[d] = fminf(fmaxf(k[d], -a.most), a.most) * k_by;
-            v[d] = fminf(fmaxf(v[d], -a.most), a.most) * v_by;
-        }
-        const uint32_t none = kNoNumberCode * 0x01010101u;
-        const long to = (long)(place + j) * s.head_dim + col * 8;
-        *reinterpret_cast<u32x2 *>(record + k_at + to) = fine ? encode8(k) : u32x2{none, none};
-        *reinterpret_cast<u32x2 *>(record + v_at + to) = fine ? encode8(v) : u32x2{0, 0};
     }
 }
 
@@ -342,6 +398,14 @@ __global__ __launch_bounds__(256) void quant_move_kernel(QuantMove a)
     }
 }
 
+// Rows of a wave of the append: one as long as that makes few waves, else as many as make about kAppendWaves.  8192 rows (16 chunks of 512, 64 heads
+// over 8, f16, 323 MB) 62 us, 5.2 TB/s; with one row a wave, most of them for nothing, 76; 320 rows 6.4 us, with two each 7.9.
+constexpr int kAppendMost = 8192, kAppendWaves = 2048;
+static int rows_each(int64_t nnz, int64_t n_kv_heads)
+{
+    const int64_t waves = nnz * n_kv_heads;
+    return waves <= kAppendMost ? 1 : (int)std::min<int64_t>((waves + kAppendWaves - 1) / kAppendWaves, 64);
+}
 // Waves that a move is cut into, about: 64 walks in 32 layers 21.8 us, with 4096 24.2, with 16384 23.4.
 constexpr int kMoveWaves = 8192;
 
@@ -371,7 +435,7 @@ static QuantRows rows_of(const dskv_quant_rows_t *r)
 }
 template <int DT> static int launch_quant_append(const QuantAppend &a, hipStream_t stream)
 {
-    const dim3 grid((unsigned)a.r.nnz, (unsigned)(a.kv_blocks + (a.table ? 1 : 0))), block(256);
+    const dim3 grid((unsigned)((a.r.nnz + a.rows_each - 1) / a.rows_each), (unsigned)(a.kv_blocks + (a.table ? 1 : 0))), block(256);
     switch (lanes_of(a.r.s.head_dim)) {
     case 1: hipLaunchKernelGGL((quant_append_kernel<DT, 1>), grid, block, 0, stream, a); break;
     case 2: hipLaunchKernelGGL((quant_append_kernel<DT, 2>), grid, block, 0, stream, a); break;
@@ -411,6 +475,7 @@ extern "C" int dskv_rope_append_quant(const dskv_quant_rows_t *rows, void *q_out
     QuantAppend a = {rows_of(rows), (char *)q_out, (char *)pages_layer, (const char *)q, (const char *)k, (const char *)v,
                      (long)q_stride * size, (long)k_stride * size, (long)v_stride * size, rope_table, n_qo_heads,
                      (rows->n_kv_heads + 3) / 4,
+                     rows_each(rows->nnz, rows->n_kv_heads),
                      // 240 * 2^8, 240 * 2^120: the code above, 256, would make an infinity of the type with that scale
                      dtype == DSKV_F16 ? 61440.f : 3.1901472e38f};
     hipStream_t st = (hipStream_t)stream;

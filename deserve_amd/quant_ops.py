@@ -19,6 +19,7 @@ is enqueued on the current stream of the tensors' device.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from dataclasses import dataclass
 from typing import Optional
@@ -66,24 +67,35 @@ class PageRecord:
         return x.transpose(-3, -2).to(dtype)
 
 
+@functools.lru_cache(maxsize=256)
+def _page_bytes(page_size: int, n_kv_heads: int, head_dim: int) -> int:
+    return PageRecord(page_size, n_kv_heads, head_dim).page_bytes
+
+
 def _check_records(name: str, pages: torch.Tensor, page_bytes: int, dims: int) -> None:
-    whole = pages.is_contiguous() or dims == 3 and (pages.shape[0] == 0 or pages[0].is_contiguous()) if pages.dim() == dims else False
-    if pages.dim() != dims or pages.dtype is not torch.uint8 or pages.shape[-1] != page_bytes or not whole:
-        what = "(num_pages, " if dims == 2 else "(L, num_pages, "
-        raise ValueError(f"{name} must be a contiguous {what}{page_bytes}) uint8 tensor, got {tuple(pages.shape)} of {pages.dtype}")
-    if pages.data_ptr() % 16 or (dims == 3 and pages.shape[0] > 1 and pages.stride(0) % 16):
+    shape = pages.shape
+    if len(shape) == dims and pages.dtype is torch.uint8 and shape[-1] == page_bytes and pages.data_ptr() % 16 == 0 and (
+            pages.is_contiguous() or (dims == 3 and (shape[0] == 0 or pages[0].is_contiguous()) and pages.stride(0) % 16 == 0)):
+        return
+    if pages.dtype is torch.uint8 and len(shape) == dims and shape[-1] == page_bytes and pages.data_ptr() % 16:
         raise ValueError(f"{name} must be 16-byte aligned")
+    what = "(num_pages, " if dims == 2 else "(L, num_pages, "
+    raise ValueError(f"{name} must be a contiguous {what}{page_bytes}) uint8 tensor, got {tuple(shape)} of {pages.dtype}")
 
 
 def _check_csr(qo_indptr: torch.Tensor, kv_indices: torch.Tensor, kv_indptr: torch.Tensor, kv_last_page_len: torch.Tensor) -> int:
-    _check_vector("qo_indptr", qo_indptr, torch.int32, 1)
     batch = qo_indptr.numel() - 1
-    _check_vector("kv_indptr", kv_indptr, torch.int32, batch + 1)
-    _check_vector("kv_indices", kv_indices, torch.int32, 0)
-    _check_vector("kv_last_page_len", kv_last_page_len, torch.int32, batch)
-    if kv_indptr.numel() != batch + 1:
-        raise ValueError("qo_indptr and kv_indptr disagree about the batch")
-    return batch
+    i32 = torch.int32
+    if qo_indptr.dtype is i32 and kv_indptr.dtype is i32 and kv_indices.dtype is i32 and kv_last_page_len.dtype is i32 and \
+            qo_indptr.dim() == kv_indptr.dim() == kv_indices.dim() == kv_last_page_len.dim() == 1 and \
+            qo_indptr.is_contiguous() and kv_indptr.is_contiguous() and kv_indices.is_contiguous() and \
+            kv_last_page_len.is_contiguous() and 0 <= batch <= kv_last_page_len.numel() and kv_indptr.numel() == batch + 1:
+        return batch
+    _check_vector("qo_indptr", qo_indptr, i32, 1)
+    _check_vector("kv_indptr", kv_indptr, i32, batch + 1)
+    _check_vector("kv_indices", kv_indices, i32, 0)
+    _check_vector("kv_last_page_len", kv_last_page_len, i32, batch)
+    raise ValueError("qo_indptr and kv_indptr disagree about the batch")
 
 
 def rope_append_quantized(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, qo_indptr: torch.Tensor,
@@ -97,16 +109,13 @@ def rope_append_quantized(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.T
     holds already, whose codes are rounded anew where it grows.  A token with a value that is no finite number makes no number of the rows
     that see it, and nothing else.  A request whose arrays contradict themselves, or a page that the pool does not have,
     takes no rows.  No page takes rows of two requests."""
-    for name, t in (("k", k), ("v", v)):
-        if t.dim() != 3:
-            raise ValueError(f"{name} must be (tokens, heads, D), got {tuple(t.shape)}")
-    _, hkv, dim = k.shape
+    if k.dim() != 3:
+        raise ValueError(f"k must be (tokens, heads, D), got {tuple(k.shape)}")
+    nnz, hkv, dim = k.shape
     dtype = k.dtype
-    record = PageRecord(page_size, hkv, dim)
-    _check_records("pages", pages, record.page_bytes, 2)
+    _check_records("pages", pages, _page_bytes(page_size, hkv, dim), 2)
     code = _lib.dtype_code(dtype)
-    k, k_stride = _token_rows("k", k, dtype, hkv, dim, None)
-    nnz = k.shape[0]
+    k, k_stride = _token_rows("k", k, dtype, hkv, dim, nnz)
     v, v_stride = _token_rows("v", v, dtype, hkv, dim, nnz)
     batch = _check_csr(qo_indptr, kv_indices, kv_indptr, kv_last_page_len)
     result, q_stride, heads = q, 0, hkv
@@ -128,7 +137,7 @@ def rope_append_quantized(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.T
     elif out is not None:
         raise ValueError("out is for the rotated q: rope_table is missing")
     rotated = rope_table is not None
-    index = _on_device(pages, k, v, qo_indptr, kv_indices, kv_indptr, kv_last_page_len, rope_table, *((q, result) if rotated else ()))
+    index = _on_device(pages, k, v, qo_indptr, kv_indices, kv_indptr, kv_last_page_len, rope_table, q if rotated else None, out)
     if nnz == 0 or pages.shape[0] == 0:
         return result
     rows = _lib.QuantRows(qo_indptr.data_ptr(), kv_indices.data_ptr(), kv_indptr.data_ptr(), kv_last_page_len.data_ptr(),
@@ -181,7 +190,7 @@ class BatchQuantizedWithPagedKVCacheWrapper:
         masks (tokens) int64, bit j: the row sees new row j of its request, at most MAX_TREE_ROWS rows a request;
         None: it sees the rows up to itself."""
         batch = _check_csr(qo_indptr, paged_kv_indices, paged_kv_indptr, paged_kv_last_page_len)
-        record = PageRecord(page_size, num_kv_heads, head_dim)
+        page_bytes = _page_bytes(page_size, num_kv_heads, head_dim)
         if masks is not None:
             _check_vector("masks", masks, torch.int64, 0)
             if max_qo_len > MAX_TREE_ROWS:
@@ -194,13 +203,13 @@ class BatchQuantizedWithPagedKVCacheWrapper:
         if num_kv_heads > 512 and self._counters.numel() < _lib.lib().dskv_quant_attn_counters(num_kv_heads):
             self._counters = self._zeros(_lib.lib().dskv_quant_attn_counters(num_kv_heads))
         counters = self._counters
-        self._held = (qo_indptr, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len, masks, record.page_bytes, counters)
-        step = _lib.TreeStep(
+        self._held = (qo_indptr, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len, masks, page_bytes, counters)
+        workspace = self._workspace
+        self._step = _lib.QuantStep((
             qo_indptr.data_ptr(), paged_kv_indptr.data_ptr(), paged_kv_indices.data_ptr(),
-            paged_kv_last_page_len.data_ptr(), _lib.ptr(masks), self._workspace.data_ptr(),
-            self._workspace.numel() * self._workspace.element_size(), paged_kv_indices.numel(), batch, 0, max_qo_len,
-            num_qo_heads, num_kv_heads, head_dim, page_size)
-        self._step = _lib.QuantStep(step, counters.data_ptr(), counters.numel(), min_qo_len)
+            paged_kv_last_page_len.data_ptr(), None if masks is None else masks.data_ptr(), workspace.data_ptr(),
+            workspace.numel() * workspace.element_size(), paged_kv_indices.numel(), batch, 0, max_qo_len,
+            num_qo_heads, num_kv_heads, head_dim, page_size), counters.data_ptr(), counters.numel(), min_qo_len)
 
     def forward(self, q: torch.Tensor, pages: torch.Tensor, sm_scale: Optional[float] = None, *,
                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -219,11 +228,12 @@ class BatchQuantizedWithPagedKVCacheWrapper:
             raise ValueError(f"masks hold {masks.numel()} rows, q has {nnz}")
         if sm_scale is not None and not sm_scale > 0:
             raise ValueError(f"sm_scale must be positive, not {sm_scale}")
-        if out is None:
+        fresh = out is None
+        if fresh:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif out.shape != q.shape or out.dtype is not dtype or not out.is_contiguous() or out.data_ptr() % 16:
             raise ValueError("out must be contiguous, 16-byte aligned and of q's shape and dtype")
-        index = _on_device(q, pages, out, self._held[0])
+        index = _on_device(q, pages, None if fresh else out, self._held[0])
         if pages.shape[0] == 0:
             raise ValueError("the pool has no pages")
         step = _lib.QuantStep.from_buffer_copy(self._step)      # calls from several threads do not share it
@@ -245,8 +255,7 @@ def move_accepted_quantized_rows(pages: torch.Tensor, qo_indptr: torch.Tensor, k
     (draft_ops.verify_drafts) to where its sequence goes on, row j of the walk from the request's new row path[j] to its new row j, in all
     layers; the tables are those of the step that was verified.  The scale of a block that rows move into grows where they need it.
     Accepted chains are there already."""
-    record = PageRecord(page_size, n_kv_heads, head_dim)
-    _check_records("pages", pages, record.page_bytes, 3)
+    _check_records("pages", pages, _page_bytes(page_size, n_kv_heads, head_dim), 3)
     batch = _check_csr(qo_indptr, kv_indices, kv_indptr, kv_last_page_len)
     _check_vector("path", path, torch.int32, 0)
     _check_vector("counts", counts, torch.int32, batch)
