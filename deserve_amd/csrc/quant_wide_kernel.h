@@ -18,21 +18,24 @@ namespace dskv {
 
 constexpr int kMergeEach = 4;                // columns that a thread of the merge launch takes
 constexpr int kWideBlock = 32;
-constexpr int kWideRegion = 1088;           // 64 lanes' 16 bytes, (4 chunk + row) * 16 of four rows, and 64 bytes of padding
+constexpr int kWideRegion = 1088;           // 64 chunks of 16 bytes, (4 chunk + row) * 16 of four rows, and 64 bytes of padding
 constexpr int kWideStage = kWideBlock / 4 * kWideRegion;
 constexpr int kWideLeast = 8;               // units a share has at least: what fills the stages takes about as long
 
 template <int kD, int kWaves> struct QuantWide {
     static constexpr int kThreads = kWaves * 64;
     static constexpr int kCols = kWaves * 32;
-    static constexpr int kPack = 128 / kD;               // blocks of a stage: rows of 64 dims lie side by side with the next block's
-    static constexpr int kChunks = kD / 8;               // 8-code chunks of a row
+    // A stage is what the workgroup's lanes fetch at once, kLane bytes each: one block or two, which lie one after the other in LDS, or, with
+    // 64 dims, side by side in rows of 128
+    static constexpr int kPack = kD == 128 && kWaves == 4 ? 1 : 2;
+    static constexpr int kLane = kPack * kWideBlock * kD / kThreads;
+    static constexpr int kLaneRows = 64 * kLane / kD;    // tokens that a wave fetches
+    static constexpr int kStageBytes = kD == 128 ? kPack * kWideStage : kWideStage;
     static constexpr int kSteps = kD / 16, kDims = kD / 32;      // matrix instructions of a block's scores; 32-dim tiles of O
-    static constexpr int kGroups = 8 / kWaves;           // regions of a stage that a wave fetches
     static constexpr int kHalf = kWaves == 8 ? 64 : 32;  // blocks that are looked up at a time; two such halves are kept
-    static constexpr int kTokens = 2 * kHalf * kWideBlock;
+    static constexpr int kTokens = 2 * kHalf * kWideBlock, kBeyond = 12;
     static constexpr int kKStages = kPack == 2 ? 2 : 4, kVStages = kPack == 2 ? 4 : 2;      // in LDS
-    static constexpr int kAhead = 2;                     // stages of K, and of V, on their way in registers
+    static constexpr int kAhead = kD == 128 && kPack == 2 ? 1 : 2;       // stages of K, and of V, on their way in registers
     // what turn u (in front of the iterations of stage u) writes: K(u + kFirst) and V(u + kBehind)
     static constexpr int kFirst = kPack == 2 ? 2 : 3, kBehind = kPack - 1;
 };
@@ -48,9 +51,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void quant_wide_kernel(QuantArgs a)
 {
     typedef Elt<DT> E;
     typedef QuantWide<kD, kWaves> W;
-    __shared__ __align__(16) char lds[(W::kKStages + W::kVStages) * kWideStage];
-    __shared__ uint32_t row_at[W::kTokens];              // where a token's K lies (see quant_row)
-    __shared__ uint16_t scale_at[W::kTokens];            // exponents of its scales, V's in the upper byte
+    __shared__ __align__(16) char lds[(W::kKStages + W::kVStages) * W::kStageBytes];
+    // Where a token's K lies (see quant_row), and the exponents of its scales, V's in the second byte; behind the two halves the first
+    // kBeyond blocks again, so that what a turn reads lies at fixed distances
+    __shared__ u32x2 token_at[W::kTokens + W::kBeyond * kWideBlock];
     __shared__ uint32_t held_at[2 * W::kHalf];           // bit per token of a block: there is one
     __shared__ int holes;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -67,12 +71,18 @@ __global__ __launch_bounds__(kWaves * 64, 2) void quant_wide_kernel(QuantArgs a)
     TreeRequest r = place.r;
     if (head == 0 && threadIdx.x < 2) a.cuts[2 * share + threadIdx.x].parts.n = 0;
 
-    auto k_stage = [&](int i) { return lds + (i & (W::kKStages - 1)) * kWideStage; };
-    auto v_stage = [&](int i) { return lds + (W::kKStages + (i & (W::kVStages - 1))) * kWideStage; };
+    auto k_stage = [&](int i) { return lds + (i & (W::kKStages - 1)) * W::kStageBytes; };
+    auto v_stage = [&](int i) { return lds + (W::kKStages + (i & (W::kVStages - 1))) * W::kStageBytes; };
     // block j in its stage of K or V
-    auto block_at = [&](auto &stage, int j) -> char * { return W::kPack == 2 ? stage(j >> 1) + (j & 1) * 512 : stage(j); };
-    // lane p of a wave fetches chunk p / 4 of row p % 4 of a region
-    const char *const pool = a.pages + head * a.head_bytes + (lane >> 2) % W::kChunks * 8;
+    auto block_at = [&](auto &stage, int j) -> char * {
+        return W::kPack == 2 ? stage(j >> 1) + (j & 1) * (kD == 128 ? kWideStage : 512) : stage(j);
+    };
+    // lane p of a wave fetches part p / kLaneRows of token p % kLaneRows of its tokens of a stage
+    const int my_token = wave * W::kLaneRows + lane % W::kLaneRows, my_part = lane / W::kLaneRows;
+    const char *const pool = a.pages + head * a.head_bytes + my_part * W::kLane;
+    const int my_row = my_token % kWideBlock, my_block = my_token / kWideBlock, my_chunk = my_part * (W::kLane / 8);
+    const int my_place = kD == 128 ? my_block * kWideStage + my_row / 4 * kWideRegion + (4 * my_chunk + my_row % 4) * 16
+                                   : my_row / 4 * kWideRegion + (4 * (my_chunk + 8 * my_block) + my_row % 4) * 16;
     const char *const none = reinterpret_cast<const char *>(kNoRow);
     const char *const scales = a.pages + 2 * a.half_bytes + head * 4;
 
@@ -148,53 +158,54 @@ __global__ __launch_bounds__(kWaves * 64, 2) void quant_wide_kernel(QuantArgs a)
                     }
                 }
                 const int at = (x & 1) * W::kHalf * kWideBlock + i;
-                row_at[at] = row;
-                scale_at[at] = (uint16_t)exponents;
+                token_at[at] = u32x2{row, exponents};
+                if (at < W::kBeyond * kWideBlock) token_at[W::kTokens + at] = u32x2{row, exponents};
                 const unsigned long long there64 = __ballot(row != kNoQuantRow);
                 if ((lane & 31) == 0) held_at[at / kWideBlock] = (uint32_t)(there64 >> (lane & 32));
             }
         };
-        // token of the walk, as the tables have it, that the lane fetches of region i of stage u; its block
-        auto block_of = [&](int u) { return W::kPack == 2 ? 2 * u + (lane >> 5) : u; };
-        auto token_of = [&](int u, int i) {
-            return (block_of(u) & (2 * W::kHalf - 1)) * kWideBlock + (wave * W::kGroups + i) * 4 + (lane & 3);
+        // what the tables say of the token that the lane fetches of stage u + more
+        const u32x2 *const mine_at = token_at + my_token;
+        auto token_of = [&](int u, int more) -> const u32x2 & {
+            return mine_at[((u * W::kPack & (2 * W::kHalf - 1)) + more * W::kPack) * kWideBlock];
         };
-        u32x2 k_codes[W::kAhead][W::kGroups], v_codes[W::kAhead][W::kGroups];
-        auto request = [&](uint32_t row, u32x2 &codes, long more) {
+        typedef uint32_t Codes __attribute__((ext_vector_type(W::kLane / 4)));
+        Codes k_codes[W::kAhead], v_codes[W::kAhead];
+        auto request = [&](uint32_t row, Codes &codes, long more) {
             const char *p = pool + (uint64_t)row * 16 + more;
             p = row != kNoQuantRow ? p : none;
-            codes = *(const __attribute__((address_space(1))) u32x2 *)p;
+            codes = *(const __attribute__((address_space(1))) Codes *)p;
         };
-        auto write = [&](u32x2 codes, uint32_t exponent, int i, char *stage) {
+        auto write = [&](const Codes &codes, uint32_t exponent, char *stage) {
             const float scale = __builtin_bit_cast(float, exponent << 23);
-            u32x4 x;
 #pragma unroll
-            for (int w = 0; w < 2; w++) {
-                if constexpr (DT == DSKV_F16) {
-                    x[2 * w] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[w], scale, false));
-                    x[2 * w + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[w], scale, true));
-                } else {
-                    x[2 * w] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[w], scale, false));
-                    x[2 * w + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[w], scale, true));
+            for (int c = 0; c < W::kLane / 8; c++) {
+                u32x4 x;
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                    const uint32_t four = codes[2 * c + w];
+                    if constexpr (DT == DSKV_F16) {
+                        x[2 * w] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(four, scale, false));
+                        x[2 * w + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(four, scale, true));
+                    } else {
+                        x[2 * w] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(four, scale, false));
+                        x[2 * w + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(four, scale, true));
+                    }
                 }
+                *reinterpret_cast<u32x4 *>(stage + my_place + c * 64) = x;
             }
-            *reinterpret_cast<u32x4 *>(stage + (wave * W::kGroups + i) * kWideRegion + lane * 16) = x;
         };
         // what turn u needs of the tables: exponents of what it writes, places of what it requests
         struct Known {
-            uint8_t k_exponent[W::kGroups], v_exponent[W::kGroups];
-            uint32_t k_row[W::kGroups], v_row[W::kGroups];
+            uint32_t k_exponent, v_exponent, k_row, v_row;
         };
-        const uint8_t *const exponent_at = reinterpret_cast<const uint8_t *>(scale_at);
         auto know = [&](int u, Known &x) {
-#pragma unroll
-            for (int i = 0; i < W::kGroups; i++) {
-                x.k_exponent[i] = exponent_at[2 * token_of(u + W::kFirst, i)];
-                x.v_exponent[i] = exponent_at[2 * token_of(u + W::kBehind, i) + 1];
-                x.k_row[i] = row_at[token_of(u + W::kFirst + W::kAhead, i)];
-                x.v_row[i] = row_at[token_of(u + W::kBehind + W::kAhead, i)];
-            }
+            x.k_exponent = *(reinterpret_cast<const uint8_t *>(&token_of(u, W::kFirst)) + 4);
+            x.v_exponent = *(reinterpret_cast<const uint8_t *>(&token_of(u, W::kBehind)) + 5);
+            x.k_row = token_of(u, W::kFirst + W::kAhead).x;
+            x.v_row = token_of(u, W::kBehind + W::kAhead).x;
         };
+        static_assert((W::kFirst + W::kAhead + 1) * W::kPack <= W::kBeyond, "a turn reads behind what is there twice");
 
         // ---- parts of an iteration
         u32x4 key[W::kSteps];                                    // K operand: token r32, dims 16 s + 8 h ..
@@ -251,7 +262,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void quant_wide_kernel(QuantArgs a)
         if (threadIdx.x == 0) holes = 0;
         __syncthreads();
         look_up(0);
-        for (int i = threadIdx.x; i < kWideStage / 16; i += W::kThreads)
+        for (int i = threadIdx.x; i < W::kStageBytes / 16; i += W::kThreads)
             reinterpret_cast<u32x4 *>(v_stage(-1))[i] = u32x4{0, 0, 0, 0};     // V(-1), which P(-1) = 0 is multiplied by
         __syncthreads();
         if (holes) mask_from = 0;
@@ -261,27 +272,21 @@ __global__ __launch_bounds__(kWaves * 64, 2) void quant_wide_kernel(QuantArgs a)
         asm volatile("" : "+v"(mask));
         // as if there were turns in front
 #pragma unroll
-        for (int u = 0; u < W::kAhead; u++)
+        for (int u = 0; u < W::kAhead; u++) {
+            const uint32_t row = token_of(0, u).x;
+            request(row, k_codes[u], 0);
+            request(row, v_codes[u], a.half_bytes);
+        }
 #pragma unroll
-            for (int i = 0; i < W::kGroups; i++) {
-                const uint32_t row = row_at[token_of(u, i)];
-                request(row, k_codes[u][i], 0);
-                request(row, v_codes[u][i], a.half_bytes);
-            }
+        for (int u = 0; u < W::kFirst; u++) {
+            write(k_codes[u % W::kAhead], token_of(0, u).y & 0xFF, k_stage(u));
+            request(token_of(0, u + W::kAhead).x, k_codes[u % W::kAhead], 0);
+        }
 #pragma unroll
-        for (int u = 0; u < W::kFirst; u++)
-#pragma unroll
-            for (int i = 0; i < W::kGroups; i++) {
-                write(k_codes[u % W::kAhead][i], exponent_at[2 * token_of(u, i)], i, k_stage(u));
-                request(row_at[token_of(u + W::kAhead, i)], k_codes[u % W::kAhead][i], 0);
-            }
-#pragma unroll
-        for (int u = 0; u < W::kBehind; u++)
-#pragma unroll
-            for (int i = 0; i < W::kGroups; i++) {
-                write(v_codes[u][i], exponent_at[2 * token_of(u, i) + 1], i, v_stage(u));
-                request(row_at[token_of(u + W::kAhead, i)], v_codes[u][i], a.half_bytes);
-            }
+        for (int u = 0; u < W::kBehind; u++) {
+            write(v_codes[u], token_of(0, u).y >> 8, v_stage(u));
+            request(token_of(0, u + W::kAhead).x, v_codes[u], a.half_bytes);
+        }
         Known known;
         know(0, known);
         __syncthreads();
@@ -295,13 +300,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void quant_wide_kernel(QuantArgs a)
         auto turn = [&](int u, int phase) {
             constexpr int kMask = W::kAhead - 1;
             const int k_at = (phase + W::kFirst) & kMask, v_at = (phase + W::kBehind) & kMask;
-#pragma unroll
-            for (int i = 0; i < W::kGroups; i++) {
-                write(k_codes[k_at][i], known.k_exponent[i], i, k_stage(u + W::kFirst));
-                write(v_codes[v_at][i], known.v_exponent[i], i, v_stage(u + W::kBehind));
-                request(known.k_row[i], k_codes[k_at][i], 0);
-                request(known.v_row[i], v_codes[v_at][i], a.half_bytes);
-            }
+            write(k_codes[k_at], known.k_exponent, k_stage(u + W::kFirst));
+            write(v_codes[v_at], known.v_exponent, v_stage(u + W::kBehind));
+            request(known.k_row, k_codes[k_at], 0);
+            request(known.v_row, v_codes[v_at], a.half_bytes);
             know(u + 1, known);
         };
         auto meet = [&](int phase) {
