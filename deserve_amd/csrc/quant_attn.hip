@@ -158,7 +158,7 @@ template <int DT, int kD, int kWaves> static int launch_quant_wide(const QuantAr
     hipLaunchKernelGGL((quant_wide_kernel<DT, kD, kWaves>), dim3((unsigned)(f.shares * a.n_kv_heads)), dim3(kWaves * 64), 0, stream, a);
     DSKV_LAUNCH_CHECK("quant_wide_kernel");
     constexpr int kColumns = 256 / (kD / 4) * kMergeEach;                // of a workgroup
-    const dim3 grid((unsigned)(2 * f.shares), (unsigned)a.n_kv_heads, (unsigned)((kWaves * 32 + kColumns - 1) / kColumns));
+    const dim3 grid((unsigned)((kWaves * 32 + kColumns - 1) / kColumns), (unsigned)a.n_kv_heads, (unsigned)(2 * f.shares));
     hipLaunchKernelGGL((quant_merge_kernel<DT, kD, kWaves * 32>), grid, dim3(256), 0, stream, a);
     DSKV_LAUNCH_CHECK("quant_merge_kernel");
     return 0;

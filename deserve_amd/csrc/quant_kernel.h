@@ -23,6 +23,12 @@ struct QuantArgs : TreeArgs {
 };
 __device__ __forceinline__ int rows_taken(const QuantArgs &a, int n) { return n >= a.rows_from && n <= a.rows_to ? n : 0; }
 
+// (beside a chunk there may be many requests that this launch has nothing of; one request in one tile is cut evenly)
+__device__ __forceinline__ bool parts_apply(const QuantArgs &a, int spans, int busy)
+{
+    return busy <= spans && (busy > 1 || a.max_rows * a.group > 128);
+}
+
 constexpr uint32_t kNoQuantRow = 0xFFFFFFFFu;
 // Where token t's K lies in the head's part of the pool, in sixteens of bytes.
 __device__ __forceinline__ uint32_t quant_row(const QuantArgs &a, int t, int page)

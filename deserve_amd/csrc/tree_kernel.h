@@ -109,6 +109,8 @@ struct TreeRequest {
 
 // Of a request's n rows those that a launch computes: here all of them.
 __device__ __forceinline__ int rows_taken(const TreeArgs &, int n) { return n; }
+// Whether a batch is small enough for parts of a common size (see tree_place), with `busy` requests that have rows.
+__device__ __forceinline__ bool parts_apply(const TreeArgs &a, int spans, int busy) { return a.batch > 1 && a.batch <= spans; }
 
 // What the arrays say about request b, within the bounds of the tensors.
 template <int kCols, int kSub, typename A> __device__ __forceinline__ TreeRequest tree_request(const A &a, int b)
@@ -281,7 +283,7 @@ __device__ __forceinline__ void tree_place(const A &a, int share, TreePlace &at)
     int before = (int)((which ? upto[1] : upto[0]) - (which ? mine[1] : mine[0]));
     const bool tells = blockIdx.x == 0;
     if constexpr (kTurn > 0) {
-        if (a.batch > 1 && a.batch <= spans && per == 1 && units > 0) {     // (`parts` is of one request a thread)
+        if (parts_apply(a, spans, requests) && per == 1 && units > 0) {     // (`parts` is of one request a thread)
             const int most = shares.each + (shares.longer > 0);
             const int cut = most <= kLeast ? kLeast : (most + kTurn - 1) / kTurn * kTurn, cut_more = (cut + 2 * kTurn - 1) / kTurn * kTurn;
             const int tiles = which ? (r.col_tiles > 0) : r.col_tiles;
