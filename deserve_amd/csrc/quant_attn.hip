@@ -115,16 +115,16 @@ struct QuantForm {
 };
 constexpr int kQuantUnits = 256;        // compute units
 static bool quant_matrix_form(int head_dim) { return head_dim == 64 || head_dim == 128; }
-static QuantForm quant_form(bool wide, int max_rows, int n_qo_heads, int n_kv_heads, int dtype)
+static QuantForm quant_form(bool wide, int max_rows, int n_qo_heads, int n_kv_heads, int head_dim, int dtype)
 {
     QuantForm f;
     const long cols = (long)max_rows * (n_qo_heads / n_kv_heads);
     f.wide_waves = !wide ? 0 : cols <= 128 ? 4 : 8;
-    const int widest = wide ? f.wide_waves * 32 : quant_columns(dtype);
+    const int widest = wide ? f.wide_waves * 32 : quant_columns(dtype, head_dim);
     f.col_tiles = (int)((cols + widest - 1) / widest);
     f.blocks = wide ? 0 : (int)((cols + 16L * f.col_tiles - 1) / (16L * f.col_tiles));
     f.cols = wide ? widest : f.blocks * 16;
-    const int resident = kQuantUnits * (wide ? (f.wide_waves == 4 ? 2 : 1) : quant_workgroups(dtype, f.blocks));
+    const int resident = kQuantUnits * (wide ? (f.wide_waves == 4 ? 2 : 1) : quant_workgroups(dtype, head_dim, f.blocks));
     f.shares = resident >= n_kv_heads ? resident / n_kv_heads : 1;
     if (f.shares > 8) f.shares = f.shares / 8 * 8;         // (see share_and_head)
     f.sides = wide && f.col_tiles > 1 && f.shares % (8 * f.col_tiles) == 0 ? f.col_tiles : 1;
@@ -133,10 +133,10 @@ static QuantForm quant_form(bool wide, int max_rows, int n_qo_heads, int n_kv_he
 // Requests of so many rows and fewer are the narrow form's (never fewer than one: a request of more columns a row than its tiles
 // hold is in several of them), the others the wide one's, which reads K and V once for all columns.  Where a step has both, those for one block of
 // 16 columns: beside a chunk they are decode rows, which would be padded to three.
-static int narrow_rows(int max_rows, int n_qo_heads, int n_kv_heads, int dtype)
+static int narrow_rows(int max_rows, int n_qo_heads, int n_kv_heads, int head_dim, int dtype)
 {
     if (dtype == DSKV_F32) return INT32_MAX;
-    const int group = n_qo_heads / n_kv_heads, all = std::max(quant_columns(dtype) / group, 1);
+    const int group = n_qo_heads / n_kv_heads, all = std::max(quant_columns(dtype, head_dim) / group, 1);
     return max_rows <= all ? all : std::max(16 / group, 1);
 }
 static int64_t units_bytes(int batch) { return ((int64_t)batch + 7) / 4 * 16; }
@@ -172,11 +172,15 @@ template <int DT, int kD> static int launch_quant_blocks(const QuantArgs &a, con
     switch (f.blocks) {
     case 1: return launch_quant<DT, kD, 1>(a, f, stream);
     case 2: return launch_quant<DT, kD, 2>(a, f, stream);
-    default:
-        if constexpr (quant_columns(DT) >= 48) return launch_quant<DT, kD, 3>(a, f, stream);
-        set_error("quant_attn: no form for %d columns", f.cols);
-        return DSKV_E_INVAL;
+    case 3:
+        if constexpr (quant_columns(DT, kD) >= 48) return launch_quant<DT, kD, 3>(a, f, stream);
+        break;
+    case 4:
+        if constexpr (quant_columns(DT, kD) >= 64) return launch_quant<DT, kD, 4>(a, f, stream);
+        break;
     }
+    set_error("quant_attn: no form for %d columns", f.cols);
+    return DSKV_E_INVAL;
 }
 template <int DT> static int launch_quant_dim(const QuantArgs &a, const QuantForm &f, hipStream_t stream)
 {
@@ -205,11 +209,11 @@ extern "C" int64_t dskv_quant_attn_workspace(int32_t batch, int32_t nnz, int32_t
 {
     using namespace dskv;
     if (batch <= 0 || nnz <= 0 || max_qo_len <= 0 || n_kv_heads <= 0 || n_qo_heads < n_kv_heads || !quant_matrix_form(head_dim)) return 0;
-    const int narrow_most = narrow_rows(max_qo_len, n_qo_heads, n_kv_heads, dtype);
-    const int64_t narrow = form_bytes(quant_form(false, max_qo_len < narrow_most ? max_qo_len : narrow_most, n_qo_heads, n_kv_heads, dtype),
+    const int narrow_most = narrow_rows(max_qo_len, n_qo_heads, n_kv_heads, head_dim, dtype);
+    const int64_t narrow = form_bytes(quant_form(false, max_qo_len < narrow_most ? max_qo_len : narrow_most, n_qo_heads, n_kv_heads, head_dim, dtype),
                                       batch, n_kv_heads, head_dim);
     if (max_qo_len <= narrow_most) return narrow;
-    const int64_t wide = form_bytes(quant_form(true, max_qo_len, n_qo_heads, n_kv_heads, dtype), batch, n_kv_heads, head_dim);
+    const int64_t wide = form_bytes(quant_form(true, max_qo_len, n_qo_heads, n_kv_heads, head_dim, dtype), batch, n_kv_heads, head_dim);
     return narrow > wide ? narrow : wide;
 }
 
@@ -253,10 +257,10 @@ extern "C" int dskv_quant_attn(const dskv_quant_step_t *step, void *out, const v
     a.page_bytes = shape.page_bytes;
     hipStream_t st = (hipStream_t)stream;
     // two launches where some requests have few rows and others many, one after the other over the same workspace
-    const int narrow_most = narrow_rows(s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->dtype);
+    const int narrow_most = narrow_rows(s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->head_dim, s->dtype);
     const bool some_narrow = step->min_qo_len <= narrow_most, some_wide = s->max_qo_len > narrow_most;
-    const QuantForm narrow = quant_form(false, some_wide ? narrow_most : s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->dtype);
-    const QuantForm wide = quant_form(true, s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->dtype);
+    const QuantForm narrow = quant_form(false, some_wide ? narrow_most : s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->head_dim, s->dtype);
+    const QuantForm wide = quant_form(true, s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->head_dim, s->dtype);
     const int64_t col_tiles = some_wide && wide.col_tiles > narrow.col_tiles ? wide.col_tiles : narrow.col_tiles;
     // (places in the pool, tokens of a request and units are numbered in 32 bits there)
     if (quant_matrix_form(s->head_dim) && s->num_pages * (shape.page_bytes / 16) < UINT32_MAX &&

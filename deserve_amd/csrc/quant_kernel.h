@@ -189,9 +189,20 @@ template <int kTerms> __device__ __forceinline__ void split8(const float *f, u32
     }
 }
 
-// Workgroups of a compute unit, with one subtile of a wave in flight.  64 requests over 256 - 4096 tokens, bf16, of one row 52.3 us; with two
-// subtiles in flight 54.5, with those and one workgroup 62.5, with three workgroups 56.7.  Of 5 rows in f16 (two blocks) 71.8; 85.6, 87.8.
-constexpr int quant_workgroups(int dtype, int blocks) { return dtype != DSKV_F32 && blocks <= 2 ? 2 : 1; }
+// Columns of a tile at most; where q's operands lie, in registers or, where these would be too many beside O and the weights' terms, in
+// LDS; and workgroups of a compute unit, with one subtile of a wave in flight.  64 requests over 256 - 4096 tokens, 128 dims:
+//   bf16, one row    52.3 us; with two subtiles in flight 54.5, with those and one workgroup 62.5, with three workgroups 56.7
+//   f16, 5 rows      67 (two blocks); 85.6, 87.8
+//   bf16, 12 rows    113 (three blocks, one workgroup); with two workgroups 128, q in registers or in LDS: they spill
+//   fp32, one row    55.6; with q in registers, one workgroup 69.7.  5 rows 108 (one workgroup); with q in LDS 111
+// and 64 dims: bf16 of 12 rows 54 (three blocks; with one workgroup 78), of 16 rows 66 (four; as wide tiles 79); fp32, one row 38; 51.
+constexpr int quant_columns(int dtype, int dim) { return dtype == DSKV_F32 ? 32 : dim == 64 ? 64 : 48; }
+constexpr bool quant_q_in_lds(int dtype, int dim, int blocks) { return dtype == DSKV_F32 && (dim == 64 || blocks == 1); }
+constexpr int quant_workgroups(int dtype, int dim, int blocks)
+{
+    return dim == 64 || blocks <= (dtype == DSKV_F32 ? 1 : 2) ? 2 : 1;
+}
+
 template <int DT, int kD, int kBlocks> struct QuantTile {
     static constexpr int kElt = DT == DSKV_F32 ? 4 : 2;
     static constexpr int kSub = 32;                                  // tokens of a subtile
@@ -207,18 +218,19 @@ template <int DT, int kD, int kBlocks> struct QuantTile {
     static constexpr int kPitch = kD + 16;                           // bytes; 16 rows' chunks at one offset meet no bank twice
     static constexpr int kWaveLds = 2 * kSub * kPitch + 2 * kSub * 4;      // K, V, their scales
     static constexpr int kOPitch = kD + 4;                           // floats
+    static constexpr bool kQInLds = quant_q_in_lds(DT, kD, kBlocks);
+    static constexpr int kQLds = kQInLds ? kBlocks * kSteps * kQTerms * 1024 : 0;
     static constexpr int kMergeLds = kTreeWaves * kCols * (kOPitch + 2) * 4;
     static constexpr int kLds = kTreeWaves * kWaveLds > kMergeLds ? kTreeWaves * kWaveLds : kMergeLds;
-    static constexpr int kWorkgroups = quant_workgroups(DT, kBlocks);      // of a compute unit
+    static constexpr int kWorkgroups = quant_workgroups(DT, kD, kBlocks);
     static constexpr int kDepth = 1;                                 // subtiles a wave has in flight
 };
-constexpr int quant_columns(int dtype) { return dtype == DSKV_F32 ? 32 : 48; }
 
 template <int DT, int kD, int kBlocks>
 __global__ __launch_bounds__(kTreeThreads, (QuantTile<DT, kD, kBlocks>::kWorkgroups)) void quant_matrix_kernel(QuantArgs a)
 {
     typedef QuantTile<DT, kD, kBlocks> S;
-    __shared__ __align__(16) char lds[S::kLds];
+    __shared__ __align__(16) char lds[S::kLds + S::kQLds];
     __shared__ int last_part;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, c = lane & 15;
@@ -305,6 +317,7 @@ __global__ __launch_bounds__(kTreeThreads, (QuantTile<DT, kD, kBlocks>::kWorkgro
     it.r = place.r;
     int cols, prior, st;
     u32x4 q[kBlocks][S::kSteps][S::kQTerms];                    // step 2 h + s: dims 64 h + 16 g + 8 s .. of the column
+    u32x4 *const q_lds = reinterpret_cast<u32x4 *>(lds + S::kLds) + lane;
     unsigned long long mask[kBlocks];
     int limit[kBlocks];
     f32x4 o[kBlocks][S::kDimTiles];
@@ -324,6 +337,7 @@ __global__ __launch_bounds__(kTreeThreads, (QuantTile<DT, kD, kBlocks>::kWorkgro
             const int apart = there ? 1 : 0;
 #pragma unroll
             for (int e = 0; e < S::kSteps; e++) {
+                if (S::kQInLds && (k * S::kSteps + e) % kTreeWaves != wave) continue;      // each wave a few
                 const char *at = row + apart * ((e >> 1) * 64 + (e & 1) * 8) * S::kElt;
                 q[k][e][0] = *(global_chunk_ptr)at;
                 if constexpr (DT == DSKV_F32) q[k][e][1] = *(global_chunk_ptr)(at + 16);
@@ -344,6 +358,7 @@ __global__ __launch_bounds__(kTreeThreads, (QuantTile<DT, kD, kBlocks>::kWorkgro
         for (int k = 0; k < kBlocks; k++) {
 #pragma unroll
             for (int e = 0; e < S::kSteps; e++) {
+                if (S::kQInLds && (k * S::kSteps + e) % kTreeWaves != wave) continue;
                 if constexpr (DT == DSKV_F32) {
                     float f[8];
                     Chunk<DSKV_F32>::unpack(q[k][e][0], f);
@@ -351,9 +366,14 @@ __global__ __launch_bounds__(kTreeThreads, (QuantTile<DT, kD, kBlocks>::kWorkgro
                     split8<3>(f, q[k][e]);
                 }
                 asm volatile("" : "+v"(q[k][e][0]));
+                if constexpr (S::kQInLds) {
+#pragma unroll
+                    for (int i = 0; i < S::kQTerms; i++) q_lds[((k * S::kSteps + e) * S::kQTerms + i) * 64] = q[k][e][i];
+                }
             }
             asm volatile("" : "+v"(mask[k]));
         }
+        if (S::kQInLds) __syncthreads();
     };
     auto subtile = [&](Held &mine) {
         const bool there = st < it.st1;                         // (else a turn without a subtile)
@@ -404,7 +424,9 @@ __global__ __launch_bounds__(kTreeThreads, (QuantTile<DT, kD, kBlocks>::kWorkgro
 #pragma unroll
                 for (int k = 0; k < kBlocks; k++)
 #pragma unroll
-                    for (int i = 0; i < S::kQTerms; i++) s[k][t] = Elt<S::kKeyType>::mfma_k32(x, q[k][e][i], s[k][t]);
+                    for (int i = 0; i < S::kQTerms; i++)
+                        s[k][t] = Elt<S::kKeyType>::mfma_k32(
+                            x, S::kQInLds ? q_lds[((k * S::kSteps + e) * S::kQTerms + i) * 64] : q[k][e][i], s[k][t]);
             }
         }
         // V's codes: eight of a lane along the tokens for every 16 dims, in the order that the scores have them: 4 g .. 4 g + 3 and
