@@ -128,11 +128,18 @@ __global__ __launch_bounds__(256, 4) void quant_append_kernel(QuantAppend a)
     const int head = blockIdx.y * 4 + (threadIdx.x >> 6);
     if (head >= s.n_kv_heads) return;
     int b = request_of_row(a.r.qo_indptr, a.r.batch, t0);
-    if (b < 0) return;
+    if (b < 0) {
+        if (t0 >= a.r.qo_indptr[0]) return;                               // rows behind the last request
+        b = 0;
+    }
     for (int t = t0; t < t1;) {
         while (b < a.r.batch && a.r.qo_indptr[b + 1] <= t) b++;           // on to the request of row t
         if (b == a.r.batch) return;
         const QuantRequest r = quant_request(a.r, b);
+        if (r.n > 0 && r.first > t) {                                     // rows in front of the first request
+            t = r.first;
+            continue;
+        }
         if (r.n == 0) {                                                   // its arrays contradict themselves
             const int next = a.r.qo_indptr[b + 1];
             if (next <= t) return;

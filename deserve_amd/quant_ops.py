@@ -22,7 +22,7 @@ import ctypes
 import functools
 import math
 from dataclasses import dataclass
-from typing import Optional
+from typing import List, Optional
 
 import torch
 
@@ -108,7 +108,7 @@ def rope_append_quantized(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.T
     A block's scale is the least power of two that its largest value takes to 448 or less, never less than that of the tokens it
     holds already, whose codes are rounded anew where it grows.  A token with a value that is no finite number makes no number of the rows
     that see it, and nothing else.  A request whose arrays contradict themselves, or a page that the pool does not have,
-    takes no rows.  No page takes rows of two requests."""
+    takes no rows.  No page takes rows of two requests, or of two entries of a table."""
     if k.dim() != 3:
         raise ValueError(f"k must be (tokens, heads, D), got {tuple(k.shape)}")
     nnz, hkv, dim = k.shape
@@ -159,7 +159,9 @@ class BatchQuantizedWithPagedKVCacheWrapper:
         if kv_layout != "HND":
             raise ValueError("8-bit pages hold their tokens by head: only the HND layout is implemented")
         self._workspace = workspace_buffer
-        # what the parts of a request count themselves in with: zero between launches, kept for good (captured ones hold its address)
+        # what the parts of a request count themselves in with: zero between launches, and kept for good, also where more heads
+        # ask for more words (captured launches hold their address)
+        self._all_counters: List[torch.Tensor] = []
         self._counters = self._zeros(_lib.lib().dskv_quant_attn_counters(1))
         self._step: Optional[_lib.QuantStep] = None
         self._held: tuple = ()
@@ -173,6 +175,7 @@ class BatchQuantizedWithPagedKVCacheWrapper:
         with torch.cuda.device(device):
             zeros = torch.zeros((n,), dtype=torch.int32, device=device)
             torch.cuda.current_stream().synchronize()        # whatever stream uses them first
+        self._all_counters.append(zeros)
         return zeros
 
     def another(self) -> "BatchQuantizedWithPagedKVCacheWrapper":

@@ -247,3 +247,34 @@ def test_append_attention_and_moves_replayed():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, eager) and torch.equal(pages, eager_pages), i
+
+
+@pytest.mark.parametrize("n", [[3, 20, 1], [700, 1, 400]], ids=["few", "many"])
+def test_rows_in_front_of_the_first_request(n):
+    """Rows that are no request's, in front: the others go where they went without them, in waves of one row and of several."""
+    from deserve_amd.quant_ops import rope_append_quantized
+
+    step = make_step(29, [13, 7, 0], n, False, 16, 8, 8, 64, "bf16")
+    k, v = (rows(s, step, torch.bfloat16).cuda() for s in (1, 2))
+    qo, indptr, indices, last = step.on("cuda")["csr"]
+    got = []
+    for front in (0, 5):
+        pages = as_quantised(step)[0].tensor().cuda()
+        x, y = (torch.cat([t[:front] * float("nan"), t]) for t in (k, v))
+        rope_append_quantized(None, x, y, qo + front, pages, indices, indptr, last, 16)
+        got.append(pages)
+    assert torch.equal(*got)
+
+
+def test_counters_of_a_captured_step_outlive_a_wider_one():
+    """A wrapper that is given more heads than its counters are for, after a capture with fewer."""
+    from deserve_amd.quant_ops import BatchQuantizedWithPagedKVCacheWrapper
+
+    step, wide = make_step(31, [3000], [1], False, 16, 8, 2, 128, "bf16"), make_step(32, [30], [1], False, 4, 600, 600, 64, "bf16")
+    w = BatchQuantizedWithPagedKVCacheWrapper(torch.empty(128 << 20, dtype=torch.uint8, device="cuda"))
+    first, on = w._counters.data_ptr(), wide.on("cuda")
+    w.begin_forward(*on["csr"], 600, 600, 64, 4, max_qo_len=1)
+    w.forward(on["q"], as_quantised(wide)[0].tensor().cuda())
+    w.end_forward()
+    assert w._counters.data_ptr() != first and first in [t.data_ptr() for t in w._all_counters]
+    near(run(step, as_quantised(step)[0].tensor().cuda()), *attention(as_quantised(step)[1]))
