@@ -193,10 +193,10 @@ template <int kTerms> __device__ __forceinline__ void split8(const float *f, u32
 // LDS; and workgroups of a compute unit, with one subtile of a wave in flight.  64 requests over 256 - 4096 tokens, 128 dims:
 //   bf16, one row    52.3 us; with two subtiles in flight 54.5, with those and one workgroup 62.5, with three workgroups 56.7
 //   f16, 5 rows      67 (two blocks); 85.6, 87.8
-//   bf16, 12 rows    113 (three blocks, one workgroup); with two workgroups 128, q in registers or in LDS: they spill
 //   fp32, one row    55.6; with q in registers, one workgroup 69.7.  5 rows 108 (one workgroup); with q in LDS 111
 // and 64 dims: bf16 of 12 rows 54 (three blocks; with one workgroup 78), of 16 rows 66 (four; as wide tiles 79); fp32, one row 38; 51.
-constexpr int quant_columns(int dtype, int dim) { return dtype == DSKV_F32 ? 32 : dim == 64 ? 64 : 48; }
+// (With 128 dims three blocks leave registers for one workgroup only, 113 us for 12 rows; see QuantWide.)
+constexpr int quant_columns(int dtype, int dim) { return dtype == DSKV_F32 || dim == 128 ? 32 : 64; }
 constexpr bool quant_q_in_lds(int dtype, int dim, int blocks) { return dtype == DSKV_F32 && (dim == 64 || blocks == 1); }
 constexpr int quant_workgroups(int dtype, int dim, int blocks)
 {

@@ -22,20 +22,24 @@ constexpr int kWideRegion = 1088;           // 64 chunks of 16 bytes, (4 chunk +
 constexpr int kWideStage = kWideBlock / 4 * kWideRegion;
 constexpr int kWideLeast = 8;               // units a share has at least: what fills the stages takes about as long
 
-template <int kD, int kWaves> struct QuantWide {
+// kFetch: waves without columns that fetch for the others, more stages ahead than there would be registers for beside O and q; 0: all do
+// both.  64 requests of 12 rows over 256 - 4096 tokens, 128 dims, two waves of columns and two that fetch: 106 us; 113 in the narrow form with three
+// blocks of columns a tile, and one such request over 4000 tokens 23.4 and 40.
+template <int kD, int kWaves, int kFetch> struct QuantWide {
     static constexpr int kThreads = kWaves * 64;
-    static constexpr int kCols = kWaves * 32;
+    static constexpr int kCompute = kWaves - kFetch, kCols = kCompute * 32;
+    static constexpr int kFetchThreads = (kFetch ? kFetch : kWaves) * 64;
     // A stage is what the workgroup's lanes fetch at once, kLane bytes each: one block or two, which lie one after the other in LDS, or, with
     // 64 dims, side by side in rows of 128
     static constexpr int kPack = kD == 128 && kWaves == 4 ? 1 : 2;
-    static constexpr int kLane = kPack * kWideBlock * kD / kThreads;
+    static constexpr int kLane = kPack * kWideBlock * kD / kFetchThreads;
     static constexpr int kLaneRows = 64 * kLane / kD;    // tokens that a wave fetches
     static constexpr int kStageBytes = kD == 128 ? kPack * kWideStage : kWideStage;
     static constexpr int kSteps = kD / 16, kDims = kD / 32;      // matrix instructions of a block's scores; 32-dim tiles of O
     static constexpr int kHalf = kWaves == 8 ? 64 : 32;  // blocks that are looked up at a time; two such halves are kept
     static constexpr int kTokens = 2 * kHalf * kWideBlock, kBeyond = 12;
     static constexpr int kKStages = kPack == 2 ? 2 : 4, kVStages = kPack == 2 ? 4 : 2;      // in LDS
-    static constexpr int kAhead = kD == 128 && kPack == 2 ? 1 : 2;       // stages of K, and of V, on their way in registers
+    static constexpr int kAhead = kFetch ? 8 : kD == 128 && kPack == 2 ? 1 : 2;      // stages of K, and of V, on their way in registers
     // what turn u (in front of the iterations of stage u) writes: K(u + kFirst) and V(u + kBehind)
     static constexpr int kFirst = kPack == 2 ? 2 : 3, kBehind = kPack - 1;
 };
@@ -46,11 +50,11 @@ struct QuantCut {
     QuantParts parts;    // n < 2: none
 };
 
-template <int DT, int kD, int kWaves>
+template <int DT, int kD, int kWaves, int kFetch>
 __global__ __launch_bounds__(kWaves * 64, 2) void quant_wide_kernel(QuantArgs a)
 {
     typedef Elt<DT> E;
-    typedef QuantWide<kD, kWaves> W;
+    typedef QuantWide<kD, kWaves, kFetch> W;
     __shared__ __align__(16) char lds[(W::kKStages + W::kVStages) * W::kStageBytes];
     // Where a token's K lies (see quant_row), and the exponents of its scales, V's in the second byte; behind the two halves the first
     // kBeyond blocks again, so that what a turn reads lies at fixed distances
@@ -78,7 +82,9 @@ __global__ __launch_bounds__(kWaves * 64, 2) void quant_wide_kernel(QuantArgs a)
         return W::kPack == 2 ? stage(j >> 1) + (j & 1) * (kD == 128 ? kWideStage : 512) : stage(j);
     };
     // lane p of a wave fetches part p / kLaneRows of token p % kLaneRows of its tokens of a stage
-    const int my_token = wave * W::kLaneRows + lane % W::kLaneRows, my_part = lane / W::kLaneRows;
+    const bool fetches = kFetch == 0 || wave >= W::kCompute;
+    const int my_token = (kFetch == 0 ? wave : fetches ? wave - W::kCompute : 0) * W::kLaneRows + lane % W::kLaneRows;
+    const int my_part = lane / W::kLaneRows;
     const char *const pool = a.pages + head * a.head_bytes + my_part * W::kLane;
     const int my_row = my_token % kWideBlock, my_block = my_token / kWideBlock, my_chunk = my_part * (W::kLane / 8);
     const int my_place = kD == 128 ? my_block * kWideStage + my_row / 4 * kWideRegion + (4 * my_chunk + my_row % 4) * 16
@@ -270,32 +276,26 @@ __global__ __launch_bounds__(kWaves * 64, 2) void quant_wide_kernel(QuantArgs a)
 #pragma unroll
         for (int s = 0; s < W::kSteps; s++) asm volatile("" : "+v"(q[s]));
         asm volatile("" : "+v"(mask));
-        // as if there were turns in front
-#pragma unroll
-        for (int u = 0; u < W::kAhead; u++) {
-            const uint32_t row = token_of(0, u).x;
-            request(row, k_codes[u], 0);
-            request(row, v_codes[u], a.half_bytes);
-        }
-#pragma unroll
-        for (int u = 0; u < W::kFirst; u++) {
-            write(k_codes[u % W::kAhead], token_of(0, u).y & 0xFF, k_stage(u));
-            request(token_of(0, u + W::kAhead).x, k_codes[u % W::kAhead], 0);
-        }
-#pragma unroll
-        for (int u = 0; u < W::kBehind; u++) {
-            write(v_codes[u], token_of(0, u).y >> 8, v_stage(u));
-            request(token_of(0, u + W::kAhead).x, v_codes[u], a.half_bytes);
-        }
         Known known;
-        know(0, known);
-        __syncthreads();
-        if (works) {
-            read_keys(block_at(k_stage, 0));
-            scores(xs[0]);
-            if ((st0 + 1) * kWideBlock > mask_from) mask_scores(0, xs[0]);
-            read_keys(block_at(k_stage, 1));
-        }
+        auto fill = [&]() {                              // as if there were turns in front
+#pragma unroll
+            for (int u = 0; u < W::kAhead; u++) {
+                const uint32_t row = token_of(0, u).x;
+                request(row, k_codes[u], 0);
+                request(row, v_codes[u], a.half_bytes);
+            }
+#pragma unroll
+            for (int u = 0; u < W::kFirst; u++) {
+                write(k_codes[u % W::kAhead], token_of(0, u).y & 0xFF, k_stage(u));
+                request(token_of(0, u + W::kAhead).x, k_codes[u % W::kAhead], 0);
+            }
+#pragma unroll
+            for (int u = 0; u < W::kBehind; u++) {
+                write(v_codes[u], token_of(0, u).y >> 8, v_stage(u));
+                request(token_of(0, u + W::kAhead).x, v_codes[u], a.half_bytes);
+            }
+            know(0, known);
+        };
         // phase: u up to a multiple of kAhead, a literal
         auto turn = [&](int u, int phase) {
             constexpr int kMask = W::kAhead - 1;
@@ -329,7 +329,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void quant_wide_kernel(QuantArgs a)
                     va[d][s] = u32x4{lo.x, lo.y, hi.x, hi.y};
                 }
             scores(xs[nxt]);                                                        // S(j + 1)
-            if (turns) turn(j / W::kPack, phase / W::kPack);
+            if (kFetch == 0 && turns) turn(j / W::kPack, phase / W::kPack);
             float sum = 0;
             weights(xs[cur], 0, pb[cur][0], sum);
             if ((st0 + j + 2) * kWideBlock > mask_from) mask_scores(j + 1, xs[nxt]);
@@ -351,7 +351,13 @@ __global__ __launch_bounds__(kWaves * 64, 2) void quant_wide_kernel(QuantArgs a)
         auto look_ahead = [&](int j) {                   // (the turns look up to 12 blocks behind the last one, too)
             if (j % W::kHalf == W::kHalf / 2 && j + W::kHalf / 2 < blocks + 16) look_up(j / W::kHalf + 1);
         };
+        if constexpr (kFetch == 0) fill();
+        if (kFetch == 0 || !fetches) __syncthreads();
         if (works) {
+            read_keys(block_at(k_stage, 0));
+            scores(xs[0]);
+            if ((st0 + 1) * kWideBlock > mask_from) mask_scores(0, xs[0]);
+            read_keys(block_at(k_stage, 1));
             for (int j = 0;; j += 4) {
                 look_ahead(j);
                 iteration(j, 0);
@@ -364,15 +370,29 @@ __global__ __launch_bounds__(kWaves * 64, 2) void quant_wide_kernel(QuantArgs a)
                 iteration(j + 3, 3);
                 if (j + 3 >= blocks) break;
             }
-        } else {
+        } else if (fetches) {
             // a wave without columns only fetches
+            if constexpr (kFetch != 0) {
+                fill();
+                __syncthreads();
+            }
             auto passes = [&](int j, int phase) {
                 if (meet(phase)) turn(j / W::kPack, phase / W::kPack);
                 return j >= blocks;
             };
-            for (int j = 0;; j += 4) {
+            for (int j = 0;; j += kFetch ? 8 : 4) {
                 look_ahead(j);
                 if (passes(j, 0) || passes(j + 1, 1) || passes(j + 2, 2) || passes(j + 3, 3)) break;
+                if constexpr (kFetch != 0) {
+                    look_ahead(j + 4);
+                    if (passes(j + 4, 4) || passes(j + 5, 5) || passes(j + 6, 6) || passes(j + 7, 7)) break;
+                }
+            }
+        } else {
+            // a wave that would have columns, of a tile that has fewer
+            for (int j = 0; j <= blocks; j++) {
+                look_ahead(j);
+                meet(0);
             }
         }
 

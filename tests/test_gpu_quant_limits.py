@@ -17,6 +17,11 @@ SHAPES = [
     ("one_kv_head_64", [100, 0, 33], [1, 1, 3], False, 16, 64, 1, 128, "bf16"),
     ("one_kv_head_71", [100, 0, 33], [1, 1, 3], False, 16, 71, 1, 64, "f16"),
     ("one_kv_head_130_fp32", [100, 0], [1, 2], False, 16, 130, 1, 64, "fp32"),
+    ("one_kv_head_33", [100, 0, 700], [2, 1, 1], False, 16, 33, 1, 128, "bf16"),
+    ("one_kv_head_40_chunk", [100, 0, 700], [1, 50, 1], False, 16, 40, 1, 128, "f16"),
+    ("9_rows", [700, 20, 0, 1300], [9, 1, 8, 5], True, 16, 8, 2, 128, "bf16"),
+    ("16_rows", [700, 20, 0, 1300], [16, 1, 8, 15], False, 12, 8, 2, 128, "f16"),
+    ("12_rows_long", [9000, 3], [12, 9], False, 16, 4, 1, 128, "bf16"),
     ("kv_heads_600", [37, 5], [1, 2], False, 4, 600, 600, 64, "bf16"),
     ("kv_heads_600_chunk", [9], [70], False, 8, 600, 600, 64, "bf16"),
     ("page_256", [300, 255, 256], [1, 1, 130], False, 256, 8, 2, 128, "bf16"),
@@ -45,7 +50,7 @@ def test_shapes(case):
 
 
 @pytest.mark.parametrize("scale", [0.02, 0.4])
-@pytest.mark.parametrize("dim,n", [(128, 2), (128, 60), (80, 2)])
+@pytest.mark.parametrize("dim,n", [(128, 2), (128, 60), (128, 14), (80, 2)])
 def test_scale_and_hints(dim, n, scale):
     """Another scale; hints that are not kept, which leave out nothing but rows behind max_qo_len."""
     step = make_step(22, [300, 40, 7], [n, 1, n], False, 16, 8, 2, dim, "bf16")
@@ -62,7 +67,7 @@ def test_scale_and_hints(dim, n, scale):
     assert torch.isnan(got[n - 1]).all() and torch.isnan(got[2 * n]).all()
 
 
-@pytest.mark.parametrize("dtype,dim,n", [("bf16", 128, 2), ("f16", 128, 60), ("bf16", 64, 30), ("fp32", 128, 2), ("bf16", 80, 2)])
+@pytest.mark.parametrize("dtype,dim,n", [("bf16", 128, 2), ("f16", 128, 60), ("bf16", 128, 14), ("bf16", 64, 30), ("fp32", 128, 2), ("bf16", 80, 2)])
 def test_rows_of_q_that_are_none(dtype, dim, n):
     """A NaN or an infinity in one head of a row: that head has no number, the others are right."""
     step = make_step(23, [200, 31], [n, 1], False, 16, 8, 2, dim, dtype)

@@ -1,5 +1,6 @@
 """Refusals of the operators over 8-bit pages, before anything is launched (all on the CPU)."""
 import ctypes
+import itertools
 
 import pytest
 import torch
@@ -147,3 +148,14 @@ def test_c_entries():
     assert lib.dskv_quant_attn_workspace(0, 2, 2, 32, 8, 128, 2) == 0 == lib.dskv_quant_attn_workspace(1, 2, 2, 32, 8, 80, 2)
     assert lib.dskv_quant_attn_counters(8) == 1024 and lib.dskv_quant_attn_counters(1000) == 2000 and lib.dskv_quant_attn_counters(0) == 0
     assert lib.dskv_quant_attn(None, 16, 16, 4096, 16, None) == _lib.E_INVAL
+
+
+def test_workspaces_of_all_forms():
+    """Every pair of heads, rows and type has a form and asks for a workspace; head dims without a matrix form ask for none."""
+    lib = _lib.lib()
+    for dtype in (_lib.F32, _lib.F16, _lib.BF16):
+        for hkv, group in itertools.product((1, 2, 8, 600), (1, 2, 4, 7, 16, 17, 31, 32, 33, 48, 64, 65, 71, 128, 130)):
+            for rows in (1, 2, 5, 8, 9, 16, 17, 64, 128, 2000):
+                for dim in (64, 128):
+                    assert lib.dskv_quant_attn_workspace(8, 8 * rows, rows, hkv * group, hkv, dim, dtype) > 0
+                assert lib.dskv_quant_attn_workspace(8, 8 * rows, rows, hkv * group, hkv, 80, dtype) == 0
