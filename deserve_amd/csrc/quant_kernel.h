@@ -104,10 +104,61 @@ __device__ __forceinline__ void put_result(const QuantArgs &a, const TreeRequest
     if constexpr (DT == DSKV_F32) *reinterpret_cast<f32x4 *>(dst) = acc * inv;
     else *reinterpret_cast<u32x2 *>(dst) = u32x2{Elt<DT>::pack2(acc.x * inv, acc.y * inv), Elt<DT>::pack2(acc.z * inv, acc.w * inv)};
 }
+// kEach quads of dims a thread, of x and every kThreads-th behind it, and kAtOnce parts requested together.
+template <int DT, int kD, int kCols, int kThreads, int kEach, int kAtOnce>
+__device__ __forceinline__ void merge_parts(const QuantArgs &a, const TreePlace &place, const TreeRequest &r, const QuantParts &p,
+                                            int head, int ct, int cols, int x)
+{
+    constexpr int kQuads = kD / 4;
+    float top[kEach], sum[kEach];
+    f32x4 acc[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; e++) {
+        top[e] = -INFINITY;
+        sum[e] = 0;
+        acc[e] = f32x4{0, 0, 0, 0};
+    }
+    for (int i0 = 0; i0 < p.n; i0 += kAtOnce) {
+        f32x4 o[kAtOnce][kEach];
+        f32x2 ml[kAtOnce][kEach];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; i++) {
+            const PartSlot<kCols, kD> part(a, head, part_slot(a, place, p, ct, min(i0 + i, p.n - 1)));
+#pragma unroll
+            for (int e = 0; e < kEach; e++) {
+                const int col = min((x + e * kThreads) / kQuads, cols - 1);
+                ml[i][e] = part.get_ml(col);
+                o[i][e] = part.get_o(col, x % kQuads * 4);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < kEach; e++) {
+            float m = top[e];
+#pragma unroll
+            for (int i = 0; i < kAtOnce; i++) m = fmaxf(m, ml[i][e].x);
+            const float from = m == -INFINITY ? 0.f : m, keep = __builtin_amdgcn_exp2f(top[e] - from);
+            top[e] = m;
+            sum[e] *= keep;
+            acc[e] *= keep;
+#pragma unroll
+            for (int i = 0; i < kAtOnce; i++)
+                if (i0 + i < p.n) {
+                    const float w = __builtin_amdgcn_exp2f(ml[i][e].x - from);
+                    sum[e] += ml[i][e].y * w;
+                    acc[e] += o[i][e] * w;
+                }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < kEach; e++) {
+        const int col = (x + e * kThreads) / kQuads;
+        if (col < cols) put_result<DT, kD>(a, r, head, ct * kCols + col, x % kQuads * 4, acc[e], sum[e]);
+    }
+}
 // By all threads of a workgroup, behind its stores of a part's partial.  last: a word of LDS.
-template <int DT, int kD, int kCols, int kThreads, int kAtOnce>
+template <int DT, int kD, int kCols, int kThreads>
 __device__ __forceinline__ void join_parts(const QuantArgs &a, const TreePlace &place, const TreeRequest &r, const QuantParts &p,
-                                           int head, int ct, int col0, int cols, int *last)
+                                           int head, int ct, int cols, int *last)
 {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");               // the partial is where other XCDs see it
     __syncthreads();
@@ -120,37 +171,13 @@ __device__ __forceinline__ void join_parts(const QuantArgs &a, const TreePlace &
     __syncthreads();
     if (!*last) return;
     asm volatile("" ::: "memory");
-    constexpr int kQuads = kD / 4;
-    for (int x = threadIdx.x; x < cols * kQuads; x += kThreads) {
-        const int col = x / kQuads, dim = x % kQuads * 4;
-        float top = -INFINITY, sum = 0;
-        f32x4 acc = {0, 0, 0, 0};
-        for (int i0 = 0; i0 < p.n; i0 += kAtOnce) {
-            f32x4 o[kAtOnce];
-            f32x2 ml[kAtOnce];
-#pragma unroll
-            for (int i = 0; i < kAtOnce; i++) {
-                const PartSlot<kCols, kD> part(a, head, part_slot(a, place, p, ct, min(i0 + i, p.n - 1)));
-                ml[i] = part.get_ml(col);
-                o[i] = part.get_o(col, dim);
-            }
-            float m = top;
-#pragma unroll
-            for (int i = 0; i < kAtOnce; i++) m = fmaxf(m, ml[i].x);
-            const float from = m == -INFINITY ? 0.f : m, keep = __builtin_amdgcn_exp2f(top - from);
-            top = m;
-            sum *= keep;
-            acc *= keep;
-#pragma unroll
-            for (int i = 0; i < kAtOnce; i++)
-                if (i0 + i < p.n) {
-                    const float w = __builtin_amdgcn_exp2f(ml[i].x - from);
-                    sum += ml[i].y * w;
-                    acc += o[i] * w;
-                }
-        }
-        put_result<DT, kD>(a, r, head, col0 + col, dim, acc, sum);
-    }
+    // few parts: all columns together; many: parts together
+    constexpr int kQuads = kD / 4, kEach = kCols * kQuads / kThreads;
+    static_assert(kThreads % kQuads == 0 && kCols * kQuads % kThreads == 0, "a thread's quads lie at one place of their columns");
+    const int x = threadIdx.x;
+    if (p.n <= 4 && cols * kQuads > kThreads) merge_parts<DT, kD, kCols, kThreads, kEach, 2>(a, place, r, p, head, ct, cols, x);
+    else
+        for (int y = x; y < cols * kQuads; y += kThreads) merge_parts<DT, kD, kCols, kThreads, 1, 8>(a, place, r, p, head, ct, cols, y);
 }
 
 // 8 codes as a matrix operand of type T
@@ -541,8 +568,8 @@ __global__ __launch_bounds__(kTreeThreads, (QuantTile<DT, kD, kBlocks>::kWorkgro
         }
         if (cut) {
             const int item = it.base + it.ct * it.r.subtiles;
-            join_parts<DT, kD, S::kCols, kTreeThreads, 8>(a, place, it.r, parts_of(a, place, item, it.r.subtiles, it.ct), head, it.ct,
-                                                          it.ct * S::kCols, cols, &last_part);
+            join_parts<DT, kD, S::kCols, kTreeThreads>(a, place, it.r, parts_of(a, place, item, it.r.subtiles, it.ct), head, it.ct,
+                                                       cols, &last_part);
         }
         __syncthreads();
     };
