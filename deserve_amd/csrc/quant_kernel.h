@@ -95,12 +95,12 @@ template <int kCols, int kD> struct PartSlot {
 };
 // Four dims of a column's row.
 template <int DT, int kD>
-__device__ __forceinline__ void put_result(const QuantArgs &a, const TreeRequest &r, int head, int at, int dim, f32x4 acc, float sum)
+__device__ __forceinline__ void put_result(const QuantArgs &a, long first, int head, int at, int dim, f32x4 acc, float sum)
 {
     constexpr int kElt = DT == DSKV_F32 ? 4 : 2;
     const int i = (int)((unsigned)at / (unsigned)a.group), hq = head * a.group + at - i * a.group;
     const float inv = sum == 0 ? 0.f : 1.f / sum;
-    char *dst = a.out + (((r.first + i) * a.n_qo_heads + hq) * kD + dim) * kElt;
+    char *dst = a.out + (((first + i) * a.n_qo_heads + hq) * kD + dim) * kElt;
     if constexpr (DT == DSKV_F32) *reinterpret_cast<f32x4 *>(dst) = acc * inv;
     else *reinterpret_cast<u32x2 *>(dst) = u32x2{Elt<DT>::pack2(acc.x * inv, acc.y * inv), Elt<DT>::pack2(acc.z * inv, acc.w * inv)};
 }
@@ -152,7 +152,7 @@ __device__ __forceinline__ void merge_parts(const QuantArgs &a, const TreePlace 
 #pragma unroll
     for (int e = 0; e < kEach; e++) {
         const int col = (x + e * kThreads) / kQuads;
-        if (col < cols) put_result<DT, kD>(a, r, head, ct * kCols + col, x % kQuads * 4, acc[e], sum[e]);
+        if (col < cols) put_result<DT, kD>(a, r.first, head, ct * kCols + col, x % kQuads * 4, acc[e], sum[e]);
     }
 }
 // By all threads of a workgroup, behind its stores of a part's partial.  last: a word of LDS.
@@ -563,7 +563,7 @@ __global__ __launch_bounds__(kTreeThreads, (QuantTile<DT, kD, kBlocks>::kWorkgro
                 part.put_o(col, quad * 4, acc);
                 if (quad == 0) part.put_ml(col, top, sum);
             } else {
-                put_result<DT, kD>(a, it.r, head, it.ct * S::kCols + col, quad * 4, acc, sum);
+                put_result<DT, kD>(a, it.r.first, head, it.ct * S::kCols + col, quad * 4, acc, sum);
             }
         }
         if (cut) {

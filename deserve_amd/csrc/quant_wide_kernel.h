@@ -46,8 +46,9 @@ template <int kD, int kWaves, int kFetch> struct QuantWide {
 
 // An item that begins in a share and ends in another.
 struct QuantCut {
-    int b, ct;
-    QuantParts parts;    // n < 2: none
+    int first, col0, cols, ct;      // row of q that the request begins with; the tile's first column and how many it has
+    bool beside;
+    QuantParts parts;               // n < 2: none
 };
 
 template <int DT, int kD, int kWaves, int kFetch>
@@ -422,7 +423,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void quant_wide_kernel(QuantArgs a)
                               E::pack2(acc[d][4 * i + 2] * inv, acc[d][4 * i + 3] * inv)};
         }
         // an item that goes on in another share is the merge launch's
-        if (cut && st0 == 0 && head == 0 && threadIdx.x == 0) a.cuts[2 * share + (unit > begin ? 1 : 0)] = {b, ct, parts_of(a, place, item, r.subtiles, ct)};
+        if (cut && st0 == 0 && head == 0 && threadIdx.x == 0) 
+            a.cuts[2 * share + (unit > begin ? 1 : 0)] = {(int)r.first, ct * r.tile, cols, ct, beside, parts_of(a, place, item, r.subtiles, ct)};
         unit = item + st1;
     }
 }
@@ -436,12 +438,10 @@ __global__ __launch_bounds__(256) void quant_merge_kernel(QuantArgs a)
     const QuantCut cut = a.cuts[blockIdx.z];
     if (cut.parts.n < 2) return;
     const int head = blockIdx.y, quad = threadIdx.x % kQuads, column = threadIdx.x / kQuads;
-    const TreeRequest r = tree_request<kCols, kWideBlock>(a, cut.b);
-    const int cols = min(r.n * a.group - cut.ct * r.tile, r.tile), col0 = (int)blockIdx.x * kColumns * kEach + column;
+    const int cols = cut.cols, col0 = (int)blockIdx.x * kColumns * kEach + column;
     if ((int)blockIdx.x * kColumns * kEach >= cols) return;
-    const bool beside = a.units_before[a.batch + 1] != 0;
     TreePlace place;
-    place.beside = beside;
+    place.beside = cut.beside;
     float top[kEach], sum[kEach];
     f32x4 acc[kEach];
 #pragma unroll
@@ -489,7 +489,7 @@ __global__ __launch_bounds__(256) void quant_merge_kernel(QuantArgs a)
     }
 #pragma unroll
     for (int e = 0; e < kEach; e++)
-        if (col0 + e * kColumns < cols) put_result<DT, kD>(a, r, head, cut.ct * r.tile + col0 + e * kColumns, quad * 4, acc[e], sum[e]);
+        if (col0 + e * kColumns < cols) put_result<DT, kD>(a, cut.first, head, cut.col0 + col0 + e * kColumns, quad * 4, acc[e], sum[e]);
 }
 
 }  // namespace dskv
