@@ -219,12 +219,13 @@ template <int kTerms> __device__ __forceinline__ void split8(const float *f, u32
 // Columns of a tile at most; where q's operands lie, in registers or, where these would be too many beside O and the weights' terms, in
 // LDS; and workgroups of a compute unit, with one subtile of a wave in flight.  64 requests over 256 - 4096 tokens, 128 dims:
 //   bf16, one row    52.3 us; with two subtiles in flight 54.5, with those and one workgroup 62.5, with three workgroups 56.7
-//   f16, 5 rows      67 (two blocks); 85.6, 87.8
+//   f16, 5 rows      64.0 (two blocks); with two subtiles in flight 85.6, with three workgroups 87.8
 //   fp32, one row    55.6; with q in registers, one workgroup 69.7.  5 rows 108 (one workgroup); with q in LDS 111
-// and 64 dims: bf16 of 12 rows 54 (three blocks; with one workgroup 78), of 16 rows 66 (four; as wide tiles 79); fp32, one row 38; 51.
+// and 64 dims: bf16 of 12 rows 54 (three blocks; with one workgroup 78), of 16 rows 66 (four; as wide tiles 79); fp32, one row 38;
+// 51.  5 rows 53.4; with one workgroup 74, with q in LDS 55.
 // (With 128 dims three blocks leave registers for one workgroup only, 113 us for 12 rows; see QuantWide.)
 constexpr int quant_columns(int dtype, int dim) { return dtype == DSKV_F32 || dim == 128 ? 32 : 64; }
-constexpr bool quant_q_in_lds(int dtype, int dim, int blocks) { return dtype == DSKV_F32 && (dim == 64 || blocks == 1); }
+constexpr bool quant_q_in_lds(int dtype, int blocks) { return dtype == DSKV_F32 && blocks == 1; }
 constexpr int quant_workgroups(int dtype, int dim, int blocks)
 {
     return dim == 64 || blocks <= (dtype == DSKV_F32 ? 1 : 2) ? 2 : 1;
@@ -245,7 +246,7 @@ template <int DT, int kD, int kBlocks> struct QuantTile {
     static constexpr int kPitch = kD + 16;                           // bytes; 16 rows' chunks at one offset meet no bank twice
     static constexpr int kWaveLds = 2 * kSub * kPitch + 2 * kSub * 4;      // K, V, their scales
     static constexpr int kOPitch = kD + 4;                           // floats
-    static constexpr bool kQInLds = quant_q_in_lds(DT, kD, kBlocks);
+    static constexpr bool kQInLds = quant_q_in_lds(DT, kBlocks);
     static constexpr int kQLds = kQInLds ? kBlocks * kSteps * kQTerms * 1024 : 0;
     static constexpr int kMergeLds = kTreeWaves * kCols * (kOPitch + 2) * 4;
     static constexpr int kLds = kTreeWaves * kWaveLds > kMergeLds ? kTreeWaves * kWaveLds : kMergeLds;
