@@ -216,6 +216,10 @@ template <int kTerms> __device__ __forceinline__ void split8(const float *f, u32
     }
 }
 
+// Units that a share has at least, two turns of its waves: shorter parts cost more to merge than they save.  8 requests of 5 rows over 300 - 1100 tokens
+// 13.8 us, with one turn 15.8, with three 14.5; one row over 1.8 K 9.6, 10.1, 10.4, over 500 8.9, 8.0, 8.9.
+constexpr int kQuantLeast = 2 * kTreeWaves;
+
 // Columns of a tile at most; where q's operands lie, in registers or, where these would be too many beside O and the weights' terms, in
 // LDS; and workgroups of a compute unit, with one subtile of a wave in flight.  64 requests over 256 - 4096 tokens, 128 dims:
 //   bf16, one row    52.3 us; with two subtiles in flight 54.5, with those and one workgroup 62.5, with three workgroups 56.7
@@ -265,7 +269,7 @@ __global__ __launch_bounds__(kTreeThreads, (QuantTile<DT, kD, kBlocks>::kWorkgro
     int share, head;
     share_and_head(a, share, head);
     TreePlace place;
-    tree_place<S::kCols, S::kSub, kTreeThreads, false, kTreeWaves, kTreeWaves * S::kDepth>(a, share, place);
+    tree_place<S::kCols, S::kSub, kTreeThreads, false, kQuantLeast, kTreeWaves * S::kDepth>(a, share, place);
     make_uniform(place);
     const int begin = place.begin, end = place.end;
     if (begin >= end) return;
