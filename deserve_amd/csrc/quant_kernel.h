@@ -7,6 +7,8 @@
 // Weights times V's scale span more than f16 holds: the second product is in bf16 for all types.  A weight is rounded to bf16 for bf16
 // results (2^-9 of it, half of what the result's own rounding is), to two bf16 terms for f16 (2^-17) and to three, that is to 32
 // bits, for fp32, whose q is three terms as well.
+// Bound by HBM: 64 requests of one row over 256 - 4096 tokens, 32 heads over 8, 128 dims, bf16, 279 MB, 52.3 us, 5.3 TB/s; its loads alone 51.  With 8
+// rows each 68, where items end: 50 if all are as long.
 #pragma once
 
 #include "quant.h"

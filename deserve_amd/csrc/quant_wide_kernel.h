@@ -1,13 +1,16 @@
 // The attention over 8-bit pages for more columns than fit a wave (head_dim 64 and 128, 16-bit types): the columns are split over the
 // waves of a workgroup, 32 each, and all of them read the same 32-token blocks of K and V from LDS, where these lie in the type of q,
-// multiplied by their scales.  See tree_kernel.h for how the work is cut.  A wave fetches its part of a block in codes, 8
-// bytes a lane and row, some blocks ahead, makes 8 numbers of them - two an instruction, which applies the scale; exact in bf16, in f16 but for
+// multiplied by their scales.  See tree_kernel.h for how the work is cut.  A lane fetches 16 or 32 bytes of a stage's codes (one block of
+// K or V, or two), some stages ahead, makes numbers of them - two an instruction, which applies the scale; exact in bf16, in f16 but for
 // what f16 itself does not hold - and writes them to LDS, so that every code is converted once a workgroup.
 //
 // Iteration j of a walk multiplies P(j - 1) into V(j - 1), turns S(j) into P(j) and computes S(j + 1), so that all of
-// its matrix instructions are independent of its exponentials.  Behind its only barrier K(j + 3) and V(j) are written to LDS, K(j + 5) and V(j + 2)
-// requested, and at its end the operands of K(j + 2) read; with 64 dims a stage holds two blocks side by side, and so it is once in two iterations.  The running maximum of a column is raised only when a block's weights under it
+// its matrix instructions are independent of its exponentials.  Behind its only barrier the next stages of K and V are written to LDS and those
+// kAhead further on requested (see kFirst, kBehind), and at its end the operands of K(j + 2) are read; where a stage holds two blocks, this is once
+// in two iterations.  The running maximum of a column is raised only when a block's weights under it
 // sum to more than most_weight in a lane.  Weights are rounded to 16 bits for the matrix product, half a step of each (see headroom).
+// Bound by the matrix and vector pipelines at the board's power cap: 16 chunks of 512 rows over up to 8 K tokens, 64 heads over 8, 128 dims, bf16, 840 us
+// with the merge, 965 TFLOP/s.
 // Where a token lies in the pool, and its scales, are looked up for some thousand tokens at a time and kept in LDS, so that pages may
 // have any size.
 #pragma once
@@ -430,7 +433,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void quant_wide_kernel(QuantArgs a)
 }
 
 // Items that were cut, two for each share that they begin in: a thread per four dims of kEach columns, workgroups along the columns (in
-// front, so that those of few items lie on all XCDs: 437 rows in 7 tiles 16.3 us with the items in front).
+// front, so that those of few items lie on all XCDs: 437 rows in 7 tiles 9.2 us, 16.3 with the items in front).  A chain of three trips and as
+// many more as there are pairs of parts.
 template <int DT, int kD, int kCols>
 __global__ __launch_bounds__(256) void quant_merge_kernel(QuantArgs a)
 {
