@@ -8,7 +8,8 @@
 namespace dskv {
 
 // Any type and head dim: one workgroup per (row, q head) whose waves take every kQuantWaves-th group of four keys.  Lane
-// (g, c) holds dims 8 c .. 8 c + 7 (and 128 more ..) of key g of the group.
+// (g, c) holds dims 8 c .. 8 c + 7 (and 128 more ..) of key g of the group.  Bound by the latency of its loads: K and V are read once per row and q
+// head, from the caches but for the first time (64 requests of one row over 256 - 4096 tokens, 32 heads over 8, 80 dims: 501 us, of five rows 1460).
 constexpr int kQuantWaves = 8;
 
 template <int DT, int kChunks>
@@ -158,10 +159,15 @@ template <int DT, int kD, int kWaves, int kFetch> static int launch_quant_wide(c
 {
     hipLaunchKernelGGL((quant_wide_kernel<DT, kD, kWaves, kFetch>), dim3((unsigned)(f.shares * a.n_kv_heads)), dim3(kWaves * 64), 0, stream, a);
     DSKV_LAUNCH_CHECK("quant_wide_kernel");
-    constexpr int kColumns = 256 / (kD / 4) * kMergeEach;                // of a workgroup
-    constexpr int kCols = QuantWide<kD, kWaves, kFetch>::kCols;
-    const dim3 grid((unsigned)((kCols + kColumns - 1) / kColumns), (unsigned)a.n_kv_heads, (unsigned)(2 * f.shares));
-    hipLaunchKernelGGL((quant_merge_kernel<DT, kD, kCols>), grid, dim3(256), 0, stream, a);
+    constexpr int kCols = QuantWide<kD, kWaves, kFetch>::kCols, kColumns = 256 / (kD / 4);
+    auto merge = [&](auto kernel, int each) {
+        const dim3 grid((unsigned)((kCols + kColumns * each - 1) / (kColumns * each)), (unsigned)a.n_kv_heads, (unsigned)(2 * f.shares));
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, a);
+    };
+    // Items of many parts: eight of them together and a column a thread.  One request of 12 rows over 4000 tokens 5.0 us, with four columns and two parts
+    // 8.6; two over 16 K 9.4, 17.9; 8 of 64 rows over 4 - 8 K, four parts an item, 10.9, 9.7.
+    if (f.shares > 4L * a.batch * f.col_tiles) merge(quant_merge_kernel<DT, kD, kCols, 1, 8>, 1);
+    else merge(quant_merge_kernel<DT, kD, kCols, 4, 2>, 4);
     DSKV_LAUNCH_CHECK("quant_merge_kernel");
     return 0;
 }

@@ -19,7 +19,6 @@
 
 namespace dskv {
 
-constexpr int kMergeEach = 4;                // columns that a thread of the merge launch takes
 constexpr int kWideBlock = 32;
 constexpr int kWideRegion = 1088;           // 64 chunks of 16 bytes, (4 chunk + row) * 16 of four rows, and 64 bytes of padding
 constexpr int kWideStage = kWideBlock / 4 * kWideRegion;
@@ -27,7 +26,7 @@ constexpr int kWideLeast = 8;               // units a share has at least: what 
 
 // kFetch: waves without columns that fetch for the others, more stages ahead than there would be registers for beside O and q; 0: all do
 // both.  64 requests of 12 rows over 256 - 4096 tokens, 128 dims, two waves of columns and two that fetch: 106 us; 113 in the narrow form with three
-// blocks of columns a tile, and one such request over 4000 tokens 23.4 and 40.
+// blocks of columns a tile, and one such request over 4000 tokens 20.0 and 40.
 template <int kD, int kWaves, int kFetch> struct QuantWide {
     static constexpr int kThreads = kWaves * 64;
     static constexpr int kCompute = kWaves - kFetch, kCols = kCompute * 32;
@@ -432,13 +431,13 @@ __global__ __launch_bounds__(kWaves * 64, 2) void quant_wide_kernel(QuantArgs a)
     }
 }
 
-// Items that were cut, two for each share that they begin in: a thread per four dims of kEach columns, workgroups along the columns (in
+// Items that were cut, two for each share that they begin in: a thread per four dims of kEach columns and kAhead parts requested together, workgroups along the columns (in
 // front, so that those of few items lie on all XCDs: 437 rows in 7 tiles 9.2 us, 16.3 with the items in front).  A chain of three trips and as
 // many more as there are pairs of parts.
-template <int DT, int kD, int kCols>
+template <int DT, int kD, int kCols, int kEach, int kAhead>
 __global__ __launch_bounds__(256) void quant_merge_kernel(QuantArgs a)
 {
-    constexpr int kQuads = kD / 4, kColumns = 256 / kQuads, kEach = kMergeEach, kAhead = 2;       // columns side by side, a thread's, parts requested together
+    constexpr int kQuads = kD / 4, kColumns = 256 / kQuads;           // columns side by side
     const QuantCut cut = a.cuts[blockIdx.z];
     if (cut.parts.n < 2) return;
     const int head = blockIdx.y, quad = threadIdx.x % kQuads, column = threadIdx.x / kQuads;
