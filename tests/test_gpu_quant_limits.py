@@ -22,6 +22,9 @@ SHAPES = [
     ("9_rows", [700, 20, 0, 1300], [9, 1, 8, 5], True, 16, 8, 2, 128, "bf16"),
     ("16_rows", [700, 20, 0, 1300], [16, 1, 8, 15], False, 12, 8, 2, 128, "f16"),
     ("12_rows_long", [9000, 3], [12, 9], False, 16, 4, 1, 128, "bf16"),
+    ("many_parts_32", [16000], [8], False, 16, 32, 8, 128, "bf16"),
+    ("many_parts_20", [9000, 4000], [5, 3], True, 16, 16, 4, 128, "f16"),
+    ("many_parts_64_dims_28", [9000], [7], False, 16, 8, 2, 64, "fp32"),
     ("many_parts_64", [6000], [12], False, 16, 32, 8, 128, "f16"),
     ("many_parts_64_dims", [6000, 5000], [9, 40], True, 16, 16, 2, 64, "bf16"),
     ("few_parts_256", [700 + 90 * i for i in range(9)], [40 + i for i in range(9)], True, 16, 16, 2, 128, "bf16"),
