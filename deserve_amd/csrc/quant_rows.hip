@@ -374,7 +374,9 @@ __global__ __launch_bounds__(256) void quant_move_kernel(QuantMove a)
             __builtin_amdgcn_s_waitcnt(0);                                // the blocks have been rounded anew
             asm volatile("" ::: "memory");
         }
-        if (moves) by_of[wave][mine] = scale != 0 ? x.from_scale * reciprocal_of(scale) : 0.f;
+        // A row of zeros asks for no scale, and its own may be so far above the one that is there that no 32 bits hold their ratio: by 0,
+        // which keeps zeros and codes of no number what they are.
+        if (moves) by_of[wave][mine] = value > 0 ? x.from_scale * reciprocal_of(scale) : 0.f;
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
