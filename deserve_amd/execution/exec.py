@@ -261,7 +261,7 @@ class BatchVerify(BatchExec):
             pool = ctx.page_pool
             if self.parents is None:                        # the rows of an accepted chain are in place
                 pass
-            elif pool.record is not None:
+            elif getattr(pool, "record", None) is not None:
                 move_accepted_quantized_rows(pool.pages, ctx.indptr, ctx.kv_page_indices, ctx.kv_page_indptr, ctx.kv_last_page_lens,
                                              verdict.path, verdict.counts, pool.page_size, pool.n_kv_heads, pool.head_dim)
             else:

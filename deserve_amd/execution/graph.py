@@ -53,7 +53,7 @@ class GraphedDecodeStep:
         self.captures = 0
 
     def _prepare(self, task_datas: Sequence[TaskData], kvcaches: Sequence[PagedKVCache]) -> Union[FlashDecodeCtx, FlashQuantCtx]:
-        if any((c.pool.record is not None) != self.quantized for c in kvcaches):
+        if any((getattr(c.pool, "record", None) is not None) != self.quantized for c in kvcaches):
             raise ValueError("the wrapper is for pages of the model's type, the caches' are in 8 bits, or the other way round")
         if self.quantized:
             if any(t.seqlen != 1 for t in task_datas):
