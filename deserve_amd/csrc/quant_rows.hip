@@ -277,8 +277,8 @@ __global__ __launch_bounds__(256) void quant_move_kernel(QuantMove a)
     const int block = blockIdx.y * 4 + wave;                               // half and head
     if (block >= 2 * s.n_kv_heads) return;
     const QuantRequest r = quant_request(a.r, b);
-    const int count = min(a.counts[b], r.n);
-    if (count < 2 || count > DSKV_MAX_TREE_ROWS) return;
+    const int walk = a.counts[b], count = min(walk, r.n);
+    if (count < 2 || walk > DSKV_MAX_TREE_ROWS) return;
     const long block_at = block * s.head_bytes, scale_at = 2 * s.half_bytes + block * 4L;
 
     const int p = lane < count ? a.path[r.first + lane] : -1;

@@ -62,3 +62,17 @@ def test_rows_of_the_least_values():
     want = move(records, step, path, counts)
     assert not np.array_equal(want.codes & 127, records.codes & 127)
     same(moved(records, step, path, counts, 16, 2, 64), want)
+
+
+@pytest.mark.parametrize("count", [65, 100, 2 ** 31 - 1])
+def test_walks_of_more_rows_than_a_tree_has(count):
+    """They move nothing, however few rows their request has; the one beside them goes where it should."""
+    print("[case] too long walks", count, flush=True)
+    step = make_step(5, [13, 7], [40, 20], False, 16, 2, 2, 64, "bf16")
+    records = quantise(step.pages.double().numpy())
+    path = np.concatenate([np.arange(0, 80, 2)[:40].clip(max=39), np.arange(0, 40, 2)[:20].clip(max=19)]).astype(np.int32)
+    counts = [count, 5]
+    want = move(records, step, path, counts)
+    first = step.request(0)[2]
+    assert np.array_equal(want.codes[first], records.codes[first]) and not np.array_equal(want.codes, records.codes)
+    same(moved(records, step, path, counts, 16, 2, 64), want)
