@@ -138,12 +138,17 @@ def rope_append_quantized(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.T
         raise ValueError("out is for the rotated q: rope_table is missing")
     rotated = rope_table is not None
     index = _on_device(pages, k, v, qo_indptr, kv_indices, kv_indptr, kv_last_page_len, rope_table, q if rotated else None, out)
-    if nnz == 0 or pages.shape[0] == 0:
+    num_pages, at = pages.shape[0], pages.data_ptr()
+    if nnz == 0 or (not rotated and (batch == 0 or num_pages == 0)):
         return result
+    if batch == 0 or num_pages == 0:
+        # no row is kept and q is rotated all the same: one request that has none, over a table without entries
+        qo_indptr = kv_indptr = kv_last_page_len = k.new_zeros((2,), dtype=torch.int32)
+        kv_indices, batch, num_pages, at = kv_indptr[:0], 1, 1, result.data_ptr()
     rows = _lib.QuantRows(qo_indptr.data_ptr(), kv_indices.data_ptr(), kv_indptr.data_ptr(), kv_last_page_len.data_ptr(),
-                          kv_indices.numel(), batch, nnz, pages.shape[0], page_size, hkv, dim)
+                          kv_indices.numel(), batch, nnz, num_pages, page_size, hkv, dim)
     _call("rope_append_quantized", index, _lib.lib().dskv_rope_append_quant, ctypes.byref(rows),
-          result.data_ptr() if rotated else None, pages.data_ptr(), q.data_ptr() if rotated else None, k.data_ptr(), v.data_ptr(),
+          result.data_ptr() if rotated else None, at, q.data_ptr() if rotated else None, k.data_ptr(), v.data_ptr(),
           q_stride, k_stride, v_stride, _lib.ptr(rope_table), heads, code)
     return result
 

@@ -672,7 +672,8 @@ typedef struct dskv_quant_rows {
  * head are no number in K and 0 in V: rows that see it get no number, others nothing of it.  Values that code * scale could only take to an
  * infinity of the type (over 61440 in f16, 240 * 2^120 else) are stored as that.
  * A request whose arrays contradict themselves, a page id outside [0, num_pages) and a table entry past n_page_indices take
- * no rows; q is rotated in every row.  No page takes rows of two requests, or of two entries of a table.  head_dim: a multiple of 8 up to 256.
+ * no rows; q is rotated in every row (with batch 0 nothing is done, to q neither).  No page takes rows of two requests, or of two entries of
+ * a table.  head_dim: a multiple of 8 up to 256.
  */
 int dskv_rope_append_quant(const dskv_quant_rows_t *rows, void *q_out, void *pages_layer, const void *q, const void *k,
                            const void *v, int64_t q_stride, int64_t k_stride, int64_t v_stride, const float *rope_table,

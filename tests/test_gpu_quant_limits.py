@@ -289,3 +289,28 @@ def test_counters_of_a_captured_step_outlive_a_wider_one():
     w.end_forward()
     assert w._counters.data_ptr() != first and first in [t.data_ptr() for t in w._all_counters]
     near(run(step, as_quantised(step)[0].tensor().cuda()), *attention(as_quantised(step)[1]))
+
+
+@pytest.mark.parametrize("dtype,dim,n", [("bf16", 128, 3), ("f16", 64, 700), ("fp32", 80, 40)])
+def test_q_is_rotated_where_no_row_is_kept(dtype, dim, n):
+    """An append without requests, and one into a pool without pages: q comes back rotated all the same."""
+    from deserve_amd.quant_ops import PageRecord, rope_append_quantized
+
+    step = make_step(33, [0], [n], False, 16, 8, 2, dim, dtype)
+    qo, indptr, indices, last = step.on("cuda")["csr"]
+    pages = as_quantised(step)[0].tensor().cuda()
+    kept = pages.clone()
+    k, q = rows(1, step, step.q.dtype).cuda(), step.q.cuda()
+    angle = torch.linspace(0, 3, n * dim // 2).view(n, dim // 2)
+    table = torch.cat([angle.cos(), angle.sin()], 1).cuda()
+    want = rope_append_quantized(q, k, k, qo, pages.clone(), indices, indptr, last, 16, table)
+    assert not torch.equal(want, q)
+    nan = lambda: torch.full_like(q, float("nan"))
+    none = torch.empty((0, PageRecord(16, 2, dim).page_bytes), dtype=torch.uint8, device="cuda")
+    for what, csr, pool in (("no requests", (qo[:1], indices, indptr[:1], last[:0]), pages), ("no rows", (qo * 0, indices, indptr, last), pages),
+                            ("no pages", (qo, indices, indptr, last), none)):
+        out = nan()
+        got = rope_append_quantized(q, k, k, csr[0], pool, *csr[1:], 16, table, out=out)
+        assert got is out and torch.equal(got, want), what
+    assert torch.equal(pages, kept)
+    assert rope_append_quantized(q, k, k, qo, none, indices, indptr, last, 16) is q
