@@ -112,7 +112,8 @@ __global__ __launch_bounds__(kQuantWaves * 64) void quant_generic_kernel(QuantAr
 // How rows of a step are computed.  wide_waves > 0: quant_wide_kernel.h with so many waves that have columns; else quant_kernel.h with tiles of
 // `blocks` * 16 columns, few and each as narrow as it can be.
 struct QuantForm {
-    int wide_waves, blocks, cols, col_tiles, shares, sides;
+    int wide_waves, blocks, cols, shares, sides;
+    long col_tiles;                     // (of max_qo_len rows, which may be any number)
 };
 constexpr int kQuantUnits = 256;        // compute units
 static bool quant_matrix_form(int head_dim) { return head_dim == 64 || head_dim == 128; }
@@ -122,8 +123,8 @@ static QuantForm quant_form(bool wide, int max_rows, int n_qo_heads, int n_kv_he
     const long cols = (long)std::max(max_rows, 1) * (n_qo_heads / n_kv_heads);
     f.wide_waves = !wide ? 0 : head_dim == 128 && cols <= 64 ? 2 : cols <= 128 ? 4 : 8;
     const int widest = wide ? f.wide_waves * 32 : quant_columns(dtype, head_dim);
-    f.col_tiles = (int)((cols + widest - 1) / widest);
-    f.blocks = wide ? 0 : (int)((cols + 16L * f.col_tiles - 1) / (16L * f.col_tiles));
+    f.col_tiles = (cols + widest - 1) / widest;
+    f.blocks = wide ? 0 : (int)((cols + 16 * f.col_tiles - 1) / (16 * f.col_tiles));
     f.cols = wide ? widest : f.blocks * 16;
     const int resident = kQuantUnits * (wide ? (f.wide_waves <= 4 ? 2 : 1) : quant_workgroups(dtype, head_dim, f.blocks));
     f.shares = resident >= n_kv_heads ? resident / n_kv_heads : 1;
@@ -275,7 +276,7 @@ extern "C" int dskv_quant_attn(const dskv_quant_step_t *step, void *out, const v
     // (places in the pool, tokens of a request and units are numbered in 32 bits there)
     if (quant_matrix_form(s->head_dim) && s->num_pages * (shape.page_bytes / 16) < UINT32_MAX &&
         s->n_page_indices < kMostTokens / s->page_size &&
-        (s->n_page_indices * s->page_size / 32 + 2LL * s->batch) * col_tiles < INT32_MAX) {
+        col_tiles <= (INT32_MAX - 1) / (s->n_page_indices * s->page_size / 32 + 2LL * s->batch)) {
         const int64_t need = dskv_quant_attn_workspace(s->batch, s->nnz, s->max_qo_len, s->n_qo_heads, s->n_kv_heads, s->head_dim, s->dtype);
         if (!s->workspace || s->workspace_bytes < need) {
             set_error("quant_attn: workspace of %lld bytes, %lld are needed", (long long)s->workspace_bytes, (long long)need);

@@ -1,6 +1,9 @@
 """Refusals of the operators over 8-bit pages, before anything is launched (all on the CPU)."""
 import ctypes
 import itertools
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -159,3 +162,16 @@ def test_workspaces_of_all_forms():
                 for dim in (64, 128):
                     assert lib.dskv_quant_attn_workspace(8, 8 * rows, rows, hkv * group, hkv, dim, dtype) > 0
                 assert lib.dskv_quant_attn_workspace(8, 8 * rows, rows, hkv * group, hkv, 80, dtype) == 0
+
+
+def test_workspaces_for_any_number_of_rows():
+    """max_qo_len as large as its type goes, with every group: an answer, and not the end of the process."""
+    code = ("from deserve_amd import _lib\n"
+            "for rows in (1 << 24, 1 << 28, 1 << 29, 1 << 30, (1 << 31) - 1):\n"
+            "    for group in (1, 4, 16, 32, 64, 128, 256, 512, 1024, 1 << 16):\n"
+            "        for dtype in (_lib.F32, _lib.F16, _lib.BF16):\n"
+            "            for dim in (64, 128):\n"
+            "                assert _lib.lib().dskv_quant_attn_workspace(3, 9, rows, group, 1, dim, dtype) > 0, (rows, group, dtype, dim)\n")
+    done = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                          capture_output=True, text=True)
+    assert done.returncode == 0, (done.returncode, done.stderr[-500:])
