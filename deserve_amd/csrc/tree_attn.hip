@@ -118,7 +118,8 @@ __global__ __launch_bounds__(kGenericWaves * 64) void tree_generic_kernel(TreeAr
 // How a step is computed.  wide_waves > 0: tree_wide_kernel.h with so many waves; else the matrix form of tree_kernel.h with
 // tiles of `blocks` * 16 columns, up to tree_columns: few tiles, each as narrow as it can be.
 struct TreeForm {
-    int wide_waves, blocks, cols, col_tiles, shares, sides;
+    int wide_waves, blocks, cols, shares, sides;
+    long col_tiles;                     // (of max_qo_len rows, which may be any number)
 };
 static bool matrix_form(int head_dim) { return head_dim == 64 || head_dim == 128; }
 static TreeForm tree_form(bool wide, int max_rows, int n_qo_heads, int n_kv_heads, int head_dim)
@@ -127,8 +128,8 @@ static TreeForm tree_form(bool wide, int max_rows, int n_qo_heads, int n_kv_head
     const long cols = (long)max_rows * (n_qo_heads / n_kv_heads);
     f.wide_waves = !wide ? 0 : cols <= 128 ? 4 : 8;
     const int widest = wide ? f.wide_waves * 32 : tree_columns(head_dim);
-    f.col_tiles = (int)((cols + widest - 1) / widest);
-    f.blocks = wide ? 0 : (int)((cols + 16L * f.col_tiles - 1) / (16L * f.col_tiles));
+    f.col_tiles = (cols + widest - 1) / widest;
+    f.blocks = wide ? 0 : (int)((cols + 16 * f.col_tiles - 1) / (16 * f.col_tiles));
     f.cols = wide ? widest : f.blocks * 16;
     // two workgroups a compute unit where their registers and LDS allow it
     const int resident = kTreeUnits * (wide ? (f.wide_waves == 4 ? 2 : 1) : tree_workgroups(head_dim, f.blocks));
@@ -161,8 +162,8 @@ template <int DT, int kD, int kCols, int kSub> static int launch_tree_merge(cons
     constexpr int kEach = kCols >= 128 ? 4 : 1;
     const int columns = 256 / (kD / 4) * (many_parts ? 1 : kEach) / (many_parts ? 4 : 1);
     const dim3 grid((unsigned)(a.batch * f.col_tiles), (unsigned)a.n_kv_heads, (unsigned)((kCols + columns - 1) / columns));
-    if (many_parts) hipLaunchKernelGGL((tree_merge_kernel<DT, kD, kCols, kSub, 4, 1>), grid, dim3(256), 0, stream, a, f.col_tiles);
-    else hipLaunchKernelGGL((tree_merge_kernel<DT, kD, kCols, kSub, 1, kEach>), grid, dim3(256), 0, stream, a, f.col_tiles);
+    if (many_parts) hipLaunchKernelGGL((tree_merge_kernel<DT, kD, kCols, kSub, 4, 1>), grid, dim3(256), 0, stream, a, (int)f.col_tiles);
+    else hipLaunchKernelGGL((tree_merge_kernel<DT, kD, kCols, kSub, 1, kEach>), grid, dim3(256), 0, stream, a, (int)f.col_tiles);
     DSKV_LAUNCH_CHECK("tree_merge_kernel");
     return 0;
 }

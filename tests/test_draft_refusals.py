@@ -1,5 +1,8 @@
 """Refusals of the drafted-token operators, before anything is launched (all on the CPU)."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -266,3 +269,16 @@ def test_a_step_is_verified_by_as_many_rows_as_it_has():
     refused("tokens holds 4", step.verify, torch.rand((5, 8)), torch.rand(5))
     step.tokens = i32(7, 8, 4, 5, 6, 9, 9)                     # padded ones are taken
     refused("on the GPU", step.verify, torch.rand((7, 8)), torch.rand(7))
+
+
+def test_workspaces_for_any_number_of_rows():
+    """max_qo_len as large as its type goes, with every group: an answer, and not the end of the process."""
+    code = ("from deserve_amd import _lib\n"
+            "for rows in (1 << 24, 1 << 28, 1 << 29, 1 << 30, (1 << 31) - 1):\n"
+            "    for group in (1, 4, 16, 32, 64, 128, 256, 512, 1024, 1 << 16):\n"
+            "        for dtype in (_lib.F32, _lib.F16, _lib.BF16):\n"
+            "            for dim in (64, 128):\n"
+            "                assert _lib.lib().dskv_tree_attn_workspace(3, 9, rows, group, 1, dim, dtype) > 0, (rows, group, dtype, dim)\n")
+    done = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                          capture_output=True, text=True)
+    assert done.returncode == 0, (done.returncode, done.stderr[-500:])
