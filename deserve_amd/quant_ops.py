@@ -165,7 +165,7 @@ class BatchQuantizedWithPagedKVCacheWrapper:
             raise ValueError("8-bit pages hold their tokens by head: only the HND layout is implemented")
         self._workspace = workspace_buffer
         # what the parts of a request count themselves in with: zero between launches, and kept for good, also where more heads
-        # ask for more words (captured launches hold their address)
+        # ask for more words (captured launches hold their address); one list for all copies (another), the longest behind
         self._all_counters: List[torch.Tensor] = []
         self._counters = self._zeros(_lib.lib().dskv_quant_attn_counters(1))
         self._step: Optional[_lib.QuantStep] = None
@@ -208,8 +208,9 @@ class BatchQuantizedWithPagedKVCacheWrapper:
         if max_qo_len < 0 or min_qo_len < 0:
             raise ValueError("max_qo_len and min_qo_len must not be negative")
         _on_device(qo_indptr, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len, masks, self._workspace)
-        if num_kv_heads > 512 and self._counters.numel() < _lib.lib().dskv_quant_attn_counters(num_kv_heads):
-            self._counters = self._zeros(_lib.lib().dskv_quant_attn_counters(num_kv_heads))
+        if num_kv_heads > 512 and self._counters.numel() < (need := _lib.lib().dskv_quant_attn_counters(num_kv_heads)):
+            made = self._all_counters[-1]                # perhaps by a copy
+            self._counters = made if made.numel() >= need else self._zeros(need)
         counters = self._counters
         self._held = (qo_indptr, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len, masks, page_bytes, counters)
         workspace = self._workspace

@@ -314,3 +314,23 @@ def test_q_is_rotated_where_no_row_is_kept(dtype, dim, n):
         assert got is out and torch.equal(got, want), what
     assert torch.equal(pages, kept)
     assert rope_append_quantized(q, k, k, qo, none, indices, indptr, last, 16) is q
+
+
+def test_counters_of_steps_planned_on_copies():
+    """Steps of more kv heads than a wrapper's first counters are for, each planned on a copy, as a stage plans them: counters are
+    made once, and all copies count in them."""
+    from deserve_amd.quant_ops import BatchQuantizedWithPagedKVCacheWrapper
+
+    step = make_step(34, [30], [1], False, 4, 520, 520, 64, "bf16")
+    records, values = as_quantised(step)
+    pages, on = records.tensor().cuda(), step.on("cuda")
+    w = BatchQuantizedWithPagedKVCacheWrapper(torch.empty(128 << 20, dtype=torch.uint8, device="cuda"))
+    used = set()
+    for heads in (520, 600, 520, 600, 520):
+        copy = w.another()
+        wide = make_step(35, [9], [1], False, 4, heads, heads, 64, "bf16") if heads != 520 else step
+        copy.begin_forward(*wide.on("cuda")["csr"], heads, heads, 64, 4, max_qo_len=1)
+        used.add((heads, copy._step.counters))
+        if heads == 520:
+            near(copy.forward(on["q"], pages), *attention(values))
+    assert len(w._all_counters) == 3 and len({c for h, c in used if h == 600}) == 1, (len(w._all_counters), used)
