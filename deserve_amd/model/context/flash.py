@@ -352,8 +352,9 @@ class FlashTreeCtx(FlashForwardCtx):
         kv_lens, qo_lens = dev[:batch], dev[batch: 2 * batch]
         tables = build_step_tables(dev[2 * batch:].view(batch, width), kv_lens, qo_lens, page_size,
                                    max_tokens=max_tokens, max_pages=int(exposed.sum()), parents=parents)
+        hint = {"min_qo_len": int(meta["seqlens"].min())} if isinstance(wrapper, BatchQuantizedWithPagedKVCacheWrapper) else {}
         wrapper.begin_forward(*tables.csr, num_qo_heads, num_kv_heads, head_dim, page_size,
-                              max_qo_len=int(meta["seqlens"].max()), masks=tables.masks)
+                              max_qo_len=int(meta["seqlens"].max()), masks=tables.masks, **hint)
         return cls(bsz=batch, seqlens=qo_lens, layer_id=0, page_pool=pool, offsets=kv_lens, indptr=tables.qo_indptr,
                    kv_page_indices=tables.kv_page_indices, kv_page_indptr=tables.kv_page_indptr,
                    kv_last_page_lens=tables.kv_last_page_lens, host={f: torch.from_numpy(meta[f]) for f in _FIELDS},

@@ -114,3 +114,23 @@ def test_drafted_trees():
                 assert np.array_equal(got.codes[page, :, :, :places] & 0x7F, want[layer].codes[page, :, :, :places] & 0x7F), (layer, page)
         for t in tasks:
             t.step()
+
+
+@pytest.mark.parametrize("rows_of", [(24, 18), (24, 3), (1, 1)])
+def test_steps_of_trees_say_how_few_rows_a_request_has(rows_of):
+    """The hint that leaves out the launch for requests of few rows, where a step has none: from the tasks, of trees and chains."""
+    from deserve_amd.execution.exec import BatchVerify
+    from deserve_amd.stage import KVStage, StageArgs
+    from deserve_amd.task import SamplingParams, TaskData
+
+    pool, caches = make_pool(80, 16)
+    stage = KVStage(StageArgs(HQ, HKV, HQ * DIM, 16, LAYERS), use_rope=False)
+    tasks = [TaskData(t, 0, 0, n, n, SamplingParams()) for t, n in zip("ab", rows_of)]
+    total = sum(rows_of)
+    chain = torch.cat([torch.arange(-1, n - 1, dtype=torch.int32) for n in rows_of]).to(DEV)
+    for parents in (None, chain):
+        ex = BatchVerify(rows_for(torch.Generator(device="cuda").manual_seed(1), total), stage, tasks, caches[:2],
+                         torch.zeros(total, dtype=torch.int32, device=DEV), parents)
+        ex.prepare()
+        assert ex.tree_ctx.tree_wrapper._step.min_qo_len == min(rows_of)
+        assert ex.tree_ctx.tree_wrapper._step.step.max_qo_len == max(rows_of)
