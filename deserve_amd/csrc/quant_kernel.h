@@ -6,7 +6,8 @@
 // token by token, so that pages may end anywhere in a subtile.
 // Weights times V's scale span more than f16 holds: the second product is in bf16 for all types.  A weight is rounded to bf16 for bf16
 // results (2^-9 of it, half of what the result's own rounding is), to two bf16 terms for f16 (2^-17) and to three, that is to 32
-// bits, for fp32, whose q is three terms as well.
+// bits, for fp32, whose q is three terms as well.  (A weight is up to most_weight, 2^8: times V, and summed, that has to fit fp32, which bounds
+// the magnitudes of V: see dskv_quant_attn in dskv.h.)
 // Bound by HBM: 64 requests of one row over 256 - 4096 tokens, 32 heads over 8, 128 dims, bf16, 279 MB, 52.3 us, 5.3 TB/s; its loads alone 51.  With 8
 // rows each 68, where items end: 50 if all are as long.
 #pragma once

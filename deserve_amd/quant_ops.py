@@ -224,7 +224,8 @@ class BatchQuantizedWithPagedKVCacheWrapper:
                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """q (tokens, Hq, D), one row for every row of the step; rows behind the last request's are left out of the
         result (as they were in out).  K and V of the new rows are in the pages (num_pages, page_bytes) uint8.  A row that sees
-        nothing gets zeros.  sm_scale: positive; None: D ** -0.5.  out: optional result tensor (contiguous, q's shape and dtype)."""
+        nothing gets zeros.  256 times a request's tokens times the largest magnitude in V is under 2 ** 128 (1e27 for any length).
+        sm_scale: positive; None: D ** -0.5.  out: optional result tensor (contiguous, q's shape and dtype)."""
         if self._step is None:
             raise RuntimeError("forward over 8-bit pages called before begin_forward")
         s = self._step.step

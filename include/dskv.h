@@ -681,6 +681,8 @@ int dskv_rope_append_quant(const dskv_quant_rows_t *rows, void *q_out, void *pag
 
 /*
  * dskv_tree_attn over such pages: same arguments and result, with sm_scale > 0 and dtype that of q and out.
+ * Weights are up to 2^8 under a running maximum that follows the scores, and sums are in fp32: rows are right as long as 256 * (tokens
+ * of the request) * (largest magnitude in V) is under 2^128, which a magnitude of 2^90 is for any length.  Beyond, a row may be no number.
  * min_qo_len: no request has fewer rows (a hint: what does not hold costs time, not results; 0 is always right).
  * counters: dskv_quant_attn_counters(n_kv_heads) words on the device that are zero before the first call that is given them and
  * used by one call at a time, like the workspace; every call leaves them zero.

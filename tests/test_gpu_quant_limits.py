@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from draftutil import attention, make_step
-from quantutil import Records, append, as_quantised, move, near, rows, same
+from quantutil import Records, append, as_quantised, move, near, quantise, rows, same
 from test_gpu_quant_attention import run
 
 pytestmark = pytest.mark.gpu
@@ -334,3 +334,34 @@ def test_counters_of_steps_planned_on_copies():
         if heads == 520:
             near(copy.forward(on["q"], pages), *attention(values))
     assert len(w._all_counters) == 3 and len({c for h, c in used if h == 600}) == 1, (len(w._all_counters), used)
+
+
+# name, cached, rows, q heads, kv heads, dim, type
+LARGE = [("narrow", 300, 1, 8, 2, 128, "bf16"), ("narrow_cut", 3000, 8, 8, 2, 128, "bf16"), ("narrow_64", 700, 3, 8, 2, 64, "bf16"),
+         ("fp32", 300, 2, 8, 2, 128, "fp32"), ("fp32_cut", 2000, 1, 8, 2, 64, "fp32"), ("wide_2", 300, 14, 8, 2, 128, "bf16"),
+         ("wide_4", 900, 30, 8, 2, 64, "bf16"), ("wide_8", 500, 100, 8, 2, 128, "bf16"), ("plain", 300, 2, 8, 2, 80, "bf16"),
+         ("plain_fp32", 300, 2, 8, 2, 256, "fp32"), ("f16", 300, 1, 8, 2, 128, "f16"), ("f16_wide", 300, 60, 8, 2, 128, "f16")]
+
+
+@pytest.mark.parametrize("case", LARGE, ids=lambda c: c[0])
+def test_the_largest_values_that_sums_hold(case):
+    """V as large as 256 * tokens * |v| < 2^128 (f16: its pages' largest) allows, under scores that rise from token to token by
+    less than what raises a running maximum, so that weights are as large as they get."""
+    print("[case] large V", *case, flush=True)
+    name, kv, n, hq, hkv, dim, dtype = case
+    step = make_step(36, [kv], [n], False, 16, hq, hkv, dim, dtype)
+    _, _, table, length = step.request(0)
+    pages = step.pages.double()
+    # log2 of a weight rises by 7.5 over the tokens
+    at = torch.arange(len(table) * 16).double().view(-1, 16)[:, :, None]
+    pages[:, 0] *= 0.01
+    pages[torch.from_numpy(table).long(), 0, :, :, 0] = (at * (7.5 / length * np.log(2))).expand(-1, -1, hkv)
+    step.q.mul_(0.01)
+    step.q[..., 0] = float(dim) ** 0.5
+    # (0.9: codes are rounded up by 2^-4 at most)
+    most = 61440.0 if dtype == "f16" else 0.9 * 2.0 ** 128 / (256 * length)
+    pages[:, 1] *= most / pages[:, 1].abs().max()
+    records = quantise(pages.numpy())
+    values = dataclasses.replace(step, pages=torch.from_numpy(records.values().transpose(0, 1, 3, 2, 4).copy()))
+    assert most * 0.9 < values.pages[:, 1].abs().max() <= most / 0.9
+    near(run(step, records.tensor().cuda()), *attention(values))
