@@ -365,3 +365,33 @@ def test_the_largest_values_that_sums_hold(case):
     values = dataclasses.replace(step, pages=torch.from_numpy(records.values().transpose(0, 1, 3, 2, 4).copy()))
     assert most * 0.9 < values.pages[:, 1].abs().max() <= most / 0.9
     near(run(step, records.tensor().cuda()), *attention(values))
+
+
+def test_a_captured_step_after_wider_ones():
+    """A captured step of cut items, replayed after the wrapper was given more heads than its first counters are for, with other
+    tensors where freed memory would be."""
+    from deserve_amd.quant_ops import BatchQuantizedWithPagedKVCacheWrapper
+
+    step, wide = make_step(31, [3000], [1], False, 16, 8, 2, 128, "bf16"), make_step(32, [30], [1], False, 4, 600, 600, 64, "bf16")
+    records, values = as_quantised(step)
+    pages, on, more = records.tensor().cuda(), step.on("cuda"), wide.on("cuda")
+    want, bound = attention(values)
+    w = BatchQuantizedWithPagedKVCacheWrapper(torch.empty(128 << 20, dtype=torch.uint8, device="cuda"))
+    w.begin_forward(*on["csr"], 8, 2, 128, 16, max_qo_len=1)
+    out = torch.empty_like(on["q"])
+    w.forward(on["q"], pages, out=out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        w.forward(on["q"], pages, out=out)
+    w.end_forward()
+    w.begin_forward(*more["csr"], 600, 600, 64, 4, max_qo_len=1)
+    wide_pages = as_quantised(wide)[0].tensor().cuda()
+    others = [torch.full((n,), 3, dtype=torch.int32, device="cuda") for n in (1024, 1024, 1200, 2400)]
+    for _ in range(3):
+        near(w.forward(more["q"], wide_pages), *attention(as_quantised(wide)[1]))
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        near(out, want, bound)
+    assert all((x == 3).all() for x in others)
