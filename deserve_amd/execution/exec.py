@@ -55,7 +55,7 @@ _quantized_wrappers: Dict[torch.device, BatchQuantizedWithPagedKVCacheWrapper] =
 
 
 def get_quantized_wrapper(device: torch.device) -> BatchQuantizedWithPagedKVCacheWrapper:
-    """The wrapper for steps over 8-bit pages, over the workspace of get_wrappers."""
+    """The wrapper for steps over 8-bit pages, over the workspace of get_wrappers: for one stream at a time, as those are."""
     device = torch.device(device)
     if device not in _quantized_wrappers:
         _quantized_wrappers[device] = BatchQuantizedWithPagedKVCacheWrapper(get_wrappers(device)[0]._workspace)

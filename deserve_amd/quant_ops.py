@@ -158,7 +158,7 @@ class BatchQuantizedWithPagedKVCacheWrapper:
     one row per request (decode), chains or trees of drafted tokens, chunks of prompts, or all of them together.  begin_forward plans
     nothing and reads nothing back: the kernels take lengths and tables from the device, so a captured step can be replayed with others.
     workspace_buffer: scratch of a forward while it runs; forwards that may run at the same time, on two streams, need a wrapper over
-    a workspace of its own each.  Making one waits for the device's current stream, once, and is not for a capture."""
+    a workspace of its own each (two over one are both wrong, and so may later ones be until reset).  Making one waits for the device's current stream, once, and is not for a capture."""
 
     def __init__(self, workspace_buffer: torch.Tensor, kv_layout: str = "HND") -> None:
         if kv_layout != "HND":
@@ -188,6 +188,12 @@ class BatchQuantizedWithPagedKVCacheWrapper:
         other = object.__new__(type(self))
         other.__dict__.update(self.__dict__, _step=None, _held=())
         return other
+
+    def reset(self) -> None:
+        """Sets back what parts count themselves in with, of this wrapper and its copies: for a program in which two forwards have run at
+        the same time over one workspace, which leaves it off zero.  On the current stream, behind all of their forwards."""
+        for counters in self._all_counters:
+            counters.zero_()
 
     def begin_forward(self, qo_indptr: torch.Tensor, paged_kv_indptr: torch.Tensor, paged_kv_indices: torch.Tensor,
                       paged_kv_last_page_len: torch.Tensor, num_qo_heads: int, num_kv_heads: int, head_dim: int,

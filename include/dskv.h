@@ -685,7 +685,7 @@ int dskv_rope_append_quant(const dskv_quant_rows_t *rows, void *q_out, void *pag
  * of the request) * (largest magnitude in V) is under 2^128, which a magnitude of 2^90 is for any length.  Beyond, a row may be no number.
  * min_qo_len: no request has fewer rows (a hint: what does not hold costs time, not results; 0 is always right).
  * counters: dskv_quant_attn_counters(n_kv_heads) words on the device that are zero before the first call that is given them and
- * used by one call at a time, like the workspace; every call leaves them zero.
+ * used by one call at a time, like the workspace; every call leaves them zero.  (Two at a time may not: they are to be cleared then.)
  */
 typedef struct dskv_quant_step {
     dskv_tree_step_t step;

@@ -395,3 +395,19 @@ def test_a_captured_step_after_wider_ones():
         torch.cuda.synchronize()
         near(out, want, bound)
     assert all((x == 3).all() for x in others)
+
+
+def test_counters_that_are_set_back():
+    """What two forwards at the same time may leave in a wrapper's counters is gone after reset, for its copies, too."""
+    from deserve_amd.quant_ops import BatchQuantizedWithPagedKVCacheWrapper
+
+    step = make_step(37, [3000, 40], [1, 2], False, 16, 8, 2, 128, "bf16")
+    records, values = as_quantised(step)
+    pages, on = records.tensor().cuda(), step.on("cuda")
+    w = BatchQuantizedWithPagedKVCacheWrapper(torch.empty(128 << 20, dtype=torch.uint8, device="cuda"))
+    copy = w.another()
+    copy.begin_forward(*on["csr"], 8, 2, 128, 16, max_qo_len=2)
+    w._counters.fill_(1)
+    w.reset()
+    near(copy.forward(on["q"], pages), *attention(values))
+    assert not w._counters.any()
