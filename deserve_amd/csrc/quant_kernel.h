@@ -263,7 +263,6 @@ template <int DT, int kD, int kBlocks> struct QuantTile {
     static constexpr int kMergeLds = kTreeWaves * kCols * (kOPitch + 2) * 4;
     static constexpr int kLds = kTreeWaves * kWaveLds > kMergeLds ? kTreeWaves * kWaveLds : kMergeLds;
     static constexpr int kWorkgroups = quant_workgroups(DT, kD, kBlocks);
-    static constexpr int kDepth = 1;                                 // subtiles a wave has in flight
 };
 
 template <int DT, int kD, int kBlocks>
@@ -277,7 +276,7 @@ __global__ __launch_bounds__(kTreeThreads, (QuantTile<DT, kD, kBlocks>::kWorkgro
     int share, head;
     share_and_head(a, share, head);
     TreePlace place;
-    tree_place<S::kCols, S::kSub, kTreeThreads, false, kQuantLeast, kTreeWaves * S::kDepth>(a, share, place);
+    tree_place<S::kCols, S::kSub, kTreeThreads, false, kQuantLeast, kTreeWaves>(a, share, place);
     make_uniform(place);
     const int begin = place.begin, end = place.end;
     if (begin >= end) return;
@@ -290,27 +289,22 @@ __global__ __launch_bounds__(kTreeThreads, (QuantTile<DT, kD, kBlocks>::kWorkgro
     const char *const scales = a.pages + 2 * a.half_bytes + ((lane >> 5) * a.n_kv_heads + head) * 4;
     const char *const none = reinterpret_cast<const char *>(kNoRow) + load_chunk * 16;
 
-    // ---- what is requested: the wave's subtiles through all items of the share, kDepth in flight, their page ids one step
+    // ---- what is requested: the wave's subtiles through all items of the share, one in flight, its page ids one step
     // further ahead (see tree_kernel.h)
     TreeItem ahead;
     ahead.b = place.b;
     ahead.base = place.base;
     ahead.r = place.r;
     open_item<S::kCols, S::kSub>(a, begin, begin, end, ahead);
-    auto walk_end = [&](const TreeItem &x) {                    // of the wave's subtiles st0 + wave, + kTreeWaves ..; whole turns of kDepth
-        constexpr int kTurn = S::kDepth * kTreeWaves;
-        return x.st0 + wave + max((x.st1 - x.st0 - wave + kTurn - 1) / kTurn, 0) * kTurn;
-    };
-    int ahead_st = ahead.st0 + wave, ahead_end = walk_end(ahead);
+    int ahead_st = ahead.st0 + wave;
     bool more = true;
     auto settle = [&]() {                                       // on to a subtile that there is
-        if (__builtin_expect(ahead_st < ahead_end, 1)) return;
-        while (more && ahead_st >= ahead_end) {
+        if (__builtin_expect(ahead_st < ahead.st1, 1)) return;
+        while (more && ahead_st >= ahead.st1) {
             more = ahead.next < end;
             if (more) {
                 open_item<S::kCols, S::kSub>(a, ahead.next, begin, end, ahead);
                 ahead_st = ahead.st0 + wave;
-                ahead_end = walk_end(ahead);
             }
         }
     };
@@ -321,7 +315,7 @@ __global__ __launch_bounds__(kTreeThreads, (QuantTile<DT, kD, kBlocks>::kWorkgro
         settle();
         Ids x;
         x.t = ahead_st * S::kSub + (lane & (S::kSub - 1));
-        x.page = more && ahead_st < ahead.st1 ? page_of(a, ahead.r, x.t) : -1;
+        x.page = more ? page_of(a, ahead.r, x.t) : -1;
         ahead_st += kTreeWaves;
         return x;
     };
@@ -330,7 +324,7 @@ __global__ __launch_bounds__(kTreeThreads, (QuantTile<DT, kD, kBlocks>::kWorkgro
         float scale;
         uint32_t there;                                         // bit per token: there is one
     };
-    Held held[S::kDepth];
+    Held held;
     auto request = [&](const Ids &x, Held &to) {
         const uint32_t mine = quant_row(a, x.t, x.page);
         to.there = (uint32_t)__ballot(mine != kNoQuantRow);     // (lanes repeat)
@@ -415,41 +409,34 @@ __global__ __launch_bounds__(kTreeThreads, (QuantTile<DT, kD, kBlocks>::kWorkgro
         }
         if (S::kQInLds) __syncthreads();
     };
-    auto subtile = [&](Held &mine) {
-        const bool there = st < it.st1;                         // (else a turn without a subtile)
-        const uint32_t there_bits = mine.there;
+    auto subtile = [&]() {
+        const uint32_t there_bits = held.there;
         const bool whole = there_bits == ~0u && (st + 1) * S::kSub <= prior + (a.masks ? 0 : 1);
         u32x4 key[S::kTiles][kD / 64];
         f32x4 k_scale[S::kTiles], v_scale[S::kTiles];
-        if (there) {
-            __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int i = 0; i < S::kLoads; i++) {
-                const int row = load_row + S::kRowsPerLoad * i;
-                *reinterpret_cast<u32x4 *>(k_lds + row * S::kPitch + load_chunk * 16) = mine.k[i];
-                *reinterpret_cast<u32x4 *>(v_lds + row * S::kPitch + load_chunk * 16) = mine.v[i];
-            }
-            scale_lds[lane] = lane < 32 ? mine.scale * a.scale : mine.scale;
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            // LDS operands are read together and ahead
+        for (int i = 0; i < S::kLoads; i++) {
+            const int row = load_row + S::kRowsPerLoad * i;
+            *reinterpret_cast<u32x4 *>(k_lds + row * S::kPitch + load_chunk * 16) = held.k[i];
+            *reinterpret_cast<u32x4 *>(v_lds + row * S::kPitch + load_chunk * 16) = held.v[i];
+        }
+        scale_lds[lane] = lane < 32 ? held.scale * a.scale : held.scale;
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        // LDS operands are read together and ahead
 #pragma unroll
-            for (int t = 0; t < S::kTiles; t++) {
+        for (int t = 0; t < S::kTiles; t++) {
 #pragma unroll
-                for (int h = 0; h < kD / 64; h++)
-                    key[t][h] = *reinterpret_cast<const u32x4 *>(k_lds + (t * 16 + c) * S::kPitch + h * 64 + g * 16);
-                k_scale[t] = *reinterpret_cast<const f32x4 *>(scale_lds + t * 16 + 4 * g);
-                v_scale[t] = *reinterpret_cast<const f32x4 *>(scale_lds + 32 + t * 16 + 4 * g);
-            }
+            for (int h = 0; h < kD / 64; h++)
+                key[t][h] = *reinterpret_cast<const u32x4 *>(k_lds + (t * 16 + c) * S::kPitch + h * 64 + g * 16);
+            k_scale[t] = *reinterpret_cast<const f32x4 *>(scale_lds + t * 16 + 4 * g);
+            v_scale[t] = *reinterpret_cast<const f32x4 *>(scale_lds + 32 + t * 16 + 4 * g);
         }
         __builtin_amdgcn_sched_barrier(0);
         const Ids ids_next = next_ids();
-        request(ids, mine);
+        request(ids, held);
         ids = ids_next;
-        if (!there) {
-            st += kTreeWaves;
-            return;
-        }
 
         // ---- scores
         f32x4 s[kBlocks][S::kTiles];
@@ -587,18 +574,12 @@ __global__ __launch_bounds__(kTreeThreads, (QuantTile<DT, kD, kBlocks>::kWorkgro
         __syncthreads();
     };
     start_item(begin);                                          // (its loads in front of those that wait for page ids)
-#pragma unroll
-    for (int i = 0; i < S::kDepth; i++) {
-        const Ids ids_next = next_ids();
-        request(ids, held[i]);
-        ids = ids_next;
-    }
+    const Ids second = next_ids();
+    request(ids, held);
+    ids = second;
     for (;;) {
         settle_item();
-        while (st < it.st1) {
-#pragma unroll
-            for (int i = 0; i < S::kDepth; i++) subtile(held[i]);
-        }
+        while (st < it.st1) subtile();
         finish_item();
         if (it.next >= end) return;
         start_item(it.next);
