@@ -235,7 +235,8 @@ constexpr int kQuantLeast = 2 * kTreeWaves;
 //   fp32, one row    55.6; with q in registers, one workgroup 69.7.  5 rows 108 (one workgroup); with q in LDS 111
 // and 64 dims: bf16 of 12 rows 54 (three blocks; with one workgroup 78), of 16 rows 66 (four; as wide tiles 79); fp32, one row 38;
 // 51.  5 rows 53.4; with one workgroup 74, with q in LDS 55.
-// (With 128 dims three blocks leave registers for one workgroup only, 113 us for 12 rows; see QuantWide.)
+// (Four blocks at 64 dims keep 4 or 5 registers, of the item, in scratch while its subtiles run.
+// With 128 dims three blocks leave registers for one workgroup only, 113 us for 12 rows; see QuantWide.)
 constexpr int quant_columns(int dtype, int dim) { return dtype == DSKV_F32 || dim == 128 ? 32 : 64; }
 constexpr bool quant_q_in_lds(int dtype, int blocks) { return dtype == DSKV_F32 && blocks == 1; }
 constexpr int quant_workgroups(int dtype, int dim, int blocks)

@@ -9,8 +9,9 @@
 // kAhead further on requested (see kFirst, kBehind), and at its end the operands of K(j + 2) are read; where a stage holds two blocks, this is once
 // in two iterations.  The running maximum of a column is raised only when a block's weights under it
 // sum to more than most_weight in a lane.  Weights are rounded to 16 bits for the matrix product, half a step of each (see headroom).
-// Bound by the matrix and vector pipelines at the board's power cap: 16 chunks of 512 rows over up to 8 K tokens, 64 heads over 8, 128 dims, bf16, 840 us
+// Bound by the matrix and vector pipelines at the board's power cap: 16 chunks of 512 rows over up to 8 K tokens, 32 heads over 8, 128 dims, bf16, 840 us
 // with the merge, 965 TFLOP/s.
+// At 128 dims, where all waves fetch, 6 or 7 registers of an item's start (rows of q and out, its place) are in scratch until its end, none of the walk's.
 // Where a token lies in the pool, and its scales, are looked up for some thousand tokens at a time and kept in LDS, so that pages may
 // have any size.
 #pragma once
@@ -425,7 +426,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void quant_wide_kernel(QuantArgs a)
                               E::pack2(acc[d][4 * i + 2] * inv, acc[d][4 * i + 3] * inv)};
         }
         // an item that goes on in another share is the merge launch's
-        if (cut && st0 == 0 && head == 0 && threadIdx.x == 0) 
+        if (cut && st0 == 0 && head == 0 && threadIdx.x == 0)
             a.cuts[2 * share + (unit > begin ? 1 : 0)] = {(int)r.first, ct * r.tile, cols, ct, beside, parts_of(a, place, item, r.subtiles, ct)};
         unit = item + st1;
     }
