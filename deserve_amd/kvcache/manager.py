@@ -50,6 +50,11 @@ class _CopyOut:
 class KVCacheManager:
     def __init__(self, virtual_page_pool: VirtualPagePool, cpu_chunk_pool: CpuChunkPool,
                  page_table_allocator: PageTableAllocator, staging_bytes: int = 128 << 20):
+        # the copies know a chunk by its address: one for smaller pages, of 8 bits for instance, would be written past its end
+        held = cpu_chunk_pool.chunks[0].numel() * cpu_chunk_pool.chunks.element_size()
+        if held < virtual_page_pool.page_bytes or cpu_chunk_pool.num_layers < virtual_page_pool.num_layers:
+            raise ValueError(f"chunks of {cpu_chunk_pool.num_layers} layers with pages of {held} bytes do not hold "
+                             f"{virtual_page_pool.num_layers} layers with pages of {virtual_page_pool.page_bytes}")
         self.virtual_page_pool = virtual_page_pool
         self.cpu_chunk_pool = cpu_chunk_pool
         self.page_table_allocator = page_table_allocator

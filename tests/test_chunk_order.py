@@ -85,3 +85,28 @@ def test_finished_copies_are_forgotten_without_anybody_waiting():
         manager.engine.arrived = i >= 80
         manager.copy_gpu_to_cpu(one, "t").free()
     assert len(chunks._writes) <= 64 and ("a", "wait") not in log
+
+
+def test_chunks_for_smaller_pages_are_refused():
+    """A chunk is written as so many of the pool's pages: one of 8-bit pages, of fewer heads or fewer layers would end before them."""
+    import pytest
+
+    f8 = torch.float8_e4m3fn
+    tables = PageTableAllocator(8, 4096, 16, CPU)
+
+    def manager(pool_type, chunk_type, pool_sizes=(2, 2, 64), chunk_sizes=(2, 2, 64)):
+        layers, heads, dim = pool_sizes
+        pool = VirtualPagePool(layers, 40, 0, 16, CPU, pool_type, n_kv_heads=heads, head_dim=dim)
+        pool.engine = Engine("a", [])
+        layers, heads, dim = chunk_sizes
+        return KVCacheManager(pool, CpuChunkPool(layers, 4, 16, chunk_type, n_kv_heads=heads, head_dim=dim), tables)
+
+    for fine in ((f8, f8), (torch.float16, torch.bfloat16), (f8, torch.float16), (torch.float16, torch.float32)):
+        manager(*fine)
+    for small in ((torch.bfloat16, f8), (torch.float32, torch.float16)):
+        with pytest.raises(ValueError, match="do not hold"):
+            manager(*small)
+    for sizes in ((2, 1, 64), (2, 2, 32), (1, 2, 64)):
+        for kind in (f8, torch.float16):
+            with pytest.raises(ValueError, match="do not hold"):
+                manager(kind, kind, chunk_sizes=sizes)
