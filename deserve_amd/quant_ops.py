@@ -30,6 +30,7 @@ from deserve_amd import _lib
 from deserve_amd.draft_ops import MAX_TREE_ROWS, _call, _check_vector, _on_device, _token_rows
 
 CODE_DTYPE = torch.float8_e4m3fn
+INT32_MAX = 2 ** 31 - 1
 
 
 @dataclass(frozen=True)
@@ -223,8 +224,8 @@ class BatchQuantizedWithPagedKVCacheWrapper:
         self._step = _lib.QuantStep((
             qo_indptr.data_ptr(), paged_kv_indptr.data_ptr(), paged_kv_indices.data_ptr(),
             paged_kv_last_page_len.data_ptr(), None if masks is None else masks.data_ptr(), workspace.data_ptr(),
-            workspace.numel() * workspace.element_size(), paged_kv_indices.numel(), batch, 0, max_qo_len,
-            num_qo_heads, num_kv_heads, head_dim, page_size), counters.data_ptr(), counters.numel(), min_qo_len)
+            workspace.numel() * workspace.element_size(), paged_kv_indices.numel(), batch, 0, min(max_qo_len, INT32_MAX),
+            num_qo_heads, num_kv_heads, head_dim, page_size), counters.data_ptr(), counters.numel(), min(min_qo_len, INT32_MAX))
 
     def forward(self, q: torch.Tensor, pages: torch.Tensor, sm_scale: Optional[float] = None, *,
                 out: Optional[torch.Tensor] = None) -> torch.Tensor:

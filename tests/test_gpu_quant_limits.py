@@ -411,3 +411,14 @@ def test_counters_that_are_set_back():
     w.reset()
     near(copy.forward(on["q"], pages), *attention(values))
     assert not w._counters.any()
+
+
+@pytest.mark.parametrize("most", [2 ** 31 - 1, 2 ** 31, 2 ** 40, 2 ** 63 - 1])
+@pytest.mark.parametrize("dtype,n", [("bf16", 1), ("bf16", 30), ("fp32", 3)])
+def test_hints_without_a_bound(dtype, n, most):
+    """max_qo_len and min_qo_len as large as a program has numbers: all rows."""
+    step = make_step(38, [70, 40], [n, 2], False, 16, 8, 2, 64, dtype)
+    records, values = as_quantised(step)
+    pages = records.tensor().cuda()
+    near(run(step, pages, max_qo_len=most), *attention(values))
+    near(run(step, pages, max_qo_len=most, min_qo_len=most), *attention(values))
