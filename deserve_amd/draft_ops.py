@@ -265,7 +265,7 @@ class BatchTreeWithPagedKVCacheWrapper:
         self._step = _lib.TreeStep(
             qo_indptr.data_ptr(), paged_kv_indptr.data_ptr(), paged_kv_indices.data_ptr(),
             paged_kv_last_page_len.data_ptr(), _lib.ptr(masks), self._workspace.data_ptr(),
-            self._workspace.numel() * self._workspace.element_size(), paged_kv_indices.numel(), batch, 0, max_qo_len,
+            self._workspace.numel() * self._workspace.element_size(), paged_kv_indices.numel(), batch, 0, min(max_qo_len, 2 ** 31 - 1),
             num_qo_heads, num_kv_heads, head_dim, page_size)
 
     def forward(self, q: torch.Tensor, paged_kv_data: torch.Tensor, sm_scale: Optional[float] = None, *,

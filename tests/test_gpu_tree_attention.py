@@ -382,3 +382,12 @@ def test_scales_that_are_not_positive_with_many_columns(dtype, dim, rows, hq):
     for scale in (0.0, -0.05, -0.3, 0.05):
         print("[case] scale", dtype, dim, rows, hq, scale, flush=True)
         compare(run(step, on, scale), *attention(step, scale))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("most", [2 ** 31 - 1, 2 ** 31, 2 ** 40, 2 ** 63 - 1])
+@pytest.mark.parametrize("dtype,n", [("bf16", 1), ("bf16", 30), ("fp32", 3)])
+def test_max_qo_len_without_a_bound(dtype, n, most):
+    """As large as a program has numbers: all rows."""
+    step = make_step(38, [70, 40], [n, 2], False, 16, 8, 2, 64, dtype)
+    compare(run(step, max_qo_len=most), *attention(step))
